@@ -21,6 +21,8 @@ SCAN_RAW, SCAN_MODEL, SCAN_BLOCK = 0, 1, 2
 ERR_UNSUPPORTED = -4   # HCLSM_ERR_UNSUPPORTED: valid arguments the entry point does not implement
 EVENT_GT_HALF, EVENT_NONZERO = 0, 1
 ATTN_TRACK_CAUSAL, ATTN_SLOTS = 0, 1
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+POS_I32, POS_I64 = 0, 1
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -89,6 +91,10 @@ _SIGNATURES: dict[str, list] = {
     "hclsm_slot_track_reorder_update": [_c_void_p] * 6 + [_i64] * 3 + [_c_void_p, _int, _c_void_p, _i64, _c_void_p],
     "hclsm_slot_track_sequence_workspace": [_i64, _i64, _i64, _i64, _int, _int],
     "hclsm_slot_track_sequence": [_c_void_p] * 7 + [_i64] * 5 + [_f32, _c_void_p, _int, _c_void_p, _i64, _c_void_p],
+    "hclsm_norm_rotary_forward": [_c_void_p] * 2 + [_i64] * 2 + [_int, _c_void_p, _f32, _f32, _int, _int, _c_void_p],
+    "hclsm_norm_rotary_backward_workspace": [_i64, _int],
+    "hclsm_norm_rotary_backward": [_c_void_p] * 2 + [_i64] * 2 + [_int, _c_void_p, _f32, _f32, _int, _c_void_p, _i64,
+                                                                 _c_void_p],
     "hclsm_issue_probe": [_int, _i64, _int, _c_void_p, _c_void_p],
 }
 _RESTYPES = {"hclsm_strerror": ctypes.c_char_p, "hclsm_slot_attn_core_workspace": ctypes.c_int64,
@@ -99,6 +105,7 @@ _RESTYPES = {"hclsm_strerror": ctypes.c_char_p, "hclsm_slot_attn_core_workspace"
              "hclsm_relation_graph_workspace": ctypes.c_int64, "hclsm_slot_track_cost_workspace": ctypes.c_int64,
              "hclsm_slot_track_reorder_update_workspace": ctypes.c_int64,
              "hclsm_slot_track_sequence_workspace": ctypes.c_int64,
+             "hclsm_norm_rotary_backward_workspace": ctypes.c_int64,
              "hclsm_event_top_down_workspace": ctypes.c_int64, "hclsm_gnn_message_pass_workspace": ctypes.c_int64}
 
 
@@ -108,6 +115,14 @@ class HclsmSlotWeights(ctypes.Structure):
         "w_q", "w_kv", "w_ih", "w_hh", "w1", "w2", "b_ih", "b_hh", "b1", "b2",
         "ln_in_w", "ln_in_b", "ln_pre_w", "ln_pre_b", "ln_mlp_w", "ln_mlp_b", "w_qt", "w_qkv",
         "w1_n", "w1_n_sum", "w1_n_bias")]
+
+
+class HclsmHeads(ctypes.Structure):
+    """Mirror of the C struct HclsmHeads (include/hclsm_amd.h)."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "g", "y", "w", "gw", "pos")] +
+                [(n, ctypes.c_int64) for n in ("x_sb", "x_sl", "x_sh", "g_sb", "g_sl", "g_sh", "pos_sb", "pos_sl",
+                                               "B", "L", "H")] +
+                [("w_dtype", ctypes.c_int), ("pos_dtype", ctypes.c_int)])
 
 _lib = None
 

@@ -41,6 +41,8 @@ from hclsm_amd.kernels.event_attention import (
     slots_attention,
 )
 
+from hclsm_amd.kernels.norm_rotary import RotaryPlan, qk_norm_rotary, rotary_embedding
+
 from hclsm_amd.kernels.slot_attention_kernel import (
     slot_attention_core,
     slot_attention_fn,
@@ -121,6 +123,9 @@ __all__ = [
     "track_causal_event_attention",
     "TrackCausalPlan",
     "slots_attention",
+    "RotaryPlan",
+    "rotary_embedding",
+    "qk_norm_rotary",
     "gnn_message_pass_fn",
     "naive_gnn_message_pass",
     "optimized_gnn_message_pass",

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 
@@ -32,6 +34,14 @@ def common_float_dtype(*tensors: torch.Tensor) -> torch.dtype:
         if dt in (torch.float32, torch.bfloat16, torch.float16):
             return dt
     return torch.float32
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(dev: torch.device):
+    """Context in which a launch for tensors on ``dev`` is made: HIP launches go to the current device."""
+    return _SAME_DEVICE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 class HipFallbackWarning(UserWarning):

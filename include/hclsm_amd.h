@@ -50,6 +50,14 @@ extern "C" {
 #define HCLSM_SCAN_BLOCK 2  /* hclsm_ssm_scan_bwd only: MODEL with dt = clamp(softplus(dt input), 1e-3, 1) inside
                                the kernel, as hclsm_ssm_block_scan_fwd computes it (level0_ssm.py:76) */
 
+/* position rotation: which elements of a head form pair i of the first `rot` */
+#define HCLSM_ROTARY_HALF        0 /* i and i + rot / 2 */
+#define HCLSM_ROTARY_INTERLEAVED 1 /* 2i and 2i + 1 */
+
+/* element types of positions */
+#define HCLSM_POS_I32 0
+#define HCLSM_POS_I64 1
+
 /* argument errors (negative) */
 #define HCLSM_ERR_NULL        (-1) /* a required pointer is NULL */
 #define HCLSM_ERR_SHAPE       (-2) /* a size is negative, zero where not allowed, or too large */
@@ -616,6 +624,44 @@ int hclsm_slot_track_sequence(const float* slots, const float* alive, float* tra
                               int64_t* perm, float* matched, float* hidden, int64_t batch, int64_t T, int64_t N,
                               int64_t D, int64_t n_iters, float temperature, const void* const* params, int dtype,
                               void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One tensor of heads for hclsm_norm_rotary_*: x [B, L, H, dh] with its own strides (in elements; the innermost is 1,
+ * 0 repeats a tensor along an axis). */
+typedef struct HclsmHeads {
+  const void* x;       /* input, element type `dtype` */
+  const void* g;       /* backward: gradient of the output, element type `dtype`; ignored by the forward */
+  void* y;             /* contiguous [B, L, H, dh]: the output, or (backward) the gradient of x */
+  const void* w;       /* [dh] weight of the norm, nullable (ones); element type w_dtype */
+  void* gw;            /* [dh] backward: gradient of w in w_dtype, nullable (not formed) */
+  const void* pos;     /* positions by (b, l), nullable (then l) */
+  int64_t x_sb, x_sl, x_sh, g_sb, g_sl, g_sh, pos_sb, pos_sl;
+  int64_t B, L, H;
+  int w_dtype;
+  int pos_dtype;       /* HCLSM_POS_I32 / _I64 */
+} HclsmHeads;
+
+/*
+ * Norm of each head and position rotation of one or two tensors (queries and keys) in one launch:
+ *   n = x * rsqrt(mean(x^2) + eps) * w  (norm != 0; else n = x),  y = the first rot elements of n turned, the rest as is,
+ *   pair (a, b) of frequency i -> amplitude * (a cos t - b sin t, b cos t + a sin t),  t = 2 pi * position * turns[i].
+ * turns: [rot / 2] float64 on the device (angular frequency / 2 pi; NULL with rot = 0).  rot is even, 0 <= rot <= dh,
+ * 1 <= dh <= 256; layout HCLSM_ROTARY_*.  k is nullable and may differ from q in B, L and H.  y may not overlap x.
+ * Angles are formed in float64, everything else in float32 with one rounding at the store.
+ */
+int hclsm_norm_rotary_forward(const HclsmHeads* q, const HclsmHeads* k, int64_t dh, int64_t rot, int layout,
+                              const double* turns, float amplitude, float eps, int norm, int dtype, void* stream);
+
+/* Workspace bytes of hclsm_norm_rotary_backward for n_tensors (1 or 2) whose gw is wanted. */
+int64_t hclsm_norm_rotary_backward_workspace(int64_t dh, int n_tensors);
+
+/*
+ * Gradients of the normed form for the same arguments: y = gradient of x, gw = gradient of w (partial sums per
+ * workgroup in the workspace, added in a fixed order by a second launch; no float atomics).  The rotation without a
+ * norm has no entry of its own: its gradient is the forward of g with the turns negated.
+ */
+int hclsm_norm_rotary_backward(const HclsmHeads* q, const HclsmHeads* k, int64_t dh, int64_t rot, int layout,
+                               const double* turns, float amplitude, float eps, int dtype, void* workspace,
+                               int64_t workspace_bytes, void* stream);
 
 /*
  * VALU issue-rate probe (measurement support; no counterpart in the reference, whose kernels have no
