@@ -95,6 +95,9 @@ _SIGNATURES: dict[str, list] = {
     "hclsm_norm_rotary_backward_workspace": [_i64, _int],
     "hclsm_norm_rotary_backward": [_c_void_p] * 2 + [_i64] * 2 + [_int, _c_void_p, _f32, _f32, _int, _c_void_p, _i64,
                                                                  _c_void_p],
+    "hclsm_cross_attention_workspace": [_i64] * 6 + [_int, _int],
+    "hclsm_cross_attention_forward": [_c_void_p, _c_void_p, _i64, _c_void_p],
+    "hclsm_cross_attention_backward": [_c_void_p, _c_void_p, _i64, _c_void_p],
     "hclsm_issue_probe": [_int, _i64, _int, _c_void_p, _c_void_p],
 }
 _RESTYPES = {"hclsm_strerror": ctypes.c_char_p, "hclsm_slot_attn_core_workspace": ctypes.c_int64,
@@ -106,6 +109,7 @@ _RESTYPES = {"hclsm_strerror": ctypes.c_char_p, "hclsm_slot_attn_core_workspace"
              "hclsm_slot_track_reorder_update_workspace": ctypes.c_int64,
              "hclsm_slot_track_sequence_workspace": ctypes.c_int64,
              "hclsm_norm_rotary_backward_workspace": ctypes.c_int64,
+             "hclsm_cross_attention_workspace": ctypes.c_int64,
              "hclsm_event_top_down_workspace": ctypes.c_int64, "hclsm_gnn_message_pass_workspace": ctypes.c_int64}
 
 
@@ -123,6 +127,17 @@ class HclsmHeads(ctypes.Structure):
                 [(n, ctypes.c_int64) for n in ("x_sb", "x_sl", "x_sh", "g_sb", "g_sl", "g_sh", "pos_sb", "pos_sl",
                                                "B", "L", "H")] +
                 [("w_dtype", ctypes.c_int), ("pos_dtype", ctypes.c_int)])
+
+
+class HclsmCrossAttention(ctypes.Structure):
+    """Mirror of the C struct HclsmCrossAttention (include/hclsm_amd.h)."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "g", "out", "lse", "dq", "dk", "dv", "key_pad",
+                                                "key_lens", "query_lens")] +
+                [(n, ctypes.c_int64) for n in ("q_sb", "q_sl", "q_sh", "k_sb", "k_sl", "k_sh", "v_sb", "v_sl", "v_sh",
+                                               "g_sb", "g_sl", "g_sh", "key_pad_sb", "B", "Lq", "Lk", "H", "Hk",
+                                               "dh")] +
+                [("scale", ctypes.c_float), ("dtype", ctypes.c_int), ("key_lens_dtype", ctypes.c_int),
+                 ("query_lens_dtype", ctypes.c_int)])
 
 _lib = None
 

@@ -38,6 +38,9 @@ FILE_FLAGS = {
     # The attention's score and output tiles are consumed by VALU code right after each MFMA; in the VGPR
     # form they need no AGPR copies and the kernel takes fewer registers (more waves per SIMD).
     "event_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "cross_attn_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "cross_attn_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "cross_attn_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -1,0 +1,232 @@
+// Shared pieces of the cross-attention kernels: arguments, operand traits, LDS tiles.
+//
+// One unit of work is a batch row and one key head.  The G = H / Hk query heads that read a key head are rows of one
+// product: row r of a unit is query r / G of head hk G + r % G, so shared heads cost no further pass over the keys
+// and their gradients are sums over rows like any other.
+//
+// Every product is formed transposed so that a lane owns one query row or one key (li = lane % 16) in all of them
+// (g = lane / 16):
+//   S^T = K Q^T     16 x 16 tile: the lane holds keys 4g .. 4g + 3 of its row li,
+//   O^T = V^T P^T   those values, rounded, are the second operand as they stand: the contraction runs over the keys in
+//                   the order 4g + r of one tile (float32) or of a pair of tiles (16 bits), and V^T is read in that
+//                   order (ds_read_b64_tr_b16: lane li gets rows 4g .. 4g + 3 of column li),
+// and the same with rows and keys exchanged for the gradients of k and v.
+#pragma once
+
+#include "internal.h"
+
+namespace hclsm {
+
+typedef float caf4 __attribute__((ext_vector_type(4)));
+typedef __bf16 cab8 __attribute__((ext_vector_type(8)));
+typedef _Float16 cah8 __attribute__((ext_vector_type(8)));
+typedef short cas4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) cas4 ca_lds_s4;
+
+struct CaArgs {
+  const char *q, *k, *v, *g;        // inputs; gradient of the output
+  char *o, *dq, *dk, *dv;           // contiguous [B, Lq, H, dh] / [B, Lk, Hk, dh]
+  float* lse;                       // [B, H, Lq] natural logarithm, -inf for rows without keys
+  float* delta;                     // [B, H, Lq] sum(g o), written by the dq kernel for the dk, dv kernel
+  float* part;                      // partial sums of a split launch
+  float* part_lse;                  // forward: log2 of the partial denominators
+  int64_t qsb, qsl, qsh, ksb, ksl, ksh, vsb, vsl, vsh, gsb, gsl, gsh;   // element strides
+  const uint8_t* pad;               // [B, Lk] nonzero: key not read; nullable
+  int64_t psb;
+  const void *klens, *qlens;        // [B] live keys / queries, nullable
+  int klens64, qlens64;
+  int Hk, G, Lq, Lk, dh;
+  uint32_t gmul;                    // row / G = (row * gmul) >> 32 >> gshift (G > 1)
+  int gshift;
+  int units, tiles, nsplit, by_xcd;
+  float scale, scale_log2;
+};
+
+// 16-byte operand fragments.  EPC: elements per 16 bytes; KS: contraction per fragment; NPT: 16-row tiles whose
+// values make one fragment of a product over rows.
+template <int DT> struct CaT;
+template <> struct CaT<HCLSM_BF16> {
+  using T = uint16_t;
+  using Frag = cab8;
+  static constexpr int EPC = 8, KS = 32, NPT = 2;
+  static __device__ __forceinline__ caf4 mma(Frag a, Frag b, caf4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack2(float a, float b) { return pack_bf16x2(a, b); }
+  static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+};
+template <> struct CaT<HCLSM_F16> {
+  using T = uint16_t;
+  using Frag = cah8;
+  static constexpr int EPC = 8, KS = 32, NPT = 2;
+  static __device__ __forceinline__ caf4 mma(Frag a, Frag b, caf4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    h2 r;
+    r.x = (_Float16)a;
+    r.y = (_Float16)b;
+    return __builtin_bit_cast(uint32_t, r);
+  }
+  static __device__ __forceinline__ float lo(uint32_t w) { return (float)__builtin_bit_cast(_Float16, (uint16_t)w); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16)); }
+};
+template <> struct CaT<HCLSM_F32> {
+  using T = float;
+  using Frag = caf4;
+  static constexpr int EPC = 4, KS = 16, NPT = 1;
+  // element e of both operands is the contraction index 4g + e: any order will do as long as both use it
+  static __device__ __forceinline__ caf4 mma(Frag a, Frag b, caf4 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <int DT> __device__ __forceinline__ typename CaT<DT>::Frag ca_frag(uint4 w) {
+  return __builtin_bit_cast(typename CaT<DT>::Frag, w);
+}
+
+// Fragment of the values of NPT tiles (t[0] alone for float32), rounded to the operand type.
+template <int DT> __device__ __forceinline__ typename CaT<DT>::Frag ca_pack(const caf4* t) {
+  if constexpr (DT == HCLSM_F32) {
+    return t[0];
+  } else {
+    using A = CaT<DT>;
+    const uint4 w = {A::pack2(t[0][0], t[0][1]), A::pack2(t[0][2], t[0][3]), A::pack2(t[1][0], t[1][1]),
+                     A::pack2(t[1][2], t[1][3])};
+    return ca_frag<DT>(w);
+  }
+}
+
+// sum over the elements of a 16-byte chunk of a * b
+template <int DT> __device__ __forceinline__ float ca_dot(uint4 a, uint4 b, float s) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == HCLSM_F32) {
+      s += __uint_as_float(x[i]) * __uint_as_float(y[i]);
+    } else {
+      s += CaT<DT>::lo(x[i]) * CaT<DT>::lo(y[i]);
+      s += CaT<DT>::hi(x[i]) * CaT<DT>::hi(y[i]);
+    }
+  }
+  return s;
+}
+
+// Four consecutive elements of an output row.
+template <int DT> __device__ __forceinline__ void ca_store4(char* base, int64_t i, caf4 v) {
+  if constexpr (DT == HCLSM_F32) {
+    *reinterpret_cast<caf4*>(base + i * 4) = v;
+  } else {
+    const uint2 w = {CaT<DT>::pack2(v[0], v[1]), CaT<DT>::pack2(v[2], v[3])};
+    *reinterpret_cast<uint2*>(base + i * 2) = w;
+  }
+}
+
+// Rows of DH elements in LDS, as 16-byte chunks.  Two reads have to be free of bank conflicts: 16 rows at one chunk
+// (operands along a row), and 32 bytes of each of 8 rows (the transposing read).  Rows of 128 bytes and more whose
+// chunk count is a power of two exchange chunks by row; others are padded by one chunk.
+template <int DT, int DH> struct CaTile {
+  static constexpr int CH = DH / CaT<DT>::EPC;
+  static constexpr bool XOR = DT != HCLSM_F32 && (CH == 8 || CH == 16 || CH == 32);
+  static constexpr int STRIDE = XOR ? CH * 16 : CH * 16 + 16;
+  static __device__ __forceinline__ int off(int row, int chunk) {
+    if constexpr (XOR) {
+      const int x = CH == 8 ? (row & 7) ^ ((row >> 3) & 1) : ((row & 7) << 1) | ((row >> 3) & 1);
+      return row * STRIDE + ((chunk ^ x) << 4);
+    } else {
+      return row * STRIDE + (chunk << 4);
+    }
+  }
+  // operand with rows row0 + li as its free index and elements KS c + 4 or 8 g .. of the row as contraction
+  static __device__ __forceinline__ typename CaT<DT>::Frag frag(const char* t, int row0, int c, int li, int g) {
+    return ca_frag<DT>(*reinterpret_cast<const uint4*>(t + off(row0 + li, 4 * c + g)));
+  }
+  // operand with columns 16 dt + li as its free index and rows row0 + 4g .. + 3 (and row0 + 16 + 4g ..) as contraction
+  static __device__ __forceinline__ typename CaT<DT>::Frag frag_t(char* t, int row0, int dt, int li, int g) {
+    if constexpr (DT == HCLSM_F32) {
+      caf4 r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        r[e] = *reinterpret_cast<const float*>(t + (row0 + 4 * g + e) * STRIDE + (16 * dt + li) * 4);
+      return r;
+    } else {
+      const int row = row0 + 4 * g + (li >> 2), chunk = 2 * dt + ((li >> 1) & 1), sub = (li & 1) * 8;
+      const cas4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ca_lds_s4*)(t + off(row, chunk) + sub));
+      const cas4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ca_lds_s4*)(t + off(row + 16, chunk) + sub));
+      typedef short s8 __attribute__((ext_vector_type(8)));
+      const s8 r = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      return __builtin_bit_cast(typename CaT<DT>::Frag, r);
+    }
+  }
+};
+
+__device__ __forceinline__ int ca_len(const void* lens, int is64, int64_t b, int most) {
+  if (lens == nullptr) return most;
+  const int64_t n = is64 ? reinterpret_cast<const int64_t*>(lens)[b] : (int64_t)reinterpret_cast<const int32_t*>(lens)[b];
+  return n < 0 ? 0 : n > most ? most : (int)n;
+}
+
+// Unit, tile and split of a workgroup.  by_xcd: workgroup i runs on XCD i % 8, each with its own L2, so the
+// tiles of one unit are given to one XCD and its keys (or rows) are fetched from HBM once.
+struct CaWork {
+  int unit, tile, split;
+  int64_t b;
+  int hk, rows, keys;       // live rows and keys (before the padding mask) of the unit
+};
+
+__device__ __forceinline__ bool ca_work(const CaArgs& a, CaWork& w) {
+  const uint32_t per = (uint32_t)a.tiles * (uint32_t)a.nsplit;
+  uint32_t i = blockIdx.x, rest;
+  if (a.by_xcd) {
+    const uint32_t j = i >> 3;
+    w.unit = (int)((j / per) * 8 + (i & 7));
+    rest = j % per;
+  } else {
+    w.unit = (int)(i / per);
+    rest = i % per;
+  }
+  if (w.unit >= a.units) return false;
+  w.split = (int)(rest / (uint32_t)a.tiles);
+  w.tile = (int)(rest % (uint32_t)a.tiles);
+  w.b = w.unit / a.Hk;
+  w.hk = w.unit - (int)w.b * a.Hk;
+  w.rows = ca_len(a.qlens, a.qlens64, w.b, a.Lq) * a.G;
+  w.keys = ca_len(a.klens, a.klens64, w.b, a.Lk);
+  return true;
+}
+
+__device__ __forceinline__ void ca_row(const CaArgs& a, int row, int& qi, int& hg) {
+  qi = row;
+  hg = 0;
+  if (a.G > 1) {
+    qi = (int)(__umulhi((uint32_t)row, a.gmul) >> a.gshift);
+    hg = row - qi * a.G;
+  }
+}
+
+// [begin, end) of a split's share of n, in whole multiples of `step` but for the end.
+__device__ __forceinline__ void ca_range(int n, int nsplit, int split, int step, int& begin, int& end) {
+  if (nsplit == 1) {
+    begin = 0;
+    end = n;
+    return;
+  }
+  const int64_t share = ((int64_t)((n + step - 1) / step) + nsplit - 1) / nsplit * step;
+  const int64_t b = share * split, e = b + share;
+  begin = b < n ? (int)b : n;
+  end = e < n ? (int)e : n;
+}
+
+// Host side: one launch per (element type, padded head size) is picked in cross_attn.hip.
+int ca_forward_f32(CaArgs a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st);
+int ca_forward_bf16(CaArgs a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st);
+int ca_forward_f16(CaArgs a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st);
+int ca_backward_f32(CaArgs a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st);
+int ca_backward_bf16(CaArgs a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st);
+int ca_backward_f16(CaArgs a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st);
+
+}  // namespace hclsm

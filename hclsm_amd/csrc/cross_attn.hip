@@ -1,0 +1,112 @@
+// Cross attention: argument checks and dispatch by element type.
+#include "cross_attn.h"
+
+namespace hclsm {
+namespace {
+
+constexpr int64_t CA_MAX_DH = 256;
+
+// Rows of 16 bytes' alignment: the kernels read and write whole 16-byte (outputs: 8-byte) vectors.
+bool ca_aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int esz) {
+  const int64_t n = 16 / esz;
+  return (uintptr_t)p % 16 == 0 && s0 % n == 0 && s1 % n == 0 && s2 % n == 0;
+}
+
+int ca_sizes(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t dh, int dtype) {
+  if (B < 0 || Lq < 0 || Lk < 0 || H < 0 || Hk < 0 || dh < 1) return HCLSM_ERR_SHAPE;
+  if (dtype < HCLSM_F32 || dtype > HCLSM_F16) return HCLSM_ERR_DTYPE;
+  if (B > 0x7fffffff || Lq > 0x7fffffff || Lk > 0x7fffffff || H > 0x7fffffff) return HCLSM_ERR_SHAPE;
+  if (H > 0 && (Hk == 0 || H % Hk != 0)) return HCLSM_ERR_SHAPE;
+  if (dh > CA_MAX_DH || dh % 8 != 0) return HCLSM_ERR_UNSUPPORTED;
+  // rows of a unit and units are int32; 128 to spare for tile arithmetic past the last row
+  if (H > 0 && Lq > (0x7fffffff - 512) / (H / Hk)) return HCLSM_ERR_UNSUPPORTED;
+  if (Lk > 0x7fffffff - 512) return HCLSM_ERR_UNSUPPORTED;
+  if (Hk > 0 && B > (0x7fffffff - 8) / Hk) return HCLSM_ERR_UNSUPPORTED;
+  return 0;
+}
+
+int ca_args(const HclsmCrossAttention* x, int bwd, CaArgs& a) {
+  if (x == nullptr) return HCLSM_ERR_NULL;
+  if (int rc = ca_sizes(x->B, x->Lq, x->Lk, x->H, x->Hk, x->dh, x->dtype)) return rc;
+  if (!(x->scale > 0.f) || !(x->scale < 3.0e38f)) return HCLSM_ERR_SHAPE;
+  const bool rows = x->B && x->Lq && x->H, keys = x->B && x->Lk && x->Hk;
+  const int esz = x->dtype == HCLSM_F32 ? 4 : 2;
+  if (rows) {
+    if (!x->q || !x->out || (bwd && (!x->g || !x->dq || !x->lse))) return HCLSM_ERR_NULL;
+    if (!ca_aligned(x->q, x->q_sb, x->q_sl, x->q_sh, esz) || !ca_aligned(x->out, 0, 0, 0, esz)) return HCLSM_ERR_UNSUPPORTED;
+    if (bwd && (!ca_aligned(x->g, x->g_sb, x->g_sl, x->g_sh, esz) || !ca_aligned(x->dq, 0, 0, 0, esz)))
+      return HCLSM_ERR_UNSUPPORTED;
+  }
+  if (keys) {
+    if (!x->k || !x->v || (bwd && (!x->dk || !x->dv))) return HCLSM_ERR_NULL;
+    if (!ca_aligned(x->k, x->k_sb, x->k_sl, x->k_sh, esz) || !ca_aligned(x->v, x->v_sb, x->v_sl, x->v_sh, esz))
+      return HCLSM_ERR_UNSUPPORTED;
+    if (bwd && (!ca_aligned(x->dk, 0, 0, 0, esz) || !ca_aligned(x->dv, 0, 0, 0, esz))) return HCLSM_ERR_UNSUPPORTED;
+  }
+  for (int code : {x->key_lens_dtype, x->query_lens_dtype})
+    if (code != HCLSM_POS_I32 && code != HCLSM_POS_I64) return HCLSM_ERR_DTYPE;
+  a.q = (const char*)x->q; a.k = (const char*)x->k; a.v = (const char*)x->v; a.g = (const char*)x->g;
+  a.o = (char*)x->out; a.dq = (char*)x->dq; a.dk = (char*)x->dk; a.dv = (char*)x->dv;
+  a.lse = x->lse;
+  a.qsb = x->q_sb; a.qsl = x->q_sl; a.qsh = x->q_sh;
+  a.ksb = x->k_sb; a.ksl = x->k_sl; a.ksh = x->k_sh;
+  a.vsb = x->v_sb; a.vsl = x->v_sl; a.vsh = x->v_sh;
+  a.gsb = x->g_sb; a.gsl = x->g_sl; a.gsh = x->g_sh;
+  a.pad = x->key_pad;
+  a.psb = x->key_pad_sb;
+  a.klens = x->key_lens; a.qlens = x->query_lens;
+  a.klens64 = x->key_lens_dtype == HCLSM_POS_I64; a.qlens64 = x->query_lens_dtype == HCLSM_POS_I64;
+  a.Hk = (int)x->Hk;
+  a.G = x->Hk ? (int)(x->H / x->Hk) : 1;
+  a.Lq = (int)x->Lq; a.Lk = (int)x->Lk; a.dh = (int)x->dh;
+  // row / G by a product: with 2^(l-1) < G <= 2^l and m = floor(2^(31+l) / G) + 1, floor(row m / 2^(31+l)) is
+  // exact for row < 2^31
+  a.gmul = 0;
+  a.gshift = 0;
+  if (a.G > 1) {
+    int l = 1;
+    while ((1ll << l) < a.G) ++l;
+    a.gmul = (uint32_t)((1ull << (31 + l)) / (uint64_t)a.G + 1);
+    a.gshift = l - 1;
+  }
+  a.scale = x->scale;
+  a.scale_log2 = x->scale * HCLSM_LOG2E;
+  return 0;
+}
+
+}  // namespace
+}  // namespace hclsm
+
+extern "C" int64_t hclsm_cross_attention_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t dh,
+                                                   int dtype, int backward) {
+  using namespace hclsm;
+  if (int rc = ca_sizes(B, Lq, Lk, H, Hk, dh, dtype)) return rc;
+  return backward ? (B * Lq * H * 4 + 255) / 256 * 256 : 0;
+}
+
+extern "C" int hclsm_cross_attention_forward(const HclsmCrossAttention* x, void* workspace, int64_t workspace_bytes,
+                                             void* stream) {
+  using namespace hclsm;
+  CaArgs a{};
+  if (int rc = ca_args(x, 0, a)) return rc;
+  if (x->B == 0 || x->Lq == 0 || x->H == 0) return 0;
+  const hipStream_t st = (hipStream_t)stream;
+  if (x->dtype == HCLSM_F32) return ca_forward_f32(a, x->B, workspace, workspace_bytes, st);
+  if (x->dtype == HCLSM_BF16) return ca_forward_bf16(a, x->B, workspace, workspace_bytes, st);
+  return ca_forward_f16(a, x->B, workspace, workspace_bytes, st);
+}
+
+extern "C" int hclsm_cross_attention_backward(const HclsmCrossAttention* x, void* workspace, int64_t workspace_bytes,
+                                              void* stream) {
+  using namespace hclsm;
+  CaArgs a{};
+  if (int rc = ca_args(x, 1, a)) return rc;
+  if (x->B == 0 || x->Hk == 0) return 0;
+  const int64_t need = hclsm_cross_attention_workspace(x->B, x->Lq, x->Lk, x->H, x->Hk, x->dh, x->dtype, 1);
+  if (need > 0 && workspace == nullptr) return HCLSM_ERR_NULL;
+  if (workspace_bytes < need) return HCLSM_ERR_SHAPE;
+  const hipStream_t st = (hipStream_t)stream;
+  if (x->dtype == HCLSM_F32) return ca_backward_f32(a, x->B, workspace, workspace_bytes, st);
+  if (x->dtype == HCLSM_BF16) return ca_backward_bf16(a, x->B, workspace, workspace_bytes, st);
+  return ca_backward_f16(a, x->B, workspace, workspace_bytes, st);
+}

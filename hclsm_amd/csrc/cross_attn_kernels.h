@@ -1,0 +1,638 @@
+// Cross-attention kernels, instantiated for one element type per source file (cross_attn_{f32,bf16,f16}.hip).
+#pragma once
+
+#include "cross_attn.h"
+
+namespace hclsm {
+
+// A tile of ROWS rows on its way from global memory to LDS: loaded into registers while the tile before it is being
+// worked on, then written.  Rows past the last one are read at the last row's address and written as zeros, as
+// are rows whose bit of `live` is clear: what a masked row holds (NaN included) never reaches a product.
+template <int DT, int DH, int NT, int ROWS> struct CaStage {
+  using A = CaT<DT>;
+  using Tile = CaTile<DT, DH>;
+  static constexpr int TOTAL = ROWS * Tile::CH, N = (TOTAL + NT - 1) / NT;
+  static constexpr int ESZ = (int)sizeof(typename A::T);
+  uint4 r[N];
+
+  // rows t0 .. of a tensor with one address per row
+  __device__ __forceinline__ void load(const char* base, int64_t stride, int t0, int last, int dh) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = (int)threadIdx.x + n * NT, row = i / Tile::CH, ch = i - row * Tile::CH;
+      r[n] = uint4{0, 0, 0, 0};
+      if (i < TOTAL && ch * A::EPC < dh) {
+        const int rr = t0 + row < last ? t0 + row : last;
+        r[n] = *reinterpret_cast<const uint4*>(base + ((int64_t)rr * stride + ch * A::EPC) * ESZ);
+      }
+    }
+  }
+  // rows t0 .. of a unit (query and head of the group)
+  __device__ __forceinline__ void load_rows(const CaArgs& a, const char* base, int64_t sl, int64_t sh, int t0, int last) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = (int)threadIdx.x + n * NT, row = i / Tile::CH, ch = i - row * Tile::CH;
+      r[n] = uint4{0, 0, 0, 0};
+      if (i < TOTAL && ch * A::EPC < a.dh) {
+        int qi, hg;
+        ca_row(a, t0 + row < last ? t0 + row : last, qi, hg);
+        r[n] = *reinterpret_cast<const uint4*>(base + (qi * sl + hg * sh + ch * A::EPC) * ESZ);
+      }
+    }
+  }
+  __device__ __forceinline__ void write(char* t, uint64_t live, bool full) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = (int)threadIdx.x + n * NT, row = i / Tile::CH, ch = i - row * Tile::CH;
+      if (i < TOTAL)
+        *reinterpret_cast<uint4*>(t + Tile::off(row, ch)) = full || (live >> row & 1) ? r[n] : uint4{0, 0, 0, 0};
+    }
+  }
+};
+
+// Bits of the live keys among t0 .. t0 + ROWS - 1: below `end` and not flagged.  p: this lane's flag.
+template <int ROWS> __device__ __forceinline__ uint64_t ca_live(int t0, int end, uint8_t p) {
+  const int lane = threadIdx.x & 63;
+  return __ballot(lane < ROWS && t0 + lane < end && p == 0);
+}
+template <int ROWS> __device__ __forceinline__ uint8_t ca_flag(const uint8_t* pad, int t0, int end) {
+  const int lane = threadIdx.x & 63;
+  return pad != nullptr && lane < ROWS && t0 + lane < end ? pad[t0 + lane] : (uint8_t)0;
+}
+template <int ROWS> constexpr uint64_t CA_FULL = ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1;
+
+// A row's operand fragments straight from global memory (zeros past dh and for rows that are not live).
+template <int DT, int DH> __device__ __forceinline__ void ca_row_frags(const char* p, int g, int dh, bool live, uint4* f) {
+  using A = CaT<DT>;
+#pragma unroll
+  for (int c = 0; c < DH / A::KS; ++c) {
+    const int e = (4 * c + g) * A::EPC;
+    f[c] = uint4{0, 0, 0, 0};
+    if (live && e < dh) f[c] = *reinterpret_cast<const uint4*>(p + e * (int)sizeof(typename A::T));
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------- forward
+//
+// NW waves of 16 QT rows each over tiles of KR keys in LDS (two buffers, one barrier per tile), with the running
+// maximum and sum of the softmax per row.  Statistics and accumulators are float32; the weights are rounded to the
+// operand type for the second product (relative 2^-9 for bf16, 2^-12 for fp16; the matrix unit has no wider operand at
+// this rate), their sum is not.
+template <int DT, int DH, int NW, int QT, int KR>
+__global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
+  using A = CaT<DT>;
+  using Tile = CaTile<DT, DH>;
+  using Frag = typename A::Frag;
+  constexpr int NT = 64 * NW, KT = KR / 16, NC = DH / A::KS, ND = DH / 16, NPT = A::NPT, ESZ = (int)sizeof(typename A::T);
+  constexpr int TB = KR * Tile::STRIDE;
+  extern __shared__ __attribute__((aligned(16))) char lds[];   // [2][K tile, V tile]
+
+  CaWork w;
+  if (!ca_work(a, w)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+  const int row0 = (w.tile * NW + wave) * 16 * QT;
+  int k0, k1;
+  ca_range(w.keys, a.nsplit, w.split, KR, k0, k1);
+  if (w.tile * NW * 16 * QT >= w.rows) k1 = k0;      // no live row in this workgroup
+
+  const char* kp = a.k + (w.b * a.ksb + w.hk * a.ksh) * ESZ;
+  const char* vp = a.v + (w.b * a.vsb + w.hk * a.vsh) * ESZ;
+  const uint8_t* pad = a.pad ? a.pad + w.b * a.psb : nullptr;
+
+  Frag q[QT][NC];
+  {
+    const char* qp = a.q + (w.b * a.qsb + (int64_t)w.hk * a.G * a.qsh) * ESZ;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const int r = row0 + 16 * t + li;
+      int qi, hg;
+      ca_row(a, r < w.rows ? r : 0, qi, hg);
+      uint4 f[NC];
+      ca_row_frags<DT, DH>(qp + (qi * a.qsl + hg * a.qsh) * ESZ, g, a.dh, r < w.rows, f);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) q[t][c] = ca_frag<DT>(f[c]);
+    }
+  }
+
+  caf4 o[QT][ND];
+  float m[QT], l[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int nt = (k1 - k0 + KR - 1) / KR;
+  CaStage<DT, DH, NT, KR> sk, sv;
+  uint8_t flag = 0;
+  uint64_t live = 0;
+  if (nt > 0) {
+    sk.load(kp, a.ksl, k0, k1 - 1, a.dh);
+    sv.load(vp, a.vsl, k0, k1 - 1, a.dh);
+    flag = ca_flag<KR>(pad, k0, k1);
+    live = ca_live<KR>(k0, k1, flag);
+    sk.write(lds, live, live == CA_FULL<KR>);
+    sv.write(lds + TB, live, live == CA_FULL<KR>);
+    if (nt > 1) {
+      sk.load(kp, a.ksl, k0 + KR, k1 - 1, a.dh);
+      sv.load(vp, a.vsl, k0 + KR, k1 - 1, a.dh);
+      flag = ca_flag<KR>(pad, k0 + KR, k1);
+    }
+  }
+  for (int i = 0; i < nt; ++i) {
+    char* tk = lds + (i & 1) * 2 * TB;
+    char* tv = tk + TB;
+    const uint64_t now = live;
+    __syncthreads();      // tile i is written, and every wave is done with the other buffer
+    if (i + 1 < nt) {
+      char* nk = lds + ((i + 1) & 1) * 2 * TB;
+      live = ca_live<KR>(k0 + (i + 1) * KR, k1, flag);
+      sk.write(nk, live, live == CA_FULL<KR>);
+      sv.write(nk + TB, live, live == CA_FULL<KR>);
+      if (i + 2 < nt) {
+        const int t0 = k0 + (i + 2) * KR;
+        sk.load(kp, a.ksl, t0, k1 - 1, a.dh);
+        sv.load(vp, a.vsl, t0, k1 - 1, a.dh);
+        flag = ca_flag<KR>(pad, t0, k1);
+      }
+    }
+
+    caf4 s[QT][KT];
+#pragma unroll
+    for (int k = 0; k < KT; ++k) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t) s[t][k] = caf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const Frag f = Tile::frag(tk, 16 * k, c, li, g);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) s[t][k] = A::mma(f, q[t][c], s[t][k]);
+      }
+    }
+    if (now != CA_FULL<KR>) {
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        const uint32_t bits = (uint32_t)(now >> (16 * k + 4 * g));
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[t][k][r] = bits >> r & 1 ? s[t][k][r] : -INFINITY;
+      }
+    }
+    Frag p[QT][KT / NPT];
+    bool grew = false;
+    float alpha[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      float mx = m[t];
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][k][r]);
+      mx = rows4_max(mx);
+      const float base = mx == -INFINITY ? 0.f : mx * a.scale_log2;
+      alpha[t] = fast_exp2(m[t] * a.scale_log2 - base);      // 0 for the first live tile (m = -inf)
+      grew |= mx > m[t];
+      m[t] = mx;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[t][k][r] = fast_exp2(s[t][k][r] * a.scale_log2 - base);
+          sum += s[t][k][r];
+        }
+      l[t] = l[t] * alpha[t] + sum;
+#pragma unroll
+      for (int u = 0; u < KT / NPT; ++u) p[t][u] = ca_pack<DT>(&s[t][u * NPT]);
+    }
+    if (__any(grew)) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[t][d] *= alpha[t];
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int u = 0; u < KT / NPT; ++u) {
+        const Frag f = Tile::frag_t(tv, 16 * NPT * u, d, li, g);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) o[t][d] = A::mma(f, p[t][u], o[t][d]);
+      }
+  }
+
+  // rows without a live key have l = 0: zeros, and a log-sum of -inf
+  const int all = a.Lq * a.G;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const float sum = rows4_sum(l[t]);
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    const int r = row0 + 16 * t + li;
+    if (r >= all) continue;
+    const bool in = r < w.rows;
+    int qi, hg;
+    ca_row(a, r, qi, hg);
+    const int h = w.hk * a.G + hg;
+    const float ls2 = in && sum > 0.f ? m[t] * a.scale_log2 + __log2f(sum) : in && sum != sum ? sum : -INFINITY;
+    if (a.nsplit > 1) {
+      const int64_t pr = ((int64_t)w.split * a.units + w.unit) * all + r;
+      if (g == 0) a.part_lse[pr] = ls2;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+        if (16 * d + 4 * g < a.dh)
+          *reinterpret_cast<caf4*>(a.part + pr * a.dh + 16 * d + 4 * g) = in ? o[t][d] * inv : caf4{0.f, 0.f, 0.f, 0.f};
+    } else {
+      if (g == 0 && a.lse) a.lse[(w.b * a.Hk * a.G + h) * a.Lq + qi] = ls2 * HCLSM_LN2;
+      const int64_t ob = ((w.b * a.Lq + qi) * a.Hk * a.G + h) * (int64_t)a.dh;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+        if (16 * d + 4 * g < a.dh) ca_store4<DT>(a.o, ob + 16 * d + 4 * g, in ? o[t][d] * inv : caf4{0.f, 0.f, 0.f, 0.f});
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------- gradient of the queries
+//
+// As the forward, with S^T and dP^T = V g^T formed per tile, p = exp(s - lse), ds = p (dP - delta) and
+// dQ^T = K^T ds^T.  delta = sum(g o) per row is formed here and left for the second kernel.  ds is rounded to the
+// operand type for its product, as the weights are in the forward.
+template <int DT, int DH, int NW, int QT, int KR>
+__global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
+  using A = CaT<DT>;
+  using Tile = CaTile<DT, DH>;
+  using Frag = typename A::Frag;
+  constexpr int NT = 64 * NW, KT = KR / 16, NC = DH / A::KS, ND = DH / 16, NPT = A::NPT, ESZ = (int)sizeof(typename A::T);
+  constexpr int TB = KR * Tile::STRIDE;
+  extern __shared__ __attribute__((aligned(16))) char lds[];   // [2][K tile, V tile]
+
+  CaWork w;
+  if (!ca_work(a, w)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+  const int row0 = (w.tile * NW + wave) * 16 * QT;
+  int k0, k1;
+  ca_range(w.keys, a.nsplit, w.split, KR, k0, k1);
+  if (w.tile * NW * 16 * QT >= w.rows) k1 = k0;
+
+  const char* kp = a.k + (w.b * a.ksb + w.hk * a.ksh) * ESZ;
+  const char* vp = a.v + (w.b * a.vsb + w.hk * a.vsh) * ESZ;
+  const uint8_t* pad = a.pad ? a.pad + w.b * a.psb : nullptr;
+
+  Frag q[QT][NC], go[QT][NC];
+  float lse2[QT], delta[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + 16 * t + li;
+    const bool in = r < w.rows;
+    int qi, hg;
+    ca_row(a, in ? r : 0, qi, hg);
+    const int h = w.hk * a.G + hg;
+    const int64_t stat = (w.b * a.Hk * a.G + h) * a.Lq + qi;
+    uint4 fq[NC], fg[NC], fo[NC];
+    ca_row_frags<DT, DH>(a.q + (w.b * a.qsb + qi * a.qsl + h * a.qsh) * ESZ, g, a.dh, in, fq);
+    ca_row_frags<DT, DH>(a.g + (w.b * a.gsb + qi * a.gsl + h * a.gsh) * ESZ, g, a.dh, in, fg);
+    ca_row_frags<DT, DH>(a.o + ((w.b * a.Lq + qi) * a.Hk * a.G + h) * (int64_t)a.dh * ESZ, g, a.dh, in, fo);
+    const float ls = in ? a.lse[stat] : -INFINITY;
+    lse2[t] = ls == -INFINITY ? INFINITY : ls * HCLSM_LOG2E;      // no key: every weight is exp(-inf)
+    float dsum = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      dsum = ca_dot<DT>(fg[c], fo[c], dsum);
+      q[t][c] = ca_frag<DT>(fq[c]);
+      go[t][c] = ca_frag<DT>(fg[c]);
+    }
+    delta[t] = rows4_sum(dsum);
+    if (in && g == 0 && w.split == 0) a.delta[stat] = delta[t];
+  }
+
+  caf4 dq[QT][ND];
+#pragma unroll
+  for (int t = 0; t < QT; ++t)
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dq[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
+
+  const int nt = (k1 - k0 + KR - 1) / KR;
+  CaStage<DT, DH, NT, KR> sk, sv;
+  uint8_t flag = 0;
+  uint64_t live = 0;
+  if (nt > 0) {
+    sk.load(kp, a.ksl, k0, k1 - 1, a.dh);
+    sv.load(vp, a.vsl, k0, k1 - 1, a.dh);
+    flag = ca_flag<KR>(pad, k0, k1);
+    live = ca_live<KR>(k0, k1, flag);
+    sk.write(lds, live, live == CA_FULL<KR>);
+    sv.write(lds + TB, live, live == CA_FULL<KR>);
+    if (nt > 1) {
+      sk.load(kp, a.ksl, k0 + KR, k1 - 1, a.dh);
+      sv.load(vp, a.vsl, k0 + KR, k1 - 1, a.dh);
+      flag = ca_flag<KR>(pad, k0 + KR, k1);
+    }
+  }
+  for (int i = 0; i < nt; ++i) {
+    char* tk = lds + (i & 1) * 2 * TB;
+    char* tv = tk + TB;
+    const uint64_t now = live;
+    __syncthreads();
+    if (i + 1 < nt) {
+      char* nk = lds + ((i + 1) & 1) * 2 * TB;
+      live = ca_live<KR>(k0 + (i + 1) * KR, k1, flag);
+      sk.write(nk, live, live == CA_FULL<KR>);
+      sv.write(nk + TB, live, live == CA_FULL<KR>);
+      if (i + 2 < nt) {
+        const int t0 = k0 + (i + 2) * KR;
+        sk.load(kp, a.ksl, t0, k1 - 1, a.dh);
+        sv.load(vp, a.vsl, t0, k1 - 1, a.dh);
+        flag = ca_flag<KR>(pad, t0, k1);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < KT / NPT; ++u) {
+      caf4 s[QT][NPT], dp[QT][NPT];
+#pragma unroll
+      for (int k = 0; k < NPT; ++k) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) s[t][k] = dp[t][k] = caf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const Frag fk = Tile::frag(tk, 16 * (u * NPT + k), c, li, g);
+          const Frag fv = Tile::frag(tv, 16 * (u * NPT + k), c, li, g);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            s[t][k] = A::mma(fk, q[t][c], s[t][k]);
+            dp[t][k] = A::mma(fv, go[t][c], dp[t][k]);
+          }
+        }
+      }
+      Frag ds[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+#pragma unroll
+        for (int k = 0; k < NPT; ++k) {
+          const uint32_t bits = (uint32_t)(now >> (16 * (u * NPT + k) + 4 * g));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = fast_exp2(s[t][k][r] * a.scale_log2 - lse2[t]);
+            dp[t][k][r] = bits >> r & 1 ? p * (dp[t][k][r] - delta[t]) : 0.f;
+          }
+        }
+        ds[t] = ca_pack<DT>(dp[t]);
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const Frag f = Tile::frag_t(tk, 16 * NPT * u, d, li, g);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) dq[t][d] = A::mma(f, ds[t], dq[t][d]);
+      }
+    }
+  }
+
+  const int all = a.Lq * a.G;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + 16 * t + li;
+    if (r >= all) continue;
+    const bool in = r < w.rows;
+    int qi, hg;
+    ca_row(a, r, qi, hg);
+    const int64_t ob = a.nsplit > 1 ? (((int64_t)w.split * a.units + w.unit) * all + r) * a.dh
+                                    : ((w.b * a.Lq + qi) * a.Hk * a.G + w.hk * a.G + hg) * (int64_t)a.dh;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      if (16 * d + 4 * g < a.dh) {
+        const caf4 v = in ? dq[t][d] * a.scale : caf4{0.f, 0.f, 0.f, 0.f};
+        if (a.nsplit > 1) *reinterpret_cast<caf4*>(a.part + ob + 16 * d + 4 * g) = v;
+        else ca_store4<DT>(a.dq, ob + 16 * d + 4 * g, v);
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------- gradients of the keys and values
+//
+// NW waves of 16 KT keys each, K and V operands in registers, over tiles of RR rows (q and g in LDS):
+// S = Q K^T and dP = g V^T with a lane per key, then dV^T = g^T p and dK^T = Q^T ds.  Shared heads are rows of the
+// unit, so their gradients are added here.  Keys that are not live get zeros.
+template <int DT, int DH, int NW, int KT, int RR>
+__global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
+  using A = CaT<DT>;
+  using Tile = CaTile<DT, DH>;
+  using Frag = typename A::Frag;
+  constexpr int NT = 64 * NW, RT = RR / 16, NC = DH / A::KS, ND = DH / 16, NPT = A::NPT, ESZ = (int)sizeof(typename A::T);
+  constexpr int TB = RR * Tile::STRIDE, BUF = 2 * TB + RR * 8;
+  extern __shared__ __attribute__((aligned(16))) char lds[];   // [2][Q tile, g tile, RR log-sums, RR deltas]
+
+  CaWork w;
+  if (!ca_work(a, w)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+  const int key0 = (w.tile * NW + wave) * 16 * KT;
+  int r0, r1;
+  ca_range(w.rows, a.nsplit, w.split, RR, r0, r1);
+  if (w.tile * NW * 16 * KT >= w.keys) r1 = r0;
+
+  const char* kp = a.k + (w.b * a.ksb + w.hk * a.ksh) * ESZ;
+  const char* vp = a.v + (w.b * a.vsb + w.hk * a.vsh) * ESZ;
+  const char* qp = a.q + (w.b * a.qsb + (int64_t)w.hk * a.G * a.qsh) * ESZ;
+  const char* gp = a.g + (w.b * a.gsb + (int64_t)w.hk * a.G * a.gsh) * ESZ;
+  const int64_t stat0 = (w.b * a.Hk + w.hk) * a.G * (int64_t)a.Lq;
+
+  Frag fk[KT][NC], fv[KT][NC];
+  bool live[KT];
+#pragma unroll
+  for (int t = 0; t < KT; ++t) {
+    const int key = key0 + 16 * t + li;
+    live[t] = key < w.keys && (a.pad == nullptr || a.pad[w.b * a.psb + key] == 0);
+    const int kk = live[t] ? key : 0;
+    uint4 f0[NC], f1[NC];
+    ca_row_frags<DT, DH>(kp + kk * a.ksl * ESZ, g, a.dh, live[t], f0);
+    ca_row_frags<DT, DH>(vp + kk * a.vsl * ESZ, g, a.dh, live[t], f1);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) { fk[t][c] = ca_frag<DT>(f0[c]); fv[t][c] = ca_frag<DT>(f1[c]); }
+  }
+  caf4 dk[KT][ND], dv[KT][ND];
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dk[t][d] = dv[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
+
+  const int nt = (r1 - r0 + RR - 1) / RR;
+  CaStage<DT, DH, NT, RR> sq, sg;
+  float st_lse = INFINITY, st_delta = 0.f;
+  auto load = [&](int t0) {
+    sq.load_rows(a, qp, a.qsl, a.qsh, t0, r1 - 1);
+    sg.load_rows(a, gp, a.gsl, a.gsh, t0, r1 - 1);
+    st_lse = INFINITY;         // rows past the last one, and rows without keys: every weight is exp(-inf)
+    st_delta = 0.f;
+    if ((int)threadIdx.x < RR && t0 + (int)threadIdx.x < r1) {
+      int qi, hg;
+      ca_row(a, t0 + (int)threadIdx.x, qi, hg);
+      const int64_t i = stat0 + (int64_t)hg * a.Lq + qi;
+      const float ls = a.lse[i];
+      if (ls != -INFINITY) st_lse = ls * HCLSM_LOG2E;
+      st_delta = a.delta[i];
+    }
+  };
+  auto write = [&](int t0, char* buf) {
+    const int n = r1 - t0;
+    const bool full = n >= RR;
+    const uint64_t mask = full ? ~0ull : (1ull << n) - 1;
+    sq.write(buf, mask, full);
+    sg.write(buf + TB, mask, full);
+    if ((int)threadIdx.x < RR) {
+      reinterpret_cast<float*>(buf + 2 * TB)[threadIdx.x] = st_lse;
+      reinterpret_cast<float*>(buf + 2 * TB)[RR + threadIdx.x] = st_delta;
+    }
+  };
+  if (nt > 0) {
+    load(r0);
+    write(r0, lds);
+    if (nt > 1) load(r0 + RR);
+  }
+  for (int i = 0; i < nt; ++i) {
+    char* tq = lds + (i & 1) * BUF;
+    char* tg = tq + TB;
+    const float* stat = reinterpret_cast<const float*>(tq + 2 * TB);
+    __syncthreads();
+    if (i + 1 < nt) {
+      write(r0 + (i + 1) * RR, lds + ((i + 1) & 1) * BUF);
+      if (i + 2 < nt) load(r0 + (i + 2) * RR);
+    }
+#pragma unroll
+    for (int u = 0; u < RT / NPT; ++u) {
+      caf4 s[KT][NPT], dp[KT][NPT];
+#pragma unroll
+      for (int k = 0; k < NPT; ++k) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) s[t][k] = dp[t][k] = caf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const Frag fq = Tile::frag(tq, 16 * (u * NPT + k), c, li, g);
+          const Frag fg = Tile::frag(tg, 16 * (u * NPT + k), c, li, g);
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
+            s[t][k] = A::mma(fq, fk[t][c], s[t][k]);
+            dp[t][k] = A::mma(fg, fv[t][c], dp[t][k]);
+          }
+        }
+      }
+      Frag p[KT], ds[KT];
+#pragma unroll
+      for (int k = 0; k < NPT; ++k) {
+        const caf4 ls = *reinterpret_cast<const caf4*>(stat + 16 * (u * NPT + k) + 4 * g);
+        const caf4 de = *reinterpret_cast<const caf4*>(stat + RR + 16 * (u * NPT + k) + 4 * g);
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float e = fast_exp2(s[t][k][r] * a.scale_log2 - ls[r]);
+            s[t][k][r] = live[t] ? e : 0.f;
+            dp[t][k][r] = s[t][k][r] * (dp[t][k][r] - de[r]);
+          }
+      }
+#pragma unroll
+      for (int t = 0; t < KT; ++t) { p[t] = ca_pack<DT>(s[t]); ds[t] = ca_pack<DT>(dp[t]); }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const Frag fg = Tile::frag_t(tg, 16 * NPT * u, d, li, g);
+        const Frag fq = Tile::frag_t(tq, 16 * NPT * u, d, li, g);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          dv[t][d] = A::mma(fg, p[t], dv[t][d]);
+          dk[t][d] = A::mma(fq, ds[t], dk[t][d]);
+        }
+      }
+    }
+  }
+
+  const int64_t half = (int64_t)a.nsplit * a.units * a.Lk * a.dh;      // split: dk sums, then dv sums
+#pragma unroll
+  for (int t = 0; t < KT; ++t) {
+    const int key = key0 + 16 * t + li;
+    if (key >= a.Lk) continue;
+    const int64_t ob = a.nsplit > 1 ? (((int64_t)w.split * a.units + w.unit) * a.Lk + key) * a.dh
+                                    : ((w.b * a.Lk + key) * a.Hk + w.hk) * (int64_t)a.dh;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      if (16 * d + 4 * g < a.dh) {
+        const int64_t i = ob + 16 * d + 4 * g;
+        if (a.nsplit > 1) {
+          *reinterpret_cast<caf4*>(a.part + i) = dk[t][d] * a.scale;
+          *reinterpret_cast<caf4*>(a.part + half + i) = dv[t][d];
+        } else {
+          ca_store4<DT>(a.dk, i, dk[t][d] * a.scale);
+          ca_store4<DT>(a.dv, i, dv[t][d]);
+        }
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------- launches
+
+// Tile sizes by the bytes of a padded row: two buffers of two tiles have to fit the 160 KB of LDS next to
+// another workgroup where rows are short, and the accumulators and operands of a wave its registers.
+template <int DT, int DH> struct CaShape {
+  static constexpr int RB = DH * (int)sizeof(typename CaT<DT>::T);
+  static constexpr int TR = RB <= 256 ? 64 : 32;      // rows of a tile
+  static constexpr int T = RB <= 256 ? 2 : 1;         // 16-row tiles per wave
+  static constexpr int LDS = 4 * TR * CaTile<DT, DH>::STRIDE;
+  static constexpr int LDS_DKV = LDS + 2 * TR * 8;
+};
+
+constexpr int CA_MAX_LDS = 160 * 1024;
+
+inline bool ca_by_xcd(int64_t units) { return units % 8 == 0 || units >= 64; }
+
+template <typename K>
+int ca_launch(K kernel, CaArgs& a, int64_t batch, int64_t rows, int per_wg, int threads, int lds, std::atomic<int>* cache,
+              hipStream_t st) {
+  int grid = 0;
+  if (int rc = device_launch_setup((const void*)kernel, threads, lds, lds > 65536 ? CA_MAX_LDS : 0, cache, &grid)) return rc;
+  const int64_t units = batch * a.Hk, tiles = (rows + per_wg - 1) / per_wg;
+  a.units = (int)units;
+  a.tiles = (int)tiles;
+  a.by_xcd = ca_by_xcd(units);
+  const int64_t blocks = (a.by_xcd ? (units + 7) / 8 * 8 : units) * tiles * a.nsplit;
+  if (blocks == 0) return 0;
+  if (blocks > 0x7fffffff / threads) return HCLSM_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, st, a);
+  HCLSM_LAUNCH_CHECK();
+  return 0;
+}
+
+template <int DT, int DH> int ca_forward_dh(CaArgs& a, int64_t batch, void*, int64_t, hipStream_t st) {
+  using S = CaShape<DT, DH>;
+  static std::atomic<int> cache[HCLSM_MAX_DEVICES];
+  a.nsplit = 1;
+  return ca_launch(ca_fwd_kernel<DT, DH, 4, S::T, S::TR>, a, batch, (int64_t)a.Lq * a.G, 64 * S::T, 256, S::LDS, cache, st);
+}
+
+template <int DT, int DH> int ca_backward_dh(CaArgs& a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st) {
+  using S = CaShape<DT, DH>;
+  static std::atomic<int> cq[HCLSM_MAX_DEVICES], ck[HCLSM_MAX_DEVICES];
+  const int64_t stats = batch * a.Hk * a.G * a.Lq;
+  if (ws_bytes < stats * 4) return HCLSM_ERR_SHAPE;
+  a.delta = (float*)ws;
+  a.nsplit = 1;
+  if (int rc = ca_launch(ca_dq_kernel<DT, DH, 4, S::T, S::TR>, a, batch, (int64_t)a.Lq * a.G, 64 * S::T, 256, S::LDS, cq, st))
+    return rc;
+  return ca_launch(ca_dkv_kernel<DT, DH, 4, S::T, S::TR>, a, batch, a.Lk, 64 * S::T, 256, S::LDS_DKV, ck, st);
+}
+
+template <int DT> int ca_forward_dt(CaArgs a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st) {
+  if (a.dh <= 32) return ca_forward_dh<DT, 32>(a, batch, ws, ws_bytes, st);
+  if (a.dh <= 64) return ca_forward_dh<DT, 64>(a, batch, ws, ws_bytes, st);
+  if (a.dh <= 96) return ca_forward_dh<DT, 96>(a, batch, ws, ws_bytes, st);
+  if (a.dh <= 128) return ca_forward_dh<DT, 128>(a, batch, ws, ws_bytes, st);
+  if (a.dh <= 192) return ca_forward_dh<DT, 192>(a, batch, ws, ws_bytes, st);
+  return ca_forward_dh<DT, 256>(a, batch, ws, ws_bytes, st);
+}
+template <int DT> int ca_backward_dt(CaArgs a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st) {
+  if (a.dh <= 32) return ca_backward_dh<DT, 32>(a, batch, ws, ws_bytes, st);
+  if (a.dh <= 64) return ca_backward_dh<DT, 64>(a, batch, ws, ws_bytes, st);
+  if (a.dh <= 96) return ca_backward_dh<DT, 96>(a, batch, ws, ws_bytes, st);
+  if (a.dh <= 128) return ca_backward_dh<DT, 128>(a, batch, ws, ws_bytes, st);
+  if (a.dh <= 192) return ca_backward_dh<DT, 192>(a, batch, ws, ws_bytes, st);
+  return ca_backward_dh<DT, 256>(a, batch, ws, ws_bytes, st);
+}
+
+}  // namespace hclsm

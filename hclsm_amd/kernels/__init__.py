@@ -41,6 +41,8 @@ from hclsm_amd.kernels.event_attention import (
     slots_attention,
 )
 
+from hclsm_amd.kernels.cross_attention import cross_attention
+
 from hclsm_amd.kernels.norm_rotary import RotaryPlan, qk_norm_rotary, rotary_embedding
 
 from hclsm_amd.kernels.slot_attention_kernel import (
@@ -123,6 +125,7 @@ __all__ = [
     "track_causal_event_attention",
     "TrackCausalPlan",
     "slots_attention",
+    "cross_attention",
     "RotaryPlan",
     "rotary_embedding",
     "qk_norm_rotary",

@@ -1,0 +1,167 @@
+"""Attention of queries against keys and values of another length (libhclsm_amd.so: hclsm_cross_attention_*).
+
+    out = cross_attention(q, k, v)                       # q (B, Lq, H, dh), k and v (B, Lk, Hk, dh)
+
+Slots or learned goal queries against the tokens of an encoder or the events of a clip: the attention core of
+``nn.MultiheadAttention`` with keys of their own (the reference's dynamics/level2_goal.py:50,63 and
+perception/multimodal_fuser.py:40; projections stay outside), with key heads shared by groups of query heads, lengths per
+batch row, a key padding mask, gradients, and a form for few queries that splits the keys over the GPU.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from hclsm_amd import _lib
+from hclsm_amd.kernels._common import on_device, require_gpu
+from hclsm_amd.kernels.ssm_scan_kernel import _no_node
+
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+MAX_HEAD_DIM = 256
+
+
+def _check(q, k, v, key_padding_mask, key_lens, query_lens, scale):
+    fn = "cross_attention"
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError(f"{fn}: {name} must be (B, L, H, dh), got shape {tuple(t.shape)}")
+        if t.dtype not in _FLOATS or t.dtype != q.dtype:
+            raise TypeError(f"{fn}: q, k, v must share one dtype among bfloat16, float16, float32, got {name} {t.dtype}")
+    B, Lq, H, dh = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != dh:
+        raise ValueError(f"{fn}: k and v must be ({B}, Lk, Hk, {dh}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    Lk, Hk = k.shape[1], k.shape[2]
+    if Hk < 1 or H % Hk:
+        raise ValueError(f"{fn}: {H} query heads cannot share {Hk} key heads")
+    if not 8 <= dh <= MAX_HEAD_DIM or dh % 8:
+        raise ValueError(f"{fn}: heads of 8, 16, .. {MAX_HEAD_DIM} elements, got {dh}")
+    if key_padding_mask is not None and tuple(key_padding_mask.shape) != (B, Lk):
+        raise ValueError(f"{fn}: key_padding_mask must be ({B}, {Lk}), got {tuple(key_padding_mask.shape)}")
+    for name, t in (("key_lens", key_lens), ("query_lens", query_lens)):
+        if t is None:
+            continue
+        if t.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{fn}: {name} must be int32 or int64, got {t.dtype}")
+        if tuple(t.shape) != (B,):
+            raise ValueError(f"{fn}: {name} must be ({B},), got {tuple(t.shape)}")
+    if not 0 < scale < float("inf"):
+        raise ValueError(f"{fn}: scale must be positive, got {scale}")
+
+
+def _rows(t):
+    """t with rows on 16-byte boundaries (t itself where they are)."""
+    n = 16 // t.element_size()
+    sb, sl, sh, s = t.stride()
+    B, L, H, dh = t.shape
+    if ((s == 1 or dh == 1) and t.data_ptr() % 16 == 0 and (sb % n == 0 or B == 1) and (sl % n == 0 or L == 1)
+            and (sh % n == 0 or H == 1)):
+        return t
+    return t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 else t.clone()
+
+
+def _strides(t):
+    sb, sl, sh, _ = t.stride()
+    B, L, H, _ = t.shape
+    return sb if B > 1 else 0, sl if L > 1 else 0, sh if H > 1 else 0
+
+
+def _struct(q, k, v, out, lse, pad, klens, qlens, scale, g=None, dq=None, dk=None, dv=None):
+    B, Lq, H, dh = q.shape
+    p = _lib.ptr
+    code = lambda t: _lib.POS_I64 if t is not None and t.dtype == torch.int64 else _lib.POS_I32
+    return _lib.HclsmCrossAttention(
+        p(q), p(k), p(v), p(g), p(out), p(lse), p(dq), p(dk), p(dv), p(pad), p(klens), p(qlens), *_strides(q),
+        *_strides(k), *_strides(v), *((0, 0, 0) if g is None else _strides(g)),
+        0 if pad is None else (pad.stride(0) if B > 1 else 0), B, Lq, k.shape[1], H, k.shape[2], dh, scale,
+        _lib.dtype_code(q.dtype), code(klens), code(qlens))
+
+
+def _workspace(q, k, backward):
+    B, Lq, H, dh = q.shape
+    n = int(_lib.lib().hclsm_cross_attention_workspace(B, Lq, k.shape[1], H, k.shape[2], dh, _lib.dtype_code(q.dtype),
+                                                       backward))
+    if n < 0:
+        _lib.check(n, "hclsm_cross_attention_workspace")
+    return (torch.empty(n, dtype=torch.uint8, device=q.device) if n else None), n
+
+
+def _forward(q, k, v, pad, klens, qlens, scale, want_lse):
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    B, Lq, H, _ = q.shape
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device) if want_lse else None
+    ws, n = _workspace(q, k, 0)
+    x = _struct(q, k, v, out, lse, pad, klens, qlens, scale)
+    with on_device(q.device):
+        rc = _lib.lib().hclsm_cross_attention_forward(ctypes.byref(x), _lib.ptr(ws), n, _lib.stream_of(q))
+    _lib.check(rc, "hclsm_cross_attention_forward")
+    return out, lse
+
+
+def _backward(q, k, v, out, lse, g, pad, klens, qlens, scale):
+    q, k, v, g = _rows(q), _rows(k), _rows(v), _rows(g.to(q.dtype))
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
+    ws, n = _workspace(q, k, 1)
+    x = _struct(q, k, v, out, lse, pad, klens, qlens, scale, g, dq, dk, dv)
+    with on_device(q.device):
+        rc = _lib.lib().hclsm_cross_attention_backward(ctypes.byref(x), _lib.ptr(ws), n, _lib.stream_of(q))
+    _lib.check(rc, "hclsm_cross_attention_backward")
+    return dq, dk, dv
+
+
+class _CrossAttention(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, k, v, pad, klens, qlens, scale):
+        out, lse = _forward(q, k, v, pad, klens, qlens, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, pad, klens, qlens)
+        ctx.scale = scale
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _):
+        q, k, v, out, lse, pad, klens, qlens = ctx.saved_tensors
+        return (*_backward(q, k, v, out, lse, g, pad, klens, qlens, ctx.scale), None, None, None, None)
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_padding_mask: torch.Tensor | None = None,
+                    key_lens: torch.Tensor | None = None, query_lens: torch.Tensor | None = None,
+                    scale: float | None = None, return_lse: bool = False):
+    """softmax(scale q k^T) v for every head.
+
+    q (B, Lq, H, dh); k, v (B, Lk, Hk, dh): head h reads key head h // (H // Hk).  One dtype among bfloat16, float16,
+        float32; dh a multiple of 8 up to 256; any strides (rows that are not contiguous or not on 16-byte boundaries
+        are copied; a batch of stride 0 is read as it stands).
+    key_padding_mask (B, Lk), True = ignore that key (nn.MultiheadAttention's convention); key_lens (B,) int32 or int64:
+        keys from key_lens[b] on are ignored.  What ignored keys hold, NaN and infinities among it, has no effect.
+    query_lens (B,): queries from query_lens[b] on give zeros, and take part in no gradient.
+    scale: dh ** -0.5 if None; positive.
+
+    Returns out (B, Lq, H, dh) [, lse (B, H, Lq) float32: the softmax's log-denominator, not differentiable].  A query
+    with no key to read gives zeros (lse -inf) and zero gradients (slots_attention gives NaN there).  Differentiable in
+    q, k and v; the same inputs give the same bits.  Scores, softmax and sums are float32; with 16-bit inputs the
+    weights (and in the backward the scores' gradients) are rounded to the inputs' type for the matrix products."""
+    require_gpu("cross_attention", q, k, v, key_padding_mask, key_lens, query_lens)
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    scale = float(scale)
+    _check(q, k, v, key_padding_mask, key_lens, query_lens, scale)
+    pad = key_padding_mask
+    if pad is not None:
+        if pad.dtype not in (torch.bool, torch.uint8):
+            pad = pad != 0
+        if pad.stride(1) != 1:
+            pad = pad.contiguous()
+    klens = key_lens if key_lens is None or key_lens.stride(0) == 1 else key_lens.contiguous()
+    qlens = query_lens if query_lens is None or query_lens.stride(0) == 1 else query_lens.contiguous()
+    if _no_node((q, k, v)):
+        out, lse = _forward(q, k, v, pad, klens, qlens, scale, return_lse)
+    else:
+        out, lse = _CrossAttention.apply(q, k, v, pad, klens, qlens, scale)
+    return (out, lse) if return_lse else out

@@ -663,6 +663,48 @@ int hclsm_norm_rotary_backward(const HclsmHeads* q, const HclsmHeads* k, int64_t
                                const double* turns, float amplitude, float eps, int dtype, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
+/* Cross attention: queries of one length against keys and values of another.  Strides in elements (innermost 1); the
+ * inputs' rows, and every output, lie on 16-byte boundaries. */
+typedef struct HclsmCrossAttention {
+  const void* q;       /* [B, Lq, H, dh] */
+  const void* k;       /* [B, Lk, Hk, dh]: query head h reads key head h / (H / Hk) */
+  const void* v;       /* [B, Lk, Hk, dh] */
+  const void* g;       /* backward: gradient of out, [B, Lq, H, dh] */
+  void* out;           /* contiguous [B, Lq, H, dh]: written by the forward, read by the backward */
+  float* lse;          /* [B, H, Lq]: written by the forward (nullable there), read by the backward */
+  void* dq;            /* backward: contiguous [B, Lq, H, dh] */
+  void* dk;            /* backward: contiguous [B, Lk, Hk, dh] */
+  void* dv;
+  const uint8_t* key_pad;   /* [B, Lk], batch stride key_pad_sb: nonzero = key not read; nullable */
+  const void* key_lens;     /* [B] live keys, nullable (all); clamped to 0 .. Lk; HCLSM_POS_I32 / _I64 */
+  const void* query_lens;   /* [B] live queries, nullable (all); clamped to 0 .. Lq */
+  int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, g_sb, g_sl, g_sh, key_pad_sb;
+  int64_t B, Lq, Lk, H, Hk, dh;
+  float scale;              /* > 0 */
+  int dtype, key_lens_dtype, query_lens_dtype;
+} HclsmCrossAttention;
+
+/* Workspace bytes of hclsm_cross_attention_forward (backward = 0) or _backward (1); HCLSM_ERR_* for sizes they refuse. */
+int64_t hclsm_cross_attention_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t dh, int dtype,
+                                        int backward);
+
+/*
+ * out[b, i, h] = sum_j p_ij v[b, j, h / G],  p = softmax over the live keys j of scale * q[b, i, h] . k[b, j, h / G],
+ * lse = the logarithm of the softmax's denominator.  A key is live if it is below key_lens[b] and not flagged; keys that
+ * are not live are not read into any product (they may hold anything).  Queries from query_lens[b] on, and queries of
+ * a batch row without a live key, get out = 0 and lse = -inf.
+ * H is a multiple of Hk; dh a multiple of 8 up to 256 (HCLSM_ERR_UNSUPPORTED otherwise).  Scores, softmax and sums in
+ * float32; 16-bit operands round the weights to their type for the product with v.
+ * (The reference runs torch's nn.MultiheadAttention here: dynamics/level2_goal.py:50,63, multimodal_fuser.py:40.)
+ */
+int hclsm_cross_attention_forward(const HclsmCrossAttention* x, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Gradients of sum(g * out): dq, dk, dv, with out and lse as the forward left them.  Queries that are not live give
+ * and get none; keys that are not live get zeros.  Sums over shared heads and over rows in a fixed order (no atomics).
+ */
+int hclsm_cross_attention_backward(const HclsmCrossAttention* x, void* workspace, int64_t workspace_bytes, void* stream);
+
 /*
  * VALU issue-rate probe (measurement support; no counterpart in the reference, whose kernels have no
  * roofline).  Launches `waves` one-wave workgroups; each runs `iters` iterations of a fixed block of
