@@ -101,6 +101,18 @@ template <int DT> __device__ __forceinline__ typename CaT<DT>::Frag ca_pack(cons
   }
 }
 
+// Maxima that pass a NaN on (v_maximum3_f32: one instruction for two values, and no step to quiet its operands first).
+__device__ __forceinline__ float ca_max3(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+// over the four lanes that share a row, as rows4_max
+__device__ __forceinline__ float ca_rows4_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __builtin_elementwise_maximum(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // sum over the elements of a 16-byte chunk of a * b
 template <int DT> __device__ __forceinline__ float ca_dot(uint4 a, uint4 b, float s) {
   const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
@@ -220,6 +232,21 @@ __device__ __forceinline__ void ca_range(int n, int nsplit, int split, int step,
   begin = b < n ? (int)b : n;
   end = e < n ? (int)e : n;
 }
+
+// How a forward is launched, a function of the sizes alone (the workspace is sized by the same rule).
+struct CaPlan {
+  int few;        // 0: tiles of many rows; 1, 2: 16 or 32 rows per workgroup of ca_few_kernel
+  int nsplit;     // workgroups that share a unit's keys; their results are joined by ca_join_kernel
+};
+constexpr int CA_MAX_SPLIT = 256;
+// Rows (in bytes, padded head) up to which ca_few_kernel is built for 16 and for 32 rows: its step of keys and values, the
+// next one, the accumulators and the queries all live in registers, and longer heads would spill.
+constexpr int CA_FEW1_BYTES = 512, CA_FEW2_BYTES = 256;
+constexpr int64_t ca_padded_dh(int64_t dh) {
+  return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : dh <= 128 ? 128 : dh <= 192 ? 192 : 256;
+}
+CaPlan ca_forward_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t dh, int dtype);
+int ca_join(const CaArgs& a, int dtype, hipStream_t st);
 
 // Host side: one launch per (element type, padded head size) is picked in cross_attn.hip.
 int ca_forward_f32(CaArgs a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st);

@@ -1,7 +1,76 @@
 // Cross attention: argument checks and dispatch by element type.
 #include "cross_attn.h"
 
+#include <cstdlib>
 namespace hclsm {
+
+CaPlan ca_forward_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t dh, int dtype) {
+  const int64_t rows = Lq * G, units = B * Hk;
+  CaPlan p{0, 1};
+  const int64_t bytes = ca_padded_dh(dh) * (dtype == HCLSM_F32 ? 4 : 2);
+  p.few = rows <= 16 && bytes <= CA_FEW1_BYTES ? 1 : rows <= 32 && bytes <= CA_FEW2_BYTES ? 2 : 0;
+  if (getenv("CA_FEW")) p.few = atoi(getenv("CA_FEW"));
+  const int64_t per = p.few ? 16 * p.few : bytes <= 256 ? 128 : 64;
+  const int64_t wgs = units * ((rows + per - 1) / per);
+  const int64_t target = getenv("CA_TARGET") ? atoi(getenv("CA_TARGET")) : 1024, least = getenv("CA_LEAST") ? atoi(getenv("CA_LEAST")) : 256;
+  int64_t n = wgs > 0 ? target / wgs : 1;
+  if (n > Lk / least) n = Lk / least;
+  p.nsplit = (int)(n < 1 ? 1 : n > CA_MAX_SPLIT ? CA_MAX_SPLIT : n);
+  return p;
+}
+
+// A row's partial results joined: weights exp2(lse_s - lse), one workgroup per row, TC lanes of four columns each and
+// 256 / TC groups of lanes that take every so many of the splits; the groups add up in order.
+template <int DT>
+__global__ void __launch_bounds__(256) ca_join_kernel(const CaArgs a, int tc) {
+  __shared__ float s_lse[CA_MAX_SPLIT];
+  __shared__ caf4 s_acc[256];
+  const int all = a.Lq * a.G;
+  const int64_t stride = (int64_t)a.units * all;
+  for (int64_t row = blockIdx.x; row < stride; row += gridDim.x) {
+    if ((int)threadIdx.x < a.nsplit) s_lse[threadIdx.x] = a.part_lse[(int64_t)threadIdx.x * stride + row];
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f;
+    for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, s_lse[s]);
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int s = 0; s < a.nsplit; ++s) sum += fast_exp2(s_lse[s] - base);
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    const int c = threadIdx.x & (tc - 1), sl = threadIdx.x / tc, n = 256 / tc;
+    caf4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (4 * c < a.dh) {
+#pragma unroll 4
+      for (int s = sl; s < a.nsplit; s += n)
+        acc += *reinterpret_cast<const caf4*>(a.part + (s * stride + row) * a.dh + 4 * c) * fast_exp2(s_lse[s] - base);
+    }
+    s_acc[threadIdx.x] = acc;
+    __syncthreads();
+    const int unit = (int)(row / all), r = (int)(row - (int64_t)unit * all);
+    int qi, hg;
+    ca_row(a, r, qi, hg);
+    const int64_t b = unit / a.Hk;
+    const int h = (unit - (int)b * a.Hk) * a.G + hg;
+    if (sl == 0 && 4 * c < a.dh) {
+      for (int i = 1; i < n; ++i) acc += s_acc[i * tc + c];
+      ca_store4<DT>(a.o, ((b * a.Lq + qi) * a.Hk * a.G + h) * (int64_t)a.dh + 4 * c, acc * inv);
+    }
+    if (threadIdx.x == 0 && a.lse)
+      a.lse[(b * a.Hk * a.G + h) * a.Lq + qi] = sum > 0.f ? (base + __log2f(sum)) * HCLSM_LN2 : sum != sum ? sum : -INFINITY;
+    __syncthreads();
+  }
+}
+
+int ca_join(const CaArgs& a, int dtype, hipStream_t st) {
+  const int64_t rows = (int64_t)a.units * a.Lq * a.G;
+  int tc = 2;
+  while (4 * tc < a.dh) tc *= 2;
+  const unsigned grid = (unsigned)(rows < 65536 ? rows : 65536);
+  if (dtype == HCLSM_F32) hipLaunchKernelGGL(ca_join_kernel<HCLSM_F32>, dim3(grid), dim3(256), 0, st, a, tc);
+  else if (dtype == HCLSM_BF16) hipLaunchKernelGGL(ca_join_kernel<HCLSM_BF16>, dim3(grid), dim3(256), 0, st, a, tc);
+  else hipLaunchKernelGGL(ca_join_kernel<HCLSM_F16>, dim3(grid), dim3(256), 0, st, a, tc);
+  HCLSM_LAUNCH_CHECK();
+  return 0;
+}
+
 namespace {
 
 constexpr int64_t CA_MAX_DH = 256;
@@ -81,7 +150,10 @@ extern "C" int64_t hclsm_cross_attention_workspace(int64_t B, int64_t Lq, int64_
                                                    int dtype, int backward) {
   using namespace hclsm;
   if (int rc = ca_sizes(B, Lq, Lk, H, Hk, dh, dtype)) return rc;
-  return backward ? (B * Lq * H * 4 + 255) / 256 * 256 : 0;
+  if (backward) return (B * Lq * H * 4 + 255) / 256 * 256;
+  if (B == 0 || Lq == 0 || H == 0) return 0;
+  const CaPlan p = ca_forward_plan(B, Lq, Lk, Hk, H / Hk, dh, dtype);
+  return p.nsplit > 1 ? p.nsplit * B * Lq * H * (dh + 1) * 4 : 0;
 }
 
 extern "C" int hclsm_cross_attention_forward(const HclsmCrossAttention* x, void* workspace, int64_t workspace_bytes,

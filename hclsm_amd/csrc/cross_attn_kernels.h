@@ -1,7 +1,7 @@
 // Cross-attention kernels, instantiated for one element type per source file (cross_attn_{f32,bf16,f16}.hip).
 #pragma once
 
-#include "cross_attn.h"
+#include "cross_attn_few.h"
 
 namespace hclsm {
 
@@ -15,37 +15,40 @@ template <int DT, int DH, int NT, int ROWS> struct CaStage {
   static constexpr int ESZ = (int)sizeof(typename A::T);
   uint4 r[N];
 
+  static __device__ __forceinline__ int row(int n) { return ((int)threadIdx.x + n * NT) / Tile::CH; }
+  static __device__ __forceinline__ int chunk(int n) { return ((int)threadIdx.x + n * NT) % Tile::CH; }
+  static __device__ __forceinline__ bool in(int n) { return TOTAL % NT == 0 || (int)threadIdx.x + n * NT < TOTAL; }
+  // byte offset of the chunk in its row; chunks past dh are read at the row's start and written as zeros
+  static __device__ __forceinline__ int col(int n, int dh) { return chunk(n) * A::EPC < dh ? chunk(n) * 16 : 0; }
+
   // rows t0 .. of a tensor with one address per row
   __device__ __forceinline__ void load(const char* base, int64_t stride, int t0, int last, int dh) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int i = (int)threadIdx.x + n * NT, row = i / Tile::CH, ch = i - row * Tile::CH;
-      r[n] = uint4{0, 0, 0, 0};
-      if (i < TOTAL && ch * A::EPC < dh) {
-        const int rr = t0 + row < last ? t0 + row : last;
-        r[n] = *reinterpret_cast<const uint4*>(base + ((int64_t)rr * stride + ch * A::EPC) * ESZ);
-      }
+      const int rr = t0 + row(n) < last ? t0 + row(n) : last;
+      if (in(n)) r[n] = *reinterpret_cast<const uint4*>(base + (int64_t)rr * stride * ESZ + col(n, dh));
     }
   }
   // rows t0 .. of a unit (query and head of the group)
   __device__ __forceinline__ void load_rows(const CaArgs& a, const char* base, int64_t sl, int64_t sh, int t0, int last) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int i = (int)threadIdx.x + n * NT, row = i / Tile::CH, ch = i - row * Tile::CH;
-      r[n] = uint4{0, 0, 0, 0};
-      if (i < TOTAL && ch * A::EPC < a.dh) {
-        int qi, hg;
-        ca_row(a, t0 + row < last ? t0 + row : last, qi, hg);
-        r[n] = *reinterpret_cast<const uint4*>(base + (qi * sl + hg * sh + ch * A::EPC) * ESZ);
-      }
+      int qi, hg;
+      ca_row(a, t0 + row(n) < last ? t0 + row(n) : last, qi, hg);
+      if (in(n)) r[n] = *reinterpret_cast<const uint4*>(base + (qi * sl + hg * sh) * ESZ + col(n, a.dh));
     }
   }
-  __device__ __forceinline__ void write(char* t, uint64_t live, bool full) const {
+  __device__ __forceinline__ void write(char* t, uint64_t live, bool full, int dh) const {
+    if (full && dh == DH) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int i = (int)threadIdx.x + n * NT, row = i / Tile::CH, ch = i - row * Tile::CH;
-      if (i < TOTAL)
-        *reinterpret_cast<uint4*>(t + Tile::off(row, ch)) = full || (live >> row & 1) ? r[n] : uint4{0, 0, 0, 0};
+      for (int n = 0; n < N; ++n)
+        if (in(n)) *reinterpret_cast<uint4*>(t + Tile::off(row(n), chunk(n))) = r[n];
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (in(n))
+          *reinterpret_cast<uint4*>(t + Tile::off(row(n), chunk(n))) =
+              chunk(n) * A::EPC < dh && (live >> row(n) & 1) ? r[n] : uint4{0, 0, 0, 0};
     }
   }
 };
@@ -76,8 +79,8 @@ template <int DT, int DH> __device__ __forceinline__ void ca_row_frags(const cha
 //
 // NW waves of 16 QT rows each over tiles of KR keys in LDS (two buffers, one barrier per tile), with the running
 // maximum and sum of the softmax per row.  Statistics and accumulators are float32; the weights are rounded to the
-// operand type for the second product (relative 2^-9 for bf16, 2^-12 for fp16; the matrix unit has no wider operand at
-// this rate), their sum is not.
+// operand type for the second product (half a step, 2^-8 of the value for bf16 and 2^-11 for fp16; the matrix unit has no
+// wider operand at this rate), their sum is not: the log-sum that the backward reads is the float32 one.
 template <int DT, int DH, int NW, int QT, int KR>
 __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
   using A = CaT<DT>;
@@ -115,7 +118,7 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
   }
 
   caf4 o[QT][ND];
-  float m[QT], l[QT];
+  float m[QT], l[QT];           // l: the running sum over this lane's keys
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     m[t] = -INFINITY;
@@ -133,8 +136,8 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
     sv.load(vp, a.vsl, k0, k1 - 1, a.dh);
     flag = ca_flag<KR>(pad, k0, k1);
     live = ca_live<KR>(k0, k1, flag);
-    sk.write(lds, live, live == CA_FULL<KR>);
-    sv.write(lds + TB, live, live == CA_FULL<KR>);
+    sk.write(lds, live, live == CA_FULL<KR>, a.dh);
+    sv.write(lds + TB, live, live == CA_FULL<KR>, a.dh);
     if (nt > 1) {
       sk.load(kp, a.ksl, k0 + KR, k1 - 1, a.dh);
       sv.load(vp, a.vsl, k0 + KR, k1 - 1, a.dh);
@@ -149,8 +152,8 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
     if (i + 1 < nt) {
       char* nk = lds + ((i + 1) & 1) * 2 * TB;
       live = ca_live<KR>(k0 + (i + 1) * KR, k1, flag);
-      sk.write(nk, live, live == CA_FULL<KR>);
-      sv.write(nk + TB, live, live == CA_FULL<KR>);
+      sk.write(nk, live, live == CA_FULL<KR>, a.dh);
+      sv.write(nk + TB, live, live == CA_FULL<KR>, a.dh);
       if (i + 2 < nt) {
         const int t0 = k0 + (i + 2) * KR;
         sk.load(kp, a.ksl, t0, k1 - 1, a.dh);
@@ -190,38 +193,41 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
 #pragma unroll
       for (int k = 0; k < KT; ++k)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][k][r]);
-      mx = rows4_max(mx);
+        for (int r = 0; r < 4; r += 2) mx = ca_max3(mx, s[t][k][r], s[t][k][r + 1]);
+      mx = ca_rows4_max(mx);
       const float base = mx == -INFINITY ? 0.f : mx * a.scale_log2;
       alpha[t] = fast_exp2(m[t] * a.scale_log2 - base);      // 0 for the first live tile (m = -inf)
-      grew |= mx > m[t];
+      grew |= !(mx == m[t]);
       m[t] = mx;
-      float sum = 0.f;
 #pragma unroll
       for (int k = 0; k < KT; ++k)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[t][k][r] = fast_exp2(s[t][k][r] * a.scale_log2 - base);
-          sum += s[t][k][r];
-        }
-      l[t] = l[t] * alpha[t] + sum;
+        for (int r = 0; r < 4; ++r) s[t][k][r] = fast_exp2(s[t][k][r] * a.scale_log2 - base);
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[r] += s[t][k][r];
+      l[t] = l[t] * alpha[t] + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
 #pragma unroll
       for (int u = 0; u < KT / NPT; ++u) p[t][u] = ca_pack<DT>(&s[t][u * NPT]);
     }
     if (__any(grew)) {
 #pragma unroll
-      for (int t = 0; t < QT; ++t)
+      for (int t = 0; t < QT; ++t) {
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[t][d] *= alpha[t];
+      }
     }
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+    for (int u = 0; u < KT / NPT; ++u) {
 #pragma unroll
-      for (int u = 0; u < KT / NPT; ++u) {
+      for (int d = 0; d < ND; ++d) {
         const Frag f = Tile::frag_t(tv, 16 * NPT * u, d, li, g);
 #pragma unroll
         for (int t = 0; t < QT; ++t) o[t][d] = A::mma(f, p[t][u], o[t][d]);
       }
+    }
   }
 
   // rows without a live key have l = 0: zeros, and a log-sum of -inf
@@ -281,7 +287,8 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
   const uint8_t* pad = a.pad ? a.pad + w.b * a.psb : nullptr;
 
   Frag q[QT][NC], go[QT][NC];
-  float lse2[QT], delta[QT];
+  float lse2[QT];
+  caf4 ndelta[QT];      // -delta of the lane's row: the accumulator that dP starts from
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int r = row0 + 16 * t + li;
@@ -303,8 +310,9 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
       q[t][c] = ca_frag<DT>(fq[c]);
       go[t][c] = ca_frag<DT>(fg[c]);
     }
-    delta[t] = rows4_sum(dsum);
-    if (in && g == 0 && w.split == 0) a.delta[stat] = delta[t];
+    dsum = rows4_sum(dsum);
+    ndelta[t] = caf4{-dsum, -dsum, -dsum, -dsum};
+    if (in && g == 0 && w.split == 0) a.delta[stat] = dsum;
   }
 
   caf4 dq[QT][ND];
@@ -322,8 +330,8 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
     sv.load(vp, a.vsl, k0, k1 - 1, a.dh);
     flag = ca_flag<KR>(pad, k0, k1);
     live = ca_live<KR>(k0, k1, flag);
-    sk.write(lds, live, live == CA_FULL<KR>);
-    sv.write(lds + TB, live, live == CA_FULL<KR>);
+    sk.write(lds, live, live == CA_FULL<KR>, a.dh);
+    sv.write(lds + TB, live, live == CA_FULL<KR>, a.dh);
     if (nt > 1) {
       sk.load(kp, a.ksl, k0 + KR, k1 - 1, a.dh);
       sv.load(vp, a.vsl, k0 + KR, k1 - 1, a.dh);
@@ -338,8 +346,8 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
     if (i + 1 < nt) {
       char* nk = lds + ((i + 1) & 1) * 2 * TB;
       live = ca_live<KR>(k0 + (i + 1) * KR, k1, flag);
-      sk.write(nk, live, live == CA_FULL<KR>);
-      sv.write(nk + TB, live, live == CA_FULL<KR>);
+      sk.write(nk, live, live == CA_FULL<KR>, a.dh);
+      sv.write(nk + TB, live, live == CA_FULL<KR>, a.dh);
       if (i + 2 < nt) {
         const int t0 = k0 + (i + 2) * KR;
         sk.load(kp, a.ksl, t0, k1 - 1, a.dh);
@@ -353,7 +361,10 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
 #pragma unroll
       for (int k = 0; k < NPT; ++k) {
 #pragma unroll
-        for (int t = 0; t < QT; ++t) s[t][k] = dp[t][k] = caf4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < QT; ++t) {
+          s[t][k] = caf4{0.f, 0.f, 0.f, 0.f};
+          dp[t][k] = ndelta[t];
+        }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const Frag fk = Tile::frag(tk, 16 * (u * NPT + k), c, li, g);
@@ -370,11 +381,12 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
       for (int t = 0; t < QT; ++t) {
 #pragma unroll
         for (int k = 0; k < NPT; ++k) {
-          const uint32_t bits = (uint32_t)(now >> (16 * (u * NPT + k) + 4 * g));
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float p = fast_exp2(s[t][k][r] * a.scale_log2 - lse2[t]);
-            dp[t][k][r] = bits >> r & 1 ? p * (dp[t][k][r] - delta[t]) : 0.f;
+          for (int r = 0; r < 4; ++r) dp[t][k][r] *= fast_exp2(s[t][k][r] * a.scale_log2 - lse2[t]);
+          if (now != CA_FULL<KR>) {
+            const uint32_t bits = (uint32_t)(now >> (16 * (u * NPT + k) + 4 * g));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) dp[t][k][r] = bits >> r & 1 ? dp[t][k][r] : 0.f;
           }
         }
         ds[t] = ca_pack<DT>(dp[t]);
@@ -449,6 +461,10 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) { fk[t][c] = ca_frag<DT>(f0[c]); fv[t][c] = ca_frag<DT>(f1[c]); }
   }
+  bool all_live = true;
+#pragma unroll
+  for (int t = 0; t < KT; ++t) all_live = all_live && live[t];
+  const bool dead = __any(!all_live);
   caf4 dk[KT][ND], dv[KT][ND];
 #pragma unroll
   for (int t = 0; t < KT; ++t)
@@ -469,15 +485,15 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
       const int64_t i = stat0 + (int64_t)hg * a.Lq + qi;
       const float ls = a.lse[i];
       if (ls != -INFINITY) st_lse = ls * HCLSM_LOG2E;
-      st_delta = a.delta[i];
+      st_delta = -a.delta[i];
     }
   };
   auto write = [&](int t0, char* buf) {
     const int n = r1 - t0;
     const bool full = n >= RR;
     const uint64_t mask = full ? ~0ull : (1ull << n) - 1;
-    sq.write(buf, mask, full);
-    sg.write(buf + TB, mask, full);
+    sq.write(buf, mask, full, a.dh);
+    sg.write(buf + TB, mask, full, a.dh);
     if ((int)threadIdx.x < RR) {
       reinterpret_cast<float*>(buf + 2 * TB)[threadIdx.x] = st_lse;
       reinterpret_cast<float*>(buf + 2 * TB)[RR + threadIdx.x] = st_delta;
@@ -503,7 +519,10 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
 #pragma unroll
       for (int k = 0; k < NPT; ++k) {
 #pragma unroll
-        for (int t = 0; t < KT; ++t) s[t][k] = dp[t][k] = caf4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < KT; ++t) {
+          s[t][k] = caf4{0.f, 0.f, 0.f, 0.f};
+          dp[t][k] = *reinterpret_cast<const caf4*>(stat + RR + 16 * (u * NPT + k) + 4 * g);      // -delta
+        }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const Frag fq = Tile::frag(tq, 16 * (u * NPT + k), c, li, g);
@@ -519,15 +538,17 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
 #pragma unroll
       for (int k = 0; k < NPT; ++k) {
         const caf4 ls = *reinterpret_cast<const caf4*>(stat + 16 * (u * NPT + k) + 4 * g);
-        const caf4 de = *reinterpret_cast<const caf4*>(stat + RR + 16 * (u * NPT + k) + 4 * g);
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+        for (int t = 0; t < KT; ++t) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float e = fast_exp2(s[t][k][r] * a.scale_log2 - ls[r]);
-            s[t][k][r] = live[t] ? e : 0.f;
-            dp[t][k][r] = s[t][k][r] * (dp[t][k][r] - de[r]);
+          for (int r = 0; r < 4; ++r) s[t][k][r] = fast_exp2(s[t][k][r] * a.scale_log2 - ls[r]);
+          if (dead) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[t][k][r] = live[t] ? s[t][k][r] : 0.f;
           }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) dp[t][k][r] *= s[t][k][r];
+        }
       }
 #pragma unroll
       for (int t = 0; t < KT; ++t) { p[t] = ca_pack<DT>(s[t]); ds[t] = ca_pack<DT>(dp[t]); }
@@ -599,11 +620,29 @@ int ca_launch(K kernel, CaArgs& a, int64_t batch, int64_t rows, int per_wg, int 
   return 0;
 }
 
-template <int DT, int DH> int ca_forward_dh(CaArgs& a, int64_t batch, void*, int64_t, hipStream_t st) {
+template <int DT, int DH> int ca_forward_dh(CaArgs& a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st) {
   using S = CaShape<DT, DH>;
-  static std::atomic<int> cache[HCLSM_MAX_DEVICES];
-  a.nsplit = 1;
-  return ca_launch(ca_fwd_kernel<DT, DH, 4, S::T, S::TR>, a, batch, (int64_t)a.Lq * a.G, 64 * S::T, 256, S::LDS, cache, st);
+  static std::atomic<int> cw[HCLSM_MAX_DEVICES], c1[HCLSM_MAX_DEVICES], c2[HCLSM_MAX_DEVICES];
+  const CaPlan p = ca_forward_plan(batch, a.Lq, a.Lk, a.Hk, a.G, a.dh, DT);
+  const int64_t rows = (int64_t)a.Lq * a.G;
+  a.nsplit = p.nsplit;
+  if (p.nsplit > 1) {
+    const int64_t n = (int64_t)p.nsplit * batch * a.Hk * rows;
+    if (ws == nullptr) return HCLSM_ERR_NULL;
+    if (ws_bytes < n * (a.dh + 1) * 4) return HCLSM_ERR_SHAPE;
+    a.part = (float*)ws;
+    a.part_lse = a.part + n * a.dh;
+  }
+  int rc = HCLSM_ERR_UNSUPPORTED;
+  if (p.few == 1) {
+    if constexpr (S::RB <= CA_FEW1_BYTES) rc = ca_launch(ca_few_kernel<DT, DH, 4, 1>, a, batch, rows, 16, 256, 0, c1, st);
+  } else if (p.few == 2) {
+    if constexpr (S::RB <= CA_FEW2_BYTES) rc = ca_launch(ca_few_kernel<DT, DH, 4, 2>, a, batch, rows, 32, 256, 0, c2, st);
+  } else {
+    rc = ca_launch(ca_fwd_kernel<DT, DH, 4, S::T, S::TR>, a, batch, rows, 64 * S::T, 256, S::LDS, cw, st);
+  }
+  if (rc || p.nsplit == 1) return rc;
+  return ca_join(a, DT, st);
 }
 
 template <int DT, int DH> int ca_backward_dh(CaArgs& a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st) {
