@@ -101,6 +101,10 @@ template <int DT> __device__ __forceinline__ typename CaT<DT>::Frag ca_pack(cons
   }
 }
 
+// A row's exponentials are taken against a reference (log2): lowest value, which no score reaches from below, and how far
+// the row's maximum may pass it before it moves.
+constexpr float CA_LOW = -3.0e38f, CA_SLACK = 8.f;
+
 // Maxima that pass a NaN on (v_maximum3_f32: one instruction for two values, and no step to quiet its operands first).
 __device__ __forceinline__ float ca_max3(float a, float b, float c) {
   return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
@@ -219,6 +223,9 @@ __device__ __forceinline__ void ca_row(const CaArgs& a, int row, int& qi, int& h
     hg = row - qi * a.G;
   }
 }
+
+// Rows of a tile of RR: whole queries where a query has no more heads than that.
+__device__ __forceinline__ int ca_row_step(int G, int RR) { return G <= RR ? RR - RR % G : RR; }
 
 // [begin, end) of a split's share of n, in whole multiples of `step` but for the end.
 __device__ __forceinline__ void ca_range(int n, int nsplit, int split, int step, int& begin, int& end) {

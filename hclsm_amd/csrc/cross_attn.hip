@@ -81,6 +81,11 @@ bool ca_aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int esz) {
   return (uintptr_t)p % 16 == 0 && s0 % n == 0 && s1 % n == 0 && s2 % n == 0;
 }
 
+// Offsets inside a tile (at most 64 rows, of a unit or of the keys) have to fit 31 bits.
+bool ca_near(int64_t sl, int64_t sh, int64_t G, int esz) {
+  return sl >= 0 && sh >= 0 && sl < (1 << 24) && sh < ((int64_t)1 << 31) && (64 / G + 2) * sl * esz + G * sh * esz < 0x7fff0000;
+}
+
 int ca_sizes(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t dh, int dtype) {
   if (B < 0 || Lq < 0 || Lk < 0 || H < 0 || Hk < 0 || dh < 1) return HCLSM_ERR_SHAPE;
   if (dtype < HCLSM_F32 || dtype > HCLSM_F16) return HCLSM_ERR_DTYPE;
@@ -100,13 +105,16 @@ int ca_args(const HclsmCrossAttention* x, int bwd, CaArgs& a) {
   if (!(x->scale > 0.f) || !(x->scale < 3.0e38f)) return HCLSM_ERR_SHAPE;
   const bool rows = x->B && x->Lq && x->H, keys = x->B && x->Lk && x->Hk;
   const int esz = x->dtype == HCLSM_F32 ? 4 : 2;
+  const int64_t G = x->Hk ? x->H / x->Hk : 1;
   if (rows) {
+    if (!ca_near(x->q_sl, x->q_sh, G, esz) || (bwd && !ca_near(x->g_sl, x->g_sh, G, esz))) return HCLSM_ERR_UNSUPPORTED;
     if (!x->q || !x->out || (bwd && (!x->g || !x->dq || !x->lse))) return HCLSM_ERR_NULL;
     if (!ca_aligned(x->q, x->q_sb, x->q_sl, x->q_sh, esz) || !ca_aligned(x->out, 0, 0, 0, esz)) return HCLSM_ERR_UNSUPPORTED;
     if (bwd && (!ca_aligned(x->g, x->g_sb, x->g_sl, x->g_sh, esz) || !ca_aligned(x->dq, 0, 0, 0, esz)))
       return HCLSM_ERR_UNSUPPORTED;
   }
   if (keys) {
+    if (!ca_near(x->k_sl, 0, 1, esz) || !ca_near(x->v_sl, 0, 1, esz)) return HCLSM_ERR_UNSUPPORTED;
     if (!x->k || !x->v || (bwd && (!x->dk || !x->dv))) return HCLSM_ERR_NULL;
     if (!ca_aligned(x->k, x->k_sb, x->k_sl, x->k_sh, esz) || !ca_aligned(x->v, x->v_sb, x->v_sl, x->v_sh, esz))
       return HCLSM_ERR_UNSUPPORTED;

@@ -27,19 +27,6 @@ template <int DT, int DH> struct CaGroups {
   static constexpr int N = count();
 };
 
-// W elements of 2 or 4 bytes as 32-bit words, in one access
-template <int WORDS> __device__ __forceinline__ void ca_load_words(const char* p, uint32_t* w) {
-  if constexpr (WORDS == 4) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else if constexpr (WORDS == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x; w[1] = v.y;
-  } else {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  }
-}
-
 // One step's operands of a wave: SK = 16 NPT keys.
 template <int DT, int DH> struct CaStep {
   using A = CaT<DT>;
@@ -48,36 +35,50 @@ template <int DT, int DH> struct CaStep {
   uint4 k[NPT][NC];
   uint32_t v[NPT * 4][VW];
 
-  // t0 .. t0 + SK - 1 of the keys; rows past the last one are read at its address
-  __device__ __forceinline__ void load(const CaArgs& a, const char* kp, const char* vp, int t0, int last, int li, int g) {
+  static constexpr uint32_t NONE = 0xffffffffu;
+  uint32_t koff, voff;       // bytes from a step's first key: row li at operand g; row 4g at this lane's columns
+
+  __device__ __forceinline__ void init(const CaArgs& a, int li, int g) {
+    koff = (uint32_t)li * (uint32_t)(a.ksl * ESZ) + 16 * g;
+    voff = (uint32_t)(4 * g) * (uint32_t)(a.vsl * ESZ);
+  }
+  // keys kp / vp point at, n of them (past them, and past dh, loads are out of the buffer's range and give zeros)
+  __device__ __forceinline__ void load(const CaArgs& a, const char* kp, const char* vp, int n, int li, int g) {
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)kp, 0, 0x7fffffff, kRawBufferWord3);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)vp, 0, 0x7fffffff, kRawBufferWord3);
 #pragma unroll
     for (int t = 0; t < NPT; ++t) {
-      const int row = t0 + 16 * t + li;
-      const char* p = kp + (row < last ? row : last) * a.ksl * ESZ;
+      const uint32_t row = 16 * t + li < n ? koff : NONE;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const int e = (4 * c + g) * A::EPC;
-        k[t][c] = uint4{0, 0, 0, 0};
-        if (e < a.dh) k[t][c] = *reinterpret_cast<const uint4*>(p + e * ESZ);
+        const uint32_t o = (4 * c + g) * A::EPC < a.dh ? row : NONE;
+        k[t][c] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+            rk, (int)(o == NONE ? o : o + 64 * c), t * 16 * (int)(a.ksl * ESZ), 0));
       }
     }
 #pragma unroll
     for (int t = 0; t < NPT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = t0 + 16 * t + 4 * g + r;
-        const char* p = vp + (row < last ? row : last) * a.vsl * ESZ;
-        load_v<0>(a, p, li, v[4 * t + r]);
-      }
+      for (int r = 0; r < 4; ++r)
+        load_v<0>(a, rv, 16 * t + 4 * g + r < n ? voff : NONE, (16 * t + r) * (int)(a.vsl * ESZ), li, v[4 * t + r]);
   }
-  template <int K> __device__ __forceinline__ void load_v(const CaArgs& a, const char* p, int li, uint32_t* w) {
+  template <int K>
+  __device__ __forceinline__ void load_v(const CaArgs& a, __amdgpu_buffer_rsrc_t rv, uint32_t off, int so, int li, uint32_t* w) {
     if constexpr (K < CaGroups<DT, DH>::N) {
       constexpr int F = CaGroups<DT, DH>::first(K), W = CaGroups<DT, DH>::width(K), WORDS = W * ESZ / 4;
       const int col = 16 * F + W * li;
-#pragma unroll
-      for (int i = 0; i < WORDS; ++i) w[F * ESZ / 4 + i] = 0;
-      if (col < a.dh) ca_load_words<WORDS>(p + col * ESZ, w + F * ESZ / 4);
-      load_v<K + 1>(a, p, li, w);
+      const int o = (int)(off != NONE && col < a.dh ? off + col * ESZ : NONE);
+      uint32_t* d = w + F * ESZ / 4;
+      if constexpr (WORDS == 4) {
+        const uint4 x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, o, so, 0));
+        d[0] = x.x; d[1] = x.y; d[2] = x.z; d[3] = x.w;
+      } else if constexpr (WORDS == 2) {
+        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rv, o, so, 0));
+        d[0] = x.x; d[1] = x.y;
+      } else {
+        d[0] = __builtin_amdgcn_raw_buffer_load_b32(rv, o, so, 0);
+      }
+      load_v<K + 1>(a, rv, off, so, li, w);
     }
   }
   // second operand of tile nt: its column of each of the lane's keys
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
 
   CaWork w;
   if (!ca_work(a, w)) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
   const int row0 = w.tile * 16 * QT;
   int k0, k1;
   ca_range(w.keys, a.nsplit, w.split, SK * NW, k0, k1);
@@ -143,9 +144,10 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
 
   const int t0 = k0 + wave * SK;
   Step st;
+  st.init(a, li, g);
   uint8_t flag = 0;
   auto get = [&](int t, Step& d) {
-    d.load(a, kp, vp, t, k1 - 1, li, g);
+    d.load(a, kp + t * a.ksl * ESZ, vp + t * a.vsl * ESZ, k1 - t, li, g);
     flag = pad != nullptr && lane < SK && t + lane < k1 ? pad[t + lane] : (uint8_t)0;
   };
   if (t0 < k1) get(t0, st);
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
   float m[QT], l[QT];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    m[t] = -INFINITY;
+    m[t] = CA_LOW;
     l[t] = 0.f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
@@ -182,7 +184,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
     const bool full = live == (SK == 32 ? 0xffffffffu : 0xffffu);
     Step cur = st;
     if (t + SK * NW < k1) get(t + SK * NW, st);
-    if (!full) {          // values of dead keys are zeros, whatever they held
+    if (pad != nullptr && !full) {          // values of masked keys are zeros, whatever they held
 #pragma unroll
       for (int p = 0; p < NPT; ++p)
 #pragma unroll
@@ -202,36 +204,46 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
 #pragma unroll
         for (int u = 0; u < QT; ++u) s[u][p] = A::mma(ca_frag<DT>(cur.k[p][c]), q[u][c], s[u][p]);
     }
-    Frag pf[QT];
+    float top[QT];
+    bool grew = false;
 #pragma unroll
     for (int u = 0; u < QT; ++u) {
-      float mx = m[u];
+      if (!full) {
+#pragma unroll
+        for (int p = 0; p < NPT; ++p)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[u][p][r] = live >> (16 * p + 4 * g + r) & 1 ? s[u][p][r] : -INFINITY;
+      }
+      float mx = s[u][0][0];
 #pragma unroll
       for (int p = 0; p < NPT; ++p)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (!full) s[u][p][r] = live >> (16 * p + 4 * g + r) & 1 ? s[u][p][r] : -INFINITY;
-          mx = fmaxf(mx, s[u][p][r]);
-        }
-      mx = rows4_max(mx);
-      const float base = mx == -INFINITY ? 0.f : mx * a.scale_log2;
-      const float alpha = fast_exp2(m[u] * a.scale_log2 - base);
-      const bool grew = mx > m[u];
-      m[u] = mx;
-      float sum = 0.f;
+        for (int r = 0; r < 4; r += 2) mx = ca_max3(mx, s[u][p][r], s[u][p][r + 1]);
+      top[u] = ca_rows4_max(mx) * a.scale_log2;
+      grew |= !(top[u] <= m[u] + CA_SLACK);
+    }
+    if (__any(grew)) {         // as in ca_fwd_kernel
 #pragma unroll
-      for (int p = 0; p < NPT; ++p)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[u][p][r] = fast_exp2(s[u][p][r] * a.scale_log2 - base);
-          sum += s[u][p][r];
-        }
-      l[u] = l[u] * alpha + sum;
-      pf[u] = ca_pack<DT>(s[u]);
-      if (__any(grew)) {
+      for (int u = 0; u < QT; ++u) {
+        const float to = top[u] <= m[u] + CA_SLACK ? m[u] : top[u];
+        const float alpha = fast_exp2(m[u] - to);
+        m[u] = to;
+        l[u] *= alpha;
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[u][d] *= alpha;
       }
+    }
+    Frag pf[QT];
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+#pragma unroll
+      for (int p = 0; p < NPT; ++p)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[u][p][r] = fast_exp2(s[u][p][r] * a.scale_log2 - m[u]);
+          l[u] += s[u][p][r];
+        }
+      pf[u] = ca_pack<DT>(s[u]);
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
@@ -255,12 +267,11 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
     for (int u = 0; u < QT; ++u) {
       top[u] = s_m[0][u][li];
 #pragma unroll
-      for (int i = 1; i < NW; ++i) top[u] = fmaxf(top[u], s_m[i][u][li]);
-      const float base = top[u] == -INFINITY ? 0.f : top[u] * a.scale_log2;
+      for (int i = 1; i < NW; ++i) top[u] = __builtin_elementwise_maximum(top[u], s_m[i][u][li]);
       sum[u] = 0.f;
 #pragma unroll
-      for (int i = 0; i < NW; ++i) sum[u] += s_l[i][u][li] * fast_exp2(s_m[i][u][li] * a.scale_log2 - base);
-      const float f = fast_exp2(m[u] * a.scale_log2 - base);
+      for (int i = 0; i < NW; ++i) sum[u] += s_l[i][u][li] * fast_exp2(s_m[i][u][li] - top[u]);
+      const float f = fast_exp2(m[u] - top[u]);
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[u][d] *= f;
     }
@@ -297,7 +308,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
     int qi, hg;
     ca_row(a, r, qi, hg);
     const int h = w.hk * a.G + hg;
-    const float ls2 = in && sum[u] > 0.f ? top[u] * a.scale_log2 + __log2f(sum[u]) : in && sum[u] != sum[u] ? sum[u] : -INFINITY;
+    const float ls2 = in && sum[u] > 0.f ? top[u] + __log2f(sum[u]) : in && sum[u] != sum[u] ? sum[u] : -INFINITY;
     const int64_t pr = ((int64_t)w.split * a.units + w.unit) * all + r;
     const int64_t ob = a.nsplit > 1 ? pr * a.dh : ((w.b * a.Lq + qi) * a.Hk * a.G + h) * (int64_t)a.dh;
     if (g == 0) {

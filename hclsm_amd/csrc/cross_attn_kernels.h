@@ -6,50 +6,58 @@
 namespace hclsm {
 
 // A tile of ROWS rows on its way from global memory to LDS: loaded into registers while the tile before it is being
-// worked on, then written.  Rows past the last one are read at the last row's address and written as zeros, as
-// are rows whose bit of `live` is clear: what a masked row holds (NaN included) never reaches a product.
+// worked on, then written.  A chunk's offset from the tile's first row does not change from tile to tile, so a load is one
+// comparison and one select: rows past the end, and chunks past dh, get an offset past the buffer resource's end, where
+// loads return zeros.  Rows whose bit of `live` is clear are written as zeros: what a masked row holds (NaN included) never
+// reaches a product.
 template <int DT, int DH, int NT, int ROWS> struct CaStage {
   using A = CaT<DT>;
   using Tile = CaTile<DT, DH>;
   static constexpr int TOTAL = ROWS * Tile::CH, N = (TOTAL + NT - 1) / NT;
   static constexpr int ESZ = (int)sizeof(typename A::T);
+  static constexpr uint32_t NONE = 0xffffffffu;
+  uint32_t off[N];
   uint4 r[N];
 
   static __device__ __forceinline__ int row(int n) { return ((int)threadIdx.x + n * NT) / Tile::CH; }
   static __device__ __forceinline__ int chunk(int n) { return ((int)threadIdx.x + n * NT) % Tile::CH; }
   static __device__ __forceinline__ bool in(int n) { return TOTAL % NT == 0 || (int)threadIdx.x + n * NT < TOTAL; }
-  // byte offset of the chunk in its row; chunks past dh are read at the row's start and written as zeros
-  static __device__ __forceinline__ int col(int n, int dh) { return chunk(n) * A::EPC < dh ? chunk(n) * 16 : 0; }
 
-  // rows t0 .. of a tensor with one address per row
-  __device__ __forceinline__ void load(const char* base, int64_t stride, int t0, int last, int dh) {
+  // rows one stride apart
+  __device__ __forceinline__ void init(int64_t stride, int dh) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int rr = t0 + row(n) < last ? t0 + row(n) : last;
-      if (in(n)) r[n] = *reinterpret_cast<const uint4*>(base + (int64_t)rr * stride * ESZ + col(n, dh));
-    }
+    for (int n = 0; n < N; ++n)
+      off[n] = in(n) && chunk(n) * A::EPC < dh ? (uint32_t)row(n) * (uint32_t)(stride * ESZ) + chunk(n) * 16 : NONE;
   }
-  // rows t0 .. of a unit (query and head of the group)
-  __device__ __forceinline__ void load_rows(const CaArgs& a, const char* base, int64_t sl, int64_t sh, int t0, int last) {
+  // rows of a unit, the first one being head `phase` of its query: `used` rows of a tile
+  __device__ __forceinline__ void init_rows(const CaArgs& a, int64_t sl, int64_t sh, int phase, int used) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       int qi, hg;
-      ca_row(a, t0 + row(n) < last ? t0 + row(n) : last, qi, hg);
-      if (in(n)) r[n] = *reinterpret_cast<const uint4*>(base + (qi * sl + hg * sh) * ESZ + col(n, a.dh));
+      ca_row(a, phase + row(n), qi, hg);
+      off[n] = in(n) && row(n) < used && chunk(n) * A::EPC < a.dh
+                   ? (uint32_t)qi * (uint32_t)(sl * ESZ) + (uint32_t)hg * (uint32_t)(sh * ESZ) + chunk(n) * 16 : NONE;
     }
   }
-  __device__ __forceinline__ void write(char* t, uint64_t live, bool full, int dh) const {
-    if (full && dh == DH) {
+  // base: first row of the tile; n_rows: rows there are from it on
+  __device__ __forceinline__ void load(const char* base, int n_rows) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, kRawBufferWord3);
 #pragma unroll
-      for (int n = 0; n < N; ++n)
-        if (in(n)) *reinterpret_cast<uint4*>(t + Tile::off(row(n), chunk(n))) = r[n];
-    } else {
-#pragma unroll
-      for (int n = 0; n < N; ++n)
-        if (in(n))
-          *reinterpret_cast<uint4*>(t + Tile::off(row(n), chunk(n))) =
-              chunk(n) * A::EPC < dh && (live >> row(n) & 1) ? r[n] : uint4{0, 0, 0, 0};
+    for (int n = 0; n < N; ++n) {
+      const uint32_t o = row(n) < n_rows ? off[n] : NONE;
+      r[n] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)o, 0, 0));
     }
+  }
+  __device__ __forceinline__ void write(char* t) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (in(n)) *reinterpret_cast<uint4*>(t + Tile::off(row(n), chunk(n))) = r[n];
+  }
+  __device__ __forceinline__ void drop(uint64_t live) {
+    asm volatile("");      // keeps the branch around this: the selects would otherwise be made for every tile
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (!(live >> (row(n) & 63) & 1)) r[n] = uint4{0, 0, 0, 0};
   }
 };
 
@@ -118,10 +126,10 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
   }
 
   caf4 o[QT][ND];
-  float m[QT], l[QT];           // l: the running sum over this lane's keys
+  float m[QT], l[QT];           // reference of the exponentials (log2); sum over this lane's keys
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    m[t] = -INFINITY;
+    m[t] = CA_LOW;
     l[t] = 0.f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
@@ -129,20 +137,28 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
 
   const int nt = (k1 - k0 + KR - 1) / KR;
   CaStage<DT, DH, NT, KR> sk, sv;
+  sk.init(a.ksl, a.dh);
+  sv.init(a.vsl, a.dh);
   uint8_t flag = 0;
   uint64_t live = 0;
-  if (nt > 0) {
-    sk.load(kp, a.ksl, k0, k1 - 1, a.dh);
-    sv.load(vp, a.vsl, k0, k1 - 1, a.dh);
-    flag = ca_flag<KR>(pad, k0, k1);
-    live = ca_live<KR>(k0, k1, flag);
-    sk.write(lds, live, live == CA_FULL<KR>, a.dh);
-    sv.write(lds + TB, live, live == CA_FULL<KR>, a.dh);
-    if (nt > 1) {
-      sk.load(kp, a.ksl, k0 + KR, k1 - 1, a.dh);
-      sv.load(vp, a.vsl, k0 + KR, k1 - 1, a.dh);
-      flag = ca_flag<KR>(pad, k0 + KR, k1);
+  auto load = [&](int t0) {
+    sk.load(kp + t0 * a.ksl * ESZ, k1 - t0);
+    sv.load(vp + t0 * a.vsl * ESZ, k1 - t0);
+    flag = ca_flag<KR>(pad, t0, k1);
+  };
+  auto write = [&](int t0, char* buf) {
+    live = ca_live<KR>(t0, k1, flag);
+    if (pad != nullptr && live != CA_FULL<KR>) {
+      sk.drop(live);
+      sv.drop(live);
     }
+    sk.write(buf);
+    sv.write(buf + TB);
+  };
+  if (nt > 0) {
+    load(k0);
+    write(k0, lds);
+    if (nt > 1) load(k0 + KR);
   }
   for (int i = 0; i < nt; ++i) {
     char* tk = lds + (i & 1) * 2 * TB;
@@ -150,16 +166,8 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
     const uint64_t now = live;
     __syncthreads();      // tile i is written, and every wave is done with the other buffer
     if (i + 1 < nt) {
-      char* nk = lds + ((i + 1) & 1) * 2 * TB;
-      live = ca_live<KR>(k0 + (i + 1) * KR, k1, flag);
-      sk.write(nk, live, live == CA_FULL<KR>, a.dh);
-      sv.write(nk + TB, live, live == CA_FULL<KR>, a.dh);
-      if (i + 2 < nt) {
-        const int t0 = k0 + (i + 2) * KR;
-        sk.load(kp, a.ksl, t0, k1 - 1, a.dh);
-        sv.load(vp, a.vsl, t0, k1 - 1, a.dh);
-        flag = ca_flag<KR>(pad, t0, k1);
-      }
+      write(k0 + (i + 1) * KR, lds + ((i + 1) & 1) * 2 * TB);
+      if (i + 2 < nt) load(k0 + (i + 2) * KR);
     }
 
     caf4 s[QT][KT];
@@ -184,40 +192,47 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
           for (int r = 0; r < 4; ++r) s[t][k][r] = bits >> r & 1 ? s[t][k][r] : -INFINITY;
       }
     }
-    Frag p[QT][KT / NPT];
+    // The reference of a row's exponentials follows its maximum only in steps of more than 2^CA_SLACK: weights then
+    // stay below 2^CA_SLACK, which float32 sums and either 16-bit type hold as exactly as weights below one, and the
+    // accumulators are hardly ever rescaled.
+    float top[QT];
     bool grew = false;
-    float alpha[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      float mx = m[t];
+      float mx = s[t][0][0];
 #pragma unroll
       for (int k = 0; k < KT; ++k)
 #pragma unroll
         for (int r = 0; r < 4; r += 2) mx = ca_max3(mx, s[t][k][r], s[t][k][r + 1]);
-      mx = ca_rows4_max(mx);
-      const float base = mx == -INFINITY ? 0.f : mx * a.scale_log2;
-      alpha[t] = fast_exp2(m[t] * a.scale_log2 - base);      // 0 for the first live tile (m = -inf)
-      grew |= !(mx == m[t]);
-      m[t] = mx;
-#pragma unroll
-      for (int k = 0; k < KT; ++k)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[t][k][r] = fast_exp2(s[t][k][r] * a.scale_log2 - base);
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < KT; ++k)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sum[r] += s[t][k][r];
-      l[t] = l[t] * alpha[t] + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-#pragma unroll
-      for (int u = 0; u < KT / NPT; ++u) p[t][u] = ca_pack<DT>(&s[t][u * NPT]);
+      top[t] = ca_rows4_max(mx) * a.scale_log2;
+      grew |= !(top[t] <= m[t] + CA_SLACK);
     }
     if (__any(grew)) {
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
+        const float to = top[t] <= m[t] + CA_SLACK ? m[t] : top[t];
+        const float alpha = fast_exp2(m[t] - to);
+        m[t] = to;
+        l[t] *= alpha;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) o[t][d] *= alpha[t];
+        for (int d = 0; d < ND; ++d) o[t][d] *= alpha;
       }
+    }
+    Frag p[QT][KT / NPT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[t][k][r] = fast_exp2(s[t][k][r] * a.scale_log2 - m[t]);
+      float sum[4] = {l[t], 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[r] += s[t][k][r];
+      l[t] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+      for (int u = 0; u < KT / NPT; ++u) p[t][u] = ca_pack<DT>(&s[t][u * NPT]);
     }
 #pragma unroll
     for (int u = 0; u < KT / NPT; ++u) {
@@ -242,7 +257,7 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
     int qi, hg;
     ca_row(a, r, qi, hg);
     const int h = w.hk * a.G + hg;
-    const float ls2 = in && sum > 0.f ? m[t] * a.scale_log2 + __log2f(sum) : in && sum != sum ? sum : -INFINITY;
+    const float ls2 = in && sum > 0.f ? m[t] + __log2f(sum) : in && sum != sum ? sum : -INFINITY;
     if (a.nsplit > 1) {
       const int64_t pr = ((int64_t)w.split * a.units + w.unit) * all + r;
       if (g == 0) a.part_lse[pr] = ls2;
@@ -323,20 +338,28 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
 
   const int nt = (k1 - k0 + KR - 1) / KR;
   CaStage<DT, DH, NT, KR> sk, sv;
+  sk.init(a.ksl, a.dh);
+  sv.init(a.vsl, a.dh);
   uint8_t flag = 0;
   uint64_t live = 0;
-  if (nt > 0) {
-    sk.load(kp, a.ksl, k0, k1 - 1, a.dh);
-    sv.load(vp, a.vsl, k0, k1 - 1, a.dh);
-    flag = ca_flag<KR>(pad, k0, k1);
-    live = ca_live<KR>(k0, k1, flag);
-    sk.write(lds, live, live == CA_FULL<KR>, a.dh);
-    sv.write(lds + TB, live, live == CA_FULL<KR>, a.dh);
-    if (nt > 1) {
-      sk.load(kp, a.ksl, k0 + KR, k1 - 1, a.dh);
-      sv.load(vp, a.vsl, k0 + KR, k1 - 1, a.dh);
-      flag = ca_flag<KR>(pad, k0 + KR, k1);
+  auto load = [&](int t0) {
+    sk.load(kp + t0 * a.ksl * ESZ, k1 - t0);
+    sv.load(vp + t0 * a.vsl * ESZ, k1 - t0);
+    flag = ca_flag<KR>(pad, t0, k1);
+  };
+  auto write = [&](int t0, char* buf) {
+    live = ca_live<KR>(t0, k1, flag);
+    if (pad != nullptr && live != CA_FULL<KR>) {
+      sk.drop(live);
+      sv.drop(live);
     }
+    sk.write(buf);
+    sv.write(buf + TB);
+  };
+  if (nt > 0) {
+    load(k0);
+    write(k0, lds);
+    if (nt > 1) load(k0 + KR);
   }
   for (int i = 0; i < nt; ++i) {
     char* tk = lds + (i & 1) * 2 * TB;
@@ -344,16 +367,8 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
     const uint64_t now = live;
     __syncthreads();
     if (i + 1 < nt) {
-      char* nk = lds + ((i + 1) & 1) * 2 * TB;
-      live = ca_live<KR>(k0 + (i + 1) * KR, k1, flag);
-      sk.write(nk, live, live == CA_FULL<KR>, a.dh);
-      sv.write(nk + TB, live, live == CA_FULL<KR>, a.dh);
-      if (i + 2 < nt) {
-        const int t0 = k0 + (i + 2) * KR;
-        sk.load(kp, a.ksl, t0, k1 - 1, a.dh);
-        sv.load(vp, a.vsl, t0, k1 - 1, a.dh);
-        flag = ca_flag<KR>(pad, t0, k1);
-      }
+      write(k0 + (i + 1) * KR, lds + ((i + 1) & 1) * 2 * TB);
+      if (i + 2 < nt) load(k0 + (i + 2) * KR);
     }
 #pragma unroll
     for (int u = 0; u < KT / NPT; ++u) {
@@ -438,8 +453,9 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
   if (!ca_work(a, w)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
   const int key0 = (w.tile * NW + wave) * 16 * KT;
+  const int step = ca_row_step(a.G, RR);      // rows of a tile: whole queries
   int r0, r1;
-  ca_range(w.rows, a.nsplit, w.split, RR, r0, r1);
+  ca_range(w.rows, a.nsplit, w.split, step, r0, r1);
   if (w.tile * NW * 16 * KT >= w.keys) r1 = r0;
 
   const char* kp = a.k + (w.b * a.ksb + w.hk * a.ksh) * ESZ;
@@ -471,29 +487,34 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[t][d] = dv[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
 
-  const int nt = (r1 - r0 + RR - 1) / RR;
+  const int nt = (r1 - r0 + step - 1) / step;
   CaStage<DT, DH, NT, RR> sq, sg;
   float st_lse = INFINITY, st_delta = 0.f;
+  int st_q = 0, st_h = 0;
+  auto init = [&](int phase) {
+    sq.init_rows(a, a.qsl, a.qsh, phase, step);
+    sg.init_rows(a, a.gsl, a.gsh, phase, step);
+    ca_row(a, phase + (int)threadIdx.x, st_q, st_h);
+  };
+  init(0);
   auto load = [&](int t0) {
-    sq.load_rows(a, qp, a.qsl, a.qsh, t0, r1 - 1);
-    sg.load_rows(a, gp, a.gsl, a.gsh, t0, r1 - 1);
+    int q0, phase;
+    ca_row(a, t0, q0, phase);
+    if (a.G > RR) init(phase);       // more heads to a query than rows to a tile: tiles begin inside a query
+    sq.load(qp + q0 * a.qsl * ESZ, r1 - t0);
+    sg.load(gp + q0 * a.gsl * ESZ, r1 - t0);
     st_lse = INFINITY;         // rows past the last one, and rows without keys: every weight is exp(-inf)
     st_delta = 0.f;
-    if ((int)threadIdx.x < RR && t0 + (int)threadIdx.x < r1) {
-      int qi, hg;
-      ca_row(a, t0 + (int)threadIdx.x, qi, hg);
-      const int64_t i = stat0 + (int64_t)hg * a.Lq + qi;
+    if ((int)threadIdx.x < step && t0 + (int)threadIdx.x < r1) {
+      const int64_t i = stat0 + (int64_t)st_h * a.Lq + q0 + st_q;
       const float ls = a.lse[i];
       if (ls != -INFINITY) st_lse = ls * HCLSM_LOG2E;
       st_delta = -a.delta[i];
     }
   };
-  auto write = [&](int t0, char* buf) {
-    const int n = r1 - t0;
-    const bool full = n >= RR;
-    const uint64_t mask = full ? ~0ull : (1ull << n) - 1;
-    sq.write(buf, mask, full, a.dh);
-    sg.write(buf + TB, mask, full, a.dh);
+  auto write = [&](char* buf) {
+    sq.write(buf);
+    sg.write(buf + TB);
     if ((int)threadIdx.x < RR) {
       reinterpret_cast<float*>(buf + 2 * TB)[threadIdx.x] = st_lse;
       reinterpret_cast<float*>(buf + 2 * TB)[RR + threadIdx.x] = st_delta;
@@ -501,8 +522,8 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
   };
   if (nt > 0) {
     load(r0);
-    write(r0, lds);
-    if (nt > 1) load(r0 + RR);
+    write(lds);
+    if (nt > 1) load(r0 + step);
   }
   for (int i = 0; i < nt; ++i) {
     char* tq = lds + (i & 1) * BUF;
@@ -510,8 +531,8 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
     const float* stat = reinterpret_cast<const float*>(tq + 2 * TB);
     __syncthreads();
     if (i + 1 < nt) {
-      write(r0 + (i + 1) * RR, lds + ((i + 1) & 1) * BUF);
-      if (i + 2 < nt) load(r0 + (i + 2) * RR);
+      write(lds + ((i + 1) & 1) * BUF);
+      if (i + 2 < nt) load(r0 + (i + 2) * step);
     }
 #pragma unroll
     for (int u = 0; u < RT / NPT; ++u) {

@@ -52,12 +52,12 @@ def _check(q, k, v, key_padding_mask, key_lens, query_lens, scale):
 
 
 def _rows(t):
-    """t with rows on 16-byte boundaries (t itself where they are)."""
+    """t with rows on 16-byte boundaries and near enough to each other (t itself where they are)."""
     n = 16 // t.element_size()
     sb, sl, sh, s = t.stride()
-    B, L, H, dh = t.shape
-    if ((s == 1 or dh == 1) and t.data_ptr() % 16 == 0 and (sb % n == 0 or B == 1) and (sl % n == 0 or L == 1)
-            and (sh % n == 0 or H == 1)):
+    B, L, H, _ = t.shape
+    if (s == 1 and t.data_ptr() % 16 == 0 and (sb % n == 0 or B == 1) and (L == 1 or (sl % n == 0 and sl < 1 << 20))
+            and (H == 1 or (sh % n == 0 and sh * H < 1 << 28))):
         return t
     return t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 else t.clone()
 
@@ -136,8 +136,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_pa
     """softmax(scale q k^T) v for every head.
 
     q (B, Lq, H, dh); k, v (B, Lk, Hk, dh): head h reads key head h // (H // Hk).  One dtype among bfloat16, float16,
-        float32; dh a multiple of 8 up to 256; any strides (rows that are not contiguous or not on 16-byte boundaries
-        are copied; a batch of stride 0 is read as it stands).
+        float32; dh a multiple of 8 up to 256; any strides (rows that are not contiguous, not on 16-byte boundaries
+        or very far apart are copied; a batch of stride 0 is read as it stands).
     key_padding_mask (B, Lk), True = ignore that key (nn.MultiheadAttention's convention); key_lens (B,) int32 or int64:
         keys from key_lens[b] on are ignored.  What ignored keys hold, NaN and infinities among it, has no effect.
     query_lens (B,): queries from query_lens[b] on give zeros, and take part in no gradient.
