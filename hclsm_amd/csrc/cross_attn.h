@@ -22,6 +22,7 @@ typedef __bf16 cab8 __attribute__((ext_vector_type(8)));
 typedef _Float16 cah8 __attribute__((ext_vector_type(8)));
 typedef short cas4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) cas4 ca_lds_s4;
+typedef __attribute__((address_space(3))) void ca_lds_void;
 
 struct CaArgs {
   const char *q, *k, *v, *g;        // inputs; gradient of the output
@@ -143,20 +144,17 @@ template <int DT> __device__ __forceinline__ void ca_store4(char* base, int64_t 
 }
 
 // Rows of DH elements in LDS, as 16-byte chunks.  Two reads have to be free of bank conflicts: 16 rows at one chunk
-// (operands along a row), and 32 bytes of each of 8 rows (the transposing read).  Rows of 128 bytes and more whose
-// chunk count is a power of two exchange chunks by row; others are padded by one chunk.
+// (operands along a row), and 32 bytes of each of 8 rows (the transposing read).  Rows of 8, 16 or 32 chunks of 16-bit
+// elements exchange their chunks by the row's low three bits (measured: no conflict cycles); others are padded by one chunk.
 template <int DT, int DH> struct CaTile {
   static constexpr int CH = DH / CaT<DT>::EPC;
   static constexpr bool XOR = DT != HCLSM_F32 && (CH == 8 || CH == 16 || CH == 32);
-  static constexpr int STRIDE = XOR ? CH * 16 : CH * 16 + 16;
-  static __device__ __forceinline__ int off(int row, int chunk) {
-    if constexpr (XOR) {
-      const int x = CH == 8 ? (row & 7) ^ ((row >> 3) & 1) : ((row & 7) << 1) | ((row >> 3) & 1);
-      return row * STRIDE + ((chunk ^ x) << 4);
-    } else {
-      return row * STRIDE + (chunk << 4);
-    }
-  }
+  static constexpr int PC = XOR ? CH : CH + 1;      // chunks of a row in LDS
+  static constexpr int STRIDE = PC * 16;
+  static __device__ __forceinline__ int swap(int row) { return !XOR ? 0 : CH == 8 ? row & 7 : (row & 7) << 1; }
+  static __device__ __forceinline__ int off(int row, int chunk) { return row * STRIDE + ((chunk ^ swap(row)) << 4); }
+  // bytes of a tile of `rows`, in whole transfers of a workgroup of `threads`
+  static constexpr int bytes(int rows, int threads) { return (rows * PC + threads - 1) / threads * threads * 16; }
   // operand with rows row0 + li as its free index and elements KS c + 4 or 8 g .. of the row as contraction
   static __device__ __forceinline__ typename CaT<DT>::Frag frag(const char* t, int row0, int c, int li, int g) {
     return ca_frag<DT>(*reinterpret_cast<const uint4*>(t + off(row0 + li, 4 * c + g)));

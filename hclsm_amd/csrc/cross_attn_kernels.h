@@ -5,29 +5,26 @@
 
 namespace hclsm {
 
-// A tile of ROWS rows on its way from global memory to LDS: loaded into registers while the tile before it is being
-// worked on, then written.  A chunk's offset from the tile's first row does not change from tile to tile, so a load is one
-// comparison and one select: rows past the end, and chunks past dh, get an offset past the buffer resource's end, where
-// loads return zeros.  Rows whose bit of `live` is clear are written as zeros: what a masked row holds (NaN included) never
-// reaches a product.
+// Transfer of a tile of ROWS rows from global memory straight to LDS (16 bytes per lane to consecutive LDS addresses of
+// a wave; which chunk of which row that is, is chosen by the lane's global address), one tile ahead of its use.  A
+// chunk's offset from the tile's first row does not change from tile to tile; rows past the end, chunks past dh and the
+// layout's padding get an offset past the buffer resource's end, for which the hardware writes zeros.
 template <int DT, int DH, int NT, int ROWS> struct CaStage {
   using A = CaT<DT>;
   using Tile = CaTile<DT, DH>;
-  static constexpr int TOTAL = ROWS * Tile::CH, N = (TOTAL + NT - 1) / NT;
+  static constexpr int BYTES = Tile::bytes(ROWS, NT), N = BYTES / (NT * 16);
   static constexpr int ESZ = (int)sizeof(typename A::T);
   static constexpr uint32_t NONE = 0xffffffffu;
   uint32_t off[N];
-  uint4 r[N];
 
-  static __device__ __forceinline__ int row(int n) { return ((int)threadIdx.x + n * NT) / Tile::CH; }
-  static __device__ __forceinline__ int chunk(int n) { return ((int)threadIdx.x + n * NT) % Tile::CH; }
-  static __device__ __forceinline__ bool in(int n) { return TOTAL % NT == 0 || (int)threadIdx.x + n * NT < TOTAL; }
+  static __device__ __forceinline__ int row(int n) { return ((int)threadIdx.x + n * NT) / Tile::PC; }
+  static __device__ __forceinline__ int chunk(int n) { return (((int)threadIdx.x + n * NT) % Tile::PC) ^ Tile::swap(row(n)); }
 
   // rows one stride apart
   __device__ __forceinline__ void init(int64_t stride, int dh) {
 #pragma unroll
     for (int n = 0; n < N; ++n)
-      off[n] = in(n) && chunk(n) * A::EPC < dh ? (uint32_t)row(n) * (uint32_t)(stride * ESZ) + chunk(n) * 16 : NONE;
+      off[n] = row(n) < ROWS && chunk(n) * A::EPC < dh ? (uint32_t)row(n) * (uint32_t)(stride * ESZ) + chunk(n) * 16 : NONE;
   }
   // rows of a unit, the first one being head `phase` of its query: `used` rows of a tile
   __device__ __forceinline__ void init_rows(const CaArgs& a, int64_t sl, int64_t sh, int phase, int used) {
@@ -35,31 +32,43 @@ template <int DT, int DH, int NT, int ROWS> struct CaStage {
     for (int n = 0; n < N; ++n) {
       int qi, hg;
       ca_row(a, phase + row(n), qi, hg);
-      off[n] = in(n) && row(n) < used && chunk(n) * A::EPC < a.dh
+      off[n] = row(n) < used && chunk(n) * A::EPC < a.dh
                    ? (uint32_t)qi * (uint32_t)(sl * ESZ) + (uint32_t)hg * (uint32_t)(sh * ESZ) + chunk(n) * 16 : NONE;
     }
   }
-  // base: first row of the tile; n_rows: rows there are from it on
-  __device__ __forceinline__ void load(const char* base, int n_rows) {
+  // base: first row of the tile; n_rows: rows there are from it on; wave: index of the wave, in a scalar register
+  __device__ __forceinline__ void load(const char* base, int n_rows, char* t, int wave) const {
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, kRawBufferWord3);
+    if (n_rows >= ROWS) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const uint32_t o = row(n) < n_rows ? off[n] : NONE;
-      r[n] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)o, 0, 0));
+      for (int n = 0; n < N; ++n)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (ca_lds_void*)(t + (n * NT + wave * 64) * 16), 16, (int)off[n], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (ca_lds_void*)(t + (n * NT + wave * 64) * 16), 16,
+                                                 (int)(row(n) < n_rows ? off[n] : NONE), 0, 0, 0);
     }
   }
-  __device__ __forceinline__ void write(char* t) const {
+  // zeros for the rows whose bit is clear: what a masked row holds (NaN included) never reaches a product
+  static __device__ __forceinline__ void drop(char* t, uint64_t live) {
 #pragma unroll
     for (int n = 0; n < N; ++n)
-      if (in(n)) *reinterpret_cast<uint4*>(t + Tile::off(row(n), chunk(n))) = r[n];
-  }
-  __device__ __forceinline__ void drop(uint64_t live) {
-    asm volatile("");      // keeps the branch around this: the selects would otherwise be made for every tile
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-      if (!(live >> (row(n) & 63) & 1)) r[n] = uint4{0, 0, 0, 0};
+      if (row(n) < ROWS && !(live >> (row(n) & 63) & 1))
+        *reinterpret_cast<uint4*>(t + ((int)threadIdx.x + n * NT) * 16) = uint4{0, 0, 0, 0};
   }
 };
+
+// This wave's transfers are in LDS (gfx9 encoding of s_waitcnt with the vector-memory count alone).
+__device__ __forceinline__ void ca_wait_vmem() { __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8)); }
+// No instruction moves across: operand reads stay ahead of the products they are to overlap with.
+__device__ __forceinline__ void ca_fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// Two LDS objects of their own, and loops that name them in turn: a read of the one then does not wait for transfers to
+// the other (with one object, or an index into two, the compiler has every LDS read wait for all transfers).
+#define CA_TWO_BUFFERS(bytes)                                       \
+  __shared__ __attribute__((aligned(16))) char buf0[bytes];         \
+  __shared__ __attribute__((aligned(16))) char buf1[bytes]
 
 // Bits of the live keys among t0 .. t0 + ROWS - 1: below `end` and not flagged.  p: this lane's flag.
 template <int ROWS> __device__ __forceinline__ uint64_t ca_live(int t0, int end, uint8_t p) {
@@ -95,12 +104,13 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
   using Tile = CaTile<DT, DH>;
   using Frag = typename A::Frag;
   constexpr int NT = 64 * NW, KT = KR / 16, NC = DH / A::KS, ND = DH / 16, NPT = A::NPT, ESZ = (int)sizeof(typename A::T);
-  constexpr int TB = KR * Tile::STRIDE;
-  extern __shared__ __attribute__((aligned(16))) char lds[];   // [2][K tile, V tile]
+  using Stage = CaStage<DT, DH, NT, KR>;
+  constexpr int TB = Stage::BYTES;
+  CA_TWO_BUFFERS(2 * TB);      // K tile, V tile
 
   CaWork w;
   if (!ca_work(a, w)) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
   const int row0 = (w.tile * NW + wave) * 16 * QT;
   int k0, k1;
   ca_range(w.keys, a.nsplit, w.split, KR, k0, k1);
@@ -136,52 +146,59 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
   }
 
   const int nt = (k1 - k0 + KR - 1) / KR;
-  CaStage<DT, DH, NT, KR> sk, sv;
+  Stage sk, sv;
   sk.init(a.ksl, a.dh);
   sv.init(a.vsl, a.dh);
   uint8_t flag = 0;
-  uint64_t live = 0;
-  auto load = [&](int t0) {
-    sk.load(kp + t0 * a.ksl * ESZ, k1 - t0);
-    sv.load(vp + t0 * a.vsl * ESZ, k1 - t0);
+  auto load = [&](int i, char* buf) __attribute__((always_inline)) {
+    const int t0 = k0 + i * KR;
+    sk.load(kp + t0 * a.ksl * ESZ, k1 - t0, buf, wave);
+    sv.load(vp + t0 * a.vsl * ESZ, k1 - t0, buf + TB, wave);
     flag = ca_flag<KR>(pad, t0, k1);
   };
-  auto write = [&](int t0, char* buf) {
-    live = ca_live<KR>(t0, k1, flag);
-    if (pad != nullptr && live != CA_FULL<KR>) {
-      sk.drop(live);
-      sv.drop(live);
-    }
-    sk.write(buf);
-    sv.write(buf + TB);
-  };
-  if (nt > 0) {
-    load(k0);
-    write(k0, lds);
-    if (nt > 1) load(k0 + KR);
-  }
-  for (int i = 0; i < nt; ++i) {
-    char* tk = lds + (i & 1) * 2 * TB;
+  if (nt > 0) load(0, buf0);
+  auto tile = [&](int i, char* tk, char* next) __attribute__((always_inline)) {
     char* tv = tk + TB;
-    const uint64_t now = live;
-    __syncthreads();      // tile i is written, and every wave is done with the other buffer
-    if (i + 1 < nt) {
-      write(k0 + (i + 1) * KR, lds + ((i + 1) & 1) * 2 * TB);
-      if (i + 2 < nt) load(k0 + (i + 2) * KR);
+    ca_wait_vmem();
+    const uint64_t now = ca_live<KR>(k0 + i * KR, k1, flag);
+    __syncthreads();      // tile i is in LDS, and every wave is done with the other buffer
+    if (pad != nullptr && now != CA_FULL<KR>) {
+      Stage::drop(tk, now);
+      Stage::drop(tv, now);
+      __syncthreads();
     }
+    if (i + 1 < nt) load(i + 1, next);
 
     caf4 s[QT][KT];
+    Frag f[2][NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) f[0][c] = Tile::frag(tk, 0, c, li, g);
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
+      if (k + 1 < KT) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) f[(k + 1) & 1][c] = Tile::frag(tk, 16 * (k + 1), c, li, g);
+      }
+      ca_fence();
 #pragma unroll
       for (int t = 0; t < QT; ++t) s[t][k] = caf4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const Frag f = Tile::frag(tk, 16 * k, c, li, g);
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int t = 0; t < QT; ++t) s[t][k] = A::mma(f, q[t][c], s[t][k]);
-      }
+        for (int t = 0; t < QT; ++t) s[t][k] = A::mma(f[k & 1][c], q[t][c], s[t][k]);
+      ca_fence();
     }
+    // operands of the second product, CV at a time, the first ones on their way during the softmax
+    constexpr int J = KT / NPT * ND, CV = J < 4 ? J : 4;
+    static_assert(J % CV == 0, "whole groups");
+    Frag fv[2][CV];
+    auto get_v = [&](int c, Frag* d) {
+#pragma unroll
+      for (int j = 0; j < CV; ++j)
+        d[j] = Tile::frag_t(tv, 16 * NPT * ((c * CV + j) / ND), (c * CV + j) % ND, li, g);
+    };
+    get_v(0, fv[0]);
+    ca_fence();
     if (now != CA_FULL<KR>) {
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
@@ -235,14 +252,20 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
       for (int u = 0; u < KT / NPT; ++u) p[t][u] = ca_pack<DT>(&s[t][u * NPT]);
     }
 #pragma unroll
-    for (int u = 0; u < KT / NPT; ++u) {
+    for (int c = 0; c < J / CV; ++c) {
+      if (c + 1 < J / CV) get_v(c + 1, fv[(c + 1) & 1]);
+      ca_fence();
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const Frag f = Tile::frag_t(tv, 16 * NPT * u, d, li, g);
+      for (int j = 0; j < CV; ++j)
 #pragma unroll
-        for (int t = 0; t < QT; ++t) o[t][d] = A::mma(f, p[t][u], o[t][d]);
-      }
+        for (int t = 0; t < QT; ++t)
+          o[t][(c * CV + j) % ND] = A::mma(fv[c & 1][j], p[t][(c * CV + j) / ND], o[t][(c * CV + j) % ND]);
+      ca_fence();
     }
+  };
+  for (int i = 0; i < nt; i += 2) {
+    tile(i, buf0, buf1);
+    if (i + 1 < nt) tile(i + 1, buf1, buf0);
   }
 
   // rows without a live key have l = 0: zeros, and a log-sum of -inf
@@ -286,12 +309,13 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
   using Tile = CaTile<DT, DH>;
   using Frag = typename A::Frag;
   constexpr int NT = 64 * NW, KT = KR / 16, NC = DH / A::KS, ND = DH / 16, NPT = A::NPT, ESZ = (int)sizeof(typename A::T);
-  constexpr int TB = KR * Tile::STRIDE;
-  extern __shared__ __attribute__((aligned(16))) char lds[];   // [2][K tile, V tile]
+  using Stage = CaStage<DT, DH, NT, KR>;
+  constexpr int TB = Stage::BYTES;
+  CA_TWO_BUFFERS(2 * TB);      // K tile, V tile
 
   CaWork w;
   if (!ca_work(a, w)) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
   const int row0 = (w.tile * NW + wave) * 16 * QT;
   int k0, k1;
   ca_range(w.keys, a.nsplit, w.split, KR, k0, k1);
@@ -337,39 +361,28 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
     for (int d = 0; d < ND; ++d) dq[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
 
   const int nt = (k1 - k0 + KR - 1) / KR;
-  CaStage<DT, DH, NT, KR> sk, sv;
+  Stage sk, sv;
   sk.init(a.ksl, a.dh);
   sv.init(a.vsl, a.dh);
   uint8_t flag = 0;
-  uint64_t live = 0;
-  auto load = [&](int t0) {
-    sk.load(kp + t0 * a.ksl * ESZ, k1 - t0);
-    sv.load(vp + t0 * a.vsl * ESZ, k1 - t0);
+  auto load = [&](int i, char* buf) __attribute__((always_inline)) {
+    const int t0 = k0 + i * KR;
+    sk.load(kp + t0 * a.ksl * ESZ, k1 - t0, buf, wave);
+    sv.load(vp + t0 * a.vsl * ESZ, k1 - t0, buf + TB, wave);
     flag = ca_flag<KR>(pad, t0, k1);
   };
-  auto write = [&](int t0, char* buf) {
-    live = ca_live<KR>(t0, k1, flag);
-    if (pad != nullptr && live != CA_FULL<KR>) {
-      sk.drop(live);
-      sv.drop(live);
-    }
-    sk.write(buf);
-    sv.write(buf + TB);
-  };
-  if (nt > 0) {
-    load(k0);
-    write(k0, lds);
-    if (nt > 1) load(k0 + KR);
-  }
-  for (int i = 0; i < nt; ++i) {
-    char* tk = lds + (i & 1) * 2 * TB;
+  if (nt > 0) load(0, buf0);
+  auto tile = [&](int i, char* tk, char* next) __attribute__((always_inline)) {
     char* tv = tk + TB;
-    const uint64_t now = live;
-    __syncthreads();
-    if (i + 1 < nt) {
-      write(k0 + (i + 1) * KR, lds + ((i + 1) & 1) * 2 * TB);
-      if (i + 2 < nt) load(k0 + (i + 2) * KR);
+    ca_wait_vmem();
+    const uint64_t now = ca_live<KR>(k0 + i * KR, k1, flag);
+    __syncthreads();      // tile i is in LDS, and every wave is done with the other buffer
+    if (pad != nullptr && now != CA_FULL<KR>) {
+      Stage::drop(tk, now);
+      Stage::drop(tv, now);
+      __syncthreads();
     }
+    if (i + 1 < nt) load(i + 1, next);
 #pragma unroll
     for (int u = 0; u < KT / NPT; ++u) {
       caf4 s[QT][NPT], dp[QT][NPT];
@@ -413,6 +426,10 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
         for (int t = 0; t < QT; ++t) dq[t][d] = A::mma(f, ds[t], dq[t][d]);
       }
     }
+  };
+  for (int i = 0; i < nt; i += 2) {
+    tile(i, buf0, buf1);
+    if (i + 1 < nt) tile(i + 1, buf1, buf0);
   }
 
   const int all = a.Lq * a.G;
@@ -446,12 +463,13 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
   using Tile = CaTile<DT, DH>;
   using Frag = typename A::Frag;
   constexpr int NT = 64 * NW, RT = RR / 16, NC = DH / A::KS, ND = DH / 16, NPT = A::NPT, ESZ = (int)sizeof(typename A::T);
-  constexpr int TB = RR * Tile::STRIDE, BUF = 2 * TB + RR * 8;
-  extern __shared__ __attribute__((aligned(16))) char lds[];   // [2][Q tile, g tile, RR log-sums, RR deltas]
+  using Stage = CaStage<DT, DH, NT, RR>;
+  constexpr int TB = Stage::BYTES, BUF = 2 * TB + RR * 8;
+  CA_TWO_BUFFERS(BUF);         // Q tile, g tile, RR log-sums, RR negated deltas
 
   CaWork w;
   if (!ca_work(a, w)) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
   const int key0 = (w.tile * NW + wave) * 16 * KT;
   const int step = ca_row_step(a.G, RR);      // rows of a tile: whole queries
   int r0, r1;
@@ -488,7 +506,7 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
     for (int d = 0; d < ND; ++d) dk[t][d] = dv[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
 
   const int nt = (r1 - r0 + step - 1) / step;
-  CaStage<DT, DH, NT, RR> sq, sg;
+  Stage sq, sg;
   float st_lse = INFINITY, st_delta = 0.f;
   int st_q = 0, st_h = 0;
   auto init = [&](int phase) {
@@ -497,12 +515,14 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
     ca_row(a, phase + (int)threadIdx.x, st_q, st_h);
   };
   init(0);
-  auto load = [&](int t0) {
+  auto load = [&](int i, char* buf) __attribute__((always_inline)) {
+    const int t0 = r0 + i * step;
     int q0, phase;
     ca_row(a, t0, q0, phase);
     if (a.G > RR) init(phase);       // more heads to a query than rows to a tile: tiles begin inside a query
-    sq.load(qp + q0 * a.qsl * ESZ, r1 - t0);
-    sg.load(gp + q0 * a.gsl * ESZ, r1 - t0);
+    const int n = r1 - t0 < step ? r1 - t0 : RR;
+    sq.load(qp + q0 * a.qsl * ESZ, n, buf, wave);
+    sg.load(gp + q0 * a.gsl * ESZ, n, buf + TB, wave);
     st_lse = INFINITY;         // rows past the last one, and rows without keys: every weight is exp(-inf)
     st_delta = 0.f;
     if ((int)threadIdx.x < step && t0 + (int)threadIdx.x < r1) {
@@ -512,28 +532,17 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
       st_delta = -a.delta[i];
     }
   };
-  auto write = [&](char* buf) {
-    sq.write(buf);
-    sg.write(buf + TB);
-    if ((int)threadIdx.x < RR) {
-      reinterpret_cast<float*>(buf + 2 * TB)[threadIdx.x] = st_lse;
-      reinterpret_cast<float*>(buf + 2 * TB)[RR + threadIdx.x] = st_delta;
-    }
-  };
-  if (nt > 0) {
-    load(r0);
-    write(lds);
-    if (nt > 1) load(r0 + step);
-  }
-  for (int i = 0; i < nt; ++i) {
-    char* tq = lds + (i & 1) * BUF;
+  if (nt > 0) load(0, buf0);
+  auto tile = [&](int i, char* tq, char* next) __attribute__((always_inline)) {
     char* tg = tq + TB;
-    const float* stat = reinterpret_cast<const float*>(tq + 2 * TB);
-    __syncthreads();
-    if (i + 1 < nt) {
-      write(lds + ((i + 1) & 1) * BUF);
-      if (i + 2 < nt) load(r0 + (i + 2) * step);
+    float* stat = reinterpret_cast<float*>(tq + 2 * TB);
+    if ((int)threadIdx.x < RR) {
+      stat[threadIdx.x] = st_lse;
+      stat[RR + threadIdx.x] = st_delta;
     }
+    ca_wait_vmem();
+    __syncthreads();
+    if (i + 1 < nt) load(i + 1, next);
 #pragma unroll
     for (int u = 0; u < RT / NPT; ++u) {
       caf4 s[KT][NPT], dp[KT][NPT];
@@ -584,6 +593,10 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
         }
       }
     }
+  };
+  for (int i = 0; i < nt; i += 2) {
+    tile(i, buf0, buf1);
+    if (i + 1 < nt) tile(i + 1, buf1, buf0);
   }
 
   const int64_t half = (int64_t)a.nsplit * a.units * a.Lk * a.dh;      // split: dk sums, then dv sums
@@ -616,19 +629,13 @@ template <int DT, int DH> struct CaShape {
   static constexpr int RB = DH * (int)sizeof(typename CaT<DT>::T);
   static constexpr int TR = RB <= 256 ? 64 : 32;      // rows of a tile
   static constexpr int T = RB <= 256 ? 2 : 1;         // 16-row tiles per wave
-  static constexpr int LDS = 4 * TR * CaTile<DT, DH>::STRIDE;
-  static constexpr int LDS_DKV = LDS + 2 * TR * 8;
+  static_assert(4 * CaTile<DT, DH>::bytes(TR, 256) + 2 * TR * 8 <= 160 * 1024, "two buffers of two tiles");
 };
-
-constexpr int CA_MAX_LDS = 160 * 1024;
 
 inline bool ca_by_xcd(int64_t units) { return units % 8 == 0 || units >= 64; }
 
 template <typename K>
-int ca_launch(K kernel, CaArgs& a, int64_t batch, int64_t rows, int per_wg, int threads, int lds, std::atomic<int>* cache,
-              hipStream_t st) {
-  int grid = 0;
-  if (int rc = device_launch_setup((const void*)kernel, threads, lds, lds > 65536 ? CA_MAX_LDS : 0, cache, &grid)) return rc;
+int ca_launch(K kernel, CaArgs& a, int64_t batch, int64_t rows, int per_wg, int threads, hipStream_t st) {
   const int64_t units = batch * a.Hk, tiles = (rows + per_wg - 1) / per_wg;
   a.units = (int)units;
   a.tiles = (int)tiles;
@@ -636,14 +643,13 @@ int ca_launch(K kernel, CaArgs& a, int64_t batch, int64_t rows, int per_wg, int 
   const int64_t blocks = (a.by_xcd ? (units + 7) / 8 * 8 : units) * tiles * a.nsplit;
   if (blocks == 0) return 0;
   if (blocks > 0x7fffffff / threads) return HCLSM_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, st, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, st, a);
   HCLSM_LAUNCH_CHECK();
   return 0;
 }
 
 template <int DT, int DH> int ca_forward_dh(CaArgs& a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st) {
   using S = CaShape<DT, DH>;
-  static std::atomic<int> cw[HCLSM_MAX_DEVICES], c1[HCLSM_MAX_DEVICES], c2[HCLSM_MAX_DEVICES];
   const CaPlan p = ca_forward_plan(batch, a.Lq, a.Lk, a.Hk, a.G, a.dh, DT);
   const int64_t rows = (int64_t)a.Lq * a.G;
   a.nsplit = p.nsplit;
@@ -656,11 +662,11 @@ template <int DT, int DH> int ca_forward_dh(CaArgs& a, int64_t batch, void* ws, 
   }
   int rc = HCLSM_ERR_UNSUPPORTED;
   if (p.few == 1) {
-    if constexpr (S::RB <= CA_FEW1_BYTES) rc = ca_launch(ca_few_kernel<DT, DH, 4, 1>, a, batch, rows, 16, 256, 0, c1, st);
+    if constexpr (S::RB <= CA_FEW1_BYTES) rc = ca_launch(ca_few_kernel<DT, DH, 4, 1>, a, batch, rows, 16, 256, st);
   } else if (p.few == 2) {
-    if constexpr (S::RB <= CA_FEW2_BYTES) rc = ca_launch(ca_few_kernel<DT, DH, 4, 2>, a, batch, rows, 32, 256, 0, c2, st);
+    if constexpr (S::RB <= CA_FEW2_BYTES) rc = ca_launch(ca_few_kernel<DT, DH, 4, 2>, a, batch, rows, 32, 256, st);
   } else {
-    rc = ca_launch(ca_fwd_kernel<DT, DH, 4, S::T, S::TR>, a, batch, rows, 64 * S::T, 256, S::LDS, cw, st);
+    rc = ca_launch(ca_fwd_kernel<DT, DH, 4, S::T, S::TR>, a, batch, rows, 64 * S::T, 256, st);
   }
   if (rc || p.nsplit == 1) return rc;
   return ca_join(a, DT, st);
@@ -668,14 +674,13 @@ template <int DT, int DH> int ca_forward_dh(CaArgs& a, int64_t batch, void* ws, 
 
 template <int DT, int DH> int ca_backward_dh(CaArgs& a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st) {
   using S = CaShape<DT, DH>;
-  static std::atomic<int> cq[HCLSM_MAX_DEVICES], ck[HCLSM_MAX_DEVICES];
   const int64_t stats = batch * a.Hk * a.G * a.Lq;
   if (ws_bytes < stats * 4) return HCLSM_ERR_SHAPE;
   a.delta = (float*)ws;
   a.nsplit = 1;
-  if (int rc = ca_launch(ca_dq_kernel<DT, DH, 4, S::T, S::TR>, a, batch, (int64_t)a.Lq * a.G, 64 * S::T, 256, S::LDS, cq, st))
+  if (int rc = ca_launch(ca_dq_kernel<DT, DH, 4, S::T, S::TR>, a, batch, (int64_t)a.Lq * a.G, 64 * S::T, 256, st))
     return rc;
-  return ca_launch(ca_dkv_kernel<DT, DH, 4, S::T, S::TR>, a, batch, a.Lk, 64 * S::T, 256, S::LDS_DKV, ck, st);
+  return ca_launch(ca_dkv_kernel<DT, DH, 4, S::T, S::TR>, a, batch, a.Lk, 64 * S::T, 256, st);
 }
 
 template <int DT> int ca_forward_dt(CaArgs a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st) {
