@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
 // As the forward, with S^T and dP^T = V g^T formed per tile, p = exp(s - lse), ds = p (dP - delta) and
 // dQ^T = K^T ds^T.  delta = sum(g o) per row is formed here and left for the second kernel.  ds is rounded to the
 // operand type for its product, as the weights are in the forward.
-template <int DT, int DH, int NW, int QT, int KR>
+template <int DT, int DH, int NW, int QT, int KR, bool PIPE>
 __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
   using A = CaT<DT>;
   using Tile = CaTile<DT, DH>;
@@ -383,47 +383,78 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
       __syncthreads();
     }
     if (i + 1 < nt) load(i + 1, next);
+    constexpr int U = KT / NPT;
+    caf4 s[2][QT][NPT], dp[2][QT][NPT];
+    // S^T and dP^T of step u (16 NPT keys): operands of a 16-key tile are read while the tile before is multiplied
+    auto scores = [&](int u, caf4 (*s)[NPT], caf4 (*dp)[NPT]) __attribute__((always_inline)) {
+      Frag fk[2][NC], fv[2][NC];
+      auto get = [&](int k, int b) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < KT / NPT; ++u) {
-      caf4 s[QT][NPT], dp[QT][NPT];
+        for (int c = 0; c < NC; ++c) {
+          fk[b][c] = Tile::frag(tk, 16 * (u * NPT + k), c, li, g);
+          fv[b][c] = Tile::frag(tv, 16 * (u * NPT + k), c, li, g);
+        }
+      };
+      get(0, 0);
 #pragma unroll
       for (int k = 0; k < NPT; ++k) {
+        if (k + 1 < NPT) get(k + 1, (k + 1) & 1);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
           s[t][k] = caf4{0.f, 0.f, 0.f, 0.f};
           dp[t][k] = ndelta[t];
         }
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const Frag fk = Tile::frag(tk, 16 * (u * NPT + k), c, li, g);
-          const Frag fv = Tile::frag(tv, 16 * (u * NPT + k), c, li, g);
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
           for (int t = 0; t < QT; ++t) {
-            s[t][k] = A::mma(fk, q[t][c], s[t][k]);
-            dp[t][k] = A::mma(fv, go[t][c], dp[t][k]);
+            s[t][k] = A::mma(fk[k & 1][c], q[t][c], s[t][k]);
+            dp[t][k] = A::mma(fv[k & 1][c], go[t][c], dp[t][k]);
           }
-        }
       }
+    };
+    if (PIPE) scores(0, s[0], dp[0]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      ca_fence();
+      if (!PIPE) scores(u, s[u & 1], dp[u & 1]);
+      else if (u + 1 < U) scores(u + 1, s[(u + 1) & 1], dp[(u + 1) & 1]);      // the vector unit works on step u meanwhile
       Frag ds[QT];
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int k = 0; k < NPT; ++k)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) dp[u & 1][t][k][r] *= fast_exp2(s[u & 1][t][k][r] * a.scale_log2 - lse2[t]);
+      if (now != CA_FULL<KR>) {
 #pragma unroll
         for (int k = 0; k < NPT; ++k) {
+          const uint32_t bits = (uint32_t)(now >> (16 * (u * NPT + k) + 4 * g));
 #pragma unroll
-          for (int r = 0; r < 4; ++r) dp[t][k][r] *= fast_exp2(s[t][k][r] * a.scale_log2 - lse2[t]);
-          if (now != CA_FULL<KR>) {
-            const uint32_t bits = (uint32_t)(now >> (16 * (u * NPT + k) + 4 * g));
+          for (int t = 0; t < QT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) dp[t][k][r] = bits >> r & 1 ? dp[t][k][r] : 0.f;
-          }
+            for (int r = 0; r < 4; ++r) dp[u & 1][t][k][r] = bits >> r & 1 ? dp[u & 1][t][k][r] : 0.f;
         }
-        ds[t] = ca_pack<DT>(dp[t]);
       }
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const Frag f = Tile::frag_t(tk, 16 * NPT * u, d, li, g);
+      for (int t = 0; t < QT; ++t) ds[t] = ca_pack<DT>(dp[u & 1][t]);
+      constexpr int CV = ND < 4 ? ND : ND % 4 == 0 ? 4 : 2;
+      Frag ft[2][CV];
+      auto get_t = [&](int c, int b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < QT; ++t) dq[t][d] = A::mma(f, ds[t], dq[t][d]);
+        for (int j = 0; j < CV; ++j) ft[b][j] = Tile::frag_t(tk, 16 * NPT * u, c * CV + j, li, g);
+      };
+      get_t(0, 0);
+      ca_fence();
+#pragma unroll
+      for (int c = 0; c < ND / CV; ++c) {
+        if (c + 1 < ND / CV) get_t(c + 1, (c + 1) & 1);
+        ca_fence();
+#pragma unroll
+        for (int j = 0; j < CV; ++j)
+#pragma unroll
+          for (int t = 0; t < QT; ++t) dq[t][c * CV + j] = A::mma(ft[c & 1][j], ds[t], dq[t][c * CV + j]);
+        ca_fence();
       }
     }
   };
@@ -457,7 +488,7 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
 // NW waves of 16 KT keys each, K and V operands in registers, over tiles of RR rows (q and g in LDS):
 // S = Q K^T and dP = g V^T with a lane per key, then dV^T = g^T p and dK^T = Q^T ds.  Shared heads are rows of the
 // unit, so their gradients are added here.  Keys that are not live get zeros.
-template <int DT, int DH, int NW, int KT, int RR>
+template <int DT, int DH, int NW, int KT, int RR, bool PIPE>
 __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
   using A = CaT<DT>;
   using Tile = CaTile<DT, DH>;
@@ -495,10 +526,6 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) { fk[t][c] = ca_frag<DT>(f0[c]); fv[t][c] = ca_frag<DT>(f1[c]); }
   }
-  bool all_live = true;
-#pragma unroll
-  for (int t = 0; t < KT; ++t) all_live = all_live && live[t];
-  const bool dead = __any(!all_live);
   caf4 dk[KT][ND], dv[KT][ND];
 #pragma unroll
   for (int t = 0; t < KT; ++t)
@@ -507,7 +534,7 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
 
   const int nt = (r1 - r0 + step - 1) / step;
   Stage sq, sg;
-  float st_lse = INFINITY, st_delta = 0.f;
+  float st_lse = -INFINITY, st_delta = 0.f;
   int st_q = 0, st_h = 0;
   auto init = [&](int phase) {
     sq.init_rows(a, a.qsl, a.qsh, phase, step);
@@ -523,74 +550,99 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
     const int n = r1 - t0 < step ? r1 - t0 : RR;
     sq.load(qp + q0 * a.qsl * ESZ, n, buf, wave);
     sg.load(gp + q0 * a.gsl * ESZ, n, buf + TB, wave);
-    st_lse = INFINITY;         // rows past the last one, and rows without keys: every weight is exp(-inf)
+    st_lse = -INFINITY;
     st_delta = 0.f;
     if ((int)threadIdx.x < step && t0 + (int)threadIdx.x < r1) {
-      const int64_t i = stat0 + (int64_t)st_h * a.Lq + q0 + st_q;
-      const float ls = a.lse[i];
-      if (ls != -INFINITY) st_lse = ls * HCLSM_LOG2E;
-      st_delta = -a.delta[i];
+      const int64_t j = stat0 + (int64_t)st_h * a.Lq + q0 + st_q;
+      st_lse = a.lse[j];          // looked at when the tile's turn comes: here it would wait for the tile
+      st_delta = a.delta[j];
     }
   };
   if (nt > 0) load(0, buf0);
   auto tile = [&](int i, char* tq, char* next) __attribute__((always_inline)) {
     char* tg = tq + TB;
     float* stat = reinterpret_cast<float*>(tq + 2 * TB);
-    if ((int)threadIdx.x < RR) {
-      stat[threadIdx.x] = st_lse;
-      stat[RR + threadIdx.x] = st_delta;
+    if ((int)threadIdx.x < RR) {       // rows past the last one, and rows without keys: every weight is exp(-inf)
+      stat[threadIdx.x] = st_lse == -INFINITY ? INFINITY : st_lse * HCLSM_LOG2E;
+      stat[RR + threadIdx.x] = -st_delta;
     }
     ca_wait_vmem();
     __syncthreads();
     if (i + 1 < nt) load(i + 1, next);
+    constexpr int U = RT / NPT;
+    caf4 s[2][KT][NPT], dp[2][KT][NPT];
+    // S and dP of step u (16 NPT rows): operands of a 16-row tile are read while the tile before is multiplied
+    auto scores = [&](int u, caf4 (*s)[NPT], caf4 (*dp)[NPT]) __attribute__((always_inline)) {
+      Frag fq[2][NC], fg[2][NC];
+      auto get = [&](int k, int b) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < RT / NPT; ++u) {
-      caf4 s[KT][NPT], dp[KT][NPT];
+        for (int c = 0; c < NC; ++c) {
+          fq[b][c] = Tile::frag(tq, 16 * (u * NPT + k), c, li, g);
+          fg[b][c] = Tile::frag(tg, 16 * (u * NPT + k), c, li, g);
+        }
+      };
+      get(0, 0);
 #pragma unroll
       for (int k = 0; k < NPT; ++k) {
+        if (k + 1 < NPT) get(k + 1, (k + 1) & 1);
+        const caf4 nd = *reinterpret_cast<const caf4*>(stat + RR + 16 * (u * NPT + k) + 4 * g);      // -delta
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
           s[t][k] = caf4{0.f, 0.f, 0.f, 0.f};
-          dp[t][k] = *reinterpret_cast<const caf4*>(stat + RR + 16 * (u * NPT + k) + 4 * g);      // -delta
+          dp[t][k] = nd;
         }
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const Frag fq = Tile::frag(tq, 16 * (u * NPT + k), c, li, g);
-          const Frag fg = Tile::frag(tg, 16 * (u * NPT + k), c, li, g);
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
           for (int t = 0; t < KT; ++t) {
-            s[t][k] = A::mma(fq, fk[t][c], s[t][k]);
-            dp[t][k] = A::mma(fg, fv[t][c], dp[t][k]);
+            s[t][k] = A::mma(fq[k & 1][c], fk[t][c], s[t][k]);
+            dp[t][k] = A::mma(fg[k & 1][c], fv[t][c], dp[t][k]);
           }
-        }
       }
+    };
+    if (PIPE) scores(0, s[0], dp[0]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      ca_fence();
+      if (!PIPE) scores(u, s[u & 1], dp[u & 1]);
+      else if (u + 1 < U) scores(u + 1, s[(u + 1) & 1], dp[(u + 1) & 1]);      // the vector unit works on step u meanwhile
       Frag p[KT], ds[KT];
 #pragma unroll
       for (int k = 0; k < NPT; ++k) {
         const caf4 ls = *reinterpret_cast<const caf4*>(stat + 16 * (u * NPT + k) + 4 * g);
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[t][k][r] = fast_exp2(s[t][k][r] * a.scale_log2 - ls[r]);
-          if (dead) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[t][k][r] = live[t] ? s[t][k][r] : 0.f;
+          for (int r = 0; r < 4; ++r) {
+            s[u & 1][t][k][r] = fast_exp2(s[u & 1][t][k][r] * a.scale_log2 - ls[r]);
+            dp[u & 1][t][k][r] *= s[u & 1][t][k][r];
           }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) dp[t][k][r] *= s[t][k][r];
-        }
       }
 #pragma unroll
-      for (int t = 0; t < KT; ++t) { p[t] = ca_pack<DT>(s[t]); ds[t] = ca_pack<DT>(dp[t]); }
+      for (int t = 0; t < KT; ++t) { p[t] = ca_pack<DT>(s[u & 1][t]); ds[t] = ca_pack<DT>(dp[u & 1][t]); }
+      constexpr int CV = ND < 2 ? ND : 2;
+      Frag tg2[2][CV], tq2[2][CV];
+      auto get_t = [&](int c, int b) __attribute__((always_inline)) {
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const Frag fg = Tile::frag_t(tg, 16 * NPT * u, d, li, g);
-        const Frag fq = Tile::frag_t(tq, 16 * NPT * u, d, li, g);
-#pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          dv[t][d] = A::mma(fg, p[t], dv[t][d]);
-          dk[t][d] = A::mma(fq, ds[t], dk[t][d]);
+        for (int j = 0; j < CV; ++j) {
+          tg2[b][j] = Tile::frag_t(tg, 16 * NPT * u, c * CV + j, li, g);
+          tq2[b][j] = Tile::frag_t(tq, 16 * NPT * u, c * CV + j, li, g);
         }
+      };
+      get_t(0, 0);
+      ca_fence();
+#pragma unroll
+      for (int c = 0; c < ND / CV; ++c) {
+        if (c + 1 < ND / CV) get_t(c + 1, (c + 1) & 1);
+        ca_fence();
+#pragma unroll
+        for (int j = 0; j < CV; ++j)
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
+            dv[t][c * CV + j] = A::mma(tg2[c & 1][j], p[t], dv[t][c * CV + j]);
+            dk[t][c * CV + j] = A::mma(tq2[c & 1][j], ds[t], dk[t][c * CV + j]);
+          }
+        ca_fence();
       }
     }
   };
@@ -599,6 +651,8 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
     if (i + 1 < nt) tile(i + 1, buf1, buf0);
   }
 
+  // Keys that are not live read as zeros: their weights exp(-lse) mean nothing (they may overflow) but stay in the key's
+  // own column of either sum, and the rows are written as zeros.
   const int64_t half = (int64_t)a.nsplit * a.units * a.Lk * a.dh;      // split: dk sums, then dv sums
 #pragma unroll
   for (int t = 0; t < KT; ++t) {
@@ -610,12 +664,13 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
     for (int d = 0; d < ND; ++d)
       if (16 * d + 4 * g < a.dh) {
         const int64_t i = ob + 16 * d + 4 * g;
+        const caf4 zero = {0.f, 0.f, 0.f, 0.f}, vk = live[t] ? dk[t][d] * a.scale : zero, vv = live[t] ? dv[t][d] : zero;
         if (a.nsplit > 1) {
-          *reinterpret_cast<caf4*>(a.part + i) = dk[t][d] * a.scale;
-          *reinterpret_cast<caf4*>(a.part + half + i) = dv[t][d];
+          *reinterpret_cast<caf4*>(a.part + i) = vk;
+          *reinterpret_cast<caf4*>(a.part + half + i) = vv;
         } else {
-          ca_store4<DT>(a.dk, i, dk[t][d] * a.scale);
-          ca_store4<DT>(a.dv, i, dv[t][d]);
+          ca_store4<DT>(a.dk, i, vk);
+          ca_store4<DT>(a.dv, i, vv);
         }
       }
   }
@@ -629,6 +684,12 @@ template <int DT, int DH> struct CaShape {
   static constexpr int RB = DH * (int)sizeof(typename CaT<DT>::T);
   static constexpr int TR = RB <= 256 ? 64 : 32;      // rows of a tile
   static constexpr int T = RB <= 256 ? 2 : 1;         // 16-row tiles per wave
+  // Scores of the next step formed while the vector unit works on this one's: a second set of score tiles, which
+  // pays where it leaves the same number of waves per SIMD.  Measured on 8 x 1024 queries, 2048 keys, bf16 (us without ->
+  // with): dq of heads of 32: 110 -> 112, 64: 170 -> 163, 96: 126 -> 121, 128: 185 -> 183, 192: 198 -> 200, 256: 174 -> 209;
+  // dk and dv 134 -> 146, 217 -> 212, 196 -> 208, 258 -> 238, 281 -> 272, 336 -> 356; float32 heads of 64 (2 batch rows):
+  // 392 -> 383 and 423 -> 415, of 128: 407 -> 397 and 463 -> 488.
+  static constexpr bool PIPE_Q = RB <= 256, PIPE_KV = RB <= 256 && DH % 64 == 0;
   static_assert(4 * CaTile<DT, DH>::bytes(TR, 256) + 2 * TR * 8 <= 160 * 1024, "two buffers of two tiles");
 };
 
@@ -678,9 +739,9 @@ template <int DT, int DH> int ca_backward_dh(CaArgs& a, int64_t batch, void* ws,
   if (ws_bytes < stats * 4) return HCLSM_ERR_SHAPE;
   a.delta = (float*)ws;
   a.nsplit = 1;
-  if (int rc = ca_launch(ca_dq_kernel<DT, DH, 4, S::T, S::TR>, a, batch, (int64_t)a.Lq * a.G, 64 * S::T, 256, st))
+  if (int rc = ca_launch(ca_dq_kernel<DT, DH, 4, S::T, S::TR, S::PIPE_Q>, a, batch, (int64_t)a.Lq * a.G, 64 * S::T, 256, st))
     return rc;
-  return ca_launch(ca_dkv_kernel<DT, DH, 4, S::T, S::TR>, a, batch, a.Lk, 64 * S::T, 256, st);
+  return ca_launch(ca_dkv_kernel<DT, DH, 4, S::T, S::TR, S::PIPE_KV>, a, batch, a.Lk, 64 * S::T, 256, st);
 }
 
 template <int DT> int ca_forward_dt(CaArgs a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st) {
