@@ -5,8 +5,8 @@ of 2^-24 of the terms' size.  Forward: 12 for the root mean square (a sum of dh 
 sequence, halved by the square root) + 2 for it and its product, 2 for the weight and the amplitude, 3.6 for the
 angle (a turn rounded to float32 is off by 2^-26, times 2 pi) and its sine, 3 for the two products and their sum:
 24 of |a| + |b| of the pair.  Backward: the rotation, the row's sum of products and the norm, each at most 24.
-The weights' gradient adds up to 340 terms in sequence per element (4 heads, then up to 256 groups, then 64 + 16
-partial sums): 400 of the sum of the terms' magnitudes."""
+The weights' gradient adds up to 400 terms in sequence per element (at most 17 heads, 256 groups, 16 + 64 partial sums
+here): 400 of the sum of the terms' magnitudes."""
 
 from __future__ import annotations
 
