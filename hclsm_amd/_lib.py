@@ -9,6 +9,7 @@ runtime, so device pointers and ``hipStream_t`` handles from torch are valid her
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 
 import torch  # noqa: F401  (must precede the CDLL load, see module docstring)
@@ -121,23 +122,28 @@ class HclsmSlotWeights(ctypes.Structure):
         "w1_n", "w1_n_sum", "w1_n_bias")]
 
 
-class HclsmHeads(ctypes.Structure):
-    """Mirror of the C struct HclsmHeads (include/hclsm_amd.h)."""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "g", "y", "w", "gw", "pos")] +
-                [(n, ctypes.c_int64) for n in ("x_sb", "x_sl", "x_sh", "g_sb", "g_sl", "g_sh", "pos_sb", "pos_sl",
-                                               "B", "L", "H")] +
-                [("w_dtype", ctypes.c_int), ("pos_dtype", ctypes.c_int)])
+# Argument blocks of the entry points that take one by pointer, in the layout of the C structs of the same name
+# (include/hclsm_amd.h).  Packed bytes are passed as they stand: building a ctypes.Structure costs several times as much.
+HEADS_FIELDS = (("x", "g", "y", "w", "gw", "pos"),
+                ("x_sb", "x_sl", "x_sh", "g_sb", "g_sl", "g_sh", "pos_sb", "pos_sl", "B", "L", "H"),
+                ("w_dtype", "pos_dtype"))
+pack_heads = struct.Struct("@6P11q2i").pack
+CROSS_FIELDS = (("q", "k", "v", "g", "out", "out_lo", "lse", "dq", "dk", "dv", "key_pad", "key_lens", "query_lens"),
+                ("q_sb", "q_sl", "q_sh", "k_sb", "k_sl", "k_sh", "v_sb", "v_sl", "v_sh", "g_sb", "g_sl", "g_sh",
+                 "key_pad_sb", "B", "Lq", "Lk", "H", "Hk", "dh"),
+                ("scale", "dtype", "key_lens_dtype", "query_lens_dtype"))
+pack_cross = struct.Struct("@13P19qf3i").pack
 
 
-class HclsmCrossAttention(ctypes.Structure):
-    """Mirror of the C struct HclsmCrossAttention (include/hclsm_amd.h)."""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "g", "out", "lse", "dq", "dk", "dv", "key_pad",
-                                                "key_lens", "query_lens")] +
-                [(n, ctypes.c_int64) for n in ("q_sb", "q_sl", "q_sh", "k_sb", "k_sl", "k_sh", "v_sb", "v_sl", "v_sh",
-                                               "g_sb", "g_sl", "g_sh", "key_pad_sb", "B", "Lq", "Lk", "H", "Hk",
-                                               "dh")] +
-                [("scale", ctypes.c_float), ("dtype", ctypes.c_int), ("key_lens_dtype", ctypes.c_int),
-                 ("query_lens_dtype", ctypes.c_int)])
+def _block(name, pointers, sizes, rest):
+    kinds = lambda n: ctypes.c_float if n == "scale" else ctypes.c_int
+    fields = ([(n, ctypes.c_void_p) for n in pointers] + [(n, ctypes.c_int64) for n in sizes] +
+              [(n, kinds(n)) for n in rest])
+    return type(name, (ctypes.Structure,), {"_fields_": fields, "__doc__": f"Mirror of the C struct {name}."})
+
+
+HclsmHeads = _block("HclsmHeads", *HEADS_FIELDS)
+HclsmCrossAttention = _block("HclsmCrossAttention", *CROSS_FIELDS)
 
 _lib = None
 

@@ -26,7 +26,7 @@ typedef __attribute__((address_space(3))) void ca_lds_void;
 
 struct CaArgs {
   const char *q, *k, *v, *g;        // inputs; gradient of the output
-  char *o, *dq, *dk, *dv;           // contiguous [B, Lq, H, dh] / [B, Lk, Hk, dh]
+  char *o, *olo, *dq, *dk, *dv;     // contiguous [B, Lq, H, dh] / [B, Lk, Hk, dh]
   float* lse;                       // [B, H, Lq] natural logarithm, -inf for rows without keys
   float* delta;                     // [B, H, Lq] sum(g o), written by the dq kernel for the dk, dv kernel
   float* part;                      // partial sums of a split launch
@@ -177,6 +177,17 @@ template <int DT, int DH> struct CaTile {
     }
   }
 };
+
+// Four consecutive elements of the output, and what their rounding dropped where that is wanted.
+template <int DT> __device__ __forceinline__ void ca_store_out(const CaArgs& a, int64_t i, caf4 v) {
+  ca_store4<DT>(a.o, i, v);
+  if constexpr (DT != HCLSM_F32) {
+    if (a.olo != nullptr) {
+      const uint32_t w0 = CaT<DT>::pack2(v[0], v[1]), w1 = CaT<DT>::pack2(v[2], v[3]);
+      ca_store4<DT>(a.olo, i, caf4{v[0] - CaT<DT>::lo(w0), v[1] - CaT<DT>::hi(w0), v[2] - CaT<DT>::lo(w1), v[3] - CaT<DT>::hi(w1)});
+    }
+  }
+}
 
 __device__ __forceinline__ int ca_len(const void* lens, int is64, int64_t b, int most) {
   if (lens == nullptr) return most;

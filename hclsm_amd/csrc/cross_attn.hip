@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(256) ca_join_kernel(const CaArgs a, int tc) {
     const int h = (unit - (int)b * a.Hk) * a.G + hg;
     if (sl == 0 && 4 * c < a.dh) {
       for (int i = 1; i < n; ++i) acc += s_acc[i * tc + c];
-      ca_store4<DT>(a.o, ((b * a.Lq + qi) * a.Hk * a.G + h) * (int64_t)a.dh + 4 * c, acc * inv);
+      ca_store_out<DT>(a, ((b * a.Lq + qi) * a.Hk * a.G + h) * (int64_t)a.dh + 4 * c, acc * inv);
     }
     if (threadIdx.x == 0 && a.lse)
       a.lse[(b * a.Hk * a.G + h) * a.Lq + qi] = sum > 0.f ? (base + __log2f(sum)) * HCLSM_LN2 : sum != sum ? sum : -INFINITY;
@@ -109,7 +109,8 @@ int ca_args(const HclsmCrossAttention* x, int bwd, CaArgs& a) {
   if (rows) {
     if (!ca_near(x->q_sl, x->q_sh, G, esz) || (bwd && !ca_near(x->g_sl, x->g_sh, G, esz))) return HCLSM_ERR_UNSUPPORTED;
     if (!x->q || !x->out || (bwd && (!x->g || !x->dq || !x->lse))) return HCLSM_ERR_NULL;
-    if (!ca_aligned(x->q, x->q_sb, x->q_sl, x->q_sh, esz) || !ca_aligned(x->out, 0, 0, 0, esz)) return HCLSM_ERR_UNSUPPORTED;
+    if (!ca_aligned(x->q, x->q_sb, x->q_sl, x->q_sh, esz) || !ca_aligned(x->out, 0, 0, 0, esz) ||
+        !ca_aligned(x->out_lo, 0, 0, 0, esz)) return HCLSM_ERR_UNSUPPORTED;
     if (bwd && (!ca_aligned(x->g, x->g_sb, x->g_sl, x->g_sh, esz) || !ca_aligned(x->dq, 0, 0, 0, esz)))
       return HCLSM_ERR_UNSUPPORTED;
   }
@@ -123,7 +124,7 @@ int ca_args(const HclsmCrossAttention* x, int bwd, CaArgs& a) {
   for (int code : {x->key_lens_dtype, x->query_lens_dtype})
     if (code != HCLSM_POS_I32 && code != HCLSM_POS_I64) return HCLSM_ERR_DTYPE;
   a.q = (const char*)x->q; a.k = (const char*)x->k; a.v = (const char*)x->v; a.g = (const char*)x->g;
-  a.o = (char*)x->out; a.dq = (char*)x->dq; a.dk = (char*)x->dk; a.dv = (char*)x->dv;
+  a.o = (char*)x->out; a.olo = (char*)x->out_lo; a.dq = (char*)x->dq; a.dk = (char*)x->dk; a.dv = (char*)x->dv;
   a.lse = x->lse;
   a.qsb = x->q_sb; a.qsl = x->q_sl; a.qsh = x->q_sh;
   a.ksb = x->k_sb; a.ksl = x->k_sl; a.ksh = x->k_sh;

@@ -112,7 +112,7 @@ __device__ __forceinline__ void ca_few_store(const CaArgs& a, int64_t ob, const 
       for (int e = 0; e < 4; ++e) v[e] = in ? o[F + (4 * j + e) % W][(4 * j + e) / W] * f : 0.f;
       if (col + 4 * j < a.dh) {
         if (a.nsplit > 1) *reinterpret_cast<caf4*>(a.part + ob + col + 4 * j) = v;
-        else ca_store4<DT>(a.o, ob + col + 4 * j, v);
+        else ca_store_out<DT>(a, ob + col + 4 * j, v);
       }
     }
     ca_few_store<DT, DH, K + 1>(a, ob, o, f, in, g);

@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
       const int64_t ob = ((w.b * a.Lq + qi) * a.Hk * a.G + h) * (int64_t)a.dh;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
-        if (16 * d + 4 * g < a.dh) ca_store4<DT>(a.o, ob + 16 * d + 4 * g, in ? o[t][d] * inv : caf4{0.f, 0.f, 0.f, 0.f});
+        if (16 * d + 4 * g < a.dh) ca_store_out<DT>(a, ob + 16 * d + 4 * g, in ? o[t][d] * inv : caf4{0.f, 0.f, 0.f, 0.f});
     }
   }
 }
@@ -340,12 +340,16 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
     ca_row_frags<DT, DH>(a.q + (w.b * a.qsb + qi * a.qsl + h * a.qsh) * ESZ, g, a.dh, in, fq);
     ca_row_frags<DT, DH>(a.g + (w.b * a.gsb + qi * a.gsl + h * a.gsh) * ESZ, g, a.dh, in, fg);
     ca_row_frags<DT, DH>(a.o + ((w.b * a.Lq + qi) * a.Hk * a.G + h) * (int64_t)a.dh * ESZ, g, a.dh, in, fo);
+    uint4 fl[NC];
+    const bool lo = a.olo != nullptr;
+    ca_row_frags<DT, DH>(a.olo + ((w.b * a.Lq + qi) * a.Hk * a.G + h) * (int64_t)a.dh * ESZ, g, a.dh, in && lo, fl);
     const float ls = in ? a.lse[stat] : -INFINITY;
     lse2[t] = ls == -INFINITY ? INFINITY : ls * HCLSM_LOG2E;      // no key: every weight is exp(-inf)
     float dsum = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       dsum = ca_dot<DT>(fg[c], fo[c], dsum);
+      dsum = ca_dot<DT>(fg[c], fl[c], dsum);
       q[t][c] = ca_frag<DT>(fq[c]);
       go[t][c] = ca_frag<DT>(fg[c]);
     }

@@ -36,6 +36,15 @@ def common_float_dtype(*tensors: torch.Tensor) -> torch.dtype:
     return torch.float32
 
 
+def once(back, ctx, *grads):
+    """back(ctx, *grads), which cannot be differentiated again: where a graph of the gradients is asked for (create_graph),
+    differentiating it raises.  Elsewhere without the wrapper, which costs several us."""
+    if not torch.is_grad_enabled():
+        return back(ctx, *grads)
+    from torch.autograd.function import once_differentiable
+    return once_differentiable(back)(ctx, *grads)
+
+
 _SAME_DEVICE = contextlib.nullcontext()
 
 

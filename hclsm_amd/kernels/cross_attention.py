@@ -10,13 +10,10 @@ batch row, a key padding mask, gradients, and a form for few queries that splits
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
-from torch.autograd.function import once_differentiable
 
 from hclsm_amd import _lib
-from hclsm_amd.kernels._common import on_device, require_gpu
+from hclsm_amd.kernels._common import on_device, once, require_gpu
 from hclsm_amd.kernels.ssm_scan_kernel import _no_node
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -62,72 +59,94 @@ def _rows(t):
     return t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 else t.clone()
 
 
+_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_WORKSPACE: dict = {}       # sizes -> bytes (a function of the sizes alone)
+
+
 def _strides(t):
     sb, sl, sh, _ = t.stride()
     B, L, H, _ = t.shape
     return sb if B > 1 else 0, sl if L > 1 else 0, sh if H > 1 else 0
 
 
-def _struct(q, k, v, out, lse, pad, klens, qlens, scale, g=None, dq=None, dk=None, dv=None):
+def _pack(q, k, v, out, out_lo, lse, masks, scale, g=None, dq=None, dk=None, dv=None):
+    """The packed HclsmCrossAttention of a call."""
+    pad, klens, qlens = masks
     B, Lq, H, dh = q.shape
-    p = _lib.ptr
-    code = lambda t: _lib.POS_I64 if t is not None and t.dtype == torch.int64 else _lib.POS_I32
-    return _lib.HclsmCrossAttention(
-        p(q), p(k), p(v), p(g), p(out), p(lse), p(dq), p(dk), p(dv), p(pad), p(klens), p(qlens), *_strides(q),
-        *_strides(k), *_strides(v), *((0, 0, 0) if g is None else _strides(g)),
-        0 if pad is None else (pad.stride(0) if B > 1 else 0), B, Lq, k.shape[1], H, k.shape[2], dh, scale,
-        _lib.dtype_code(q.dtype), code(klens), code(qlens))
+    p = lambda t: 0 if t is None else t.data_ptr()
+    code = lambda t: _lib.POS_I64 if t is not None and t.dtype is torch.int64 else _lib.POS_I32
+    return _lib.pack_cross(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), p(g), out.data_ptr(), p(out_lo), p(lse), p(dq), p(dk), p(dv), p(pad),
+        p(klens), p(qlens), *_strides(q), *_strides(k), *_strides(v), *((0, 0, 0) if g is None else _strides(g)),
+        pad.stride(0) if pad is not None and B > 1 else 0, B, Lq, k.shape[1], H, k.shape[2], dh, scale, _CODE[q.dtype],
+        code(klens), code(qlens))
 
 
 def _workspace(q, k, backward):
-    B, Lq, H, dh = q.shape
-    n = int(_lib.lib().hclsm_cross_attention_workspace(B, Lq, k.shape[1], H, k.shape[2], dh, _lib.dtype_code(q.dtype),
-                                                       backward))
-    if n < 0:
-        _lib.check(n, "hclsm_cross_attention_workspace")
+    key = (*q.shape, k.shape[1], k.shape[2], q.dtype, backward)
+    n = _WORKSPACE.get(key)
+    if n is None:
+        B, Lq, H, dh = q.shape
+        n = int(_lib.lib().hclsm_cross_attention_workspace(B, Lq, k.shape[1], H, k.shape[2], dh, _CODE[q.dtype], backward))
+        if n < 0:
+            _lib.check(n, "hclsm_cross_attention_workspace")
+        if len(_WORKSPACE) > 4096:
+            _WORKSPACE.clear()
+        _WORKSPACE[key] = n
     return (torch.empty(n, dtype=torch.uint8, device=q.device) if n else None), n
 
 
-def _forward(q, k, v, pad, klens, qlens, scale, want_lse):
+def _like(t):
+    """A new contiguous tensor of t's shape."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _forward(q, k, v, masks, scale, want_lse, want_lo):
     q, k, v = _rows(q), _rows(k), _rows(v)
     B, Lq, H, _ = q.shape
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = _like(q)
+    lo = _like(q) if want_lo else None
     lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device) if want_lse else None
     ws, n = _workspace(q, k, 0)
-    x = _struct(q, k, v, out, lse, pad, klens, qlens, scale)
+    x = _pack(q, k, v, out, lo, lse, masks, scale)
     with on_device(q.device):
-        rc = _lib.lib().hclsm_cross_attention_forward(ctypes.byref(x), _lib.ptr(ws), n, _lib.stream_of(q))
-    _lib.check(rc, "hclsm_cross_attention_forward")
-    return out, lse
+        rc = _lib.lib().hclsm_cross_attention_forward(x, None if ws is None else ws.data_ptr(), n, _lib.stream_of(q))
+    if rc:
+        _lib.check(rc, "hclsm_cross_attention_forward")
+    return out, lse, lo
 
 
-def _backward(q, k, v, out, lse, g, pad, klens, qlens, scale):
-    q, k, v, g = _rows(q), _rows(k), _rows(v), _rows(g.to(q.dtype))
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
+def _backward(q, k, v, out, lo, lse, g, masks, scale):
+    q, k, v, g = _rows(q), _rows(k), _rows(v), _rows(g if g.dtype is q.dtype else g.to(q.dtype))
+    dq, dk, dv = _like(q), _like(k), _like(v)
     ws, n = _workspace(q, k, 1)
-    x = _struct(q, k, v, out, lse, pad, klens, qlens, scale, g, dq, dk, dv)
+    x = _pack(q, k, v, out, lo, lse, masks, scale, g, dq, dk, dv)
     with on_device(q.device):
-        rc = _lib.lib().hclsm_cross_attention_backward(ctypes.byref(x), _lib.ptr(ws), n, _lib.stream_of(q))
-    _lib.check(rc, "hclsm_cross_attention_backward")
+        rc = _lib.lib().hclsm_cross_attention_backward(x, None if ws is None else ws.data_ptr(), n, _lib.stream_of(q))
+    if rc:
+        _lib.check(rc, "hclsm_cross_attention_backward")
     return dq, dk, dv
 
 
 class _CrossAttention(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, q, k, v, pad, klens, qlens, scale):
-        out, lse = _forward(q, k, v, pad, klens, qlens, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, pad, klens, qlens)
+    def forward(ctx, q, k, v, masks, scale):
+        # 16-bit outputs: what their rounding dropped is kept too, for the backward's sum(g out)
+        out, lse, lo = _forward(q, k, v, masks, scale, True, q.dtype is not torch.float32)
+        ctx.save_for_backward(q, k, v, out, lo, lse, *masks)
         ctx.scale = scale
         ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g, _):
-        q, k, v, out, lse, pad, klens, qlens = ctx.saved_tensors
-        return (*_backward(q, k, v, out, lse, g, pad, klens, qlens, ctx.scale), None, None, None, None)
+        return once(_CrossAttention._back, ctx, g)
+
+    @staticmethod
+    def _back(ctx, g):
+        q, k, v, out, lo, lse, *masks = ctx.saved_tensors
+        return (*_backward(q, k, v, out, lo, lse, g, masks, ctx.scale), None, None)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_padding_mask: torch.Tensor | None = None,
@@ -161,7 +180,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_pa
     klens = key_lens if key_lens is None or key_lens.stride(0) == 1 else key_lens.contiguous()
     qlens = query_lens if query_lens is None or query_lens.stride(0) == 1 else query_lens.contiguous()
     if _no_node((q, k, v)):
-        out, lse = _forward(q, k, v, pad, klens, qlens, scale, return_lse)
+        out, lse, _ = _forward(q, k, v, (pad, klens, qlens), scale, return_lse, False)
     else:
-        out, lse = _CrossAttention.apply(q, k, v, pad, klens, qlens, scale)
+        out, lse = _CrossAttention.apply(q, k, v, (pad, klens, qlens), scale)
     return (out, lse) if return_lse else out

@@ -15,14 +15,12 @@ are contiguous and new.  The reference rotates the heads of its vision encoder (
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from hclsm_amd import _lib
-from hclsm_amd.kernels._common import on_device, require_gpu
+from hclsm_amd.kernels._common import on_device, once, require_gpu
 from hclsm_amd.kernels.ssm_scan_kernel import _no_node
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -133,60 +131,73 @@ def _rows(x):
     return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
 
 
+_POS = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64}
+_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _like(x):
+    """A new contiguous tensor of x's shape."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def _heads(x, y, w, pos, g=None, gw=None):
+    """The packed HclsmHeads of one tensor."""
     B, L, H, _ = x.shape
     sb, sl, sh, _ = x.stride()
-    gs = (0, 0, 0) if g is None else g.stride()[:3]
-    ps, pd = (0, 0), 0
+    gb, gl, gh, _ = (0, 0, 0, 0) if g is None else g.stride()
+    pb = pl = pd = pp = 0
     if pos is not None:
-        ps = (0, pos.stride(0)) if pos.dim() == 1 else pos.stride()
-        pd = _lib.POS_I32 if pos.dtype == torch.int32 else _lib.POS_I64
-    return _lib.HclsmHeads(x.data_ptr(), None if g is None else g.data_ptr(), y.data_ptr(),
-                           None if w is None else w.data_ptr(), None if gw is None else gw.data_ptr(),
-                           None if pos is None else pos.data_ptr(), sb, sl, sh, *gs, *ps, B, L, H,
-                           0 if w is None else _lib.dtype_code(w.dtype), pd)
+        pb, pl = (0, pos.stride(0)) if pos.dim() == 1 else pos.stride()
+        pd, pp = _POS[pos.dtype], pos.data_ptr()
+    return _lib.pack_heads(x.data_ptr(), 0 if g is None else g.data_ptr(), y.data_ptr(), 0 if w is None else w.data_ptr(),
+                           0 if gw is None else gw.data_ptr(), pp, sb, sl, sh, gb, gl, gh, pb, pl, B, L, H,
+                           0 if w is None else _CODE[w.dtype], pd)
 
 
 def _plan_args(plan, back=False):
     """rot, layout, device pointer of the turns, amplitude."""
     if plan is None:
         return 0, _lib.ROTARY_HALF, None, 1.0
-    t = plan._turns
-    return plan.rot_dim, plan._code, t.data_ptr() + (plan.rot_dim // 2 * 8 if back else 0), plan.amplitude
+    return plan.rot_dim, plan._code, plan._turns.data_ptr() + (plan.rot_dim // 2 * 8 if back else 0), plan.amplitude
 
 
 def _forward(tensors, plan, eps, norm, back=False):
     """tensors: [(x, w, positions)], one or two; returns the outputs."""
-    xs = [_rows(x) for x, _, _ in tensors]
-    ys = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
-    hs = [_heads(x, y, w, pos) for x, y, (_, w, pos) in zip(xs, ys, tensors)]
+    ys, hs = [], []
+    for x, w, pos in tensors:
+        x = _rows(x)
+        y = _like(x)
+        ys.append(y)
+        hs.append((_heads(x, y, w, pos), x))        # x: a copy has to live until the launch
     rot, layout, turns, amp = _plan_args(plan, back)
-    x = xs[0]
+    x = hs[0][1]
     with on_device(x.device):
-        rc = _lib.lib().hclsm_norm_rotary_forward(
-            ctypes.byref(hs[0]), ctypes.byref(hs[1]) if len(hs) > 1 else None, x.shape[3], rot, layout, turns, amp,
-            eps, norm, _lib.dtype_code(x.dtype), _lib.stream_of(x))
-    _lib.check(rc, "hclsm_norm_rotary_forward")
+        rc = _lib.lib().hclsm_norm_rotary_forward(hs[0][0], hs[1][0] if len(hs) > 1 else None, x.shape[3], rot, layout,
+                                                  turns, amp, eps, norm, _CODE[x.dtype], _lib.stream_of(x))
+    if rc:
+        _lib.check(rc, "hclsm_norm_rotary_forward")
     return ys
 
 
 def _norm_backward(tensors, plan, eps):
     """tensors: [(x, w, positions, g, want gradient of w)], one or two; returns [(gx, gw or None)]."""
-    xs = [_rows(t[0]) for t in tensors]
-    gs = [_rows(t[3].to(t[0].dtype)) for t in tensors]
-    out = [(torch.empty(x.shape, dtype=x.dtype, device=x.device),
-            torch.empty_like(t[1]) if t[1] is not None and t[4] else None) for x, t in zip(xs, tensors)]
-    hs = [_heads(x, gx, t[1], t[2], g, gw) for x, g, (gx, gw), t in zip(xs, gs, out, tensors)]
+    out, hs = [], []
+    for x, w, pos, g, want in tensors:
+        x = _rows(x)
+        g = _rows(g if g.dtype is x.dtype else g.to(x.dtype))
+        gx, gw = _like(x), torch.empty_like(w) if want and w is not None else None
+        out.append((gx, gw))
+        hs.append((_heads(x, gx, w, pos, g, gw), x, g))
     rot, layout, turns, amp = _plan_args(plan)
-    x = xs[0]
+    x = hs[0][1]
     L = _lib.lib()
-    wsb = int(L.hclsm_norm_rotary_backward_workspace(x.shape[3], len(hs)))
+    wsb = L.hclsm_norm_rotary_backward_workspace(x.shape[3], len(hs))
     ws = torch.empty(wsb, dtype=torch.uint8, device=x.device)
     with on_device(x.device):
-        rc = L.hclsm_norm_rotary_backward(
-            ctypes.byref(hs[0]), ctypes.byref(hs[1]) if len(hs) > 1 else None, x.shape[3], rot, layout, turns, amp,
-            eps, _lib.dtype_code(x.dtype), _lib.ptr(ws), wsb, _lib.stream_of(x))
-    _lib.check(rc, "hclsm_norm_rotary_backward")
+        rc = L.hclsm_norm_rotary_backward(hs[0][0], hs[1][0] if len(hs) > 1 else None, x.shape[3], rot, layout, turns,
+                                          amp, eps, _CODE[x.dtype], ws.data_ptr(), wsb, _lib.stream_of(x))
+    if rc:
+        _lib.check(rc, "hclsm_norm_rotary_backward")
     return out
 
 
@@ -201,10 +212,15 @@ class _Rotary(torch.autograd.Function):
         return _forward([(x, None, positions)], plan, 0.0, 0)[0]
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        return once(_Rotary._back, ctx, g)
+
+    @staticmethod
+    def _back(ctx, g):
         (positions,) = ctx.saved_tensors
-        return _forward([(g.to(ctx.dtype), None, positions)], ctx.plan, 0.0, 0, back=True)[0], None, None
+        if g.dtype is not ctx.dtype:
+            g = g.to(ctx.dtype)
+        return _forward([(g, None, positions)], ctx.plan, 0.0, 0, back=True)[0], None, None
 
 
 def rotary_embedding(x: torch.Tensor, plan: RotaryPlan, positions: torch.Tensor | None = None) -> torch.Tensor:
@@ -231,8 +247,11 @@ class _QKNormRotary(torch.autograd.Function):
         return (ys[0], ys[1] if k is not None else None)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gq, gk):
+        return once(_QKNormRotary._back, ctx, gq, gk)
+
+    @staticmethod
+    def _back(ctx, gq, gk):
         q, k, wq, wk, pos, kpos = ctx.saved_tensors
         need = ctx.needs_input_grad
         grads = [None] * 8

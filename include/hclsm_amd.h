@@ -671,6 +671,9 @@ typedef struct HclsmCrossAttention {
   const void* v;       /* [B, Lk, Hk, dh] */
   const void* g;       /* backward: gradient of out, [B, Lq, H, dh] */
   void* out;           /* contiguous [B, Lq, H, dh]: written by the forward, read by the backward */
+  void* out_lo;        /* as out, nullable: the forward writes what rounding out to `dtype` dropped, rounded to `dtype`;
+                          the backward adds it to out in sum(g out) (without it that sum is off by up to half a step of
+                          out, which matters where the scores' gradients are small next to it) */
   float* lse;          /* [B, H, Lq]: written by the forward (nullable there), read by the backward */
   void* dq;            /* backward: contiguous [B, Lq, H, dh] */
   void* dk;            /* backward: contiguous [B, Lk, Hk, dh] */
