@@ -249,20 +249,28 @@ __device__ __forceinline__ void ca_range(int n, int nsplit, int split, int step,
   end = e < n ? (int)e : n;
 }
 
-// How a forward is launched, a function of the sizes alone (the workspace is sized by the same rule).
+// How a call is launched, a function of the sizes alone (the workspace is sized by the same rules).
 struct CaPlan {
-  int few;        // 0: tiles of many rows; 1, 2: 16 or 32 rows per workgroup of ca_few_kernel
-  int nsplit;     // workgroups that share a unit's keys; their results are joined by ca_join_kernel
+  int few;        // 0: tiles of many rows; 1, 2: at most 16 or 32 rows of a unit, ca_few_kernel (backward: ca_few_bwd_kernel)
+  int nsplit;     // workgroups that share a unit's keys (out, dq); their results are joined by ca_join / ca_sum
+  int nrows;      // backward: workgroups that share a unit's rows (dk, dv)
 };
 constexpr int CA_MAX_SPLIT = 256;
-// Rows (in bytes, padded head) up to which ca_few_kernel is built for 16 and for 32 rows: its step of keys and values, the
-// next one, the accumulators and the queries all live in registers, and longer heads would spill.
-constexpr int CA_FEW1_BYTES = 512, CA_FEW2_BYTES = 256;
+// Rows (in bytes, padded head) up to which ca_few_kernel is built for 16 and for 32 rows, and ca_few_bwd_kernel: a
+// step's keys and values, the accumulators and the queries all live in registers, and longer heads would spill.
+constexpr int CA_FEW1_BYTES = 512, CA_FEW2_BYTES = 256, CA_FEW_BWD_BYTES = 256;
 constexpr int64_t ca_padded_dh(int64_t dh) {
   return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : dh <= 128 ? 128 : dh <= 192 ? 192 : 256;
 }
+// Rows (or keys) of a workgroup's tile: 128, or 64 where there are no more or the operands are too wide for two 16-row
+// tiles per wave.
+constexpr int64_t ca_tile_rows(int64_t n, int64_t bytes) { return bytes <= 256 && n > 64 ? 128 : 64; }
 CaPlan ca_forward_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t dh, int dtype);
+CaPlan ca_backward_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t dh, int dtype);
+int64_t ca_backward_bytes(const CaPlan& p, int64_t B, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t dh);
+// out = partial outputs joined by their log-sums; sums of partial dq (keys = 0) or of dk and dv (keys = 1)
 int ca_join(const CaArgs& a, int dtype, hipStream_t st);
+int ca_sum(const CaArgs& a, int keys, int dtype, hipStream_t st);
 
 // Host side: one launch per (element type, padded head size) is picked in cross_attn.hip.
 int ca_forward_f32(CaArgs a, int64_t batch, void* ws, int64_t ws_bytes, hipStream_t st);

@@ -1,22 +1,51 @@
 // Cross attention: argument checks and dispatch by element type.
 #include "cross_attn.h"
 
-#include <cstdlib>
 namespace hclsm {
 
+namespace {
+
+// Workgroups that share a unit's n keys or rows: as many as fill `slots` workgroups, of `least` each or more.
+int ca_split(int64_t workgroups, int64_t slots, int64_t n, int64_t least) {
+  int64_t s = workgroups > 0 ? slots / workgroups : 1;
+  s = s > n / least ? n / least : s;
+  return (int)(s < 1 ? 1 : s > CA_MAX_SPLIT ? CA_MAX_SPLIT : s);
+}
+
+int64_t ca_row_bytes(int64_t dh, int dtype) { return ca_padded_dh(dh) * (dtype == HCLSM_F32 ? 4 : 2); }
+
+}  // namespace
+
 CaPlan ca_forward_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t dh, int dtype) {
-  const int64_t rows = Lq * G, units = B * Hk;
-  CaPlan p{0, 1};
-  const int64_t bytes = ca_padded_dh(dh) * (dtype == HCLSM_F32 ? 4 : 2);
+  const int64_t rows = Lq * G, units = B * Hk, bytes = ca_row_bytes(dh, dtype);
+  CaPlan p{0, 1, 1};
   p.few = rows <= 16 && bytes <= CA_FEW1_BYTES ? 1 : rows <= 32 && bytes <= CA_FEW2_BYTES ? 2 : 0;
-  if (getenv("CA_FEW")) p.few = atoi(getenv("CA_FEW"));
-  const int64_t per = p.few ? 16 * p.few : bytes <= 256 ? 128 : 64;
-  const int64_t wgs = units * ((rows + per - 1) / per);
-  const int64_t target = getenv("CA_TARGET") ? atoi(getenv("CA_TARGET")) : 1024, least = getenv("CA_LEAST") ? atoi(getenv("CA_LEAST")) : 256;
-  int64_t n = wgs > 0 ? target / wgs : 1;
-  if (n > Lk / least) n = Lk / least;
-  p.nsplit = (int)(n < 1 ? 1 : n > CA_MAX_SPLIT ? CA_MAX_SPLIT : n);
+  const int64_t per = p.few ? 16 * p.few : ca_tile_rows(rows, bytes);
+  // workgroups that are on the chip at once (registers: 4 to 1 a CU for few rows, 3 to 2 for many)
+  const int64_t slots = p.few ? (bytes <= 64 ? 1024 : bytes <= 128 ? 768 : bytes <= 192 ? 512 : 256) : bytes <= 128 ? 768 : 512;
+  p.nsplit = ca_split(units * ((rows + per - 1) / per), slots, Lk, p.few ? 256 : 128);
   return p;
+}
+
+CaPlan ca_backward_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t dh, int dtype) {
+  const int64_t rows = Lq * G, units = B * Hk, bytes = ca_row_bytes(dh, dtype);
+  CaPlan p{0, 1, 1};
+  if (rows <= 32 && bytes <= CA_FEW_BWD_BYTES) {
+    p.few = 2;
+    p.nsplit = ca_split(units, 512, Lk, 256);
+    return p;
+  }
+  const int64_t slots = 512, pq = ca_tile_rows(rows, bytes), pk = ca_tile_rows(Lk, bytes);
+  p.nsplit = ca_split(units * ((rows + pq - 1) / pq), slots, Lk, 128);
+  p.nrows = ca_split(units * ((Lk + pk - 1) / pk), slots, rows, 128);
+  return p;
+}
+
+int64_t ca_backward_bytes(const CaPlan& p, int64_t B, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t dh) {
+  const int64_t units = B * Hk, rows = Lq * G;
+  const int64_t dq = p.nsplit > 1 ? p.nsplit * units * rows * dh * 4 : 0;
+  if (p.few) return dq;
+  return (units * rows * 4 + 255) / 256 * 256 + dq + (p.nrows > 1 ? 2 * p.nrows * units * Lk * dh * 4 : 0);
 }
 
 // A row's partial results joined: weights exp2(lse_s - lse), one workgroup per row, TC lanes of four columns each and
@@ -59,7 +88,47 @@ __global__ void __launch_bounds__(256) ca_join_kernel(const CaArgs a, int tc) {
   }
 }
 
+// The same with one thread per four columns of a row, for many rows of few splits.
+template <int DT>
+__global__ void __launch_bounds__(256) ca_join_rows_kernel(const CaArgs a) {
+  const int all = a.Lq * a.G;
+  const uint32_t c4 = (uint32_t)a.dh / 4;
+  const int64_t rows = (int64_t)a.units * all;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * c4; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / c4;
+    const int col = (int)(i - row * c4) * 4;
+    float top = -INFINITY, sum = 0.f;
+    for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, a.part_lse[s * rows + row]);
+    const float base = top == -INFINITY ? 0.f : top;
+    caf4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < a.nsplit; ++s) {
+      const float f = fast_exp2(a.part_lse[s * rows + row] - base);
+      sum += f;
+      acc += *reinterpret_cast<const caf4*>(a.part + (s * rows + row) * a.dh + col) * f;
+    }
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    const int unit = (int)(row / all), r = (int)(row - (int64_t)unit * all);
+    int qi, hg;
+    ca_row(a, r, qi, hg);
+    const int64_t b = unit / a.Hk;
+    const int h = (unit - (int)b * a.Hk) * a.G + hg;
+    ca_store_out<DT>(a, ((b * a.Lq + qi) * a.Hk * a.G + h) * (int64_t)a.dh + col, acc * inv);
+    if (col == 0 && a.lse)
+      a.lse[(b * a.Hk * a.G + h) * a.Lq + qi] = sum > 0.f ? (base + __log2f(sum)) * HCLSM_LN2 : sum != sum ? sum : -INFINITY;
+  }
+}
+
 int ca_join(const CaArgs& a, int dtype, hipStream_t st) {
+  if (a.nsplit <= 8) {
+    const int64_t n = (int64_t)a.units * a.Lq * a.G * (a.dh / 4);
+    const unsigned grid = (unsigned)((n + 255) / 256 < 8192 ? (n + 255) / 256 : 8192);
+    if (dtype == HCLSM_F32) hipLaunchKernelGGL(ca_join_rows_kernel<HCLSM_F32>, dim3(grid), dim3(256), 0, st, a);
+    else if (dtype == HCLSM_BF16) hipLaunchKernelGGL(ca_join_rows_kernel<HCLSM_BF16>, dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(ca_join_rows_kernel<HCLSM_F16>, dim3(grid), dim3(256), 0, st, a);
+    HCLSM_LAUNCH_CHECK();
+    return 0;
+  }
   const int64_t rows = (int64_t)a.units * a.Lq * a.G;
   int tc = 2;
   while (4 * tc < a.dh) tc *= 2;
@@ -67,6 +136,43 @@ int ca_join(const CaArgs& a, int dtype, hipStream_t st) {
   if (dtype == HCLSM_F32) hipLaunchKernelGGL(ca_join_kernel<HCLSM_F32>, dim3(grid), dim3(256), 0, st, a, tc);
   else if (dtype == HCLSM_BF16) hipLaunchKernelGGL(ca_join_kernel<HCLSM_BF16>, dim3(grid), dim3(256), 0, st, a, tc);
   else hipLaunchKernelGGL(ca_join_kernel<HCLSM_F16>, dim3(grid), dim3(256), 0, st, a, tc);
+  HCLSM_LAUNCH_CHECK();
+  return 0;
+}
+
+// Partial sums of a split backward added in the splits' order, four columns to a thread.
+template <int DT>
+__global__ void __launch_bounds__(256) ca_sum_kernel(const CaArgs a, int keys) {
+  const int rows = keys ? a.Lk : a.Lq * a.G;
+  const uint32_t c4 = (uint32_t)a.dh / 4;
+  const int64_t n = (int64_t)a.units * rows * c4, half = n * 4 * a.nsplit;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n * (keys ? 2 : 1); i += (int64_t)gridDim.x * 256) {
+    const bool second = i >= n;
+    const int64_t e = second ? i - n : i;
+    const float* p = a.part + (second ? half : 0) + e * 4;
+    caf4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < a.nsplit; ++k) s += *reinterpret_cast<const caf4*>(p + (int64_t)k * n * 4);
+    const int64_t row = e / c4;
+    const int col = (int)(e - row * c4) * 4, unit = (int)(row / rows), r = (int)(row - (int64_t)unit * rows);
+    const int64_t b = unit / a.Hk;
+    const int hk = unit - (int)b * a.Hk;
+    if (keys) {
+      ca_store4<DT>(second ? a.dv : a.dk, ((b * a.Lk + r) * a.Hk + hk) * (int64_t)a.dh + col, s);
+    } else {
+      int qi, hg;
+      ca_row(a, r, qi, hg);
+      ca_store4<DT>(a.dq, ((b * a.Lq + qi) * a.Hk * a.G + hk * a.G + hg) * (int64_t)a.dh + col, s);
+    }
+  }
+}
+
+int ca_sum(const CaArgs& a, int keys, int dtype, hipStream_t st) {
+  const int64_t n = (int64_t)a.units * (keys ? 2 * (int64_t)a.Lk : (int64_t)a.Lq * a.G) * (a.dh / 4);
+  const unsigned grid = (unsigned)((n + 255) / 256 < 4096 ? (n + 255) / 256 : 4096);
+  if (dtype == HCLSM_F32) hipLaunchKernelGGL(ca_sum_kernel<HCLSM_F32>, dim3(grid), dim3(256), 0, st, a, keys);
+  else if (dtype == HCLSM_BF16) hipLaunchKernelGGL(ca_sum_kernel<HCLSM_BF16>, dim3(grid), dim3(256), 0, st, a, keys);
+  else hipLaunchKernelGGL(ca_sum_kernel<HCLSM_F16>, dim3(grid), dim3(256), 0, st, a, keys);
   HCLSM_LAUNCH_CHECK();
   return 0;
 }
@@ -159,8 +265,9 @@ extern "C" int64_t hclsm_cross_attention_workspace(int64_t B, int64_t Lq, int64_
                                                    int dtype, int backward) {
   using namespace hclsm;
   if (int rc = ca_sizes(B, Lq, Lk, H, Hk, dh, dtype)) return rc;
-  if (backward) return (B * Lq * H * 4 + 255) / 256 * 256;
-  if (B == 0 || Lq == 0 || H == 0) return 0;
+  if (B == 0 || Hk == 0) return 0;
+  if (backward) return ca_backward_bytes(ca_backward_plan(B, Lq, Lk, Hk, H / Hk, dh, dtype), B, Lq, Lk, Hk, H / Hk, dh);
+  if (Lq == 0 || H == 0) return 0;
   const CaPlan p = ca_forward_plan(B, Lq, Lk, Hk, H / Hk, dh, dtype);
   return p.nsplit > 1 ? p.nsplit * B * Lq * H * (dh + 1) * 4 : 0;
 }

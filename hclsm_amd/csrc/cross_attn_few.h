@@ -2,7 +2,7 @@
 // reading the keys and values is the work.
 #pragma once
 
-#include "cross_attn.h"
+#include "cross_attn_stage.h"
 
 namespace hclsm {
 
@@ -63,7 +63,7 @@ template <int DT, int DH> struct CaStep {
         load_v<0>(a, rv, 16 * t + 4 * g + r < n ? voff : NONE, (16 * t + r) * (int)(a.vsl * ESZ), li, v[4 * t + r]);
   }
   template <int K>
-  __device__ __forceinline__ void load_v(const CaArgs& a, __amdgpu_buffer_rsrc_t rv, uint32_t off, int so, int li, uint32_t* w) {
+  static __device__ __forceinline__ void load_v(const CaArgs& a, __amdgpu_buffer_rsrc_t rv, uint32_t off, int so, int li, uint32_t* w) {
     if constexpr (K < CaGroups<DT, DH>::N) {
       constexpr int F = CaGroups<DT, DH>::first(K), W = CaGroups<DT, DH>::width(K), WORDS = W * ESZ / 4;
       const int col = 16 * F + W * li;
@@ -82,7 +82,8 @@ template <int DT, int DH> struct CaStep {
     }
   }
   // second operand of tile nt: its column of each of the lane's keys
-  __device__ __forceinline__ typename A::Frag vfrag(int nt) const {
+  __device__ __forceinline__ typename A::Frag vfrag(int nt) const { return column(v, nt); }
+  static __device__ __forceinline__ typename A::Frag column(const uint32_t (*v)[VW], int nt) {
     if constexpr (DT == HCLSM_F32) {
       return caf4{__uint_as_float(v[0][nt]), __uint_as_float(v[1][nt]), __uint_as_float(v[2][nt]), __uint_as_float(v[3][nt])};
     } else {
@@ -98,24 +99,21 @@ template <int DT, int DH> struct CaStep {
   }
 };
 
-// Result of a row: in group K the lane holds columns c0 + 4 W g + W r + nt of tile nt, element r.
-template <int DT, int DH, int K>
-__device__ __forceinline__ void ca_few_store(const CaArgs& a, int64_t ob, const caf4* o, float f, bool in, int g) {
+// Result of a row: in group K the lane holds columns c0 + 4 W g + W r + nt of tile nt, element r.  put(column, four values).
+template <int DT, int DH, int K = 0, typename F>
+__device__ __forceinline__ void ca_few_store(int dh, const caf4* o, float f, bool in, int g, F put) {
   using Gr = CaGroups<DT, DH>;
   if constexpr (K < Gr::N) {
-    constexpr int F = Gr::first(K), W = Gr::width(K);
-    const int col = 16 * F + 4 * W * g;
+    constexpr int F0 = Gr::first(K), W = Gr::width(K);
+    const int col = 16 * F0 + 4 * W * g;
 #pragma unroll
     for (int j = 0; j < W; ++j) {       // four columns at a time: elements 4j .. 4j + 3 of (r, nt) in order
       caf4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = in ? o[F + (4 * j + e) % W][(4 * j + e) / W] * f : 0.f;
-      if (col + 4 * j < a.dh) {
-        if (a.nsplit > 1) *reinterpret_cast<caf4*>(a.part + ob + col + 4 * j) = v;
-        else ca_store_out<DT>(a, ob + col + 4 * j, v);
-      }
+      for (int e = 0; e < 4; ++e) v[e] = in ? o[F0 + (4 * j + e) % W][(4 * j + e) / W] * f : 0.f;
+      if (col + 4 * j < dh) put(col + 4 * j, v);
     }
-    ca_few_store<DT, DH, K + 1>(a, ob, o, f, in, g);
+    ca_few_store<DT, DH, K + 1>(dh, o, f, in, g, put);
   }
 }
 
@@ -315,7 +313,266 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
       if (a.nsplit > 1) a.part_lse[pr] = ls2;
       else if (a.lse) a.lse[(w.b * a.Hk * a.G + h) * a.Lq + qi] = ls2 * HCLSM_LN2;
     }
-    ca_few_store<DT, DH, 0>(a, ob, o[u], in ? inv : 0.f, in, g);
+    ca_few_store<DT, DH>(a.dh, o[u], inv, in, g, [&](int col, caf4 v) {
+      if (a.nsplit > 1) *reinterpret_cast<caf4*>(a.part + ob + col) = v;
+      else ca_store_out<DT>(a, ob + col, v);
+    });
+  }
+}
+
+// Gradients of at most 32 rows of a unit in one pass over its keys: all rows are at hand, so a key's dk and dv are whole
+// as soon as the key has been read, and only dq is summed over the keys (over the waves and, when the keys are
+// split over workgroups, by ca_sum_kernel).  Both orientations of the scores are formed, S^T (a lane per row) for
+// dQ^T = K^T ds^T and S (a lane per key) for dV^T = g^T p and dK^T = Q^T ds: the key's operand registers serve both, and
+// moving ds between the lanes would cost more than the second product.  What bounds it: reading q, g, out and k, v once
+// and writing dq, dk, dv.
+template <int DT, int DH, int NW>
+__global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
+  using A = CaT<DT>;
+  using Frag = typename A::Frag;
+  using Tile = CaTile<DT, DH>;
+  using Step = CaStep<DT, DH>;
+  constexpr int NT = 64 * NW, QT = 2, R = 16 * QT, NC = DH / A::KS, ND = DH / 16, NPT = A::NPT, SK = Step::SK;
+  constexpr int ESZ = (int)sizeof(typename A::T), VW = Step::VW, RU = QT / NPT;
+  using Stage = CaStage<DT, DH, NT, R>;
+  __shared__ __attribute__((aligned(16))) char tq[Stage::BYTES];
+  __shared__ __attribute__((aligned(16))) char tg[Stage::BYTES];
+  __shared__ __attribute__((aligned(16))) float stat[2 * R];       // log-sums (log2), negated deltas
+  __shared__ caf4 s_dq[NW / 2][QT][ND][64];
+
+  CaWork w;
+  if (!ca_work(a, w)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
+  int k0, k1;
+  ca_range(a.Lk, a.nsplit, w.split, SK * NW, k0, k1);        // every key: dk and dv are written for all of them
+  const char* kp = a.k + (w.b * a.ksb + w.hk * a.ksh) * ESZ;
+  const char* vp = a.v + (w.b * a.vsb + w.hk * a.vsh) * ESZ;
+  const uint8_t* pad = a.pad ? a.pad + w.b * a.psb : nullptr;
+  const int h0 = w.hk * a.G;
+
+  const uint32_t koff = (uint32_t)li * (uint32_t)(a.ksl * ESZ) + 16 * g, voff = (uint32_t)li * (uint32_t)(a.vsl * ESZ) + 16 * g;
+  const uint32_t coff = (uint32_t)(4 * g) * (uint32_t)(a.ksl * ESZ);
+  constexpr uint32_t NONE = 0xffffffffu;
+  uint4 k[NPT][NC], v[NPT][NC];       // a step's keys and values along their rows, and the keys by column
+  uint32_t kc[NPT * 4][VW];
+  uint8_t flag = 0;
+  auto load = [&](int t0) __attribute__((always_inline)) {
+    const int n = w.keys - t0;
+    flag = pad != nullptr && lane < SK && lane < n ? pad[t0 + lane] : (uint8_t)0;
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + t0 * a.ksl * ESZ), 0, 0x7fffffff, kRawBufferWord3);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)(vp + t0 * a.vsl * ESZ), 0, 0x7fffffff, kRawBufferWord3);
+#pragma unroll
+    for (int p = 0; p < NPT; ++p) {
+      const bool in = 16 * p + li < n;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const bool have = in && (4 * c + g) * A::EPC < a.dh;
+        k[p][c] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+            rk, (int)(have ? koff + 64 * c : NONE), 16 * p * (int)(a.ksl * ESZ), 0));
+        v[p][c] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+            rv, (int)(have ? voff + 64 * c : NONE), 16 * p * (int)(a.vsl * ESZ), 0));
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < NPT; ++p)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        Step::template load_v<0>(a, rk, 16 * p + 4 * g + r < n ? coff : NONE, (16 * p + r) * (int)(a.ksl * ESZ), li, kc[4 * p + r]);
+  };
+
+  Stage sq, sg;
+  sq.init_rows(a, a.qsl, a.qsh, 0, R);
+  sg.init_rows(a, a.gsl, a.gsh, 0, R);
+  sq.load(a.q + (w.b * a.qsb + h0 * a.qsh) * ESZ, w.rows, tq, wave);
+  sg.load(a.g + (w.b * a.gsb + h0 * a.gsh) * ESZ, w.rows, tg, wave);
+  if (k0 + wave * SK < k1) load(k0 + wave * SK);      // on their way while the rows are prepared
+  ca_wait_vmem();
+  __syncthreads();
+  Frag q[QT][NC], go[QT][NC];
+#pragma unroll
+  for (int t = 0; t < QT; ++t)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) { q[t][c] = Tile::frag(tq, 16 * t, c, li, g); go[t][c] = Tile::frag(tg, 16 * t, c, li, g); }
+  static_assert(NW >= QT, "a wave per tile of rows");
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    if (wave != t) continue;
+    const int r = 16 * t + li;
+    const bool in = r < w.rows;
+    int qi, hg;
+    ca_row(a, in ? r : 0, qi, hg);
+    const int64_t ob = ((w.b * a.Lq + qi) * a.Hk * a.G + h0 + hg) * (int64_t)a.dh * ESZ;
+    uint4 fo[NC], fl[NC];
+    ca_row_frags<DT, DH>(a.o + ob, g, a.dh, in, fo);
+    ca_row_frags<DT, DH>(a.olo + ob, g, a.dh, in && a.olo != nullptr, fl);
+    float d = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      d = ca_dot<DT>(__builtin_bit_cast(uint4, go[t][c]), fo[c], d);
+      d = ca_dot<DT>(__builtin_bit_cast(uint4, go[t][c]), fl[c], d);
+    }
+    d = rows4_sum(d);
+    const float ls = in ? a.lse[(w.b * a.Hk * a.G + h0 + hg) * a.Lq + qi] : -INFINITY;
+    if (g == 0) {
+      stat[r] = ls == -INFINITY ? INFINITY : ls * HCLSM_LOG2E;
+      stat[R + r] = -d;
+    }
+  }
+  __syncthreads();
+  float lse2[QT];
+  caf4 nd[QT], lsr[QT], ndr[QT];        // of row li; of rows 4g .. 4g + 3
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    lse2[t] = stat[16 * t + li];
+    const float d = stat[R + 16 * t + li];
+    nd[t] = caf4{d, d, d, d};
+    lsr[t] = *reinterpret_cast<const caf4*>(stat + 16 * t + 4 * g);
+    ndr[t] = *reinterpret_cast<const caf4*>(stat + R + 16 * t + 4 * g);
+  }
+
+  caf4 dq[QT][ND];
+#pragma unroll
+  for (int t = 0; t < QT; ++t)
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dq[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
+
+  for (int t0 = k0 + wave * SK; t0 < k1; t0 += SK * NW) {
+    const int n = w.keys - t0;                                      // keys there are from t0 on
+    const uint32_t live = (uint32_t)__ballot(lane < SK && lane < n && flag == 0);
+    const bool full = live == (SK == 32 ? 0xffffffffu : 0xffffu);
+    if (pad != nullptr && !full) {
+#pragma unroll
+      for (int p = 0; p < NPT; ++p)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!(live >> (16 * p + 4 * g + r) & 1)) {
+#pragma unroll
+            for (int i = 0; i < VW; ++i) kc[4 * p + r][i] = 0;
+          }
+    }
+
+    // dq: a lane per row
+    {
+      caf4 s[QT][NPT], dp[QT][NPT];
+#pragma unroll
+      for (int p = 0; p < NPT; ++p) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          s[t][p] = caf4{0.f, 0.f, 0.f, 0.f};
+          dp[t][p] = nd[t];
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            s[t][p] = A::mma(ca_frag<DT>(k[p][c]), q[t][c], s[t][p]);
+            dp[t][p] = A::mma(ca_frag<DT>(v[p][c]), go[t][c], dp[t][p]);
+          }
+      }
+      Frag ds[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+#pragma unroll
+        for (int p = 0; p < NPT; ++p)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            dp[t][p][r] *= fast_exp2(s[t][p][r] * a.scale_log2 - lse2[t]);
+            if (!full) dp[t][p][r] = live >> (16 * p + 4 * g + r) & 1 ? dp[t][p][r] : 0.f;
+          }
+        ds[t] = ca_pack<DT>(dp[t]);
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const Frag f = Step::column(kc, d);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) dq[t][d] = A::mma(f, ds[t], dq[t][d]);
+      }
+    }
+    // dk, dv: a lane per key; a key that is not live spoils no column but its own, which is written as zeros
+    Frag p2[NPT][RU], ds2[NPT][RU];
+#pragma unroll
+    for (int p = 0; p < NPT; ++p) {
+      caf4 s[QT], dp[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        s[t] = caf4{0.f, 0.f, 0.f, 0.f};
+        dp[t] = ndr[t];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          s[t] = A::mma(q[t][c], ca_frag<DT>(k[p][c]), s[t]);
+          dp[t] = A::mma(go[t][c], ca_frag<DT>(v[p][c]), dp[t]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[t][r] = fast_exp2(s[t][r] * a.scale_log2 - lsr[t][r]);
+          dp[t][r] *= s[t][r];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < RU; ++u) { p2[p][u] = ca_pack<DT>(&s[u * NPT]); ds2[p][u] = ca_pack<DT>(&dp[u * NPT]); }
+    }
+    if (t0 + SK * NW < k1) load(t0 + SK * NW);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      caf4 dk[NPT], dv[NPT];
+#pragma unroll
+      for (int p = 0; p < NPT; ++p) dk[p] = dv[p] = caf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < RU; ++u) {
+        const Frag fg = Tile::frag_t(tg, 16 * NPT * u, d, li, g);
+        const Frag fq = Tile::frag_t(tq, 16 * NPT * u, d, li, g);
+#pragma unroll
+        for (int p = 0; p < NPT; ++p) {
+          dv[p] = A::mma(fg, p2[p][u], dv[p]);
+          dk[p] = A::mma(fq, ds2[p][u], dk[p]);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < NPT; ++p) {
+        const int key = t0 + 16 * p + li;
+        if (key < k1 && 16 * d + 4 * g < a.dh) {
+          const bool in = live >> (16 * p + li) & 1;
+          const caf4 zero = {0.f, 0.f, 0.f, 0.f};
+          const int64_t i = ((w.b * a.Lk + key) * a.Hk + w.hk) * (int64_t)a.dh + 16 * d + 4 * g;
+          ca_store4<DT>(a.dk, i, in ? dk[p] * a.scale : zero);
+          ca_store4<DT>(a.dv, i, in ? dv[p] : zero);
+        }
+      }
+    }
+  }
+
+  // dq of the waves, added in a fixed order
+#pragma unroll
+  for (int h = NW / 2; h >= 1; h >>= 1) {
+    if (wave >= h && wave < 2 * h) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) s_dq[wave - h][t][d][lane] = dq[t][d];
+    }
+    __syncthreads();
+    if (wave < h) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dq[t][d] += s_dq[wave][t][d][lane];
+    }
+    __syncthreads();
+  }
+  if (wave != 0) return;
+  const int all = a.Lq * a.G;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = 16 * t + li;
+    if (r >= all) continue;
+    int qi, hg;
+    ca_row(a, r, qi, hg);
+    const int64_t ob = a.nsplit > 1 ? (((int64_t)w.split * a.units + w.unit) * all + r) * a.dh
+                                    : ((w.b * a.Lq + qi) * a.Hk * a.G + h0 + hg) * (int64_t)a.dh;
+    ca_few_store<DT, DH>(a.dh, dq[t], a.scale, r < w.rows, g, [&](int col, caf4 x) {
+      if (a.nsplit > 1) *reinterpret_cast<caf4*>(a.part + ob + col) = x;
+      else ca_store4<DT>(a.dq, ob + col, x);
+    });
   }
 }
 

@@ -77,7 +77,8 @@ def test_abi_refusals_before_launch():
         assert call(**{n: None}) == -1
     for n in ("g", "lse", "dq", "dk", "dv"):
         assert call(True, **{n: None}) == -1
-    assert call(True, ws=None) == -1 and call(True, ws_bytes=4) == -2
+    assert call(True, ws=None, Lq=40) == -1 and call(True, ws_bytes=4, Lq=40) == -2
+    assert call(ws=None, Lk=5000) == -1 and call(ws_bytes=4, Lk=5000) == -2          # keys split over workgroups
     for kw in (dict(B=-1), dict(Hk=3), dict(Hk=0), dict(dh=0), dict(scale=0.0), dict(scale=float("nan")),
                dict(Lq=1 << 31)):
         assert call(**kw) == -2, kw
@@ -88,4 +89,5 @@ def test_abi_refusals_before_launch():
         assert call(**kw) == -4, kw
     assert call(B=0) == 0 and call(Lq=0) == 0 and call(True, B=0) == 0
     ws = L.hclsm_cross_attention_workspace
-    assert ws(2, 3, 5, 4, 2, 16, 1, 1) > 0 and ws(2, 3, 5, 4, 2, 12, 1, 1) == -4 and ws(2, 3, 5, 4, 3, 16, 1, 0) == -2
+    assert ws(2, 3, 5, 4, 2, 16, 1, 0) == 0 and ws(2, 40, 5, 4, 2, 16, 1, 1) > 0 and ws(2, 3, 5000, 4, 2, 16, 1, 0) > 0
+    assert ws(2, 3, 5, 4, 2, 12, 1, 1) == -4 and ws(2, 3, 5, 4, 3, 16, 1, 0) == -2

@@ -71,6 +71,25 @@ def test_all_keys(shape, dtype):
     _compare(q, k, v, g, np.ones((shape[0], shape[2]), bool), dtype, f"{shape} {dtype}")
 
 
+SPLIT = [  # keys of a unit shared by several workgroups, rows too in the backward; many heads to a key head
+    (1, 3, 1500, 4, 2, 64), (1, 1, 5000, 8, 1, 128), (2, 16, 900, 4, 2, 32), (1, 200, 700, 2, 1, 64), (2, 150, 1000, 6, 2, 128),
+    (1, 70, 600, 2, 1, 256), (1, 9, 100, 40, 1, 32), (1, 4, 90, 40, 1, 256), (1, 3, 50, 70, 1, 64), (1, 40, 300, 7, 1, 200),
+    (1, 33, 530, 3, 1, 96),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SPLIT)
+def test_split_keys_and_rows(shape, dtype):
+    print(f"split {shape} {dtype}", flush=True)
+    q, k, v, g = _data(*shape, dtype, 12)
+    _compare(q, k, v, g, np.ones((shape[0], shape[2]), bool), dtype, f"{shape} {dtype}")
+    lens = torch.tensor([shape[2] - 37, 3][:shape[0]])
+    live = np.arange(shape[2]) < lens.numpy()[:, None]
+    k[~torch.tensor(live)] = float("nan")
+    _compare(q, k, v, g, live, dtype, f"{shape} {dtype} lengths", key_lens=lens.cuda())
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(5, 3, 70, 4, 2, 64), (4, 40, 200, 2, 2, 32), (5, 70, 140, 3, 1, 128),
                                    (4, 1, 300, 6, 2, 64), (4, 9, 90, 2, 1, 200)])
