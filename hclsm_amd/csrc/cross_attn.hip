@@ -19,7 +19,7 @@ int64_t ca_row_bytes(int64_t dh, int dtype) { return ca_padded_dh(dh) * (dtype =
 CaPlan ca_forward_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t dh, int dtype) {
   const int64_t rows = Lq * G, units = B * Hk, bytes = ca_row_bytes(dh, dtype);
   CaPlan p{0, 1, 1};
-  p.few = rows <= 16 && bytes <= CA_FEW1_BYTES ? 1 : rows <= 32 && bytes <= CA_FEW2_BYTES ? 2 : 0;
+  p.few = rows <= 16 && bytes <= CA_FEW1_BYTES ? 1 : rows <= 32 && dtype == HCLSM_F32 && bytes <= CA_FEW2_F32_BYTES ? 2 : 0;
   const int64_t per = p.few ? 16 * p.few : ca_tile_rows(rows, bytes);
   // workgroups that are on the chip at once (registers: 4 to 1 a CU for few rows, 3 to 2 for many)
   const int64_t slots = p.few ? (bytes <= 64 ? 1024 : bytes <= 128 ? 768 : bytes <= 192 ? 512 : 256) : bytes <= 128 ? 768 : 512;
@@ -214,7 +214,7 @@ int ca_args(const HclsmCrossAttention* x, int bwd, CaArgs& a) {
   const int64_t G = x->Hk ? x->H / x->Hk : 1;
   if (rows) {
     if (!ca_near(x->q_sl, x->q_sh, G, esz) || (bwd && !ca_near(x->g_sl, x->g_sh, G, esz))) return HCLSM_ERR_UNSUPPORTED;
-    if (!x->q || !x->out || (bwd && (!x->g || !x->dq || !x->lse))) return HCLSM_ERR_NULL;
+    if (!x->q || !x->out || (bwd && (!x->g || !x->lse))) return HCLSM_ERR_NULL;
     if (!ca_aligned(x->q, x->q_sb, x->q_sl, x->q_sh, esz) || !ca_aligned(x->out, 0, 0, 0, esz) ||
         !ca_aligned(x->out_lo, 0, 0, 0, esz)) return HCLSM_ERR_UNSUPPORTED;
     if (bwd && (!ca_aligned(x->g, x->g_sb, x->g_sl, x->g_sh, esz) || !ca_aligned(x->dq, 0, 0, 0, esz)))
@@ -222,7 +222,7 @@ int ca_args(const HclsmCrossAttention* x, int bwd, CaArgs& a) {
   }
   if (keys) {
     if (!ca_near(x->k_sl, 0, 1, esz) || !ca_near(x->v_sl, 0, 1, esz)) return HCLSM_ERR_UNSUPPORTED;
-    if (!x->k || !x->v || (bwd && (!x->dk || !x->dv))) return HCLSM_ERR_NULL;
+    if (!x->k || !x->v || (bwd && (!x->dk != !x->dv))) return HCLSM_ERR_NULL;
     if (!ca_aligned(x->k, x->k_sb, x->k_sl, x->k_sh, esz) || !ca_aligned(x->v, x->v_sb, x->v_sl, x->v_sh, esz))
       return HCLSM_ERR_UNSUPPORTED;
     if (bwd && (!ca_aligned(x->dk, 0, 0, 0, esz) || !ca_aligned(x->dv, 0, 0, 0, esz))) return HCLSM_ERR_UNSUPPORTED;
@@ -289,7 +289,7 @@ extern "C" int hclsm_cross_attention_backward(const HclsmCrossAttention* x, void
   using namespace hclsm;
   CaArgs a{};
   if (int rc = ca_args(x, 1, a)) return rc;
-  if (x->B == 0 || x->Hk == 0) return 0;
+  if (x->B == 0 || x->Hk == 0 || (!x->dq && !x->dk)) return 0;
   const int64_t need = hclsm_cross_attention_workspace(x->B, x->Lq, x->Lk, x->H, x->Hk, x->dh, x->dtype, 1);
   if (need > 0 && workspace == nullptr) return HCLSM_ERR_NULL;
   if (workspace_bytes < need) return HCLSM_ERR_SHAPE;

@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
     }
 
     // dq: a lane per row
-    {
+    if (a.dq != nullptr) {
       caf4 s[QT][NPT], dp[QT][NPT];
 #pragma unroll
       for (int p = 0; p < NPT; ++p) {
@@ -512,6 +512,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
       for (int u = 0; u < RU; ++u) { p2[p][u] = ca_pack<DT>(&s[u * NPT]); ds2[p][u] = ca_pack<DT>(&dp[u * NPT]); }
     }
     if (t0 + SK * NW < k1) load(t0 + SK * NW);
+    if (a.dk == nullptr) continue;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       caf4 dk[NPT], dv[NPT];
@@ -540,6 +541,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
       }
     }
   }
+  if (a.dq == nullptr) return;
 
   // dq of the waves, added in a fixed order
 #pragma unroll

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
   const int row0 = (w.tile * NW + wave) * 16 * QT;
   int k0, k1;
   ca_range(w.keys, a.nsplit, w.split, KR, k0, k1);
-  if (w.tile * NW * 16 * QT >= w.rows) k1 = k0;
+  if (w.tile * NW * 16 * QT >= w.rows || a.dq == nullptr) k1 = k0;      // (dq not wanted: delta alone)
 
   const char* kp = a.k + (w.b * a.ksb + w.hk * a.ksh) * ESZ;
   const char* vp = a.v + (w.b * a.vsb + w.hk * a.vsh) * ESZ;
@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
     if (i + 1 < nt) tile(i + 1, buf1, buf0);
   }
 
+  if (a.dq == nullptr) return;
   const int all = a.Lq * a.G;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -659,7 +660,7 @@ template <int DT, int DH> int ca_forward_dh(CaArgs& a, int64_t batch, void* ws, 
   if (p.few == 1) {
     if constexpr (S::RB <= CA_FEW1_BYTES) rc = ca_launch(ca_few_kernel<DT, DH, 4, 1>, a, batch, rows, 16, 256, st);
   } else if (p.few == 2) {
-    if constexpr (S::RB <= CA_FEW2_BYTES) rc = ca_launch(ca_few_kernel<DT, DH, 4, 2>, a, batch, rows, 32, 256, st);
+    if constexpr (DT == HCLSM_F32 && S::RB <= CA_FEW2_F32_BYTES) rc = ca_launch(ca_few_kernel<DT, DH, 4, 2>, a, batch, rows, 32, 256, st);
   } else {
     rc = ca_tile_rows(rows, S::RB) == 64 ? ca_launch(ca_fwd_kernel<DT, DH, 4, 1, S::TR>, a, batch, rows, 64, 256, st)
                                          : ca_launch(ca_fwd_kernel<DT, DH, 4, S::T, S::TR>, a, batch, rows, 128, 256, st);
@@ -679,19 +680,21 @@ template <int DT, int DH> int ca_backward_dh(CaArgs& a, int64_t batch, void* ws,
     a.part = (float*)w;
     int rc = HCLSM_ERR_UNSUPPORTED;
     if constexpr (S::RB <= CA_FEW_BWD_BYTES) rc = ca_launch(ca_few_bwd_kernel<DT, DH, 4>, a, batch, 1, 1, 256, st);
-    return rc || p.nsplit == 1 ? rc : ca_sum(a, 0, DT, st);
+    return rc || p.nsplit == 1 || a.dq == nullptr ? rc : ca_sum(a, 0, DT, st);
   }
   a.delta = (float*)w;
   w += (units * rows * 4 + 255) / 256 * 256;
   a.part = (float*)w;
+  if (a.dq == nullptr) a.nsplit = 1;
   if (int rc = ca_tile_rows(rows, S::RB) == 64
                    ? ca_launch(ca_dq_kernel<DT, DH, 4, 1, S::TR, S::PIPE_Q>, a, batch, rows, 64, 256, st)
                    : ca_launch(ca_dq_kernel<DT, DH, 4, S::T, S::TR, S::PIPE_Q>, a, batch, rows, 128, 256, st))
     return rc;
-  if (p.nsplit > 1) {
+  if (a.nsplit > 1) {
     if (int rc = ca_sum(a, 0, DT, st)) return rc;
-    w += p.nsplit * units * rows * a.dh * 4;
+    w += a.nsplit * units * rows * a.dh * 4;
   }
+  if (a.dk == nullptr) return 0;
   a.nsplit = p.nrows;
   a.part = (float*)w;
   if (int rc = ca_tile_rows(a.Lk, S::RB) == 64

@@ -116,9 +116,9 @@ def _forward(q, k, v, masks, scale, want_lse, want_lo):
     return out, lse, lo
 
 
-def _backward(q, k, v, out, lo, lse, g, masks, scale):
+def _backward(q, k, v, out, lo, lse, g, masks, scale, want_q=True, want_kv=True):
     q, k, v, g = _rows(q), _rows(k), _rows(v), _rows(g if g.dtype is q.dtype else g.to(q.dtype))
-    dq, dk, dv = _like(q), _like(k), _like(v)
+    dq, dk, dv = _like(q) if want_q else None, _like(k) if want_kv else None, _like(v) if want_kv else None
     ws, n = _workspace(q, k, 1)
     x = _pack(q, k, v, out, lo, lse, masks, scale, g, dq, dk, dv)
     with on_device(q.device):
@@ -146,7 +146,9 @@ class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def _back(ctx, g):
         q, k, v, out, lo, lse, *masks = ctx.saved_tensors
-        return (*_backward(q, k, v, out, lo, lse, g, masks, ctx.scale), None, None)
+        need = ctx.needs_input_grad
+        dq, dk, dv = _backward(q, k, v, out, lo, lse, g, masks, ctx.scale, need[0], need[1] or need[2])
+        return dq, dk if need[1] else None, dv if need[2] else None, None, None
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_padding_mask: torch.Tensor | None = None,

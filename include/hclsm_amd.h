@@ -675,8 +675,8 @@ typedef struct HclsmCrossAttention {
                           the backward adds it to out in sum(g out) (without it that sum is off by up to half a step of
                           out, which matters where the scores' gradients are small next to it) */
   float* lse;          /* [B, H, Lq]: written by the forward (nullable there), read by the backward */
-  void* dq;            /* backward: contiguous [B, Lq, H, dh] */
-  void* dk;            /* backward: contiguous [B, Lk, Hk, dh] */
+  void* dq;            /* backward: contiguous [B, Lq, H, dh]; nullable (not formed) */
+  void* dk;            /* backward: contiguous [B, Lk, Hk, dh]; dk and dv are nullable together (not formed) */
   void* dv;
   const uint8_t* key_pad;   /* [B, Lk], batch stride key_pad_sb: nonzero = key not read; nullable */
   const void* key_lens;     /* [B] live keys, nullable (all); clamped to 0 .. Lk; HCLSM_POS_I32 / _I64 */

@@ -75,8 +75,9 @@ def test_abi_refusals_before_launch():
     assert L.hclsm_cross_attention_forward(None, None, 0, None) == -1
     for n in ("q", "k", "v", "out"):
         assert call(**{n: None}) == -1
-    for n in ("g", "lse", "dq", "dk", "dv"):
+    for n in ("g", "lse", "dk", "dv"):
         assert call(True, **{n: None}) == -1
+    assert call(True, dq=None, dk=None, dv=None) == 0                   # nothing wanted
     assert call(True, ws=None, Lq=40) == -1 and call(True, ws_bytes=4, Lq=40) == -2
     assert call(ws=None, Lk=5000) == -1 and call(ws_bytes=4, Lk=5000) == -2          # keys split over workgroups
     for kw in (dict(B=-1), dict(Hk=3), dict(Hk=0), dict(dh=0), dict(scale=0.0), dict(scale=float("nan")),

@@ -219,9 +219,14 @@ def test_same_bits_partial_gradients_and_side_stream():
     first = torch.autograd.grad(out, ins, g, retain_graph=True)
     again = torch.autograd.grad(out, ins, g)
     assert all(torch.equal(a, b) for a, b in zip(first, again))
-    only = k.clone().requires_grad_()
-    (dk,) = torch.autograd.grad(cross_attention(q, only, v), only, g)
-    assert torch.equal(dk, first[1])
+    for Lq in (50, 5):                    # tiles of rows, and few rows
+        qs, gs = q[:, :Lq].contiguous(), g[:, :Lq].contiguous()
+        ref = torch.autograd.grad(cross_attention(qs.requires_grad_(), *ins[1:]), [qs, *ins[1:]], gs)
+        for i in range(3):                # a frozen encoder, learned keys: gradients of one input alone
+            parts = [qs.detach(), k, v]
+            parts[i] = parts[i].clone().requires_grad_()
+            (one,) = torch.autograd.grad(cross_attention(*parts), parts[i], gs)
+            assert torch.equal(one, ref[i])
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -300,3 +305,51 @@ def test_norm_rotation_and_attention_together(dtype):
         d = 2 * big(_np(go))
         assert_within(gx, rx, eps * np.abs(rx) + 72 * 2.0 ** -24 * r * d * np.abs(_np(w)).max() * (1 + n * n), "d" + name)
         assert_within(gw, rw, 400 * 2.0 ** -24 * (d * n).sum((0, 1, 2)) + 2.0 ** -23 * np.abs(rw), "dw" + name)
+
+
+def test_second_derivatives_are_refused():
+    from hclsm_amd.kernels import RotaryPlan, cross_attention, qk_norm_rotary, rotary_embedding
+    x = torch.randn(1, 4, 2, 16, device="cuda", requires_grad=True)
+    plan = RotaryPlan(16)
+    for f in (lambda x: cross_attention(x, x, x), lambda x: qk_norm_rotary(x, None, None, None, plan)[0],
+              lambda x: rotary_embedding(x, plan)):
+        y = f(x)
+        (g,) = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
+        first = torch.autograd.grad(f(x), x, torch.ones_like(y))[0]
+        assert torch.equal(g, first)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x)
+
+
+def test_offsets_past_32_bits():
+    """Keys and values of 4.6 GB each: the last keys of a long cache, for one query and for a tile of them, forward and
+    backward, and the rotation of as long a tensor."""
+    from hclsm_amd.kernels import RotaryPlan, cross_attention, rotary_embedding
+    L, Hk, dh, n = 2_200_013, 8, 128, 100
+    gen = torch.Generator("cuda").manual_seed(13)
+    k = torch.zeros(1, L, Hk, dh, dtype=torch.bfloat16, device="cuda")
+    v = torch.full_like(k, float("nan"))
+    tail = [torch.randn(1, n, Hk, dh, generator=gen, device="cuda").bfloat16() for _ in range(2)]
+    k[:, -n:], v[:, -n:] = tail
+    pad = torch.ones(1, L, dtype=torch.bool, device="cuda")
+    pad[:, -n:] = False
+    for Lq in (1, 40):
+        print(f"offsets past 32 bits, {Lq} queries", flush=True)
+        q = torch.randn(1, Lq, Hk, dh, generator=gen, device="cuda").bfloat16()
+        g = torch.randn(q.shape, generator=gen, device="cuda").bfloat16()
+        live = np.ones((1, n), bool)
+        vals = [_np(t) for t in (q, *tail)]
+        refs = (oh.cross_attention(*vals, live)[0], *oh.cross_attention_grads(*vals, live, _np(g)))
+        ins = [t.requires_grad_() for t in (q, k, v)]
+        out = cross_attention(*ins, key_padding_mask=pad)
+        dq, dk, dv = torch.autograd.grad(out, ins, g)
+        assert not dk[:, :-n].any() and not dv[:, :-n].any()
+        for name, got, ref, b in zip(("out", "dq", "dk", "dv"), (out, dq, dk[:, -n:], dv[:, -n:]), refs,
+                                     bounds(*vals, live, _np(g), None, torch.bfloat16)):
+            assert_within(got, ref, b, f"{Lq} queries {name}")
+        del out, dq, dk, dv
+    plan = RotaryPlan(dh)
+    with torch.no_grad():
+        k[:, -n:] = tail[0]
+        y = rotary_embedding(k, plan)[:, -n:]
+        assert torch.equal(y, rotary_embedding(tail[0], plan, torch.arange(L - n, L, device="cuda")))
