@@ -48,6 +48,18 @@ def _check(q, k, v, key_padding_mask, key_lens, query_lens, scale):
         raise ValueError(f"{fn}: scale must be positive, got {scale}")
 
 
+def _masks(key_padding_mask, key_lens, query_lens):
+    """The masks as the kernels read them: bytes with contiguous rows, contiguous lengths."""
+    pad = key_padding_mask
+    if pad is not None:
+        if pad.dtype not in (torch.bool, torch.uint8):
+            pad = pad != 0
+        if pad.stride(1) != 1:
+            pad = pad.contiguous()
+    return (pad, key_lens if key_lens is None or key_lens.stride(0) == 1 else key_lens.contiguous(),
+            query_lens if query_lens is None or query_lens.stride(0) == 1 else query_lens.contiguous())
+
+
 def _rows(t):
     """t with rows on 16-byte boundaries and near enough to each other (t itself where they are)."""
     n = 16 // t.element_size()
@@ -173,16 +185,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_pa
         scale = q.shape[-1] ** -0.5
     scale = float(scale)
     _check(q, k, v, key_padding_mask, key_lens, query_lens, scale)
-    pad = key_padding_mask
-    if pad is not None:
-        if pad.dtype not in (torch.bool, torch.uint8):
-            pad = pad != 0
-        if pad.stride(1) != 1:
-            pad = pad.contiguous()
-    klens = key_lens if key_lens is None or key_lens.stride(0) == 1 else key_lens.contiguous()
-    qlens = query_lens if query_lens is None or query_lens.stride(0) == 1 else query_lens.contiguous()
+    masks = _masks(key_padding_mask, key_lens, query_lens)
     if _no_node((q, k, v)):
-        out, lse, _ = _forward(q, k, v, (pad, klens, qlens), scale, return_lse, False)
+        out, lse, _ = _forward(q, k, v, masks, scale, return_lse, False)
     else:
-        out, lse = _CrossAttention.apply(q, k, v, (pad, klens, qlens), scale)
+        out, lse = _CrossAttention.apply(q, k, v, masks, scale)
     return (out, lse) if return_lse else out

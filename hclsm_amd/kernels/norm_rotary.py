@@ -98,6 +98,29 @@ class RotaryPlan:
         return self._turns.device
 
 
+class _RawPlan:
+    """What the kernels need of a plan, from tensors (the torch.library ops)."""
+
+    def __init__(self, turns, rot_dim, code, amplitude):
+        self._turns, self.rot_dim, self._code, self.amplitude = turns, rot_dim, code, amplitude
+
+    @classmethod
+    def of(cls, fn, turns, rot_dim, layout, amplitude, x):
+        if rot_dim == 0:
+            return None
+        if rot_dim < 0 or rot_dim % 2 or rot_dim > x.shape[3] or layout not in _LAYOUTS.values():
+            raise ValueError(f"{fn}: rot_dim must be even and at most {x.shape[3]}, layout 0 or 1, got {rot_dim} and {layout}")
+        if turns is None or turns.dtype != torch.float64 or turns.shape != (rot_dim // 2,) or not turns.is_contiguous():
+            raise ValueError(f"{fn}: turns must be {rot_dim // 2} contiguous float64 values")
+        return cls(turns, rot_dim, layout, amplitude)
+
+
+def _check_weight(fn, name, w, x):
+    if w is not None and (w.shape != (x.shape[3],) or w.dtype not in _FLOATS or not w.is_contiguous()):
+        raise ValueError(f"{fn}: {name} must be a contiguous float tensor of {x.shape[3]} elements, got "
+                         f"{w.dtype} {tuple(w.shape)}")
+
+
 def _check_heads(fn, name, x):
     if x.dim() != 4:
         raise ValueError(f"{fn}: {name} must be (B, L, H, dh), got shape {tuple(x.shape)}")
@@ -288,9 +311,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tens
     elif k_weight is not None or key_positions is not None:
         raise ValueError(f"{fn}: k_weight and key_positions need k")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.shape != (q.shape[3],) or w.dtype not in _FLOATS or not w.is_contiguous()):
-            raise ValueError(f"{fn}: {name} must be a contiguous float tensor of {q.shape[3]} elements, got "
-                             f"{w.dtype} {tuple(w.shape)}")
+        _check_weight(fn, name, w, q)
     if not eps >= 0:
         raise ValueError(f"{fn}: eps must be >= 0, got {eps}")
     if _no_node([t for t in (q, k, q_weight, k_weight) if t is not None]):

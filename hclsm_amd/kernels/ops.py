@@ -43,6 +43,16 @@ adds tens of microseconds of Python dispatch per call, which is the size of the 
     hclsm_hip::slot_track_sequence(slots, alive?, params, with_hidden, n_iters, temperature, compute_dtype)
         -> (tracked, alive', perm, matched, hidden): the tracking loop of model.py:229-252 over
         SlotTracker's 10 tensors (state-dict order); alive' is empty without alive, hidden without with_hidden
+    hclsm_hip::cross_attention_fwd(q, k, v, key_padding_mask?, key_lens?, query_lens?, scale, for_grad)
+        -> (out, lse, out_lo): softmax(scale q k^T) v against keys of another length; out_lo, what rounding out
+        dropped, has shape (0,) without for_grad or for float32 (dynamics/level2_goal.py:50,63)
+    hclsm_hip::cross_attention_bwd(q, k, v, out, lse, out_lo, g, key_padding_mask?, key_lens?, query_lens?, scale)
+        -> (dq, dk, dv)
+    hclsm_hip::norm_rotary_fwd(x, weight?, turns?, positions?, rot_dim, layout, amplitude, eps, norm) -> y
+        rms norm of each head (norm) and its rotation (rot_dim > 0; turns = frequency / 2 pi in float64; layout 0 half,
+        1 interleaved) (perception/vision_encoder.py:171-259)
+    hclsm_hip::norm_rotary_bwd(x, weight?, turns?, positions?, g, rot_dim, layout, amplitude, eps) -> (gx, gweight)
+        of the normed form; gweight has shape (0,) without a weight
 """
 
 from __future__ import annotations
@@ -53,7 +63,11 @@ import torch
 
 from hclsm_amd import _lib
 from hclsm_amd.kernels._common import require_gpu
+from hclsm_amd.kernels.cross_attention import (_backward as _cross_backward, _check as _cross_check,
+                                               _forward as _cross_forward, _masks as _cross_masks)
 from hclsm_amd.kernels.event_attention import event_attention as _event_attention
+from hclsm_amd.kernels.norm_rotary import (_check_heads, _check_positions, _check_weight, _forward as _nr_forward,
+                                           _norm_backward as _nr_backward, _RawPlan)
 from hclsm_amd.kernels.slot_attention_kernel import _core_raw
 from hclsm_amd.kernels.slot_iteration import SlotMode, SlotWeights, slot_attention_forward as _slot_forward
 from hclsm_amd.kernels.level1_packed import Level1Weights, level1_forward_packed
@@ -321,3 +335,84 @@ def _(slots, alive, params, with_hidden, n_iters, temperature, compute_dtype):
             slots.new_empty((B, T, N) if alive is not None else (0,), **f32),
             slots.new_empty((B, T, N), dtype=torch.int64), slots.new_empty((B, T, N), **f32),
             slots.new_empty((B, N, D) if with_hidden else (0,), **f32))
+
+
+# --------------------------------------------------------------------------- cross attention, norms and rotations
+
+def _opt(t, like, dtype=None):
+    return like.new_empty((0,), dtype=dtype or like.dtype) if t is None else t
+
+
+@torch.library.custom_op("hclsm_hip::cross_attention_fwd", mutates_args=())
+def cross_attention_fwd(q: Tensor, k: Tensor, v: Tensor, key_padding_mask: Optional[Tensor], key_lens: Optional[Tensor],
+                        query_lens: Optional[Tensor], scale: float, for_grad: bool) -> tuple[Tensor, Tensor, Tensor]:
+    require_gpu("cross_attention_fwd", q, k, v, key_padding_mask, key_lens, query_lens)
+    _cross_check(q, k, v, key_padding_mask, key_lens, query_lens, scale)
+    out, lse, lo = _cross_forward(q, k, v, _cross_masks(key_padding_mask, key_lens, query_lens), scale, True,
+                                  bool(for_grad) and q.dtype is not torch.float32)
+    return out, lse, _opt(lo, q)
+
+
+@cross_attention_fwd.register_fake
+def _(q, k, v, key_padding_mask, key_lens, query_lens, scale, for_grad):
+    B, Lq, H, _ = q.shape
+    return (q.new_empty(q.shape), q.new_empty((B, H, Lq), dtype=torch.float32),
+            q.new_empty(q.shape if for_grad and q.dtype is not torch.float32 else (0,)))
+
+
+@torch.library.custom_op("hclsm_hip::cross_attention_bwd", mutates_args=())
+def cross_attention_bwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, out_lo: Tensor, g: Tensor,
+                        key_padding_mask: Optional[Tensor], key_lens: Optional[Tensor], query_lens: Optional[Tensor],
+                        scale: float) -> tuple[Tensor, Tensor, Tensor]:
+    require_gpu("cross_attention_bwd", q, k, v, out, lse, out_lo, g, key_padding_mask, key_lens, query_lens)
+    _cross_check(q, k, v, key_padding_mask, key_lens, query_lens, scale)
+    B, Lq, H, _ = q.shape
+    lo = out_lo if out_lo.numel() or not q.numel() else None
+    for name, t, shape, dt in (("out", out, q.shape, q.dtype), ("lse", lse, (B, H, Lq), torch.float32),
+                               ("out_lo", lo, q.shape, q.dtype)):
+        if t is not None and (t.shape != shape or t.dtype != dt or not t.is_contiguous()):
+            raise ValueError(f"cross_attention_bwd: {name} must be the forward's contiguous {tuple(shape)} {dt} tensor, "
+                             f"got {tuple(t.shape)} {t.dtype}")
+    if g.shape != q.shape:
+        raise ValueError(f"cross_attention_bwd: g must be {tuple(q.shape)}, got {tuple(g.shape)}")
+    return _cross_backward(q, k, v, out, lo, lse, g, _cross_masks(key_padding_mask, key_lens, query_lens), scale)
+
+
+@cross_attention_bwd.register_fake
+def _(q, k, v, out, lse, out_lo, g, key_padding_mask, key_lens, query_lens, scale):
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+
+
+@torch.library.custom_op("hclsm_hip::norm_rotary_fwd", mutates_args=())
+def norm_rotary_fwd(x: Tensor, weight: Optional[Tensor], turns: Optional[Tensor], positions: Optional[Tensor],
+                    rot_dim: int, layout: int, amplitude: float, eps: float, norm: bool) -> Tensor:
+    require_gpu("norm_rotary_fwd", x, weight, turns, positions)
+    _check_heads("norm_rotary_fwd", "x", x)
+    _check_weight("norm_rotary_fwd", "weight", weight, x)
+    _check_positions("norm_rotary_fwd", "positions", positions, x)
+    plan = _RawPlan.of("norm_rotary_fwd", turns, rot_dim, layout, amplitude, x)
+    return _nr_forward([(x, weight, positions)], plan, eps, int(norm))[0]
+
+
+@norm_rotary_fwd.register_fake
+def _(x, weight, turns, positions, rot_dim, layout, amplitude, eps, norm):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op("hclsm_hip::norm_rotary_bwd", mutates_args=())
+def norm_rotary_bwd(x: Tensor, weight: Optional[Tensor], turns: Optional[Tensor], positions: Optional[Tensor], g: Tensor,
+                    rot_dim: int, layout: int, amplitude: float, eps: float) -> tuple[Tensor, Tensor]:
+    require_gpu("norm_rotary_bwd", x, weight, turns, positions, g)
+    _check_heads("norm_rotary_bwd", "x", x)
+    _check_weight("norm_rotary_bwd", "weight", weight, x)
+    _check_positions("norm_rotary_bwd", "positions", positions, x)
+    if g.shape != x.shape:
+        raise ValueError(f"norm_rotary_bwd: g must be {tuple(x.shape)}, got {tuple(g.shape)}")
+    plan = _RawPlan.of("norm_rotary_bwd", turns, rot_dim, layout, amplitude, x)
+    gx, gw = _nr_backward([(x, weight, positions, g, True)], plan, eps)[0]
+    return gx, _opt(gw, x)
+
+
+@norm_rotary_bwd.register_fake
+def _(x, weight, turns, positions, g, rot_dim, layout, amplitude, eps):
+    return x.new_empty(x.shape), (weight.new_empty(weight.shape) if weight is not None else x.new_empty((0,)))
