@@ -211,7 +211,7 @@ int ca_args(const HclsmCrossAttention* x, int bwd, CaArgs& a) {
   if (!(x->scale > 0.f) || !(x->scale < 3.0e38f)) return HCLSM_ERR_SHAPE;
   const bool rows = x->B && x->Lq && x->H, keys = x->B && x->Lk && x->Hk;
   const int esz = x->dtype == HCLSM_F32 ? 4 : 2;
-  const int64_t G = x->Hk ? x->H / x->Hk : 1;
+  const int64_t G = x->H ? x->H / x->Hk : 1;
   if (rows) {
     if (!ca_near(x->q_sl, x->q_sh, G, esz) || (bwd && !ca_near(x->g_sl, x->g_sh, G, esz))) return HCLSM_ERR_UNSUPPORTED;
     if (!x->q || !x->out || (bwd && (!x->g || !x->lse))) return HCLSM_ERR_NULL;
@@ -241,8 +241,9 @@ int ca_args(const HclsmCrossAttention* x, int bwd, CaArgs& a) {
   a.klens = x->key_lens; a.qlens = x->query_lens;
   a.klens64 = x->key_lens_dtype == HCLSM_POS_I64; a.qlens64 = x->query_lens_dtype == HCLSM_POS_I64;
   a.Hk = (int)x->Hk;
-  a.G = x->Hk ? (int)(x->H / x->Hk) : 1;
-  a.Lq = (int)x->Lq; a.Lk = (int)x->Lk; a.dh = (int)x->dh;
+  a.G = x->H ? (int)(x->H / x->Hk) : 1;
+  a.Lq = x->H ? (int)x->Lq : 0;        // no query head: no rows, whatever their length
+  a.Lk = (int)x->Lk; a.dh = (int)x->dh;
   // row / G by a product: with 2^(l-1) < G <= 2^l and m = floor(2^(31+l) / G) + 1, floor(row m / 2^(31+l)) is
   // exact for row < 2^31
   a.gmul = 0;

@@ -209,6 +209,13 @@ def test_empty_sizes():
             assert not out.any() and torch.isneginf(lse).all() and not grads[0].any()
         if Lq == 0:
             assert not grads[1].any() and not grads[2].any()
+    for dh in (16, 256):                  # no query head; queries of length zero
+        for Lq, H in ((3, 0), (0, 2)):
+            q = torch.empty(2, Lq, H, dh, device="cuda", requires_grad=True)
+            k, v = (torch.randn(2, 70, 2, dh, device="cuda", requires_grad=True) for _ in range(2))
+            out = cross_attention(q, k, v)
+            grads = torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+            assert out.shape == q.shape and not grads[1].any() and not grads[2].any()
 
 
 def test_same_bits_partial_gradients_and_side_stream():
@@ -353,3 +360,29 @@ def test_offsets_past_32_bits():
         k[:, -n:] = tail[0]
         y = rotary_embedding(k, plan)[:, -n:]
         assert torch.equal(y, rotary_embedding(tail[0], plan, torch.arange(L - n, L, device="cuda")))
+
+
+def test_two_streams_at_once():
+    """Calls on two streams in flight together, each with a workspace of its own (keys split, partial gradients)."""
+    from hclsm_amd.kernels import cross_attention
+    data = [_data(1, Lq, 3000, 4, 2, 64, torch.bfloat16, 20 + Lq) for Lq in (2, 90)]
+    sets = [[t.cuda() for t in d] for d in data]
+
+    def step(q, k, v, g):
+        ins = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+        out = cross_attention(*ins)
+        return (out.detach(), *torch.autograd.grad(out, ins, g))
+
+    refs = [step(*d) for d in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got[i].append(step(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, refs[i]))
