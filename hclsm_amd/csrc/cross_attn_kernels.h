@@ -28,6 +28,16 @@ template <int ROWS> constexpr uint64_t CA_FULL = ROWS == 64 ? ~0ull : (1ull << (
 // maximum and sum of the softmax per row.  Statistics and accumulators are float32; the weights are rounded to the
 // operand type for the second product (half a step, 2^-8 of the value for bf16 and 2^-11 for fp16; the matrix unit has no
 // wider operand at this rate), their sum is not: the log-sum that the backward reads is the float32 one.
+//
+// What bounds it: the exponentials and the matrix unit in turn.  Heads of 64 need 512 matrix cycles and about 650 of
+// the vector unit (a multiply-add, an exponential, an addition, half a conversion and half a maximum per score) for a
+// wave's tile; counted on 8 x 2048 queries, 4099 keys, 12 heads of 64: matrix unit busy 35% of the cycles, vector unit 65%, LDS
+// without conflicts 17%.  The waves of a SIMD do the two parts at the same time rather than in turn: step u's exponentials
+// next to step u + 1's scores in one wave, raised priorities around the products or for every other wave, 8 waves to a
+// workgroup, 16 or 48 rows to a wave were all measured and gave nothing or lost 5 to 20%.
+// Measured (bf16): 174 us there (0.80 PFLOP/s over the live keys); 8 x 2048 queries, 4096 keys, 12 heads of 128: 388 us
+// (1.06 PFLOP/s); 8 x 1024, 2048 keys, 12 heads of 128 on 4: 118 us (0.87: 768 workgroups on 512 places).  A matrix
+// product of 8192^3 by the library reaches 1.27 PFLOP/s on the same card.
 template <int DT, int DH, int NW, int QT, int KR>
 __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
   using A = CaT<DT>;
@@ -233,6 +243,9 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
 // As the forward, with S^T and dP^T = V g^T formed per tile, p = exp(s - lse), ds = p (dP - delta) and
 // dQ^T = K^T ds^T.  delta = sum(g o) per row is formed here and left for the second kernel.  ds is rounded to the
 // operand type for its product, as the weights are in the forward.
+// Three products, two of which the kernel for dk and dv forms again: that costs two products in seven, and leaves no sum
+// of dq over key tiles to atomics.  Measured: 8 x 1024 queries, 2048 keys, 12 heads of 128 on 4, bf16:
+// 186 us, 0.83 PFLOP/s; matrix unit busy 34%.
 template <int DT, int DH, int NW, int QT, int KR, bool PIPE>
 __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
   using A = CaT<DT>;
@@ -423,6 +436,8 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
 // NW waves of 16 KT keys each, K and V operands in registers, over tiles of RR rows (q and g in LDS):
 // S = Q K^T and dP = g V^T with a lane per key, then dV^T = g^T p and dK^T = Q^T ds.  Shared heads are rows of the
 // unit, so their gradients are added here.  Keys that are not live get zeros.
+// Four products.  Measured on the sizes above: 236 us, 0.87 PFLOP/s; matrix unit busy 37%, one wave per SIMD (the accumulators
+// and operands of 32 keys of 128 take 300 registers; 16 keys per wave and two waves per SIMD measured the same).
 template <int DT, int DH, int NW, int KT, int RR, bool PIPE>
 __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
   using A = CaT<DT>;
