@@ -187,6 +187,9 @@ bool ca_aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int esz) {
   return (uintptr_t)p % 16 == 0 && s0 % n == 0 && s1 % n == 0 && s2 % n == 0;
 }
 
+// Partial sums are read and written as 16-byte vectors.
+bool ca_workspace_aligned(const void* ws) { return (uintptr_t)ws % 16 == 0; }
+
 // Offsets inside a tile (at most 64 rows, of a unit or of the keys) have to fit 31 bits.
 bool ca_near(int64_t sl, int64_t sh, int64_t G, int esz) {
   return sl >= 0 && sh >= 0 && sl < (1 << 24) && sh < ((int64_t)1 << 31) && (64 / G + 2) * sl * esz + G * sh * esz < 0x7fff0000;
@@ -208,7 +211,7 @@ int ca_sizes(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t d
 int ca_args(const HclsmCrossAttention* x, int bwd, CaArgs& a) {
   if (x == nullptr) return HCLSM_ERR_NULL;
   if (int rc = ca_sizes(x->B, x->Lq, x->Lk, x->H, x->Hk, x->dh, x->dtype)) return rc;
-  if (!(x->scale > 0.f) || !(x->scale < 3.0e38f)) return HCLSM_ERR_SHAPE;
+  if (!(x->scale > 0.f) || !(x->scale <= 2.0e38f)) return HCLSM_ERR_SHAPE;      // times log2(e) it is still finite
   const bool rows = x->B && x->Lq && x->H, keys = x->B && x->Lk && x->Hk;
   const int esz = x->dtype == HCLSM_F32 ? 4 : 2;
   const int64_t G = x->H ? x->H / x->Hk : 1;
@@ -279,6 +282,7 @@ extern "C" int hclsm_cross_attention_forward(const HclsmCrossAttention* x, void*
   CaArgs a{};
   if (int rc = ca_args(x, 0, a)) return rc;
   if (x->B == 0 || x->Lq == 0 || x->H == 0) return 0;
+  if (!ca_workspace_aligned(workspace)) return HCLSM_ERR_UNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;
   if (x->dtype == HCLSM_F32) return ca_forward_f32(a, x->B, workspace, workspace_bytes, st);
   if (x->dtype == HCLSM_BF16) return ca_forward_bf16(a, x->B, workspace, workspace_bytes, st);
@@ -294,6 +298,7 @@ extern "C" int hclsm_cross_attention_backward(const HclsmCrossAttention* x, void
   const int64_t need = hclsm_cross_attention_workspace(x->B, x->Lq, x->Lk, x->H, x->Hk, x->dh, x->dtype, 1);
   if (need > 0 && workspace == nullptr) return HCLSM_ERR_NULL;
   if (workspace_bytes < need) return HCLSM_ERR_SHAPE;
+  if (!ca_workspace_aligned(workspace)) return HCLSM_ERR_UNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;
   if (x->dtype == HCLSM_F32) return ca_backward_f32(a, x->B, workspace, workspace_bytes, st);
   if (x->dtype == HCLSM_BF16) return ca_backward_bf16(a, x->B, workspace, workspace_bytes, st);

@@ -44,8 +44,8 @@ def _check(q, k, v, key_padding_mask, key_lens, query_lens, scale):
             raise TypeError(f"{fn}: {name} must be int32 or int64, got {t.dtype}")
         if tuple(t.shape) != (B,):
             raise ValueError(f"{fn}: {name} must be ({B},), got {tuple(t.shape)}")
-    if not 0 < scale < float("inf"):
-        raise ValueError(f"{fn}: scale must be positive, got {scale}")
+    if not 1e-45 <= scale <= 2e38:
+        raise ValueError(f"{fn}: scale must be positive, as a float32 too, and at most 2e38, got {scale}")
 
 
 def _masks(key_padding_mask, key_lens, query_lens):

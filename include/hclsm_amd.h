@@ -664,7 +664,8 @@ int hclsm_norm_rotary_backward(const HclsmHeads* q, const HclsmHeads* k, int64_t
                                int64_t workspace_bytes, void* stream);
 
 /* Cross attention: queries of one length against keys and values of another.  Strides in elements (innermost 1); the
- * inputs' rows, and every output, lie on 16-byte boundaries. */
+ * inputs' rows, every output, and the workspace lie on 16-byte boundaries (HCLSM_ERR_UNSUPPORTED otherwise; so are
+ * calls of more than 2^31 / 256 workgroups, one or more of which serve a batch row's key head). */
 typedef struct HclsmCrossAttention {
   const void* q;       /* [B, Lq, H, dh] */
   const void* k;       /* [B, Lk, Hk, dh]: query head h reads key head h / (H / Hk) */
@@ -683,7 +684,7 @@ typedef struct HclsmCrossAttention {
   const void* query_lens;   /* [B] live queries, nullable (all); clamped to 0 .. Lq */
   int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, g_sb, g_sl, g_sh, key_pad_sb;
   int64_t B, Lq, Lk, H, Hk, dh;
-  float scale;              /* > 0 */
+  float scale;              /* > 0, at most 2e38 */
   int dtype, key_lens_dtype, query_lens_dtype;
 } HclsmCrossAttention;
 

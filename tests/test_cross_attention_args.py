@@ -92,3 +92,25 @@ def test_abi_refusals_before_launch():
     ws = L.hclsm_cross_attention_workspace
     assert ws(2, 3, 5, 4, 2, 16, 1, 0) == 0 and ws(2, 40, 5, 4, 2, 16, 1, 1) > 0 and ws(2, 3, 5000, 4, 2, 16, 1, 0) > 0
     assert ws(2, 3, 5, 4, 2, 12, 1, 1) == -4 and ws(2, 3, 5, 4, 3, 16, 1, 0) == -2
+
+
+def test_abi_refuses_unaligned_workspaces_and_scales_past_float32():
+    from hclsm_amd import _lib
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("libhclsm_amd.so not built")
+    L, P = _lib.lib(), 4096
+    x = _lib.HclsmCrossAttention(B=2, Lq=40, Lk=5000, H=4, Hk=2, dh=16, scale=0.25, dtype=1)
+    for n in ("q", "k", "v", "g", "out", "lse", "dq", "dk", "dv"):
+        setattr(x, n, P)
+    big = 1 << 40
+    assert L.hclsm_cross_attention_forward(ctypes.byref(x), P + 4, big, None) == -4
+    assert L.hclsm_cross_attention_backward(ctypes.byref(x), P + 8, big, None) == -4
+    x.scale = 2.5e38      # times log2(e): past float32
+    assert L.hclsm_cross_attention_forward(ctypes.byref(x), P, big, None) == -2
+    assert L.hclsm_cross_attention_backward(ctypes.byref(x), P, big, None) == -2
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e39, 2.5e38])
+def test_scales_that_float32_does_not_hold(scale):
+    with pytest.raises(ValueError, match="scale"):
+        _check(scale=scale)
