@@ -29,12 +29,14 @@ template <int ROWS> constexpr uint64_t CA_FULL = ROWS == 64 ? ~0ull : (1ull << (
 // operand type for the second product (half a step, 2^-8 of the value for bf16 and 2^-11 for fp16; the matrix unit has no
 // wider operand at this rate), their sum is not: the log-sum that the backward reads is the float32 one.
 //
-// What bounds it: the exponentials and the matrix unit in turn.  Heads of 64 need 512 matrix cycles and about 650 of
+// What bounds it: the exponentials and the matrix unit together.  Heads of 64 need 512 matrix cycles and about 650 of
 // the vector unit (a multiply-add, an exponential, an addition, half a conversion and half a maximum per score) for a
 // wave's tile; counted on 8 x 2048 queries, 4099 keys, 12 heads of 64: matrix unit busy 35% of the cycles, vector unit 65%, LDS
-// without conflicts 17%.  The waves of a SIMD do the two parts at the same time rather than in turn: step u's exponentials
-// next to step u + 1's scores in one wave, raised priorities around the products or for every other wave, 8 waves to a
-// workgroup, 16 or 48 rows to a wave were all measured and gave nothing or lost 5 to 20%.
+// without conflicts 17%.  What was measured to have the one run under the other, and not kept: step u's exponentials
+// next to step u + 1's scores in one wave; two halves of a workgroup that a barrier keeps in opposite phases (19 to 45%
+// slower); raised priorities around the products or for every other wave; 8 waves to a workgroup; 16 or 48 rows to a
+// wave.  Two or three tiles on their way instead of one change nothing (heads of 64: 144 and 143 us; of 128 with tiles of
+// 64 keys: 118 both; with tiles of 32, which leave room for three, 137), so the transfers are not what it waits for.
 // Measured (bf16): 174 us there (0.80 PFLOP/s over the live keys); 8 x 2048 queries, 4096 keys, 12 heads of 128: 388 us
 // (1.06 PFLOP/s); 8 x 1024, 2048 keys, 12 heads of 128 on 4: 118 us (0.87: 768 workgroups on 512 places).  A matrix
 // product of 8192^3 by the library reaches 1.27 PFLOP/s on the same card.
