@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
   using Frag = typename A::Frag;
   using Step = CaStep<DT, DH>;
   constexpr int NC = DH / A::KS, ND = DH / 16, NPT = A::NPT, ESZ = (int)sizeof(typename A::T), SK = Step::SK;
+  constexpr int PARTS = DT == HCLSM_F32 ? 1 : 2;
   __shared__ float s_m[NW][QT][16], s_l[NW][QT][16];
   __shared__ caf4 s_o[NW > 1 ? NW / 2 : 1][QT][ND][64];
 
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
         for (int d = 0; d < ND; ++d) o[u][d] *= alpha;
       }
     }
-    Frag pf[QT];
+    Frag pf[QT][PARTS];
 #pragma unroll
     for (int u = 0; u < QT; ++u) {
 #pragma unroll
@@ -244,13 +245,15 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
           s[u][p][r] = fast_exp2(s[u][p][r] * a.scale_log2 - m[u]);
           l[u] += s[u][p][r];
         }
-      pf[u] = ca_pack<DT>(s[u]);
+      ca_pack_parts<DT, PARTS>(s[u], pf[u]);
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       const Frag f = cur.vfrag(d);
 #pragma unroll
-      for (int u = 0; u < QT; ++u) o[u][d] = A::mma(f, pf[u], o[u][d]);
+      for (int u = 0; u < QT; ++u)
+#pragma unroll
+        for (int e = 0; e < PARTS; ++e) o[u][d] = A::mma(f, pf[u][e], o[u][d]);
     }
   }
 
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
 // split over workgroups, by ca_sum_kernel).  Both orientations of the scores are formed, S^T (a lane per row) for
 // dQ^T = K^T ds^T and S (a lane per key) for dV^T = g^T p and dK^T = Q^T ds: the key's operand registers serve both, and
 // moving ds between the lanes would cost more than the second product.  What bounds it: reading q, g, out and k, v once
-// and writing dq, dk, dv.  Measured: 32 slots on 196 tokens of 256 frames, 6 heads of 64, bf16: 52 us, 3.5 TB/s (the two
+// and writing dq, dk, dv.  Measured: 32 slots on 196 tokens of 256 frames, 6 heads of 64, bf16: 53 us, 3.4 TB/s (the two
 // tiled kernels: 83 us).
 template <int DT, int DH, int NW>
 __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
@@ -338,6 +341,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
   using Step = CaStep<DT, DH>;
   constexpr int NT = 64 * NW, QT = 2, R = 16 * QT, NC = DH / A::KS, ND = DH / 16, NPT = A::NPT, SK = Step::SK;
   constexpr int ESZ = (int)sizeof(typename A::T), VW = Step::VW, RU = QT / NPT;
+  constexpr int PARTS = DT == HCLSM_F32 ? 1 : 2;
   using Stage = CaStage<DT, DH, NT, R>;
   __shared__ __attribute__((aligned(16))) char tq[Stage::BYTES];
   __shared__ __attribute__((aligned(16))) char tg[Stage::BYTES];
@@ -473,7 +477,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
             dp[t][p] = A::mma(ca_frag<DT>(v[p][c]), go[t][c], dp[t][p]);
           }
       }
-      Frag ds[QT];
+      Frag ds[QT][PARTS];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
 #pragma unroll
@@ -483,17 +487,19 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
             dp[t][p][r] *= fast_exp2(s[t][p][r] * a.scale_log2 - lse2[t]);
             if (!full) dp[t][p][r] = live >> (16 * p + 4 * g + r) & 1 ? dp[t][p][r] : 0.f;
           }
-        ds[t] = ca_pack<DT>(dp[t]);
+        ca_pack_parts<DT, PARTS>(dp[t], ds[t]);
       }
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         const Frag f = Step::column(kc, d);
 #pragma unroll
-        for (int t = 0; t < QT; ++t) dq[t][d] = A::mma(f, ds[t], dq[t][d]);
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int e = 0; e < PARTS; ++e) dq[t][d] = A::mma(f, ds[t][e], dq[t][d]);
       }
     }
     // dk, dv: a lane per key; a key that is not live spoils no column but its own, which is written as zeros
-    Frag p2[NPT][RU], ds2[NPT][RU];
+    Frag p2[NPT][RU][PARTS], ds2[NPT][RU][PARTS];
 #pragma unroll
     for (int p = 0; p < NPT; ++p) {
       caf4 s[QT], dp[QT];
@@ -513,7 +519,10 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
         }
       }
 #pragma unroll
-      for (int u = 0; u < RU; ++u) { p2[p][u] = ca_pack<DT>(&s[u * NPT]); ds2[p][u] = ca_pack<DT>(&dp[u * NPT]); }
+      for (int u = 0; u < RU; ++u) {
+        ca_pack_parts<DT, PARTS>(&s[u * NPT], p2[p][u]);
+        ca_pack_parts<DT, PARTS>(&dp[u * NPT], ds2[p][u]);
+      }
     }
     if (t0 + SK * NW < k1) load(t0 + SK * NW);
     if (a.dk == nullptr) continue;
@@ -527,10 +536,12 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
         const Frag fg = Tile::frag_t(tg, 16 * NPT * u, d, li, g);
         const Frag fq = Tile::frag_t(tq, 16 * NPT * u, d, li, g);
 #pragma unroll
-        for (int p = 0; p < NPT; ++p) {
-          dv[p] = A::mma(fg, p2[p][u], dv[p]);
-          dk[p] = A::mma(fq, ds2[p][u], dk[p]);
-        }
+        for (int p = 0; p < NPT; ++p)
+#pragma unroll
+          for (int e = 0; e < PARTS; ++e) {
+            dv[p] = A::mma(fg, p2[p][u][e], dv[p]);
+            dk[p] = A::mma(fq, ds2[p][u][e], dk[p]);
+          }
       }
 #pragma unroll
       for (int p = 0; p < NPT; ++p) {

@@ -26,7 +26,7 @@ template <int ROWS> constexpr uint64_t CA_FULL = ROWS == 64 ? ~0ull : (1ull << (
 //
 // NW waves of 16 QT rows each over tiles of KR keys in LDS (two buffers, one barrier per tile), with the running
 // maximum and sum of the softmax per row.  Statistics and accumulators are float32; the weights are rounded to the
-// operand type for the second product (half a step, 2^-8 of the value for bf16 and 2^-11 for fp16; the matrix unit has no
+// operand type (PARTS operands, 2 for few keys) for the second product (half a step, 2^-8 of the value for bf16 and 2^-11 for fp16; the matrix unit has no
 // wider operand at this rate), their sum is not: the log-sum that the backward reads is the float32 one.
 //
 // What bounds it: the exponentials and the matrix unit together.  Heads of 64 need 512 matrix cycles and about 650 of
@@ -40,7 +40,7 @@ template <int ROWS> constexpr uint64_t CA_FULL = ROWS == 64 ? ~0ull : (1ull << (
 // Measured (bf16): 174 us there (0.80 PFLOP/s over the live keys); 8 x 2048 queries, 4096 keys, 12 heads of 128: 388 us
 // (1.06 PFLOP/s); 8 x 1024, 2048 keys, 12 heads of 128 on 4: 118 us (0.87: 768 workgroups on 512 places).  A matrix
 // product of 8192^3 by the library reaches 1.27 PFLOP/s on the same card.
-template <int DT, int DH, int NW, int QT, int KR>
+template <int DT, int DH, int NW, int QT, int KR, int PARTS>
 __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
   using A = CaT<DT>;
   using Tile = CaTile<DT, DH>;
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
       ca_fence();
     }
     // operands of the second product, CV at a time, the first ones on their way during the softmax
-    constexpr int J = KT / NPT * ND, CV = J < 4 ? J : 4;
+    constexpr int J = KT / NPT * ND, CV = J % 4 == 0 ? 4 : 2;
     static_assert(J % CV == 0, "whole groups");
     Frag fv[2][CV];
     auto get_v = [&](int c, Frag* d) {
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
         for (int d = 0; d < ND; ++d) o[t][d] *= alpha;
       }
     }
-    Frag p[QT][KT / NPT];
+    Frag p[QT][KT / NPT][PARTS];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
 #pragma unroll
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
         for (int r = 0; r < 4; ++r) sum[r] += s[t][k][r];
       l[t] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-      for (int u = 0; u < KT / NPT; ++u) p[t][u] = ca_pack<DT>(&s[t][u * NPT]);
+      for (int u = 0; u < KT / NPT; ++u) ca_pack_parts<DT, PARTS>(&s[t][u * NPT], p[t][u]);
     }
 #pragma unroll
     for (int c = 0; c < J / CV; ++c) {
@@ -201,7 +201,9 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
       for (int j = 0; j < CV; ++j)
 #pragma unroll
         for (int t = 0; t < QT; ++t)
-          o[t][(c * CV + j) % ND] = A::mma(fv[c & 1][j], p[t][(c * CV + j) / ND], o[t][(c * CV + j) % ND]);
+#pragma unroll
+          for (int e = 0; e < PARTS; ++e)
+            o[t][(c * CV + j) % ND] = A::mma(fv[c & 1][j], p[t][(c * CV + j) / ND][e], o[t][(c * CV + j) % ND]);
       ca_fence();
     }
   };
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
 // Three products, two of which the kernel for dk and dv forms again: that costs two products in seven, and leaves no sum
 // of dq over key tiles to atomics.  Measured: 8 x 1024 queries, 2048 keys, 12 heads of 128 on 4, bf16:
 // 186 us, 0.83 PFLOP/s; matrix unit busy 34%.
-template <int DT, int DH, int NW, int QT, int KR, bool PIPE>
+template <int DT, int DH, int NW, int QT, int KR, bool PIPE, int PARTS>
 __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
   using A = CaT<DT>;
   using Tile = CaTile<DT, DH>;
@@ -368,7 +370,7 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
       ca_fence();
       if (!PIPE) scores(u, s[u & 1], dp[u & 1]);
       else if (u + 1 < U) scores(u + 1, s[(u + 1) & 1], dp[(u + 1) & 1]);      // the vector unit works on step u meanwhile
-      Frag ds[QT];
+      Frag ds[QT][PARTS];
 #pragma unroll
       for (int t = 0; t < QT; ++t)
 #pragma unroll
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
         }
       }
 #pragma unroll
-      for (int t = 0; t < QT; ++t) ds[t] = ca_pack<DT>(dp[u & 1][t]);
+      for (int t = 0; t < QT; ++t) ca_pack_parts<DT, PARTS>(dp[u & 1][t], ds[t]);
       constexpr int CV = ND < 4 ? ND : ND % 4 == 0 ? 4 : 2;
       Frag ft[2][CV];
       auto get_t = [&](int c, int b) __attribute__((always_inline)) {
@@ -402,7 +404,9 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
 #pragma unroll
         for (int j = 0; j < CV; ++j)
 #pragma unroll
-          for (int t = 0; t < QT; ++t) dq[t][c * CV + j] = A::mma(ft[c & 1][j], ds[t], dq[t][c * CV + j]);
+          for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int e = 0; e < PARTS; ++e) dq[t][c * CV + j] = A::mma(ft[c & 1][j], ds[t][e], dq[t][c * CV + j]);
         ca_fence();
       }
     }
@@ -440,7 +444,7 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
 // unit, so their gradients are added here.  Keys that are not live get zeros.
 // Four products.  Measured on the sizes above: 236 us, 0.87 PFLOP/s; matrix unit busy 37%, one wave per SIMD (the accumulators
 // and operands of 32 keys of 128 take 300 registers; 16 keys per wave and two waves per SIMD measured the same).
-template <int DT, int DH, int NW, int KT, int RR, bool PIPE>
+template <int DT, int DH, int NW, int KT, int RR, bool PIPE, int PARTS>
 __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
   using A = CaT<DT>;
   using Tile = CaTile<DT, DH>;
@@ -558,7 +562,7 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
       ca_fence();
       if (!PIPE) scores(u, s[u & 1], dp[u & 1]);
       else if (u + 1 < U) scores(u + 1, s[(u + 1) & 1], dp[(u + 1) & 1]);      // the vector unit works on step u meanwhile
-      Frag p[KT], ds[KT];
+      Frag p[KT][PARTS], ds[KT][PARTS];
 #pragma unroll
       for (int k = 0; k < NPT; ++k) {
         const caf4 ls = *reinterpret_cast<const caf4*>(stat + 16 * (u * NPT + k) + 4 * g);
@@ -571,7 +575,10 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
           }
       }
 #pragma unroll
-      for (int t = 0; t < KT; ++t) { p[t] = ca_pack<DT>(s[u & 1][t]); ds[t] = ca_pack<DT>(dp[u & 1][t]); }
+      for (int t = 0; t < KT; ++t) {
+        ca_pack_parts<DT, PARTS>(s[u & 1][t], p[t]);
+        ca_pack_parts<DT, PARTS>(dp[u & 1][t], ds[t]);
+      }
       constexpr int CV = ND < 2 ? ND : 2;
       Frag tg2[2][CV], tq2[2][CV];
       auto get_t = [&](int c, int b) __attribute__((always_inline)) {
@@ -590,10 +597,12 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
 #pragma unroll
         for (int j = 0; j < CV; ++j)
 #pragma unroll
-          for (int t = 0; t < KT; ++t) {
-            dv[t][c * CV + j] = A::mma(tg2[c & 1][j], p[t], dv[t][c * CV + j]);
-            dk[t][c * CV + j] = A::mma(tq2[c & 1][j], ds[t], dk[t][c * CV + j]);
-          }
+          for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int e = 0; e < PARTS; ++e) {
+              dv[t][c * CV + j] = A::mma(tg2[c & 1][j], p[t][e], dv[t][c * CV + j]);
+              dk[t][c * CV + j] = A::mma(tq2[c & 1][j], ds[t][e], dk[t][c * CV + j]);
+            }
         ca_fence();
       }
     }
@@ -642,8 +651,11 @@ template <int DT, int DH> struct CaShape {
   // dk and dv 134 -> 146, 217 -> 212, 196 -> 208, 258 -> 238, 281 -> 272, 336 -> 356; float32 heads of 64 (2 batch rows):
   // 392 -> 383 and 423 -> 415, of 128: 407 -> 397 and 463 -> 488.
   static constexpr bool PIPE_Q = RB <= 256, PIPE_KV = RB <= 256 && DH % 64 == 0;
+  static constexpr int FINE = DT == HCLSM_F32 ? 1 : 2;      // operands that hold the weights of few keys
   static_assert(4 * CaTile<DT, DH>::bytes(TR, 256) + 2 * TR * 8 <= 160 * 1024, "two buffers of two tiles");
 };
+
+template <int DT> inline bool ca_fine(const CaArgs& a) { return DT != HCLSM_F32 && a.Lk <= CA_FINE_KEYS; }
 
 inline bool ca_by_xcd(int64_t units) { return units % 8 == 0 || units >= 64; }
 
@@ -679,8 +691,9 @@ template <int DT, int DH> int ca_forward_dh(CaArgs& a, int64_t batch, void* ws, 
   } else if (p.few == 2) {
     if constexpr (DT == HCLSM_F32 && S::RB <= CA_FEW2_F32_BYTES) rc = ca_launch(ca_few_kernel<DT, DH, 4, 2>, a, batch, rows, 32, 256, st);
   } else {
-    rc = ca_tile_rows(rows, S::RB) == 64 ? ca_launch(ca_fwd_kernel<DT, DH, 4, 1, S::TR>, a, batch, rows, 64, 256, st)
-                                         : ca_launch(ca_fwd_kernel<DT, DH, 4, S::T, S::TR>, a, batch, rows, 128, 256, st);
+    rc = ca_fine<DT>(a)                      ? ca_launch(ca_fwd_kernel<DT, DH, 4, 1, CA_FINE_KEYS, S::FINE>, a, batch, rows, 64, 256, st)
+         : ca_tile_rows(rows, S::RB) == 64 ? ca_launch(ca_fwd_kernel<DT, DH, 4, 1, S::TR, 1>, a, batch, rows, 64, 256, st)
+                                           : ca_launch(ca_fwd_kernel<DT, DH, 4, S::T, S::TR, 1>, a, batch, rows, 128, 256, st);
   }
   if (rc || p.nsplit == 1) return rc;
   return ca_join(a, DT, st);
@@ -703,9 +716,11 @@ template <int DT, int DH> int ca_backward_dh(CaArgs& a, int64_t batch, void* ws,
   w += (units * rows * 4 + 255) / 256 * 256;
   a.part = (float*)w;
   if (a.dq == nullptr) a.nsplit = 1;
-  if (int rc = ca_tile_rows(rows, S::RB) == 64
-                   ? ca_launch(ca_dq_kernel<DT, DH, 4, 1, S::TR, S::PIPE_Q>, a, batch, rows, 64, 256, st)
-                   : ca_launch(ca_dq_kernel<DT, DH, 4, S::T, S::TR, S::PIPE_Q>, a, batch, rows, 128, 256, st))
+  const bool fine = ca_fine<DT>(a);
+  if (int rc = fine ? ca_launch(ca_dq_kernel<DT, DH, 4, 1, CA_FINE_KEYS, false, S::FINE>, a, batch, rows, 64, 256, st)
+               : ca_tile_rows(rows, S::RB) == 64
+                   ? ca_launch(ca_dq_kernel<DT, DH, 4, 1, S::TR, S::PIPE_Q, 1>, a, batch, rows, 64, 256, st)
+                   : ca_launch(ca_dq_kernel<DT, DH, 4, S::T, S::TR, S::PIPE_Q, 1>, a, batch, rows, 128, 256, st))
     return rc;
   if (a.nsplit > 1) {
     if (int rc = ca_sum(a, 0, DT, st)) return rc;
@@ -714,9 +729,10 @@ template <int DT, int DH> int ca_backward_dh(CaArgs& a, int64_t batch, void* ws,
   if (a.dk == nullptr) return 0;
   a.nsplit = p.nrows;
   a.part = (float*)w;
-  if (int rc = ca_tile_rows(a.Lk, S::RB) == 64
-                   ? ca_launch(ca_dkv_kernel<DT, DH, 4, 1, S::TR, S::PIPE_KV>, a, batch, a.Lk, 64, 256, st)
-                   : ca_launch(ca_dkv_kernel<DT, DH, 4, S::T, S::TR, S::PIPE_KV>, a, batch, a.Lk, 128, 256, st))
+  if (int rc = fine ? ca_launch(ca_dkv_kernel<DT, DH, 4, 1, S::TR, false, S::FINE>, a, batch, a.Lk, 64, 256, st)
+               : ca_tile_rows(a.Lk, S::RB) == 64
+                   ? ca_launch(ca_dkv_kernel<DT, DH, 4, 1, S::TR, S::PIPE_KV, 1>, a, batch, a.Lk, 64, 256, st)
+                   : ca_launch(ca_dkv_kernel<DT, DH, 4, S::T, S::TR, S::PIPE_KV, 1>, a, batch, a.Lk, 128, 256, st))
     return rc;
   return p.nrows > 1 ? ca_sum(a, 1, DT, st) : 0;
 }

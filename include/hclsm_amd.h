@@ -698,7 +698,8 @@ int64_t hclsm_cross_attention_workspace(int64_t B, int64_t Lq, int64_t Lk, int64
  * are not live are not read into any product (they may hold anything).  Queries from query_lens[b] on, and queries of
  * a batch row without a live key, get out = 0 and lse = -inf.
  * H is a multiple of Hk; dh a multiple of 8 up to 256 (HCLSM_ERR_UNSUPPORTED otherwise).  Scores, softmax and sums in
- * float32; 16-bit operands round the weights to their type for the product with v.
+ * float32; 16-bit operands round the weights to their type for the product with v (few rows or at most 32 keys: the
+ * rounding's rest is a second operand).
  * (The reference runs torch's nn.MultiheadAttention here: dynamics/level2_goal.py:50,63, multimodal_fuser.py:40.)
  */
 int hclsm_cross_attention_forward(const HclsmCrossAttention* x, void* workspace, int64_t workspace_bytes, void* stream);

@@ -11,7 +11,10 @@ up to flush whatever its size, and so is a sum; tiny = half the smallest fp16 st
   delta      sum(g out) from the rounded out: e sum(|g| |out|) + the error of out + dh U.
   ds         p (error of dP + error of delta) + (2 rel + e) |ds| with |dP error| <= dh U sum|g v|; tiny for fp16.
   dq, dk     scale times the sum of |ds error| |k| (|q|) and (n + 40) U of the terms for n of them in sequence; e |dq|.
-  dv         (2 rel + e) sum(p |g|), (n + 40) U, tiny sum|g|; e |dv|."""
+  dv         (2 rel + e) sum(p |g|), (n + 40) U, tiny sum|g|; e |dv|.
+
+fine: weights and ds in two operands, the second one the rounding's rest: e^2 in place of e (tiny as before) but for the
+rounding of the results, and delta from out and its rest: e^2 |out| in place of e |out|."""
 
 from __future__ import annotations
 
@@ -21,11 +24,13 @@ import torch
 U = 2.0 ** -24
 
 
-def bounds(q, k, v, live, g=None, scale=None, dtype=torch.float32, qk_units=0.0):
+def bounds(q, k, v, live, g=None, scale=None, dtype=torch.float32, qk_units=0.0, fine=False):
     """Bounds for (out,) or (out, dq, dk, dv); qk_units: relative error of q and k themselves, in units of U.  All
     inputs float64, masked keys and dead queries finite."""
     e = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
     end = torch.finfo(dtype).eps / 2
+    e = e * e if fine else e
+    rest = end * end if fine else end
     flush = 2.0 ** -126
     tiny = 2.0 ** -25 if dtype == torch.float16 else flush
     B, Lq, H, dh = q.shape
@@ -51,13 +56,14 @@ def bounds(q, k, v, live, g=None, scale=None, dtype=torch.float32, qk_units=0.0)
     pv = np.einsum("bhlm,bmhd->blhd", p, A(vr))
     out = np.einsum("bhlm,bmhd->blhd", p, vr)
     rel_o = rel[..., 0].transpose(0, 2, 1)[..., None]
-    b_out = (rel_o + e + seq) * pv + end * A(out) + tiny * (1 + A(vr).sum(1)[:, None])
+    b_sum = (rel_o + e + seq) * pv + tiny * (1 + A(vr).sum(1)[:, None])
+    b_out = b_sum + end * A(out)
     if g is None:
         return (b_out * (1 + 4 * e),)
     dp = np.einsum("blhd,bmhd->bhlm", g, vr)
     dpabs = np.einsum("blhd,bmhd->bhlm", A(g), A(vr))
     delta = (g * out).sum(-1).transpose(0, 2, 1)[..., None]
-    err_delta = ((A(g) * b_out).sum(-1) + (dh + 4) * U * (A(g) * pv).sum(-1)).transpose(0, 2, 1)[..., None]
+    err_delta = ((A(g) * (b_sum + rest * A(out))).sum(-1) + (dh + 4) * U * (A(g) * pv).sum(-1)).transpose(0, 2, 1)[..., None]
     ds = p * (dp - delta)
     err_ds = p * (dh * U * dpabs + err_delta + 3 * U * (dpabs + A(delta))) * (1 + e) + (2 * rel + e) * A(ds)
     err_ds = np.where(dead, 0, err_ds + tiny + flush * (A(dp) + A(delta)))

@@ -71,6 +71,39 @@ def test_all_keys(shape, dtype):
     _compare(q, k, v, g, np.ones((shape[0], shape[2]), bool), dtype, f"{shape} {dtype}")
 
 
+FINE = [  # at most 16 rows to a unit, or 32 in the backward and few keys
+    (2, 1, 65, 4, 4, 64), (3, 1, 200, 12, 3, 64), (1, 2, 1500, 8, 2, 128), (2, 16, 196, 3, 3, 64), (2, 32, 32, 6, 6, 64),
+    (2, 13, 12, 20, 5, 80), (2, 300, 5, 2, 1, 64), (1, 129, 32, 5, 5, 136), (1, 70, 31, 2, 2, 256), (2, 40, 2, 4, 2, 96),
+    (1, 100, 1, 2, 2, 32), (1, 1100, 17, 2, 2, 128),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", FINE)
+def test_weights_of_few_rows_and_few_keys_keep_their_rest(shape, dtype):
+    from hclsm_amd.kernels import cross_attention
+    print(f"cross attention {shape} {dtype}", flush=True)
+    q, k, v, g = _data(*shape, dtype, 11)
+    ins = [t.cuda().requires_grad_() for t in (q, k, v)]
+    out = cross_attention(*ins)
+    grads = torch.autograd.grad(out, ins, g.cuda())
+    vals, live = [_np(t) for t in (q, k, v)], np.ones((shape[0], shape[2]), bool)
+    refs = (oh.cross_attention(*vals, live, None)[0], *oh.cross_attention_grads(*vals, live, _np(g), None))
+    for name, got, ref, b in zip(("out", "dq", "dk", "dv"), (out, *grads), refs,
+                                 bounds(*vals, live, _np(g), None, dtype, fine=True)):
+        assert_within(got, ref, b, f"{shape} {dtype} {name}")
+
+
+def test_scores_gradients_past_float16():
+    """dP = +-960000, ds = 0.5 dP past 65504: inf 1 + (-inf)(-1) = inf in dq, no NaN from the rounding's rest."""
+    from hclsm_amd.kernels import cross_attention
+    one = torch.ones(1, 1, 1, 8)
+    ins = [t.half().cuda().requires_grad_()
+           for t in (0 * one, torch.cat((one, -one), 1), torch.cat((60000 * one, -60000 * one), 1))]
+    dq, _, dv = torch.autograd.grad(cross_attention(*ins, scale=1.0), ins, (2 * one).half().cuda())
+    assert torch.isposinf(dq).all() and torch.equal(dv, torch.full_like(dv, 1.0))
+
+
 SPLIT = [  # keys of a unit shared by several workgroups, rows too in the backward; many heads to a key head
     (1, 3, 1500, 4, 2, 64), (1, 1, 5000, 8, 1, 128), (2, 16, 900, 4, 2, 32), (1, 200, 700, 2, 1, 64), (2, 150, 1000, 6, 2, 128),
     (1, 70, 600, 2, 1, 256), (1, 9, 100, 40, 1, 32), (1, 4, 90, 40, 1, 256), (1, 3, 50, 70, 1, 64), (1, 40, 300, 7, 1, 200),
