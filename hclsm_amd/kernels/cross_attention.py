@@ -68,7 +68,9 @@ def _rows(t):
     if (s == 1 and t.data_ptr() % 16 == 0 and (sb % n == 0 or B == 1) and (L == 1 or (sl % n == 0 and sl < 1 << 20))
             and (H == 1 or (sh % n == 0 and sh * H < 1 << 28))):
         return t
-    return t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 else t.clone()
+    if not t.is_contiguous():
+        return t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
 
 
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
