@@ -360,19 +360,25 @@ def _(q, k, v, key_padding_mask, key_lens, query_lens, scale, for_grad):
             q.new_empty(q.shape if for_grad and q.dtype is not torch.float32 else (0,)))
 
 
+def _saved_lo(q, out, lse, out_lo):
+    """out_lo, or None where the forward wrote none (or nothing, for no queries); out, lse and out_lo are checked."""
+    B, Lq, H, _ = q.shape
+    lo = out_lo if out_lo.numel() else None
+    for name, t, shape, dt in (("out", out, q.shape, q.dtype), ("lse", lse, (B, H, Lq), torch.float32),
+                               ("out_lo", lo, q.shape, q.dtype)):
+        if t is not None and (t.shape != shape or t.dtype != dt or not t.is_contiguous()):
+            raise ValueError(f"cross_attention_bwd: {name} must be the forward's contiguous {tuple(shape)} {dt} tensor, "
+                             f"got {tuple(t.shape)} {t.dtype}")
+    return lo
+
+
 @torch.library.custom_op("hclsm_hip::cross_attention_bwd", mutates_args=())
 def cross_attention_bwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, out_lo: Tensor, g: Tensor,
                         key_padding_mask: Optional[Tensor], key_lens: Optional[Tensor], query_lens: Optional[Tensor],
                         scale: float) -> tuple[Tensor, Tensor, Tensor]:
     require_gpu("cross_attention_bwd", q, k, v, out, lse, out_lo, g, key_padding_mask, key_lens, query_lens)
     _cross_check(q, k, v, key_padding_mask, key_lens, query_lens, scale)
-    B, Lq, H, _ = q.shape
-    lo = out_lo if out_lo.numel() or not q.numel() else None
-    for name, t, shape, dt in (("out", out, q.shape, q.dtype), ("lse", lse, (B, H, Lq), torch.float32),
-                               ("out_lo", lo, q.shape, q.dtype)):
-        if t is not None and (t.shape != shape or t.dtype != dt or not t.is_contiguous()):
-            raise ValueError(f"cross_attention_bwd: {name} must be the forward's contiguous {tuple(shape)} {dt} tensor, "
-                             f"got {tuple(t.shape)} {t.dtype}")
+    lo = _saved_lo(q, out, lse, out_lo)
     if g.shape != q.shape:
         raise ValueError(f"cross_attention_bwd: g must be {tuple(q.shape)}, got {tuple(g.shape)}")
     return _cross_backward(q, k, v, out, lo, lse, g, _cross_masks(key_padding_mask, key_lens, query_lens), scale)
