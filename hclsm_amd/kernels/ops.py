@@ -49,8 +49,8 @@ adds tens of microseconds of Python dispatch per call, which is the size of the 
     hclsm_hip::cross_attention_bwd(q, k, v, out, lse, out_lo, g, key_padding_mask?, key_lens?, query_lens?, scale)
         -> (dq, dk, dv)
     hclsm_hip::norm_rotary_fwd(x, weight?, turns?, positions?, rot_dim, layout, amplitude, eps, norm) -> y
-        rms norm of each head (norm) and its rotation (rot_dim > 0; turns = frequency / 2 pi in float64; layout 0 half,
-        1 interleaved) (perception/vision_encoder.py:171-259)
+        rms norm of each head (norm; the weight belongs to it) and its rotation (rot_dim > 0; turns = frequency / 2 pi in
+        float64; layout 0 half, 1 interleaved) (perception/vision_encoder.py:171-259)
     hclsm_hip::norm_rotary_bwd(x, weight?, turns?, positions?, g, rot_dim, layout, amplitude, eps) -> (gx, gweight)
         of the normed form; gweight has shape (0,) without a weight
 """
@@ -389,6 +389,13 @@ def _(q, k, v, out, lse, out_lo, g, key_padding_mask, key_lens, query_lens, scal
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 
+def _check_norm(fn, weight, eps, norm):
+    if weight is not None and not norm:
+        raise ValueError(f"{fn}: a weight belongs to the norm, which is not asked for")
+    if norm and not eps >= 0:
+        raise ValueError(f"{fn}: eps must be >= 0, got {eps}")
+
+
 @torch.library.custom_op("hclsm_hip::norm_rotary_fwd", mutates_args=())
 def norm_rotary_fwd(x: Tensor, weight: Optional[Tensor], turns: Optional[Tensor], positions: Optional[Tensor],
                     rot_dim: int, layout: int, amplitude: float, eps: float, norm: bool) -> Tensor:
@@ -396,6 +403,7 @@ def norm_rotary_fwd(x: Tensor, weight: Optional[Tensor], turns: Optional[Tensor]
     _check_heads("norm_rotary_fwd", "x", x)
     _check_weight("norm_rotary_fwd", "weight", weight, x)
     _check_positions("norm_rotary_fwd", "positions", positions, x)
+    _check_norm("norm_rotary_fwd", weight, eps, norm)
     plan = _RawPlan.of("norm_rotary_fwd", turns, rot_dim, layout, amplitude, x)
     return _nr_forward([(x, weight, positions)], plan, eps, int(norm))[0]
 
@@ -412,6 +420,7 @@ def norm_rotary_bwd(x: Tensor, weight: Optional[Tensor], turns: Optional[Tensor]
     _check_heads("norm_rotary_bwd", "x", x)
     _check_weight("norm_rotary_bwd", "weight", weight, x)
     _check_positions("norm_rotary_bwd", "positions", positions, x)
+    _check_norm("norm_rotary_bwd", weight, eps, True)
     if g.shape != x.shape:
         raise ValueError(f"norm_rotary_bwd: g must be {tuple(x.shape)}, got {tuple(g.shape)}")
     plan = _RawPlan.of("norm_rotary_bwd", turns, rot_dim, layout, amplitude, x)

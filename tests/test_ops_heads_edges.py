@@ -1,5 +1,5 @@
-"""torch.library ops of cross attention and of norms and rotations: empty sizes (their argument checks on the CPU, results
-on the GPU)."""
+"""torch.library ops of cross attention and of norms and rotations: empty sizes and refusals (argument checks on the CPU,
+results on the GPU)."""
 
 from __future__ import annotations
 
@@ -48,3 +48,25 @@ def test_empty_queries(sizes, dtype, for_grad):
     dq, dk, dv = OPS.cross_attention_bwd(q, k, v, out, lse, lo, g, None, None, None, 0.25)
     assert (dq.shape, dk.shape, dv.shape) == (q.shape, k.shape, v.shape)
     assert not dk.any() and not dv.any()
+
+
+def test_weights_without_a_norm_and_bad_eps_are_refused():
+    w = torch.ones(16)
+    ops._check_norm("f", w, 0.0, True)
+    ops._check_norm("f", None, float("nan"), False)          # no norm: eps is not looked at
+    with pytest.raises(ValueError, match="belongs to the norm"):
+        ops._check_norm("f", w, 1e-6, False)
+    for eps in (-1e-6, float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            ops._check_norm("f", w, eps, True)
+
+
+@pytest.mark.gpu
+def test_norm_refusals_of_the_ops():
+    x, w = torch.ones(1, 2, 3, 16, device="cuda"), torch.ones(16, device="cuda")
+    with pytest.raises(ValueError, match="belongs to the norm"):
+        OPS.norm_rotary_fwd(x, w, None, None, 0, 0, 1.0, 1e-6, False)
+    with pytest.raises(ValueError, match="eps"):
+        OPS.norm_rotary_fwd(x, w, None, None, 0, 0, 1.0, -1.0, True)
+    with pytest.raises(ValueError, match="eps"):
+        OPS.norm_rotary_bwd(x, w, None, None, x, 0, 0, 1.0, float("nan"))
