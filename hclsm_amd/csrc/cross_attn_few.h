@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
 // and writing dq, dk, dv.  Measured: 32 slots on 196 tokens of 256 frames, 6 heads of 64, bf16: 53 us, 3.4 TB/s (the two
 // tiled kernels: 83 us).
 template <int DT, int DH, int NW>
-__global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
+__global__ void __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) ca_few_bwd_kernel(const CaArgs a) {
   using A = CaT<DT>;
   using Frag = typename A::Frag;
   using Tile = CaTile<DT, DH>;
@@ -439,10 +439,13 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
   }
 
   caf4 dq[QT][ND];
+  float up[QT];         // float16: factor of the row's ds in this wave
 #pragma unroll
-  for (int t = 0; t < QT; ++t)
+  for (int t = 0; t < QT; ++t) {
+    up[t] = ca_pow2(CA_F16_START);
 #pragma unroll
     for (int d = 0; d < ND; ++d) dq[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
+  }
 
   for (int t0 = k0 + wave * SK; t0 < k1; t0 += SK * NW) {
     const int n = w.keys - t0;                                      // keys there are from t0 on
@@ -487,6 +490,17 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
             dp[t][p][r] *= fast_exp2(s[t][p][r] * a.scale_log2 - lse2[t]);
             if (!full) dp[t][p][r] = live >> (16 * p + 4 * g + r) & 1 ? dp[t][p][r] : 0.f;
           }
+        if constexpr (CA_RANGED<DT>) {
+          const float most = ca_scale_most<NPT>(dp[t], up[t]);
+          if (__any(most > CA_F16_MOST)) {
+            const float f = ca_lowered(ca_rows4_max(most));
+            up[t] *= f;
+#pragma unroll
+            for (int p = 0; p < NPT; ++p) dp[t][p] *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) dq[t][d] *= f;
+          }
+        }
         ca_pack_parts<DT, PARTS>(dp[t], ds[t]);
       }
 #pragma unroll
@@ -500,6 +514,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
     }
     // dk, dv: a lane per key; a key that is not live spoils no column but its own, which is written as zeros
     Frag p2[NPT][RU][PARTS], ds2[NPT][RU][PARTS];
+    float down[NPT];      // float16: 1 / factor of the key's ds
 #pragma unroll
     for (int p = 0; p < NPT; ++p) {
       caf4 s[QT], dp[QT];
@@ -517,6 +532,12 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
           s[t][r] = fast_exp2(s[t][r] * a.scale_log2 - lsr[t][r]);
           dp[t][r] *= s[t][r];
         }
+      }
+      if constexpr (CA_RANGED<DT>) {
+        const float f = ca_fitted(ca_rows4_max(ca_scale_most<QT>(dp, 1.f)));
+        down[p] = ca_unscaled(f);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) dp[t] *= f;
       }
 #pragma unroll
       for (int u = 0; u < RU; ++u) {
@@ -550,6 +571,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
           const bool in = live >> (16 * p + li) & 1;
           const caf4 zero = {0.f, 0.f, 0.f, 0.f};
           const int64_t i = ((w.b * a.Lk + key) * a.Hk + w.hk) * (int64_t)a.dh + 16 * d + 4 * g;
+          if constexpr (CA_RANGED<DT>) dk[p] *= down[p];
           ca_store4<DT>(a.dk, i, in ? dk[p] * a.scale : zero);
           ca_store4<DT>(a.dv, i, in ? dv[p] : zero);
         }
@@ -559,6 +581,12 @@ __global__ void __launch_bounds__(64 * NW) ca_few_bwd_kernel(const CaArgs a) {
   if (a.dq == nullptr) return;
 
   // dq of the waves, added in a fixed order
+  if constexpr (CA_RANGED<DT>) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) dq[t][d] *= ca_unscaled(up[t]);
+  }
 #pragma unroll
   for (int h = NW / 2; h >= 1; h >>= 1) {
     if (wave >= h && wave < 2 * h) {

@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
 //
 // As the forward, with S^T and dP^T = V g^T formed per tile, p = exp(s - lse), ds = p (dP - delta) and
 // dQ^T = K^T ds^T.  delta = sum(g o) per row is formed here and left for the second kernel.  ds is rounded to the
-// operand type for its product, as the weights are in the forward.
+// operand type for its product, as the weights are in the forward (float16: at a power of two of its own, CA_RANGED).
 // Three products, two of which the kernel for dk and dv forms again: that costs two products in seven, and leaves no sum
 // of dq over key tiles to atomics.  Measured: 8 x 1024 queries, 2048 keys, 12 heads of 128 on 4, bf16:
 // 186 us, 0.83 PFLOP/s; matrix unit busy 34%.
@@ -306,10 +306,13 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
   }
 
   caf4 dq[QT][ND];
+  float up[QT];         // float16: factor of the row's ds
 #pragma unroll
-  for (int t = 0; t < QT; ++t)
+  for (int t = 0; t < QT; ++t) {
+    up[t] = ca_pow2(CA_F16_START);
 #pragma unroll
     for (int d = 0; d < ND; ++d) dq[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
+  }
 
   const int nt = (k1 - k0 + KR - 1) / KR;
   Stage sk, sv;
@@ -387,6 +390,26 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
             for (int r = 0; r < 4; ++r) dp[u & 1][t][k][r] = bits >> r & 1 ? dp[u & 1][t][k][r] : 0.f;
         }
       }
+      if constexpr (CA_RANGED<DT>) {
+        float most[QT];
+        bool past = false;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          most[t] = ca_scale_most<NPT>(dp[u & 1][t], up[t]);
+          past |= most[t] > CA_F16_MOST;
+        }
+        if (__any(past)) {
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            const float f = ca_lowered(ca_rows4_max(most[t]));
+            up[t] *= f;
+#pragma unroll
+            for (int k = 0; k < NPT; ++k) dp[u & 1][t][k] *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) dq[t][d] *= f;
+          }
+        }
+      }
 #pragma unroll
       for (int t = 0; t < QT; ++t) ca_pack_parts<DT, PARTS>(dp[u & 1][t], ds[t]);
       constexpr int CV = ND < 4 ? ND : ND % 4 == 0 ? 4 : 2;
@@ -427,6 +450,10 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
     ca_row(a, r, qi, hg);
     const int64_t ob = a.nsplit > 1 ? (((int64_t)w.split * a.units + w.unit) * all + r) * a.dh
                                     : ((w.b * a.Lq + qi) * a.Hk * a.G + w.hk * a.G + hg) * (int64_t)a.dh;
+    if constexpr (CA_RANGED<DT>) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d) dq[t][d] *= ca_unscaled(up[t]);
+    }
 #pragma unroll
     for (int d = 0; d < ND; ++d)
       if (16 * d + 4 * g < a.dh) {
@@ -483,10 +510,13 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
     for (int c = 0; c < NC; ++c) { fk[t][c] = ca_frag<DT>(f0[c]); fv[t][c] = ca_frag<DT>(f1[c]); }
   }
   caf4 dk[KT][ND], dv[KT][ND];
+  float up[KT];         // float16: factor of the key's ds
 #pragma unroll
-  for (int t = 0; t < KT; ++t)
+  for (int t = 0; t < KT; ++t) {
+    up[t] = ca_pow2(CA_F16_START);
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[t][d] = dv[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
+  }
 
   const int nt = (r1 - r0 + step - 1) / step;
   Stage sq, sg;
@@ -574,6 +604,26 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
             dp[u & 1][t][k][r] *= s[u & 1][t][k][r];
           }
       }
+      if constexpr (CA_RANGED<DT>) {
+        float most[KT];
+        bool past = false;
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          most[t] = ca_scale_most<NPT>(dp[u & 1][t], up[t]);
+          past |= live[t] && most[t] > CA_F16_MOST;
+        }
+        if (__any(past)) {
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
+            const float f = ca_lowered(ca_rows4_max(most[t]));
+            up[t] *= f;
+#pragma unroll
+            for (int k = 0; k < NPT; ++k) dp[u & 1][t][k] *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) dk[t][d] *= f;
+          }
+        }
+      }
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
         ca_pack_parts<DT, PARTS>(s[u & 1][t], p[t]);
@@ -621,6 +671,10 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
     if (key >= a.Lk) continue;
     const int64_t ob = a.nsplit > 1 ? (((int64_t)w.split * a.units + w.unit) * a.Lk + key) * a.dh
                                     : ((w.b * a.Lk + key) * a.Hk + w.hk) * (int64_t)a.dh;
+    if constexpr (CA_RANGED<DT>) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d) dk[t][d] *= ca_unscaled(up[t]);
+    }
 #pragma unroll
     for (int d = 0; d < ND; ++d)
       if (16 * d + 4 * g < a.dh) {

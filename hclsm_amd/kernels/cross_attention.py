@@ -183,7 +183,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_pa
     q, k and v; the same inputs give the same bits.  Scores, softmax and sums are float32; with 16-bit inputs the
     weights (and in the backward the scores' gradients) are rounded to the inputs' type for the matrix products, with what
     the rounding drops as a second operand where a key head has at most 16 query rows (32 in the backward, heads up to
-    128) or there are at most 32 keys; float16 gradients of scores past float16's range (65504) are infinite, as with any float16 product."""
+    128) or there are at most 32 keys; float16 gradients of scores are rounded relative to the largest of their row or key,
+    whatever their size."""
     require_gpu("cross_attention", q, k, v, key_padding_mask, key_lens, query_lens)
     if scale is None:
         scale = q.shape[-1] ** -0.5
