@@ -148,6 +148,11 @@ template <int DT> constexpr bool CA_RANGED = DT == HCLSM_F16;
 constexpr float CA_F16_MOST = 32768.f;
 constexpr int CA_F16_EXP = 11, CA_F16_START = 32;      // values are brought below 2^11
 __device__ __forceinline__ float ca_pow2(int e) { return __builtin_ldexpf(1.f, e); }
+// Weights p are rounded for the gradient of v as p 2^12 (the log-sum lowered by as much), so that they keep all their bits
+// down to 2^-26, the even weight of 67 million keys; p itself would have lost some from 16 thousand keys on.  A p past one,
+// from scores so large that float32 does not hold their differences, may be 2^4 before it overflows.
+template <int DT> constexpr float CA_P_SHIFT = DT == HCLSM_F16 ? 12.f : 0.f;
+template <int DT> constexpr float CA_P_DOWN = DT == HCLSM_F16 ? 0x1p-12f : 1.f;
 // N tiles of a row's values times up; the largest magnitude among them (NaN where there is one).
 template <int N> __device__ __forceinline__ float ca_scale_most(caf4* v, float up) {
   float m = 0.f;

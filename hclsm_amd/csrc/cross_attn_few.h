@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) ca_few_bwd_kernel(c
     lse2[t] = stat[16 * t + li];
     const float d = stat[R + 16 * t + li];
     nd[t] = caf4{d, d, d, d};
-    lsr[t] = *reinterpret_cast<const caf4*>(stat + 16 * t + 4 * g);
+    lsr[t] = *reinterpret_cast<const caf4*>(stat + 16 * t + 4 * g) - CA_P_SHIFT<DT>;
     ndr[t] = *reinterpret_cast<const caf4*>(stat + R + 16 * t + 4 * g);
   }
 
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) ca_few_bwd_kernel(c
       }
       if constexpr (CA_RANGED<DT>) {
         const float f = ca_fitted(ca_rows4_max(ca_scale_most<QT>(dp, 1.f)));
-        down[p] = ca_unscaled(f);
+        down[p] = ca_unscaled(f) * CA_P_DOWN<DT>;
 #pragma unroll
         for (int t = 0; t < QT; ++t) dp[t] *= f;
       }
@@ -571,7 +571,10 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) ca_few_bwd_kernel(c
           const bool in = live >> (16 * p + li) & 1;
           const caf4 zero = {0.f, 0.f, 0.f, 0.f};
           const int64_t i = ((w.b * a.Lk + key) * a.Hk + w.hk) * (int64_t)a.dh + 16 * d + 4 * g;
-          if constexpr (CA_RANGED<DT>) dk[p] *= down[p];
+          if constexpr (CA_RANGED<DT>) {
+            dk[p] *= down[p];
+            dv[p] *= CA_P_DOWN<DT>;
+          }
           ca_store4<DT>(a.dk, i, in ? dk[p] * a.scale : zero);
           ca_store4<DT>(a.dv, i, in ? dv[p] : zero);
         }

@@ -510,10 +510,10 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
     for (int c = 0; c < NC; ++c) { fk[t][c] = ca_frag<DT>(f0[c]); fv[t][c] = ca_frag<DT>(f1[c]); }
   }
   caf4 dk[KT][ND], dv[KT][ND];
-  float up[KT];         // float16: factor of the key's ds
+  float up[KT];         // float16: factor of the key's ds, formed from weights that have one of 2^12 already
 #pragma unroll
   for (int t = 0; t < KT; ++t) {
-    up[t] = ca_pow2(CA_F16_START);
+    up[t] = ca_pow2(CA_F16_START) * CA_P_DOWN<DT>;
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[t][d] = dv[t][d] = caf4{0.f, 0.f, 0.f, 0.f};
   }
@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
     char* tg = tq + TB;
     float* stat = reinterpret_cast<float*>(tq + 2 * TB);
     if ((int)threadIdx.x < RR) {       // rows past the last one, and rows without keys: every weight is exp(-inf)
-      stat[threadIdx.x] = st_lse == -INFINITY ? INFINITY : st_lse * HCLSM_LOG2E;
+      stat[threadIdx.x] = st_lse == -INFINITY ? INFINITY : st_lse * HCLSM_LOG2E - CA_P_SHIFT<DT>;
       stat[RR + threadIdx.x] = -st_delta;
     }
     ca_wait_vmem();
@@ -673,7 +673,10 @@ __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
                                     : ((w.b * a.Lk + key) * a.Hk + w.hk) * (int64_t)a.dh;
     if constexpr (CA_RANGED<DT>) {
 #pragma unroll
-      for (int d = 0; d < ND; ++d) dk[t][d] *= ca_unscaled(up[t]);
+      for (int d = 0; d < ND; ++d) {
+        dk[t][d] *= ca_unscaled(up[t]) * CA_P_DOWN<DT>;
+        dv[t][d] *= CA_P_DOWN<DT>;
+      }
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d)

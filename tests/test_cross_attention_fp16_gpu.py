@@ -7,7 +7,8 @@ sums of independent relative roundings:
           as much again only if something else is lost.  At most 2 is allowed.
   bound   elementwise that of cross_attention_bounds.py, for gradients 2^K times as large and divided by 2^K: the formulas are
           linear in g, and its allowance for subnormal roundings, 2^-25 in each ds, stands for values near one.  K is 10 - log2(max|ds|),
-          since a row's or key's largest ds is rounded at 2^10 or above: a step of 2^-35 of it.
+          since a row's or key's largest ds is rounded at 2^10 or above: a step of 2^-35 of it.  K is at most 12 for dv, whose
+          weights are rounded at 2^12 times their size.
 """
 
 from __future__ import annotations
@@ -57,11 +58,14 @@ def _check(case, what, scale=None, live=None, names=("dq", "dk"), **masks):
     vals[1], vals[2] = (np.where(live[:, :, None, None], t, 0) for t in vals[1:])
     refs = dict(zip(("dq", "dk", "dv"), oh.cross_attention_grads(*vals, live, gn, s)))
     K = int(np.floor(10 - np.log2(_most_ds(*vals, live, gn, s))))
-    bs = dict(zip(("out", "dq", "dk", "dv"), bounds(*vals, live, gn * 2.0 ** K, s, torch.float16)))
+    bs = {}
     for name in names:
+        K = min(K, 12) if name == "dv" else K
+        if K not in bs:
+            bs[K] = dict(zip(("out", "dq", "dk", "dv"), bounds(*vals, live, gn * 2.0 ** K, s, torch.float16)))
         got, ref = _np(grads[name]), refs[name]
         assert np.isfinite(got).all(), f"{what} {name}: not finite"
-        over = np.abs(got - ref) - (bs[name] * 2.0 ** -K + 2.0 ** -25)
+        over = np.abs(got - ref) - (bs[K][name] * 2.0 ** -K + 2.0 ** -25)
         assert (over <= 0).all(), f"{what} {name}: {over.max():.3e} over the bound"
         own = _rms(np.float64(np.float16(ref)) - ref)
         err = _rms(got - ref)
@@ -78,6 +82,18 @@ FEW = [(2, 1, 4096, 8, 2, 64), (1, 4, 32768, 2, 1, 64), (2, 32, 196, 3, 3, 64), 
 @pytest.mark.parametrize("shape", TILED + FEW)
 def test_gradients_of_any_size(shape, g_size):
     _check(_case(*shape, g_size, 1.0, 41), f"{shape} g {g_size}")
+
+
+@pytest.mark.parametrize("shape", [(1, 64, 32768, 2, 2, 64), (1, 40, 131072, 1, 1, 32), (1, 4, 131072, 2, 1, 64),
+                                   (1, 70, 40000, 1, 1, 256)])
+def test_weights_of_long_keys(shape):
+    """Weights near 2^-17, of which float16 holds some 7 bits."""
+    _check(_case(*shape, 30.0, 1.0, 46), f"{shape} long", names=("dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("shape", TILED + FEW)
+def test_gradients_of_the_values(shape):
+    _check(_case(*shape, 1.0, 1.0, 47), f"{shape}", names=("dv",))
 
 
 @pytest.mark.parametrize("shape", [(1, 64, 40, 2, 2, 64), (1, 64, 300, 2, 2, 128), (2, 8, 40, 4, 2, 64), (1, 64, 30, 1, 1, 32)])
