@@ -120,9 +120,13 @@ template <int DT, int PARTS> __device__ __forceinline__ void ca_pack_parts(const
   }
 }
 
-// A row's exponentials are taken against a reference (log2): lowest value, which no score reaches from below, and how far
-// the row's maximum may pass it before it moves.
-constexpr float CA_LOW = -3.0e38f, CA_SLACK = 8.f;
+// A row's exponentials are taken against a reference (log2): its lowest value, which no score reaches from below; how far the
+// row's maximum may pass it before it moves; and how far below the maximum it is put then.  float16 weights use the range
+// up to 2^15: what lies 2^36 below the largest weight is lost (with the largest at one it would be what lies 2^25 below, and
+// where one key of a hundred thousand stands out that adds up to 2^-8 of the softmax).
+constexpr float CA_LOW = -3.0e38f;
+template <int DT> constexpr float CA_SLACK = DT == HCLSM_F16 ? 15.f : 8.f;
+template <int DT> constexpr float CA_BELOW = DT == HCLSM_F16 ? 11.f : 0.f;
 
 // Maxima that pass a NaN on (v_maximum3_f32: one instruction for two values, and no step to quiet its operands first).
 __device__ __forceinline__ float ca_max3(float a, float b, float c) {

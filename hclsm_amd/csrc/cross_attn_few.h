@@ -222,12 +222,12 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; r += 2) mx = ca_max3(mx, s[u][p][r], s[u][p][r + 1]);
       top[u] = ca_rows4_max(mx) * a.scale_log2;
-      grew |= !(top[u] <= m[u] + CA_SLACK);
+      grew |= !(top[u] <= m[u] + CA_SLACK<DT>);
     }
     if (__any(grew)) {         // as in ca_fwd_kernel
 #pragma unroll
       for (int u = 0; u < QT; ++u) {
-        const float to = top[u] <= m[u] + CA_SLACK ? m[u] : top[u];
+        const float to = top[u] <= m[u] + CA_SLACK<DT> ? m[u] : top[u] - CA_BELOW<DT>;
         const float alpha = fast_exp2(m[u] - to);
         m[u] = to;
         l[u] *= alpha;

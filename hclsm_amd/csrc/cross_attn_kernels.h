@@ -151,8 +151,8 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
           for (int r = 0; r < 4; ++r) s[t][k][r] = bits >> r & 1 ? s[t][k][r] : -INFINITY;
       }
     }
-    // The reference of a row's exponentials follows its maximum only in steps of more than 2^CA_SLACK: weights then
-    // stay below 2^CA_SLACK, which float32 sums and either 16-bit type hold as exactly as weights below one, and the
+    // The reference of a row's exponentials follows its maximum only when it falls more than CA_SLACK behind: weights
+    // then stay below 2^CA_SLACK, which float32 sums and either 16-bit type hold as exactly as weights below one, and the
     // accumulators are hardly ever rescaled.
     float top[QT];
     bool grew = false;
@@ -164,12 +164,12 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; r += 2) mx = ca_max3(mx, s[t][k][r], s[t][k][r + 1]);
       top[t] = ca_rows4_max(mx) * a.scale_log2;
-      grew |= !(top[t] <= m[t] + CA_SLACK);
+      grew |= !(top[t] <= m[t] + CA_SLACK<DT>);
     }
     if (__any(grew)) {
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
-        const float to = top[t] <= m[t] + CA_SLACK ? m[t] : top[t];
+        const float to = top[t] <= m[t] + CA_SLACK<DT> ? m[t] : top[t] - CA_BELOW<DT>;
         const float alpha = fast_exp2(m[t] - to);
         m[t] = to;
         l[t] *= alpha;

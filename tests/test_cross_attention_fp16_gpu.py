@@ -127,3 +127,30 @@ def test_masked_keys_do_not_move_the_factor(shape):
     v[torch.tensor(pad)], k[torch.tensor(pad)] = float("inf"), float("nan")
     k[2][torch.tensor(pad[2])] = 60000.0
     _check((q, k, v, g), f"{shape} masked", live=~pad, key_padding_mask=torch.tensor(pad).cuda())
+
+
+@pytest.mark.parametrize("gap", [14.0, 18.0, 21.0])
+@pytest.mark.parametrize("where", [0, -1])
+@pytest.mark.parametrize("shape", [(1, 64, 32768, 1, 1, 64), (1, 2, 32768, 2, 1, 64), (1, 1, 50000, 4, 1, 128), (1, 70, 9000, 1, 1, 256)])
+def test_many_weights_far_below_the_largest(shape, where, gap):
+    """One key `gap` above all others with a value near zero: the others are what the output is made of.  Its weight is at
+    least 2^11, so a rounding of the smallest ones is off by at most 2^-36 of the softmax.  One batch row expanded to 800, so
+    that no row's keys are split over workgroups (each with a largest weight of its own)."""
+    from hclsm_amd.kernels import cross_attention
+    B, Lq, Lk, H, Hk, dh = shape
+    q, k, v, _ = _case(*shape, 1.0, 1.0, 48)
+    q, k, v = 0.3 * q, 0.3 * k, 1 + 0.1 * v
+    q[..., 0], k[..., 0] = 16, 0
+    k[:, where], v[:, where] = 0, 0.01
+    k[:, where, :, 0] = gap / (16 * dh ** -0.5)
+    with torch.no_grad():
+        rows = cross_attention(*(t.cuda().expand(800, -1, -1, -1) for t in (q, k, v)))
+        assert torch.equal(rows, rows[:1].expand(800, -1, -1, -1))
+        got = _np(rows[:1])
+    vals, live = [_np(t) for t in (q, k, v)], np.ones((B, Lk), bool)
+    ref, _ = oh.cross_attention(*vals, live)
+    (b,) = bounds(*vals, live, None, None, torch.float16)
+    least = 1 + np.abs(vals[2]).sum(1)[:, None].repeat(H // Hk, 2)
+    over = np.abs(got - ref) - (b - (1 - 2.0 ** -11) * 2.0 ** -25 * least + 2.0 ** -25)
+    print(f"{shape} gap {gap}: off by {np.abs(got - ref).max():.2e} of {np.abs(ref).max():.2e}", flush=True)
+    assert (over <= 0).all(), f"{over.max():.3e} over the bound"
