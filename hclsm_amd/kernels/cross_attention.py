@@ -10,6 +10,8 @@ batch row, a key padding mask, gradients, and a form for few queries that splits
 
 from __future__ import annotations
 
+import warnings
+
 import torch
 
 from hclsm_amd import _lib
@@ -52,6 +54,10 @@ def _masks(key_padding_mask, key_lens, query_lens):
     """The masks as the kernels read them: bytes with contiguous rows, contiguous lengths."""
     pad = key_padding_mask
     if pad is not None:
+        if pad.is_floating_point():
+            warnings.warn("cross_attention: a key_padding_mask of a float type is read as flags (nonzero = ignore that key), "
+                          "not added to the scores as nn.MultiheadAttention would; pass mask != 0 if that is meant",
+                          UserWarning, stacklevel=3)
         if pad.dtype not in (torch.bool, torch.uint8):
             pad = pad != 0
         if pad.stride(1) != 1:
@@ -173,8 +179,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_pa
     q (B, Lq, H, dh); k, v (B, Lk, Hk, dh): head h reads key head h // (H // Hk).  One dtype among bfloat16, float16,
         float32; dh a multiple of 8 up to 256; any strides (rows that are not contiguous, not on 16-byte boundaries
         or very far apart are copied; a batch of stride 0 is read as it stands).
-    key_padding_mask (B, Lk), True = ignore that key (nn.MultiheadAttention's convention); key_lens (B,) int32 or int64:
-        keys from key_lens[b] on are ignored.  What ignored keys hold, NaN and infinities among it, has no effect.
+    key_padding_mask (B, Lk), True (or nonzero) = ignore that key, nn.MultiheadAttention's convention for boolean masks.  A
+        mask of a float type is read the same way, with a warning: it is not added to the scores.  key_lens (B,) int32 or
+        int64: keys from key_lens[b] on are ignored.  What ignored keys hold, NaN and infinities among it, has no effect.
     query_lens (B,): queries from query_lens[b] on give zeros, and take part in no gradient.
     scale: dh ** -0.5 if None; positive.
 
