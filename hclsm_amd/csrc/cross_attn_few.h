@@ -1,5 +1,5 @@
-// Cross attention of few rows: at most 32 rows of a unit (one query and its shared heads, or a frame's slots), where
-// reading the keys and values is the work.
+// Cross attention of few rows of a unit (one query and its shared heads, or a frame's slots), where reading the keys and
+// values is the work: at most 16 rows, 32 of float32 and in the backward (longer heads aside, ca_forward_plan).
 #pragma once
 
 #include "cross_attn_stage.h"
@@ -131,7 +131,8 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
   constexpr int NC = DH / A::KS, ND = DH / 16, NPT = A::NPT, ESZ = (int)sizeof(typename A::T), SK = Step::SK;
   constexpr int PARTS = DT == HCLSM_F32 ? 1 : 2;
   __shared__ float s_m[NW][QT][16], s_l[NW][QT][16];
-  __shared__ caf4 s_o[NW > 1 ? NW / 2 : 1][QT][ND][64];
+  static_assert(NW >= 2 && (NW & (NW - 1)) == 0, "waves are joined by halves");
+  __shared__ caf4 s_o[NW / 2][QT][ND][64];
 
   CaWork w;
   if (!ca_work(a, w)) return;
@@ -261,46 +262,41 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
 #pragma unroll
   for (int u = 0; u < QT; ++u) l[u] = rows4_sum(l[u]);
   float top[QT], sum[QT];
-  if constexpr (NW > 1) {
-    if (g == 0) {
+  if (g == 0) {
 #pragma unroll
-      for (int u = 0; u < QT; ++u) { s_m[wave][u][li] = m[u]; s_l[wave][u][li] = l[u]; }
+    for (int u = 0; u < QT; ++u) { s_m[wave][u][li] = m[u]; s_l[wave][u][li] = l[u]; }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < QT; ++u) {
+    top[u] = s_m[0][u][li];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) top[u] = __builtin_elementwise_maximum(top[u], s_m[i][u][li]);
+    sum[u] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) sum[u] += s_l[i][u][li] * fast_exp2(s_m[i][u][li] - top[u]);
+    const float f = fast_exp2(m[u] - top[u]);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[u][d] *= f;
+  }
+#pragma unroll
+  for (int h = NW / 2; h >= 1; h >>= 1) {
+    if (wave >= h && wave < 2 * h) {
+#pragma unroll
+      for (int u = 0; u < QT; ++u)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) s_o[wave - h][u][d][lane] = o[u][d];
     }
     __syncthreads();
+    if (wave < h) {
 #pragma unroll
-    for (int u = 0; u < QT; ++u) {
-      top[u] = s_m[0][u][li];
+      for (int u = 0; u < QT; ++u)
 #pragma unroll
-      for (int i = 1; i < NW; ++i) top[u] = __builtin_elementwise_maximum(top[u], s_m[i][u][li]);
-      sum[u] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) sum[u] += s_l[i][u][li] * fast_exp2(s_m[i][u][li] - top[u]);
-      const float f = fast_exp2(m[u] - top[u]);
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[u][d] *= f;
+        for (int d = 0; d < ND; ++d) o[u][d] += s_o[wave][u][d][lane];
     }
-#pragma unroll
-    for (int h = NW / 2; h >= 1; h >>= 1) {
-      if (wave >= h && wave < 2 * h) {
-#pragma unroll
-        for (int u = 0; u < QT; ++u)
-#pragma unroll
-          for (int d = 0; d < ND; ++d) s_o[wave - h][u][d][lane] = o[u][d];
-      }
-      __syncthreads();
-      if (wave < h) {
-#pragma unroll
-        for (int u = 0; u < QT; ++u)
-#pragma unroll
-          for (int d = 0; d < ND; ++d) o[u][d] += s_o[wave][u][d][lane];
-      }
-      __syncthreads();
-    }
-    if (wave != 0) return;
-  } else {
-#pragma unroll
-    for (int u = 0; u < QT; ++u) { top[u] = m[u]; sum[u] = l[u]; }
+    __syncthreads();
   }
+  if (wave != 0) return;
 
   const int all = a.Lq * a.G;
 #pragma unroll
