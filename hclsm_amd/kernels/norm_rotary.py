@@ -6,7 +6,8 @@
 
 Every head is turned in pairs: pair i of the plan's first ``rot_dim`` elements by position * frequency_i.  The norm is
 the root mean square over a head's dh elements, in the same pass.  Both are differentiable (gradients of x, q, k and
-the weights), with float32 arithmetic between the load and the one rounding at the store, and angles in float64.
+the weights), with float32 arithmetic between the load and the one rounding at the store, and angles in float64; their
+sines and cosines are float32 values within 1.4 times 2^-24.
 
 x, q and k are (B, L, H, dh) tensors on the GPU (bfloat16, float16 or float32) of any strides whose last dimension is
 contiguous (others are copied), 1 <= dh <= 256.  positions: int32 or int64, (L,) or (B, L); None counts from 0.  Outputs
