@@ -66,13 +66,15 @@ def _masks(key_padding_mask, key_lens, query_lens):
             query_lens if query_lens is None or query_lens.stride(0) == 1 else query_lens.contiguous())
 
 
-def _rows(t):
-    """t with rows on 16-byte boundaries and near enough to each other (t itself where they are)."""
+def _rows(t, keys=False):
+    """t with rows on 16-byte boundaries and near enough to each other (t itself where they are).  The kernels' offsets from a
+    tile's first row are 31 bits: of keys and values a tile has one head, of queries all heads that share a key head."""
     n = 16 // t.element_size()
     sb, sl, sh, s = t.stride()
     B, L, H, _ = t.shape
-    if (s == 1 and t.data_ptr() % 16 == 0 and (sb % n == 0 or B == 1) and (L == 1 or (sl % n == 0 and sl < 1 << 20))
-            and (H == 1 or (sh % n == 0 and sh * H < 1 << 28))):
+    if (s == 1 and t.data_ptr() % 16 == 0 and (sb % n == 0 or B == 1)
+            and (L == 1 or (sl % n == 0 and (sl < 1 << 20 or (keys and sl < 1 << 22))))
+            and (H == 1 or (sh % n == 0 and (keys or sh * H < 1 << 28)))):
         return t
     if not t.is_contiguous():
         return t.contiguous()
@@ -122,7 +124,7 @@ def _like(t):
 
 
 def _forward(q, k, v, masks, scale, want_lse, want_lo):
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    q, k, v = _rows(q), _rows(k, True), _rows(v, True)
     B, Lq, H, _ = q.shape
     out = _like(q)
     lo = _like(q) if want_lo else None
@@ -137,7 +139,7 @@ def _forward(q, k, v, masks, scale, want_lse, want_lo):
 
 
 def _backward(q, k, v, out, lo, lse, g, masks, scale, want_q=True, want_kv=True):
-    q, k, v, g = _rows(q), _rows(k), _rows(v), _rows(g if g.dtype is q.dtype else g.to(q.dtype))
+    q, k, v, g = _rows(q), _rows(k, True), _rows(v, True), _rows(g if g.dtype is q.dtype else g.to(q.dtype))
     dq, dk, dv = _like(q) if want_q else None, _like(k) if want_kv else None, _like(v) if want_kv else None
     ws, n = _workspace(q, k, 1)
     x = _pack(q, k, v, out, lo, lse, masks, scale, g, dq, dk, dv)

@@ -65,3 +65,36 @@ def test_contiguous_tensors_off_a_boundary(Lq, dtype):
     for which in ((0,), (1,), (2,), (3,), (0, 1, 2, 3)):
         moved = [_off(t) if i in which else t for i, t in enumerate(ts)]
         assert all(torch.equal(a, b) for a, b in zip(step(*moved), ref)), which
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_caches_with_heads_first_are_read_as_they_stand(dtype):
+    """Heads of keys far apart, (B, H, L, dh) in memory, and tokens far apart, (L, B, H, dh): no copy.  (Nothing is touched here.)"""
+    rows = importlib.import_module("hclsm_amd.kernels.cross_attention")._rows
+    heads = torch.empty(1, 4, 1 << 20, 64, dtype=dtype).permute(0, 2, 1, 3)
+    assert heads.stride(2) * 4 == 1 << 28 and rows(heads, True) is heads
+    tokens = torch.empty(64, 1 << 21, dtype=dtype).as_strided((2, 60, 2, 64), (128, 1 << 21, 64, 1))
+    assert rows(tokens, True) is tokens
+    near = tokens[:, :1]
+    assert rows(near) is near
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Lq", [2, 70])
+def test_long_caches_with_heads_first(Lq):
+    """The same bits from a cache with 2^27 elements between heads, or 2^21 between tokens, as from a compact one."""
+    from hclsm_amd.kernels import cross_attention
+    gen = torch.Generator().manual_seed(32)
+    q, g = (torch.randn(1, Lq, 4, 64, generator=gen).bfloat16().cuda() for _ in range(2))
+    k, v = (torch.randn(1, 150, 4, 64, generator=gen).bfloat16().cuda() for _ in range(2))
+    far = torch.zeros(1, 4, 1 << 21, 64, dtype=torch.bfloat16, device="cuda").permute(0, 2, 1, 3)[:, :150]
+    apart = torch.zeros(150, 1 << 21, dtype=torch.bfloat16, device="cuda").as_strided((1, 150, 4, 64), (256, 1 << 21, 64, 1))
+    far.copy_(k), apart.copy_(v)
+
+    def step(k, v):
+        ins = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = cross_attention(*ins)
+        return (out.detach(), *torch.autograd.grad(out, ins, g))
+
+    assert far.stride(2) == 1 << 27
+    assert all(torch.equal(a, b) for a, b in zip(step(far, apart), step(k, v)))
