@@ -318,13 +318,16 @@ struct CaPlan {
   int nrows;      // backward: workgroups that share a unit's rows (dk, dv)
 };
 constexpr int CA_MAX_SPLIT = 256;
-// Rows (in bytes, padded head) up to which ca_few_kernel is built for 16 rows, for 32 rows of float32, and ca_few_bwd_kernel:
-// a step's keys and values, the accumulators and the queries all live in registers, and longer heads would spill.
-// Measured against the tiled kernels (us, 64 batch rows, 6 heads, 1500 keys; then 256 and 196): 1 row, bf16 heads of 64: 35
-// against 33 and 19 against 21, of 128: 58, 57 and 33, 37, float32 of 64: 58, 109 and 32, 65; 32 rows: float32 of 64: 69,
-// 111 and 49, 69, but bf16 of 64: 37, 36 and 23, 23 and of 128: 66, 58 and 61, 40, so 16-bit rows past 16 take the tiles.
-// Backward of 32 rows: bf16 of 64: 111, 124 and 61, 130, of 128: 238, 260 and 132, 173; float32 of 64: 263, 412 and 156, 262.
-constexpr int CA_FEW1_BYTES = 512, CA_FEW2_F32_BYTES = 256, CA_FEW_BWD_BYTES = 256;
+// Rows (in bytes, padded head) up to which ca_few_kernel is built for 16 rows and for 32 rows (float32, 16 bits), and
+// ca_few_bwd_kernel: a step's keys and values, the accumulators and the queries all live in registers, and longer heads
+// would spill.  Measured against the tiled kernels (us, 64 batch rows, 6 heads, 1500 keys; then 256 and 196): 1 row, bf16
+// heads of 64: 29 against 28 and 17 against 19, of 128: 57, 54 and 32, 34, float32 of 64: 57, 110 and 31, 65; 32 rows:
+// float32 of 64: 83, 109 and 52, 71, bf16 of 64: 44, 41 and 25, 24, where the weights keep their second operand for the
+// difference, but of 128: 82, 68 and 70, 49, which take the tiles.  Backward of 32 rows: bf16 of 64: 95, 101 and 54, 67, of
+// 128: 194, 236 and 125, 157; float32 of 64: 227, 406 and 121, 252.  Single float32 queries with heads past 128 take the
+// tiles too: 64 x 1568 keys, 12 heads of 192: 570 us, of 256: 770, 3.2 TB/s, where heads of 128 take 211, 5.9 TB/s.
+constexpr int CA_FEW1_BYTES = 512, CA_FEW2_F32_BYTES = 256, CA_FEW2_16BIT_BYTES = 128, CA_FEW_BWD_BYTES = 256;
+constexpr int64_t ca_few2_bytes(int dtype) { return dtype == HCLSM_F32 ? CA_FEW2_F32_BYTES : CA_FEW2_16BIT_BYTES; }
 constexpr int64_t ca_padded_dh(int64_t dh) {
   return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : dh <= 128 ? 128 : dh <= 192 ? 192 : 256;
 }

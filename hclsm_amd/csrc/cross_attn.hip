@@ -19,7 +19,7 @@ int64_t ca_row_bytes(int64_t dh, int dtype) { return ca_padded_dh(dh) * (dtype =
 CaPlan ca_forward_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t dh, int dtype) {
   const int64_t rows = Lq * G, units = B * Hk, bytes = ca_row_bytes(dh, dtype);
   CaPlan p{0, 1, 1};
-  p.few = rows <= 16 && bytes <= CA_FEW1_BYTES ? 1 : rows <= 32 && dtype == HCLSM_F32 && bytes <= CA_FEW2_F32_BYTES ? 2 : 0;
+  p.few = rows <= 16 && bytes <= CA_FEW1_BYTES ? 1 : rows <= 32 && bytes <= ca_few2_bytes(dtype) ? 2 : 0;
   const int64_t per = p.few ? 16 * p.few : ca_tile_rows(rows, bytes);
   // workgroups that are on the chip at once (registers: 4 to 1 a CU for few rows, 3 to 2 for many)
   const int64_t slots = p.few ? (bytes <= 64 ? 1024 : bytes <= 128 ? 768 : bytes <= 192 ? 512 : 256) : bytes <= 128 ? 768 : 512;

@@ -1,5 +1,5 @@
 // Cross attention of few rows of a unit (one query and its shared heads, or a frame's slots), where reading the keys and
-// values is the work: at most 16 rows, 32 of float32 and in the backward (longer heads aside, ca_forward_plan).
+// values is the work: at most 16 rows, or 32 of short heads and in the backward (ca_forward_plan, ca_backward_plan).
 #pragma once
 
 #include "cross_attn_stage.h"

@@ -746,7 +746,7 @@ template <int DT, int DH> int ca_forward_dh(CaArgs& a, int64_t batch, void* ws, 
   if (p.few == 1) {
     if constexpr (S::RB <= CA_FEW1_BYTES) rc = ca_launch(ca_few_kernel<DT, DH, 4, 1>, a, batch, rows, 16, 256, st);
   } else if (p.few == 2) {
-    if constexpr (DT == HCLSM_F32 && S::RB <= CA_FEW2_F32_BYTES) rc = ca_launch(ca_few_kernel<DT, DH, 4, 2>, a, batch, rows, 32, 256, st);
+    if constexpr (S::RB <= ca_few2_bytes(DT)) rc = ca_launch(ca_few_kernel<DT, DH, 4, 2>, a, batch, rows, 32, 256, st);
   } else {
     rc = ca_fine<DT>(a)                      ? ca_launch(ca_fwd_kernel<DT, DH, 4, 1, CA_FINE_KEYS, S::FINE>, a, batch, rows, 64, 256, st)
          : ca_tile_rows(rows, S::RB) == 64 ? ca_launch(ca_fwd_kernel<DT, DH, 4, 1, S::TR, 1>, a, batch, rows, 64, 256, st)

@@ -191,9 +191,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_pa
     with no key to read gives zeros (lse -inf) and zero gradients (slots_attention gives NaN there).  Differentiable in
     q, k and v; the same inputs give the same bits.  Scores, softmax and sums are float32; with 16-bit inputs the
     weights (and in the backward the scores' gradients) are rounded to the inputs' type for the matrix products, with what
-    the rounding drops as a second operand where a key head has at most 16 query rows (32 in the backward, heads up to
-    128) or there are at most 32 keys; float16 gradients of scores are rounded relative to the largest of their row or key,
-    whatever their size."""
+    the rounding drops as a second operand where a key head has at most 16 query rows (32 of heads up to 64, and in the
+    backward of heads up to 128) or there are at most 32 keys; float16 gradients of scores are rounded relative to the
+    largest of their row or key, whatever their size."""
     require_gpu("cross_attention", q, k, v, key_padding_mask, key_lens, query_lens)
     if scale is None:
         scale = q.shape[-1] ** -0.5
