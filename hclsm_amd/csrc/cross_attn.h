@@ -341,8 +341,10 @@ constexpr int64_t ca_tile_rows(int64_t n, int64_t bytes) { return bytes <= 256 &
 // own rounding (6700 and 2000 random calls).  It costs next to nothing there (us, bf16, one and two operands): 256 frames,
 // 32 slots, 196 tokens, 6 heads of 64: backward 50.5, 53; 8 slots, heads of 128: 121, 126; 64 single queries on 1568 keys,
 // 12 heads of 64: 50.8, 50.5; in tiles of 32 keys, 16 x 1024 queries, 32 keys, 12 heads of 64: 23.5 + 49.5, 22.3 + 49.8, of
-// 128: 42.5 + 99.6, 40.6 + 85.4; of 256 with 512 queries: 43.0 + 95.1, 43.6 + 100.8.  For many rows and keys it would add
-// a third to a half to the products that bound those kernels, for errors that are 1.41 times those of the results' rounding.
+// 128: 42.5 + 99.6, 40.6 + 85.4; of 256 with 512 queries: 43.0 + 95.1, 43.6 + 100.8.  For many rows and keys, where the
+// products bound the kernels, results of either 16-bit type are off by 1.41 times their own rounding, and two operands
+// would cost (forward, backward): 8 x 1024 queries, 2048 keys, 12 heads of 64: 65, 190 against 105, 280; of 128 on 4: 105,
+// 389 against 178, 573; 8 x 2048 queries, 4099 keys: 180 against 282.
 constexpr int CA_FINE_KEYS = 32;
 CaPlan ca_forward_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t dh, int dtype);
 CaPlan ca_backward_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hk, int64_t G, int64_t dh, int dtype);

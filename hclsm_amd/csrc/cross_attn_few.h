@@ -122,7 +122,8 @@ __device__ __forceinline__ void ca_few_store(int dh, const caf4* o, float f, boo
 // registers, one step ahead: no value is read by two waves, so LDS would only add a copy.
 // What bounds it: reading k and v.  Measured (bf16): one query on 100352 keys, 16 heads of 128 on 4, keys split over 64
 // workgroups per key head: 41 us, 4.9 TB/s, and 5 us to join; 64 single queries on up to 1568 keys, 12 heads of 64: 46 us,
-// 4.2 TB/s; float32, 32 slots on 196 tokens of 64 frames, 6 heads of 64: 18 us, 2.5 TB/s.  A 1 GiB copy reaches 5.1 TB/s.
+// 4.2 TB/s; float32, 32 slots on 196 tokens of 64 frames, 6 heads of 64: 17 us, 2.6 TB/s (two steps of keys to a wave: its
+// time is the wait for the first and the joining).  A 1 GiB copy reaches 5.1 TB/s.
 template <int DT, int DH, int NW, int QT>
 __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
   using A = CaT<DT>;
@@ -327,8 +328,9 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
 // split over workgroups, by ca_sum_kernel).  Both orientations of the scores are formed, S^T (a lane per row) for
 // dQ^T = K^T ds^T and S (a lane per key) for dV^T = g^T p and dK^T = Q^T ds: the key's operand registers serve both, and
 // moving ds between the lanes would cost more than the second product.  What bounds it: reading q, g, out and k, v once
-// and writing dq, dk, dv.  Measured: 32 slots on 196 tokens of 256 frames, 6 heads of 64, bf16: 53 us, 3.4 TB/s (the two
-// tiled kernels: 83 us).
+// and writing dq, dk, dv.  Measured: 32 slots on 196 tokens of 256 frames, 6 heads of 64, bf16: 54 us, 3.4 TB/s (the two
+// tiled kernels: 67 us); matrix unit busy 10% of the cycles, vector unit 32%: a wave has one or two steps of keys and waits
+// for the rows, and for each step's keys, with nothing else to do.
 template <int DT, int DH, int NW>
 __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) ca_few_bwd_kernel(const CaArgs a) {
   using A = CaT<DT>;

@@ -26,8 +26,9 @@ template <int ROWS> constexpr uint64_t CA_FULL = ROWS == 64 ? ~0ull : (1ull << (
 //
 // NW waves of 16 QT rows each over tiles of KR keys in LDS (two buffers, one barrier per tile), with the running
 // maximum and sum of the softmax per row.  Statistics and accumulators are float32; the weights are rounded to the
-// operand type (PARTS operands, 2 for few keys) for the second product (half a step, 2^-8 of the value for bf16 and 2^-11 for fp16; the matrix unit has no
-// wider operand at this rate), their sum is not: the log-sum that the backward reads is the float32 one.
+// operand type (PARTS operands, 2 for few keys) for the second product (half a step, 2^-8 of the value for bf16 and 2^-11
+// for fp16; the matrix unit has no wider operand at this rate), their sum is not: the log-sum that the backward reads is
+// the float32 one.
 //
 // What bounds it: the exponentials and the matrix unit together.  Heads of 64 need 512 matrix cycles and about 650 of
 // the vector unit (a multiply-add, an exponential, an addition, half a conversion and half a maximum per score) for a
@@ -37,9 +38,11 @@ template <int ROWS> constexpr uint64_t CA_FULL = ROWS == 64 ? ~0ull : (1ull << (
 // slower); raised priorities around the products or for every other wave; 8 waves to a workgroup; 16 or 48 rows to a
 // wave.  Two or three tiles on their way instead of one change nothing (heads of 64: 144 and 143 us; of 128 with tiles of
 // 64 keys: 118 both; with tiles of 32, which leave room for three, 137), so the transfers are not what it waits for.
-// Measured (bf16): 174 us there (0.80 PFLOP/s over the live keys); 8 x 2048 queries, 4096 keys, 12 heads of 128: 388 us
-// (1.06 PFLOP/s); 8 x 1024, 2048 keys, 12 heads of 128 on 4: 118 us (0.87: 768 workgroups on 512 places).  A matrix
-// product of 8192^3 by the library reaches 1.27 PFLOP/s on the same card.
+// Measured (bf16): 176 to 182 us there (0.77 PFLOP/s over the live keys); 8 x 2048 queries, 4096 keys, 12 heads of 128: 394 us
+// (1.05 PFLOP/s); 8 x 1024, 2048 keys, 12 heads of 128 on 4: 105 us (0.98).  Heads of 128: matrix unit 36%, vector unit
+// 41%; the rest is the barrier of every tile and the last round (768 workgroups on 512 places).  A matrix product of
+// 8192^3 by the library reaches 1.23 to 1.27 PFLOP/s on the same cards.  Float32, 2 x 1024 queries, 2048 keys, 12 heads of 64: 142
+// us with the join of two splits (91 TFLOP/s of the library's 154), of 128: 264 (98), of 256: 654 (79).
 template <int DT, int DH, int NW, int QT, int KR, int PARTS>
 __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
   using A = CaT<DT>;
@@ -248,8 +251,9 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
 // dQ^T = K^T ds^T.  delta = sum(g o) per row is formed here and left for the second kernel.  ds is rounded to the
 // operand type for its product, as the weights are in the forward (float16: at a power of two of its own, CA_RANGED).
 // Three products, two of which the kernel for dk and dv forms again: that costs two products in seven, and leaves no sum
-// of dq over key tiles to atomics.  Measured: 8 x 1024 queries, 2048 keys, 12 heads of 128 on 4, bf16:
-// 186 us, 0.83 PFLOP/s; matrix unit busy 34%.
+// of dq over key tiles to atomics.  Measured: 8 x 1024 queries, 2048 keys, 12 heads of 128 on 4, bf16: 174 us, 0.89 PFLOP/s;
+// matrix unit busy 34% of the cycles, vector unit 29%: a third of them neither works (one wave per SIMD, a barrier per tile,
+// 768 workgroups on 512 places).  Float32, 2 x 1024, 2048 keys, 12 heads of 64: 199 us (97 TFLOP/s), of 128: 400 (97).
 template <int DT, int DH, int NW, int QT, int KR, bool PIPE, int PARTS>
 __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
   using A = CaT<DT>;
@@ -469,8 +473,9 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
 // NW waves of 16 KT keys each, K and V operands in registers, over tiles of RR rows (q and g in LDS):
 // S = Q K^T and dP = g V^T with a lane per key, then dV^T = g^T p and dK^T = Q^T ds.  Shared heads are rows of the
 // unit, so their gradients are added here.  Keys that are not live get zeros.
-// Four products.  Measured on the sizes above: 236 us, 0.87 PFLOP/s; matrix unit busy 37%, one wave per SIMD (the accumulators
-// and operands of 32 keys of 128 take 300 registers; 16 keys per wave and two waves per SIMD measured the same).
+// Four products.  Measured on the sizes above: 389 us with dq, so 215 of its own, 0.96 PFLOP/s; matrix unit busy 37% of the
+// cycles, vector unit 31%, one wave per SIMD (the accumulators and operands of 32 keys of 128 take 300 registers; 16 keys per wave and
+// two waves per SIMD measured the same).  Float32: 266 us (97 TFLOP/s) and 430 (120).
 template <int DT, int DH, int NW, int KT, int RR, bool PIPE, int PARTS>
 __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
   using A = CaT<DT>;
@@ -703,10 +708,10 @@ template <int DT, int DH> struct CaShape {
   static constexpr int TR = RB <= 256 ? 64 : 32;      // rows of a tile
   static constexpr int T = RB <= 256 ? 2 : 1;         // 16-row tiles per wave
   // Scores of the next step formed while the vector unit works on this one's: a second set of score tiles, which
-  // pays where it leaves the same number of waves per SIMD.  Measured on 8 x 1024 queries, 2048 keys, bf16 (us without ->
-  // with): dq of heads of 32: 110 -> 112, 64: 170 -> 163, 96: 126 -> 121, 128: 185 -> 183, 192: 198 -> 200, 256: 174 -> 209;
-  // dk and dv 134 -> 146, 217 -> 212, 196 -> 208, 258 -> 238, 281 -> 272, 336 -> 356; float32 heads of 64 (2 batch rows):
-  // 392 -> 383 and 423 -> 415, of 128: 407 -> 397 and 463 -> 488.
+  // pays where it leaves the same number of waves per SIMD.  Measured on 8 x 1024 queries, 2048 keys, 12 heads, bf16 (us
+  // without -> with): dq of heads of 32: 69 -> 66, 64: 103 -> 96, 96: 128 -> 127, 128: 177 -> 181, 192: 301 -> 289, 256: 328
+  // -> 356; dk and dv 78 -> 77, 126 -> 122, 211 -> 225, 284 -> 253, 419 -> 389, 637 -> 690; float32 (2 batch rows), heads of
+  // 64: 194 -> 194 and 265 -> 266, of 128: 397 -> 394 and 431 -> 460.
   static constexpr bool PIPE_Q = RB <= 256, PIPE_KV = RB <= 256 && DH % 64 == 0;
   static constexpr int FINE = DT == HCLSM_F32 ? 1 : 2;      // operands that hold the weights of few keys
   static_assert(4 * CaTile<DT, DH>::bytes(TR, 256) + 2 * TR * 8 <= 160 * 1024, "two buffers of two tiles");

@@ -13,7 +13,7 @@
 // What bounds it: HBM.  A row is spread over G lanes that hold V pairs each: two vectors of V elements per lane and row,
 // V = 4 where rot, dh, the strides and the addresses allow it (16 B loads of float32, 8 B of 16-bit elements), else 2 or 1.
 // 16-byte loads of 16-bit elements would halve the lanes and double what each keeps (weights, their gradients, angles):
-// 52 -> 90 us for the backward below, 35 -> 38 us for its forward.  A lane group takes a token's heads one after another,
+// 52 -> 73 us for the backward below, 36 -> 41 us for its forward.  A lane group takes a token's heads one after another,
 // the next loads in flight, so that an angle (about 40 instructions, some in float64) serves all of them; where the tokens
 // alone do not fill the chip, a token's heads are shared by several groups.
 // Measured (bf16, 32 x 1568 tokens, 6 + 6 heads of 64): forward 35 us and backward 52 us, 4.4 TB/s of the bytes that have to

@@ -646,6 +646,7 @@ typedef struct HclsmHeads {
  *   pair (a, b) of frequency i -> amplitude * (a cos t - b sin t, b cos t + a sin t),  t = 2 pi * position * turns[i].
  * turns: [rot / 2] float64 on the device (angular frequency / 2 pi; NULL with rot = 0).  rot is even, 0 <= rot <= dh,
  * 1 <= dh <= 256; layout HCLSM_ROTARY_*.  k is nullable and may differ from q in B, L and H.  y may not overlap x.
+ * B L H past 2^31 - 1 is HCLSM_ERR_UNSUPPORTED.
  * Angles are formed in float64, everything else in float32 with one rounding at the store.
  */
 int hclsm_norm_rotary_forward(const HclsmHeads* q, const HclsmHeads* k, int64_t dh, int64_t rot, int layout,
@@ -699,7 +700,7 @@ int64_t hclsm_cross_attention_workspace(int64_t B, int64_t Lq, int64_t Lk, int64
  * a batch row without a live key, get out = 0 and lse = -inf.
  * H is a multiple of Hk; dh a multiple of 8 up to 256 (HCLSM_ERR_UNSUPPORTED otherwise).  Scores, softmax and sums in
  * float32; 16-bit operands round the weights to their type for the product with v (few rows or at most 32 keys: the
- * rounding's rest is a second operand).
+ * rounding's rest is a second operand; float16: scaled so that the largest is 2^11 to 2^15).
  * (The reference runs torch's nn.MultiheadAttention here: dynamics/level2_goal.py:50,63, multimodal_fuser.py:40.)
  */
 int hclsm_cross_attention_forward(const HclsmCrossAttention* x, void* workspace, int64_t workspace_bytes, void* stream);
@@ -707,6 +708,7 @@ int hclsm_cross_attention_forward(const HclsmCrossAttention* x, void* workspace,
 /*
  * Gradients of sum(g * out): dq, dk, dv, with out and lse as the forward left them.  Queries that are not live give
  * and get none; keys that are not live get zeros.  Sums over shared heads and over rows in a fixed order (no atomics).
+ * float16 gradients of scores are rounded at a power of two of their own per row of dq and key of dk, whatever g's size.
  */
 int hclsm_cross_attention_backward(const HclsmCrossAttention* x, void* workspace, int64_t workspace_bytes, void* stream);
 
