@@ -142,9 +142,9 @@ __device__ __forceinline__ float ca_rows4_max(float x) {
 
 // Scores' gradients ds = p (dP - delta) of a row lie around |g| / Lk, which float16 (2^-24 to 65504) does not hold for small g
 // or many keys, nor for large g and v.  They are rounded as ds times a power of two, one for each row of dq and each key
-// of dk (a lane's own result column, so the factor leaves the sum again exactly): it starts at 2^CA_F16_START and is lowered, the sums so far
-// with it, when a value would pass 2^15, so that the largest one lies at 2^10 or above and values down to 2^-24 of it keep
-// all their bits.  The rms error of dq and dk is then 1.41 times that of the results' rounding for g of any size (two
+// of dk (a lane's own result column, so the factor leaves the sum again exactly): it starts at 2^CA_F16_START and is lowered,
+// the sums so far with it, when a value would pass 2^15, so that the largest one lies at 2^10 or above and values down to
+// 2^-24 of it keep all their bits.  The rms error of dq and dk is then 1.41 times that of the results' rounding for g of any size (two
 // operands: 1.0), where plain rounding gave 5 to 22 times for g of 1e-3 and 4096 to 32768 keys.  Measured (us, without and
 // with it): 8 x 1024 queries, 2048 keys, 12 heads of 64: dq 93, 104, dk and dv 118, 128; of 128 on 4: 205, 220 and 269, 293;
 // 256 frames, 32 slots, 196 tokens, 6 heads of 64: 50, 52.

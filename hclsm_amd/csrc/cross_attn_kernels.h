@@ -39,10 +39,10 @@ template <int ROWS> constexpr uint64_t CA_FULL = ROWS == 64 ? ~0ull : (1ull << (
 // wave.  Two or three tiles on their way instead of one change nothing (heads of 64: 144 and 143 us; of 128 with tiles of
 // 64 keys: 118 both; with tiles of 32, which leave room for three, 137), so the transfers are not what it waits for.
 // Measured (bf16): 176 to 182 us there (0.77 PFLOP/s over the live keys); 8 x 2048 queries, 4096 keys, 12 heads of 128: 394 us
-// (1.05 PFLOP/s); 8 x 1024, 2048 keys, 12 heads of 128 on 4: 105 us (0.98).  Heads of 128: matrix unit 36%, vector unit
-// 41%; the rest is the barrier of every tile and the last round (768 workgroups on 512 places).  A matrix product of
-// 8192^3 by the library reaches 1.23 to 1.27 PFLOP/s on the same cards.  Float32, 2 x 1024 queries, 2048 keys, 12 heads of 64: 142
-// us with the join of two splits (91 TFLOP/s of the library's 154), of 128: 264 (98), of 256: 654 (79).
+// (1.05 PFLOP/s); 8 x 1024, 2048 keys, 12 heads of 128 on 4: 105 us (0.98), matrix unit 36%, vector unit 41% of the
+// cycles with 1.46 waves per SIMD on average of the 2 that fit (768 workgroups on 512 places: the last round is half full).
+// A matrix product of 8192^3 by the library reaches 1.23 to 1.27 PFLOP/s on the same cards.  Float32, 2 x 1024 queries, 2048
+// keys, 12 heads of 64: 142 us with the join of two splits (91 TFLOP/s of the library's 154), of 128: 264 (98), of 256: 654 (79).
 template <int DT, int DH, int NW, int QT, int KR, int PARTS>
 __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
   using A = CaT<DT>;
@@ -252,8 +252,9 @@ __global__ void __launch_bounds__(64 * NW) ca_fwd_kernel(const CaArgs a) {
 // operand type for its product, as the weights are in the forward (float16: at a power of two of its own, CA_RANGED).
 // Three products, two of which the kernel for dk and dv forms again: that costs two products in seven, and leaves no sum
 // of dq over key tiles to atomics.  Measured: 8 x 1024 queries, 2048 keys, 12 heads of 128 on 4, bf16: 174 us, 0.89 PFLOP/s;
-// matrix unit busy 34% of the cycles, vector unit 29%: a third of them neither works (one wave per SIMD, a barrier per tile,
-// 768 workgroups on 512 places).  Float32, 2 x 1024, 2048 keys, 12 heads of 64: 199 us (97 TFLOP/s), of 128: 400 (97).
+// matrix unit busy 34% of the cycles, vector unit 29%, 0.92 waves per SIMD of the one that its registers leave (three whole
+// rounds): in what is left that wave waits, hardly for LDS (2% of its time).  Float32, 2 x 1024, 2048 keys, 12 heads of 64: 199
+// us (97 TFLOP/s), of 128: 400 (97).
 template <int DT, int DH, int NW, int QT, int KR, bool PIPE, int PARTS>
 __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
   using A = CaT<DT>;
@@ -474,8 +475,9 @@ __global__ void __launch_bounds__(64 * NW) ca_dq_kernel(const CaArgs a) {
 // S = Q K^T and dP = g V^T with a lane per key, then dV^T = g^T p and dK^T = Q^T ds.  Shared heads are rows of the
 // unit, so their gradients are added here.  Keys that are not live get zeros.
 // Four products.  Measured on the sizes above: 389 us with dq, so 215 of its own, 0.96 PFLOP/s; matrix unit busy 37% of the
-// cycles, vector unit 31%, one wave per SIMD (the accumulators and operands of 32 keys of 128 take 300 registers; 16 keys per wave and
-// two waves per SIMD measured the same).  Float32: 266 us (97 TFLOP/s) and 430 (120).
+// cycles, vector unit 31%, one wave per SIMD, which waits for the rest as in ca_dq_kernel (the accumulators and operands of 32
+// keys of 128 take 300 registers; 16 keys per wave and two waves per SIMD measured the same).  Float32: 266 us (97 TFLOP/s)
+// and 430 (120).
 template <int DT, int DH, int NW, int KT, int RR, bool PIPE, int PARTS>
 __global__ void __launch_bounds__(64 * NW) ca_dkv_kernel(const CaArgs a) {
   using A = CaT<DT>;
