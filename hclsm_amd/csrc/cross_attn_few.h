@@ -331,6 +331,7 @@ __global__ void __launch_bounds__(64 * NW) ca_few_kernel(const CaArgs a) {
 // and writing dq, dk, dv.  Measured: 32 slots on 196 tokens of 256 frames, 6 heads of 64, bf16: 54 us, 3.4 TB/s (the two
 // tiled kernels: 67 us); matrix unit busy 10% of the cycles, vector unit 32%: a wave has one or two steps of keys and waits
 // for the rows, and for each step's keys, with nothing else to do.
+// Two workgroups to a CU are asked for with heads up to 64: float16 would take one register more than that leaves.
 template <int DT, int DH, int NW>
 __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 2 : 1) ca_few_bwd_kernel(const CaArgs a) {
   using A = CaT<DT>;
