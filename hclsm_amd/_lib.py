@@ -99,6 +99,14 @@ _SIGNATURES: dict[str, list] = {
     "hclsm_cross_attention_workspace": [_i64] * 6 + [_int, _int],
     "hclsm_cross_attention_forward": [_c_void_p, _c_void_p, _i64, _c_void_p],
     "hclsm_cross_attention_backward": [_c_void_p, _c_void_p, _i64, _c_void_p],
+    "hclsm_linear_attention_workspace": [_i64] * 6 + [_int, _int],
+    "hclsm_linear_attention_forward": [_c_void_p, _c_void_p, _i64, _c_void_p],
+    "hclsm_linear_attention_backward": [_c_void_p, _c_void_p, _i64, _c_void_p],
+    "hclsm_linear_attention_step": [_c_void_p, _c_void_p],
+    "hclsm_residual_norm_forward": [_c_void_p, _c_void_p],
+    "hclsm_residual_norm_fp8": [_c_void_p, _c_void_p],
+    "hclsm_residual_norm_backward_workspace": [_i64, _i64],
+    "hclsm_residual_norm_backward": [_c_void_p, _c_void_p, _i64, _c_void_p],
     "hclsm_issue_probe": [_int, _i64, _int, _c_void_p, _c_void_p],
 }
 _RESTYPES = {"hclsm_strerror": ctypes.c_char_p, "hclsm_slot_attn_core_workspace": ctypes.c_int64,
@@ -111,6 +119,8 @@ _RESTYPES = {"hclsm_strerror": ctypes.c_char_p, "hclsm_slot_attn_core_workspace"
              "hclsm_slot_track_sequence_workspace": ctypes.c_int64,
              "hclsm_norm_rotary_backward_workspace": ctypes.c_int64,
              "hclsm_cross_attention_workspace": ctypes.c_int64,
+             "hclsm_linear_attention_workspace": ctypes.c_int64,
+             "hclsm_residual_norm_backward_workspace": ctypes.c_int64,
              "hclsm_event_top_down_workspace": ctypes.c_int64, "hclsm_gnn_message_pass_workspace": ctypes.c_int64}
 
 
@@ -133,10 +143,23 @@ CROSS_FIELDS = (("q", "k", "v", "g", "out", "out_lo", "lse", "dq", "dk", "dv", "
                  "key_pad_sb", "B", "Lq", "Lk", "H", "Hk", "dh"),
                 ("scale", "dtype", "key_lens_dtype", "query_lens_dtype"))
 pack_cross = struct.Struct("@13P19qf3i").pack
+LINEAR_FIELDS = (("q", "k", "v", "g", "log_decay", "state_in", "state_out", "dstate_out", "dstate_in", "out", "dq", "dk_out",
+                  "dv_out", "seq_lens"),
+                 ("q_sb", "q_sl", "q_sh", "k_sb", "k_sl", "k_sh", "v_sb", "v_sl", "v_sh", "g_sb", "g_sl", "g_sh", "B", "L", "H",
+                  "Hk", "dk", "dv"), ("scale", "dtype", "seq_lens_dtype"))
+pack_linear = struct.Struct("@14P18qf2i0q").pack
+STEP_FIELDS = (("q", "k", "v", "log_decay", "state", "rows", "out"),
+               ("q_sb", "q_sh", "k_sb", "k_sh", "v_sb", "v_sh", "state_sb", "n_states", "B", "H", "Hk", "dk", "dv"),
+               ("scale", "dtype", "rows_dtype"))
+pack_step = struct.Struct("@7P13qf2i0q").pack
+RESIDUAL_FIELDS = (("x", "r", "w", "h", "gy", "gh", "y", "h_out", "scale", "dx", "dr", "dw"),
+                   ("x_sr", "r_sr", "h_sr", "gy_sr", "gh_sr", "rows", "D", "group"),
+                   ("eps", "dtype", "stream_dtype", "w_dtype"))
+pack_residual = struct.Struct("@12P8qf3i").pack
 
 
 def _block(name, pointers, sizes, rest):
-    kinds = lambda n: ctypes.c_float if n == "scale" else ctypes.c_int
+    kinds = lambda n: ctypes.c_float if n in ("scale", "eps") else ctypes.c_int
     fields = ([(n, ctypes.c_void_p) for n in pointers] + [(n, ctypes.c_int64) for n in sizes] +
               [(n, kinds(n)) for n in rest])
     return type(name, (ctypes.Structure,), {"_fields_": fields, "__doc__": f"Mirror of the C struct {name}."})
@@ -144,6 +167,9 @@ def _block(name, pointers, sizes, rest):
 
 HclsmHeads = _block("HclsmHeads", *HEADS_FIELDS)
 HclsmCrossAttention = _block("HclsmCrossAttention", *CROSS_FIELDS)
+HclsmLinearAttention = _block("HclsmLinearAttention", *LINEAR_FIELDS)
+HclsmLinearAttentionStep = _block("HclsmLinearAttentionStep", *STEP_FIELDS)
+HclsmResidualNorm = _block("HclsmResidualNorm", *RESIDUAL_FIELDS)
 
 _lib = None
 

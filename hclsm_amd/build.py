@@ -41,6 +41,9 @@ FILE_FLAGS = {
     "cross_attn_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "cross_attn_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "cross_attn_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "linear_attn_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "linear_attn_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "linear_attn_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -1,0 +1,10 @@
+// Linear attention on bfloat16 inputs.
+#include "linear_attn_kernels.h"
+
+namespace hclsm {
+
+int la_launch_bf16(const LaArgs& a, int da, int xt, bool sum, hipStream_t st) {
+  return la_launch<HCLSM_BF16>(a, da, xt, sum, st);
+}
+
+}  // namespace hclsm

@@ -45,6 +45,10 @@ from hclsm_amd.kernels.cross_attention import cross_attention
 
 from hclsm_amd.kernels.norm_rotary import RotaryPlan, qk_norm_rotary, rotary_embedding
 
+from hclsm_amd.kernels.linear_attention import linear_attention, linear_attention_step
+
+from hclsm_amd.kernels.residual_norm import residual_rms_norm, residual_rms_norm_fp8
+
 from hclsm_amd.kernels.slot_attention_kernel import (
     slot_attention_core,
     slot_attention_fn,
@@ -129,6 +133,10 @@ __all__ = [
     "RotaryPlan",
     "rotary_embedding",
     "qk_norm_rotary",
+    "linear_attention",
+    "linear_attention_step",
+    "residual_rms_norm",
+    "residual_rms_norm_fp8",
     "gnn_message_pass_fn",
     "naive_gnn_message_pass",
     "optimized_gnn_message_pass",

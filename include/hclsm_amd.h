@@ -712,6 +712,114 @@ int hclsm_cross_attention_forward(const HclsmCrossAttention* x, void* workspace,
  */
 int hclsm_cross_attention_backward(const HclsmCrossAttention* x, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Linear attention with a decay for each head.  Strides in elements (innermost 1); rows of q, k, v and g, every output of
+ * their type, and the workspace lie on 16-byte boundaries (HCLSM_ERR_UNSUPPORTED otherwise).  States are float32, contiguous
+ * [B, H, dk, dv]. */
+typedef struct HclsmLinearAttention {
+  const void* q;             /* [B, L, H, dk] */
+  const void* k;             /* [B, L, Hk, dk]: head h reads key head h / (H / Hk) */
+  const void* v;             /* [B, L, Hk, dv] */
+  const void* g;             /* backward: gradient of out, [B, L, H, dv] */
+  const float* log_decay;    /* [H], <= 0 (-inf: no memory) */
+  const float* state_in;     /* state in front of the first token, nullable (zeros) */
+  float* state_out;          /* forward: state behind the last live token, nullable (not written) */
+  const float* dstate_out;   /* backward: gradient of state_out, nullable (zeros) */
+  float* dstate_in;          /* backward: gradient of state_in, nullable (not formed) */
+  void* out;                 /* forward: contiguous [B, L, H, dv] */
+  void* dq;                  /* backward: contiguous as q, k, v; each nullable (not formed) */
+  void* dk_out;
+  void* dv_out;
+  const void* seq_lens;      /* [B] live tokens, nullable (all); clamped to 0 .. L; HCLSM_POS_I32 / _I64 */
+  int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, g_sb, g_sl, g_sh;
+  int64_t B, L, H, Hk, dk, dv;
+  float scale;               /* > 0 */
+  int dtype, seq_lens_dtype;
+} HclsmLinearAttention;
+
+/* Workspace bytes of hclsm_linear_attention_forward (backward = 0) or _backward (1); HCLSM_ERR_* for sizes they refuse. */
+int64_t hclsm_linear_attention_workspace(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t dk, int64_t dv, int dtype,
+                                         int backward);
+
+/*
+ * S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T (S_{-1} = state_in),  out_t = scale * q_t^T S_t,  state_out = S behind the last
+ * live token.  Tokens from seq_lens[b] on are not read, get out = 0 and leave the state as it is.
+ * dk and dv are multiples of 8 up to 256, H a multiple of Hk, B H at most 2^20 (HCLSM_ERR_UNSUPPORTED otherwise).
+ * Operands of the matrix products are float32 values in two bf16 parts (three for float32 inputs and for the state's own
+ * update), sums and states float32.  No counterpart in the reference, whose time mixing is the selective scan
+ * (kernels/ssm_scan_kernel.py).
+ */
+int hclsm_linear_attention_forward(const HclsmLinearAttention* x, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Gradients of sum(g * out) + sum(dstate_out * state_out) for q, k, v and state_in (log_decay has none).  Tokens that
+ * are not live get zeros.  Gradients of shared heads are summed in float32 in a fixed order; no atomics.
+ */
+int hclsm_linear_attention_backward(const HclsmLinearAttention* x, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One token of B streams. */
+typedef struct HclsmLinearAttentionStep {
+  const void* q;             /* [B, H, dk] */
+  const void* k;             /* [B, Hk, dk] */
+  const void* v;             /* [B, Hk, dv] */
+  const float* log_decay;    /* [H] */
+  float* state;              /* [n_states, H, dk, dv], batch stride state_sb, 16-byte boundaries: updated in place */
+  const void* rows;          /* [B] the state of each stream, nullable (stream b has state b); HCLSM_POS_I32 / _I64 */
+  void* out;                 /* contiguous [B, H, dv] */
+  int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh, state_sb;
+  int64_t n_states, B, H, Hk, dk, dv;
+  float scale;
+  int dtype, rows_dtype;
+} HclsmLinearAttentionStep;
+
+/*
+ * S = exp(log_decay[h]) S + k v^T in place, out = scale * q^T S.  A stream whose row is negative or past n_states gets
+ * out = 0 and touches no state (padding of a batch).  Rows have to differ: a state that two streams name is left with
+ * either's update, or a mixture.
+ */
+int hclsm_linear_attention_step(const HclsmLinearAttentionStep* x, void* stream);
+
+/* Root-mean-square norm with the residual's addition, for hclsm_residual_norm_*.  Rows have strides of their own (in elements;
+ * their columns are contiguous); outputs are contiguous [rows, D]. */
+typedef struct HclsmResidualNorm {
+  const void* x;       /* forward: [rows, D], element type `dtype` */
+  const void* r;       /* forward: [rows, D] residual, element type stream_dtype; nullable (then the stream is x) */
+  const void* w;       /* [D] weight, nullable (ones); element type w_dtype */
+  const void* h;       /* backward: the stream as the forward wrote it (x where there was no residual) */
+  const void* gy;      /* backward: gradient of y, `dtype`; nullable (zeros) */
+  const void* gh;      /* backward: gradient of the stream, stream_dtype; nullable (zeros) */
+  void* y;             /* forward: `dtype`; 8 bits: e4m3 (no infinities, largest value 448) */
+  void* h_out;         /* forward: the stream x + r in stream_dtype; nullable (not written) */
+  float* scale;        /* 8 bits: [rows, D / group], group 0: [rows] */
+  void* dx;            /* backward: gradient of x in `dtype`; nullable */
+  void* dr;            /* backward: gradient of r in stream_dtype (the same values); nullable */
+  void* dw;            /* backward: [D] gradient of w in w_dtype; nullable (not formed) */
+  int64_t x_sr, r_sr, h_sr, gy_sr, gh_sr;
+  int64_t rows, D, group;
+  float eps;           /* >= 0 */
+  int dtype, stream_dtype, w_dtype;      /* stream_dtype: `dtype` or HCLSM_F32 (`dtype` without a residual) */
+} HclsmResidualNorm;
+
+/*
+ * h = x + r rounded to stream_dtype,  y = h * rsqrt(mean(h^2) + eps) * w  with float32 arithmetic and one rounding.
+ * 1 <= D <= 16384 (HCLSM_ERR_UNSUPPORTED otherwise).  y and h_out may not overlap the inputs.
+ */
+int hclsm_residual_norm_forward(const HclsmResidualNorm* x, void* stream);
+
+/*
+ * The same with y in 8 bits: scale = max(max |y|, 2^-100) / 448 over a row (group 0) or over each `group` of 32, 64 or 128
+ * columns (D a multiple of it, rows on 16-byte boundaries), y8 = y / scale rounded to the nearest e4m3 value.
+ */
+int hclsm_residual_norm_fp8(const HclsmResidualNorm* x, void* stream);
+
+/* Workspace bytes of hclsm_residual_norm_backward where dw is wanted. */
+int64_t hclsm_residual_norm_backward_workspace(int64_t rows, int64_t D);
+
+/*
+ * dh = gh + i (gy w - n mean(gy w n)) with i = rsqrt(mean(h^2) + eps), n = h i, written as dx and dr;  dw = sum over rows of
+ * gy n (partial sums per workgroup in the workspace, added in a fixed order by a second launch; no float atomics).
+ */
+int hclsm_residual_norm_backward(const HclsmResidualNorm* x, void* workspace, int64_t workspace_bytes, void* stream);
+
 /*
  * VALU issue-rate probe (measurement support; no counterpart in the reference, whose kernels have no
  * roofline).  Launches `waves` one-wave workgroups; each runs `iters` iterations of a fixed block of
