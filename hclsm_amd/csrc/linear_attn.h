@@ -37,14 +37,16 @@ struct LaJob {
   const float* s0;         // [B, H] states, nullable (zeros)
   float* s1;               // states behind the last token, nullable
   float* seg;              // [B * H][nseg][da][dx]: sums of segments, then the states in front of them (nseg > 1)
-  int64_t s_r, s_c;        // element strides of a state's da and dx
+  int s_r, s_c;            // element strides of a state's da and dx
   int da, dx, xtiles, shift, y32, back;
   float cp, ci, cu;
 };
 
 struct LaArgs {
   LaJob job[3];
-  uint32_t first[4];       // workgroups of the jobs: job i has first[i] .. first[i + 1] - 1
+  uint32_t per;            // workgroups of a segment: the column tiles of all jobs
+  int items, by_xcd;       // B H nseg segments; whether they are dealt out to the XCDs
+  int fine;                // the state is a result: its sums take X in three planes, not two
   const float* log_decay;  // [H]
   const void* lens;        // [B] live tokens, nullable
   int lens64, njobs;
@@ -52,15 +54,19 @@ struct LaArgs {
   int seg_tokens;          // tokens of a segment, whole chunks (nseg > 1)
 };
 
-// Tokens of a chunk: 64, or 32 where the planes of wide heads would not fit the LDS.
-constexpr int la_chunk(int dtype, int da) { return dtype == HCLSM_F32 || (dtype == HCLSM_F16 && da > 128) ? 32 : 64; }
+// Tokens of a chunk: 64, or 32 where the planes (bf16: the two tiles) of wide heads would not fit the LDS.
+constexpr int la_chunk(int dtype, int da) { return dtype == HCLSM_F32 || da > 128 || (dtype == HCLSM_F16 && da > 64) ? 32 : 64; }
 constexpr int la_padded(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-constexpr int la_xt(int64_t dx) { return dx <= 64 ? 64 : 128; }
+constexpr int LA_THREADS = 256, LA_XT = 64;
+// Waves per SIMD that the registers are to leave room for (the LDS holds no more workgroups).
+constexpr int la_waves(int dtype, int da) {
+  return dtype == HCLSM_BF16 ? (da <= 64 ? 3 : 2) : da == 64 ? (dtype == HCLSM_F32 ? 3 : 2) : da == 128 ? 2 : 1;
+}
 
-// One launch of jobs that share padded sizes (sum: the sums of segments alone).
-int la_launch_f32(const LaArgs& a, int da, int xt, bool sum, hipStream_t st);
-int la_launch_bf16(const LaArgs& a, int da, int xt, bool sum, hipStream_t st);
-int la_launch_f16(const LaArgs& a, int da, int xt, bool sum, hipStream_t st);
+// One launch of jobs that share a padded size (sum: the sums of segments alone).
+int la_launch_f32(const LaArgs& a, int da, bool sum, hipStream_t st);
+int la_launch_bf16(const LaArgs& a, int da, bool sum, hipStream_t st);
+int la_launch_f16(const LaArgs& a, int da, bool sum, hipStream_t st);
 
 // The decay of a head as the kernels use it: -inf (no memory) as a number whose multiples stay finite.
 __device__ __forceinline__ float la_log_decay(const float* g, int h) {

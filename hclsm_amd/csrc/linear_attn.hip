@@ -13,7 +13,7 @@ struct LaPlan {
 
 LaPlan la_plan(int64_t workgroups, int64_t L, int chunk) {
   const int64_t chunks = (L + chunk - 1) / chunk;
-  int64_t n = workgroups > 0 ? 768 / workgroups : 1;
+  int64_t n = workgroups > 0 ? (workgroups < 256 ? 768 / workgroups : 1) : 1;
   n = n > chunks / 4 ? chunks / 4 : n;
   n = n > LA_MAX_SEGMENTS ? LA_MAX_SEGMENTS : n;
   if (n <= 1) return {1, 0};
@@ -27,7 +27,7 @@ struct LaSizes {
   int64_t B, L, H, Hk, dk, dv;
   int dtype;
   int64_t units() const { return B * H; }
-  int64_t tiles(int64_t dx) const { return (dx + la_xt(dx) - 1) / la_xt(dx); }
+  int64_t tiles(int64_t dx) const { return (dx + LA_XT - 1) / LA_XT; }
   // chunks of the widest job decide for all jobs of a call
   int chunk(bool bwd) const {
     const int c = la_chunk(dtype, la_padded(dk)), d = la_chunk(dtype, la_padded(dv));
@@ -51,11 +51,16 @@ int la_sizes(const LaSizes& z) {
   if (z.dtype < HCLSM_F32 || z.dtype > HCLSM_F16) return HCLSM_ERR_DTYPE;
   if (z.H > 0 && (z.Hk == 0 || z.H % z.Hk != 0)) return HCLSM_ERR_SHAPE;
   if (z.dk > LA_MAX_DIM || z.dv > LA_MAX_DIM || z.dk % 8 || z.dv % 8) return HCLSM_ERR_UNSUPPORTED;
-  // workgroups of one launch (three jobs of up to two column tiles and LA_MAX_SEGMENTS segments) have fewer than 2^32 threads
+  // workgroups of one launch (three jobs of up to four column tiles) have fewer than 2^32 threads
   if (z.B > 0x7fffffff || z.H > 0x7fffffff || z.L > 0x7fffffff - 1024) return HCLSM_ERR_UNSUPPORTED;
   if (z.H > 0 && z.B > (1 << 20) / z.H) return HCLSM_ERR_UNSUPPORTED;
+  // a chunk's outputs lie within 31 bits of each other
+  if (z.H * (z.dk > z.dv ? z.dk : z.dv) >= 1 << 23) return HCLSM_ERR_UNSUPPORTED;
   return 0;
 }
+
+// and so do its inputs
+bool la_near(int64_t sl, int esz) { return sl >= 0 && sl * esz < (1 << 24); }
 
 bool la_aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int esz) {
   const int64_t n = 16 / esz;
@@ -74,12 +79,13 @@ __global__ void __launch_bounds__(256) la_prefix_kernel(const LaArgs a) {
   const int d = e / j.dx, c = e - d * j.dx;
   float* p = j.seg + (int64_t)unit * a.nseg * n + e;
   float s = j.s0 ? j.s0[(int64_t)unit * n + d * j.s_r + c * j.s_c] : 0.f;
-  for (int k0 = 0; k0 < a.nseg; k0 += 8) {
-    float u[8];
+  constexpr int NB = 16;
+  for (int k0 = 0; k0 < a.nseg; k0 += NB) {
+    float u[NB];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) u[k] = k0 + k < a.nseg ? p[(int64_t)(k0 + k) * n] : 0.f;
+    for (int k = 0; k < NB; ++k) u[k] = k0 + k < a.nseg ? p[(int64_t)(k0 + k) * n] : 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < NB; ++k) {
       if (k0 + k >= a.nseg) break;
       const int64_t t0 = (int64_t)(j.back ? a.nseg - 1 - k0 - k : k0 + k) * a.seg_tokens;
       const int64_t m = live - t0 < 0 ? 0 : live - t0 > a.seg_tokens ? a.seg_tokens : live - t0;
@@ -111,10 +117,10 @@ int la_group(const float* ws, void* y, int64_t rows, int G, int64_t d, int dtype
   return 0;
 }
 
-int la_launch_any(const LaArgs& a, int dtype, int da, int xt, bool sum, hipStream_t st) {
-  if (dtype == HCLSM_F32) return la_launch_f32(a, da, xt, sum, st);
-  if (dtype == HCLSM_BF16) return la_launch_bf16(a, da, xt, sum, st);
-  return la_launch_f16(a, da, xt, sum, st);
+int la_launch_any(const LaArgs& a, int dtype, int da, bool sum, hipStream_t st) {
+  if (dtype == HCLSM_F32) return la_launch_f32(a, da, sum, st);
+  if (dtype == HCLSM_BF16) return la_launch_bf16(a, da, sum, st);
+  return la_launch_f16(a, da, sum, st);
 }
 
 // All jobs of a call: sums of segments, states in front of them, outputs.  Jobs of the same padded sizes share a launch.
@@ -131,16 +137,17 @@ int la_run(LaArgs a, int dtype, hipStream_t st) {
       if (done[i]) continue;
       LaArgs one = a;
       one.njobs = 0;
-      one.first[0] = 0;
-      const int da = la_padded(a.job[i].da), xt = (int)la_xt(a.job[i].dx);
+      one.per = 0;
+      const int da = la_padded(a.job[i].da);
       for (int k = i; k < a.njobs; ++k) {
-        if (done[k] || la_padded(a.job[k].da) != da || la_xt(a.job[k].dx) != xt) continue;
+        if (done[k] || la_padded(a.job[k].da) != da) continue;
         done[k] = true;
-        one.job[one.njobs] = a.job[k];
-        one.first[one.njobs + 1] = one.first[one.njobs] + (uint32_t)a.B * a.H * a.job[k].xtiles * a.nseg;
-        ++one.njobs;
+        one.per += (uint32_t)a.job[k].xtiles;
+        one.job[one.njobs++] = a.job[k];
       }
-      if (int rc = la_launch_any(one, dtype, da, xt, pass == 0, st)) return rc;
+      one.items = a.B * a.H * a.nseg;
+      one.by_xcd = one.items >= 64;
+      if (int rc = la_launch_any(one, dtype, da, pass == 0, st)) return rc;
     }
   }
   return 0;
@@ -159,6 +166,8 @@ int la_args(const HclsmLinearAttention* x, bool bwd, LaSizes& z) {
     if (!x->q || !x->k || !x->v || (bwd ? !x->g : !x->out)) return HCLSM_ERR_NULL;
     if (!la_aligned(x->q, x->q_sb, x->q_sl, x->q_sh, esz) || !la_aligned(x->k, x->k_sb, x->k_sl, x->k_sh, esz) ||
         !la_aligned(x->v, x->v_sb, x->v_sl, x->v_sh, esz)) return HCLSM_ERR_UNSUPPORTED;
+    if (!la_near(x->q_sl, esz) || !la_near(x->k_sl, esz) || !la_near(x->v_sl, esz) || (bwd && !la_near(x->g_sl, esz)))
+      return HCLSM_ERR_UNSUPPORTED;
     if (bwd ? !la_aligned(x->g, x->g_sb, x->g_sl, x->g_sh, esz) : !la_aligned(x->out, 0, 0, 0, esz)) return HCLSM_ERR_UNSUPPORTED;
     if (bwd && (!la_aligned(x->dq, 0, 0, 0, esz) || !la_aligned(x->dk_out, 0, 0, 0, esz) || !la_aligned(x->dv_out, 0, 0, 0, esz)))
       return HCLSM_ERR_UNSUPPORTED;
@@ -292,8 +301,9 @@ extern "C" int hclsm_linear_attention_forward(const HclsmLinearAttention* x, voi
   o.s0 = x->state_in;
   o.s1 = x->state_out;
   o.seg = (float*)workspace;
-  o.s_r = z.dv;
+  o.s_r = (int)z.dv;
   o.s_c = 1;
+  a.fine = x->state_out != nullptr;
   o.da = (int)z.dk; o.dx = (int)z.dv;
   o.xtiles = (int)z.tiles(z.dv);
   o.cp = o.ci = x->scale;
@@ -317,6 +327,7 @@ extern "C" int hclsm_linear_attention_backward(const HclsmLinearAttention* x, vo
   float* wk = (float*)(ws + 3 * seg);
   float* wv = (float*)(ws + 3 * seg + la_up(z.B * z.L * z.H * z.dk * 4));
   LaArgs a = la_common(x, z.plan(true));
+  a.fine = x->dstate_in || x->state_in;      // whether its gradient is wanted or not: the others have the same bits
   const LaTensor q = la_tensor(x->q, x->q_sb, x->q_sl, x->q_sh, 1), k = la_tensor(x->k, x->k_sb, x->k_sl, x->k_sh, G),
                  v = la_tensor(x->v, x->v_sb, x->v_sl, x->v_sh, G), g = la_tensor(x->g, x->g_sb, x->g_sl, x->g_sh, 1);
   auto job = [&](const LaTensor& ta, const LaTensor& tb, const LaTensor& tx, int64_t da, int64_t dx, bool turned) {
@@ -324,8 +335,8 @@ extern "C" int hclsm_linear_attention_backward(const HclsmLinearAttention* x, vo
     j.a = ta; j.b = tb; j.x = tx;
     j.da = (int)da; j.dx = (int)dx;
     j.xtiles = (int)z.tiles(dx);
-    j.s_r = turned ? 1 : z.dv;
-    j.s_c = turned ? z.dv : 1;
+    j.s_r = turned ? 1 : (int)z.dv;
+    j.s_c = turned ? (int)z.dv : 1;
     j.seg = (float*)(ws + a.njobs * seg);
     j.cp = x->scale;
     ++a.njobs;

@@ -3,8 +3,8 @@
 
 namespace hclsm {
 
-int la_launch_bf16(const LaArgs& a, int da, int xt, bool sum, hipStream_t st) {
-  return la_launch<HCLSM_BF16>(a, da, xt, sum, st);
+int la_launch_bf16(const LaArgs& a, int da, bool sum, hipStream_t st) {
+  return la_launch<HCLSM_BF16>(a, da, sum, st);
 }
 
 }  // namespace hclsm

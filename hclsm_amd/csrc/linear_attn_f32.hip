@@ -3,8 +3,8 @@
 
 namespace hclsm {
 
-int la_launch_f32(const LaArgs& a, int da, int xt, bool sum, hipStream_t st) {
-  return la_launch<HCLSM_F32>(a, da, xt, sum, st);
+int la_launch_f32(const LaArgs& a, int da, bool sum, hipStream_t st) {
+  return la_launch<HCLSM_F32>(a, da, sum, st);
 }
 
 }  // namespace hclsm

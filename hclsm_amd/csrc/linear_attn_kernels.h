@@ -1,6 +1,7 @@
 // The chunked kernel of linear attention, instantiated for one element type per source file (linear_attn_*.hip).
 #pragma once
 
+#include "cross_attn_stage.h"
 #include "linear_attn.h"
 
 namespace hclsm {
@@ -30,6 +31,7 @@ template <int N> __device__ __forceinline__ void la_split(const float* v, uint4*
     for (int i = 0; i < 4; ++i) {
       w[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
       if (p + 1 < N) {
+        asm("" : "+v"(w[i]));      // (the pair as it is: otherwise each element's conversion is repeated for its rest)
         r[2 * i] -= LaB::lo(w[i]);
         r[2 * i + 1] -= LaB::hi(w[i]);
       }
@@ -55,38 +57,54 @@ template <int NA, int NB, int MOST> __device__ __forceinline__ caf4 la_mma(const
   return acc;
 }
 
-// Rows of one chunk on their way from global memory: eight elements of a row per unit.
+// Rows of one chunk on their way from global memory to LDS: row r of the tile is token r, or n - 1 - r backwards, of the chunk's n
+// live ones; other rows and columns past d are zeros (a load past the buffer resource's end gives zeros).  bf16 goes straight
+// to LDS, the other types through registers, in which they are split into their planes.  The offsets stand for a number of live
+// tokens: they are formed again when that changes.
 template <int DT, int C, int D, int NT> struct LaStage {
-  static constexpr int U = (C * (D / 8) + NT - 1) / NT, RAW = LaT<DT>::RAW, NP = LaT<DT>::NP, ESZ = DT == HCLSM_F32 ? 4 : 2;
+  static constexpr bool DMA = DT == HCLSM_BF16;
+  static constexpr int U = C * (D / 8) / NT, RAW = LaT<DT>::RAW, NP = LaT<DT>::NP, ESZ = DT == HCLSM_F32 ? 4 : 2;
   using Tile = CaTile<HCLSM_BF16, D>;
-  static constexpr int PLANE = C * Tile::STRIDE;
-  uint4 raw[U][RAW];
+  static_assert(Tile::PC == D / 8 && C * (D / 8) % NT == 0, "rows without padding, whole units");
+  static constexpr int PLANE = C * Tile::STRIDE, BYTES = NP * PLANE;
+  static constexpr uint32_t NONE = 0xffffffffu;
+  static constexpr int STEP = NT / (D / 8);     // rows between a thread's units, which therefore have the same chunk
+  static_assert(STEP % 8 == 0, "rows of a thread differ by multiples of 8");
+  uint4 raw[DMA ? 1 : U][RAW];
 
   static __device__ __forceinline__ int row(int u) { return ((int)threadIdx.x + u * NT) / (D / 8); }
-  static __device__ __forceinline__ int chunk(int u) { return ((int)threadIdx.x + u * NT) % (D / 8); }
+  static __device__ __forceinline__ int chunk(int u) { return (((int)threadIdx.x + u * NT) % (D / 8)) ^ Tile::swap(row(u)); }
 
-  // base: the first live token of the chunk at column 0; n live tokens, taken backwards where `back`; d columns
-  __device__ __forceinline__ void load(const char* base, int64_t sl, int n, int d, bool back) {
+  // base: the chunk's first token at column 0; sb: bytes between tokens; n live tokens, d columns
+  __device__ __forceinline__ void load(const char* base, int sb, int n, int d, bool back, char* t, int wave) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, kRawBufferWord3);
+    const int r0 = row(0), c0 = chunk(0) * 8;
+    auto one = [&](int u, int off, int so) __attribute__((always_inline)) {
+      if constexpr (DMA) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (ca_lds_void*)(t + (u * NT + wave * 64) * 16), 16, off, so, 0, 0);
+      } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = row(u), c = chunk(u) * 8;
+        for (int k = 0; k < RAW; ++k)
+          raw[u][k] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, so + 16 * k, 0));
+      }
+    };
+    if (n == C) {
+      // row r0 + u STEP, backwards C - 1 - r0 - u STEP
+      const int off = c0 < d ? (back ? C - 1 - (U - 1) * STEP - r0 : r0) * sb + c0 * ESZ : (int)NONE;
 #pragma unroll
-      for (int k = 0; k < RAW; ++k) raw[u][k] = uint4{0, 0, 0, 0};
-      if (r < n && c < d) {
-        const char* p = base + ((back ? n - 1 - r : r) * sl + c) * ESZ;
+      for (int u = 0; u < U; ++u) one(u, off, (back ? U - 1 - u : u) * STEP * sb);
+    } else {
 #pragma unroll
-        for (int k = 0; k < RAW; ++k) raw[u][k] = reinterpret_cast<const uint4*>(p)[k];
+      for (int u = 0; u < U; ++u) {
+        const int r = r0 + u * STEP;
+        one(u, r < n && c0 < d ? (back ? n - 1 - r : r) * sb + c0 * ESZ : (int)NONE, 0);
       }
     }
   }
   __device__ __forceinline__ void store(char* t) const {
+    if constexpr (!DMA) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (row(u) >= C) break;
-      uint4 w[NP];
-      if constexpr (DT == HCLSM_BF16) {
-        w[0] = raw[u][0];
-      } else {
+      for (int u = 0; u < U; ++u) {
         float v[8];
         if constexpr (DT == HCLSM_F16) {
           const uint32_t x[4] = {raw[u][0].x, raw[u][0].y, raw[u][0].z, raw[u][0].w};
@@ -97,10 +115,11 @@ template <int DT, int C, int D, int NT> struct LaStage {
 #pragma unroll
           for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
         }
+        uint4 w[NP];
         la_split<NP>(v, w);
-      }
 #pragma unroll
-      for (int p = 0; p < NP; ++p) *reinterpret_cast<uint4*>(t + p * PLANE + Tile::off(row(u), chunk(u))) = w[p];
+        for (int p = 0; p < NP; ++p) *reinterpret_cast<uint4*>(t + p * PLANE + ((int)threadIdx.x + u * NT) * 16) = w[p];
+      }
     }
   }
 };
@@ -118,44 +137,115 @@ template <int D> __device__ __forceinline__ LaFrag la_frag_cols(char* t, int row
   return __builtin_bit_cast(LaFrag, r);
 }
 
-// One workgroup: a head of a batch row, XT = 16 NW columns of X (and of the state and the output), one segment of the
+// acc[t] += a b[t] for every t, over the planes as la_mma: products in a row have results of their own.
+template <int NA, int NB, int MOST, int T> __device__ __forceinline__ void la_mma_all(const LaFrag* a, const LaFrag (*b)[NB], caf4* acc) {
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (i + j <= MOST)
+#pragma unroll
+        for (int t = 0; t < T; ++t) acc[t] = LaB::mma(a[i], b[t][j], acc[t]);
+}
+template <int NA, int NB, int MOST, int T> __device__ __forceinline__ void la_mma_all(const LaFrag (*a)[NA], const LaFrag* b, caf4* acc) {
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (i + j <= MOST)
+#pragma unroll
+        for (int t = 0; t < T; ++t) acc[t] = LaB::mma(a[t][i], b[j], acc[t]);
+}
+
+// A barrier for what went through LDS: transfers from global memory to LDS stay in flight (__syncthreads waits for them).
+__device__ __forceinline__ void la_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);      // LDS counter zero (gfx9 encoding), the others as they are
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// S += B^T X for 32 tokens' weighted X (v, the lane's column and tokens) in N planes; four tiles of S at a time, the
+// operands of the next four on their way.
+template <int DA, int NP, int N, int PLANE>
+__device__ __forceinline__ void la_update(char* tb, int row0, const float* v, caf4* s, int li, int g) {
+  constexpr int M = DA / 16;
+  LaFrag fb[2][4][NP];
+  auto get = [&](int m0, LaFrag (*f)[NP]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int p = 0; p < NP; ++p) f[m][p] = la_frag_cols<DA>(tb + p * PLANE, row0, (m0 + m) >> 1, (m0 + m) & 1, li, g);
+  };
+  get(0, fb[0]);
+  uint4 w[N];
+  la_split<N>(v, w);
+  LaFrag fw[N];
+#pragma unroll
+  for (int p = 0; p < N; ++p) fw[p] = ca_frag<HCLSM_BF16>(w[p]);
+#pragma unroll
+  for (int m = 0; m < M; m += 4) {
+    if (m + 4 < M) get(m + 4, fb[(m >> 2) + 1 & 1]);
+    ca_fence();
+    la_mma_all<NP, N, N - 1, 4>(fb[(m >> 2) & 1], fw, s + m);
+    ca_fence();
+  }
+}
+
+// One workgroup of four waves: a head of a batch row, 64 columns of X (and of the state and the output), one segment of the
 // tokens, chunk after chunk.  Wave w owns 16 columns of the state, in registers for the whole segment; the weights of
 // pairs (A_r . B_s) a^(r-s) are shared out over the waves and passed through LDS in the order in which the matrix unit
-// reads them.  SUM: the state alone, from zero (the sum of a segment).
-template <int DT, int DA, int NW, bool SUM>
-__global__ void __launch_bounds__(64 * NW) la_kernel(const LaArgs args) {
-  constexpr int NT = 64 * NW, XT = 16 * NW, C = la_chunk(DT, DA), KT = C / 16, NS = DA / 16, NP = LaT<DT>::NP, NC = LaT<DT>::NC;
+// reads them.  Several workgroups of a CU hide each other's waits.  SUM: the state alone, from zero (the sum of a segment).
+template <int DT, int DA, bool SUM>
+__global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const LaArgs args) {
+  constexpr int NT = LA_THREADS, NW = NT / 64, XT = LA_XT, C = la_chunk(DT, DA), KT = C / 16, NS = DA / 16, NP = LaT<DT>::NP,
+                NC = LaT<DT>::NC;
   constexpr int ESZ = DT == HCLSM_F32 ? 4 : 2, MOST = NC - 1;
-  constexpr int NF = KT == 4 ? 6 : 2;       // pairs of 16-token tiles at or below the diagonal
+  constexpr int NF = KT == 4 ? 6 : 2, NFW = (NF + NW - 1) / NW;     // pairs of 16-token tiles at or below the diagonal
   using SA = LaStage<DT, C, DA, NT>;
   using SX = LaStage<DT, C, XT, NT>;
   using TA = CaTile<HCLSM_BF16, DA>;
   using TX = CaTile<HCLSM_BF16, XT>;
-  __shared__ __attribute__((aligned(16))) char ta[SUM ? 16 : NP * SA::PLANE];
-  __shared__ __attribute__((aligned(16))) char tb[NP * SA::PLANE];
-  __shared__ __attribute__((aligned(16))) char tx[NP * SX::PLANE];
+  constexpr bool DMA = SA::DMA;
+  __shared__ __attribute__((aligned(16))) char ta[SUM ? 16 : SA::BYTES];
+  __shared__ __attribute__((aligned(16))) char buf0[SA::BYTES + SX::BYTES];      // B, X
+  __shared__ __attribute__((aligned(16))) char buf1[DMA ? SA::BYTES + SX::BYTES : 16];
   __shared__ uint4 tp[SUM ? 1 : NF * NC * 64];
-  __shared__ float pw[C + 1];               // powers of the decay
-  __shared__ float em[C + 1];               // a^n - 1
+  __shared__ __attribute__((aligned(16))) float rx[C];      // cu a^(n - 1 - r + shift): of row r in the state's sum
 
-  uint32_t i = blockIdx.x;
+  // Workgroup i runs on XCD i % 8, each with its own L2: the jobs and column tiles of a segment, which read the same rows, are
+  // given to one of them.
+  uint32_t item = blockIdx.x / args.per, rest = blockIdx.x - item * args.per;
+  if (args.by_xcd) {
+    const uint32_t k = blockIdx.x >> 3, o = k / args.per;
+    rest = k - o * args.per;
+    item = o * 8 + (blockIdx.x & 7);
+    if (item >= (uint32_t)args.items) return;
+  }
   int ji = 0;
-  while (ji + 1 < args.njobs && i >= args.first[ji + 1]) ++ji;
+  while (rest >= (uint32_t)args.job[ji].xtiles) rest -= (uint32_t)args.job[ji++].xtiles;
   const LaJob& j = args.job[ji];
-  i -= args.first[ji];
-  const int seg = (int)(i % (uint32_t)args.nseg);
-  i /= (uint32_t)args.nseg;
-  const int xt = (int)(i % (uint32_t)j.xtiles), unit = (int)(i / (uint32_t)j.xtiles);
+  const int xt = (int)rest, unit = (int)(item / (uint32_t)args.nseg), seg = (int)(item - (uint32_t)unit * (uint32_t)args.nseg);
   const int b = unit / args.H, h = unit - b * args.H;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
   const int live = ca_len(args.lens, args.lens64, b, args.L);
   const bool back = j.back != 0;
   const int x0 = xt * XT, xc = x0 + 16 * wave;      // first column of the workgroup, of the wave
 
-  if ((int)threadIdx.x <= C) {
-    const float gd = la_log_decay(args.log_decay, h);
-    pw[threadIdx.x] = expf(gd * (float)threadIdx.x);
-    em[threadIdx.x] = expm1f(gd * (float)threadIdx.x);
+  const float gd = la_log_decay(args.log_decay, h);
+  // factors of pairs of tiles by the lane's rows: on the diagonal (zero above it), one tile apart, 16 more rows; of what the
+  // state gives a row
+  float wd[4], w1[4], w16 = 0.f, wy[KT];
+  if constexpr (!SUM) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int gap = li - 4 * g - r;
+      wd[r] = gap >= 0 ? j.cp * expf(gd * (float)gap) : 0.f;
+      w1[r] = j.cp * expf(gd * (float)(gap + 16));
+    }
+    w16 = expf(gd * 16.f);
+#pragma unroll
+    for (int u = 0; u < KT; ++u) wy[u] = j.ci * expf(gd * (float)(16 * u + li + 1 - j.shift));
   }
 
   // tokens of this segment (taken backwards: segment 0 is the last)
@@ -170,179 +260,279 @@ __global__ void __launch_bounds__(64 * NW) la_kernel(const LaArgs args) {
   caf4 s[NS];
   const int64_t state = (int64_t)j.da * j.dx;
 #pragma unroll
-  for (int m = 0; m < NS; ++m) {
-    s[m] = caf4{0.f, 0.f, 0.f, 0.f};
-    if constexpr (!SUM) {
-      const float* p = args.nseg > 1 ? j.seg + ((int64_t)unit * args.nseg + seg) * state : j.s0 ? j.s0 + unit * state : nullptr;
-      const int64_t sr = args.nseg > 1 ? j.dx : j.s_r, sc = args.nseg > 1 ? 1 : j.s_c;
-      if (p != nullptr && xc + li < j.dx) {
+  for (int m = 0; m < NS; ++m) s[m] = caf4{0.f, 0.f, 0.f, 0.f};
+  if constexpr (!SUM) {
+    const float* p = args.nseg > 1 ? j.seg + ((int64_t)unit * args.nseg + seg) * state : j.s0 ? j.s0 + unit * state : nullptr;
+    const int sr = args.nseg > 1 ? j.dx : j.s_r, sc = args.nseg > 1 ? 1 : j.s_c;
+    if (p != nullptr && xc + li < j.dx) {
+#pragma unroll
+      for (int m = 0; m < NS; ++m)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int d = 32 * (m >> 1) + 8 * g + 4 * (m & 1) + r;
           if (d < j.da) s[m][r] = p[d * sr + (xc + li) * sc];
         }
-      }
     }
   }
 
-  const char* pa = j.a.p + (b * j.a.sb + (h / j.a.group) * j.a.sh) * ESZ;
-  const char* pb = j.b.p + (b * j.b.sb + (h / j.b.group) * j.b.sh) * ESZ;
-  const char* px = j.x.p + (b * j.x.sb + (h / j.x.group) * j.x.sh + x0) * ESZ;
+  const int64_t base_a = (b * j.a.sb + (h / j.a.group) * j.a.sh) * ESZ, base_b = (b * j.b.sb + (h / j.b.group) * j.b.sh) * ESZ,
+                base_x = (b * j.x.sb + (h / j.x.group) * j.x.sh + x0) * ESZ;
+  const char *pa = j.a.p + base_a, *pb = j.b.p + base_b, *px = j.x.p + base_x;
+  const int sa_b = (int)j.a.sl * ESZ, sb_b = (int)j.b.sl * ESZ, sx_b = (int)j.x.sl * ESZ;      // bytes between tokens
+  const int da = j.da, dx = j.dx, ysz = j.y32 ? 4 : ESZ, yrow = args.H * dx * ysz;
+  const bool wanted = j.y != nullptr, wide = DT == HCLSM_F32 || j.y32 != 0, fine = NC == 3 || args.fine != 0;
+  char* py = j.y + ((int64_t)b * args.L * args.H + h) * dx * ysz;
+  const float cu = j.cu;
+  const int shift = j.shift;
   SA ra, rb;
-  SX rx;
+  SX rxs;
   auto tokens = [&](int k, int& t0, int& n) __attribute__((always_inline)) {
     t0 = first + (back ? nch - 1 - k : k) * C;
     const int e = live < t_end ? live : t_end;
     n = e - t0;
     n = n < 0 ? 0 : n > C ? C : n;
   };
-  auto load = [&](int k) __attribute__((always_inline)) {
-    int t0, n;
-    tokens(k, t0, n);
-    if constexpr (!SUM) ra.load(pa + t0 * j.a.sl * ESZ, j.a.sl, n, j.da, back);
-    rb.load(pb + t0 * j.b.sl * ESZ, j.b.sl, n, j.da, back);
-    rx.load(px + t0 * j.x.sl * ESZ, j.x.sl, n, j.dx - x0, back);
+  auto load_a = [&](int t0, int n) __attribute__((always_inline)) {
+    if constexpr (!SUM) ra.load(pa + (int64_t)t0 * sa_b, sa_b, n, da, back, ta, wave);
   };
-  if (nch > 0) load(0);
-  for (int k = 0; k < nch; ++k) {
-    int t0, n;
-    tokens(k, t0, n);
-    __syncthreads();      // every wave is done with the chunk before
-    if (n > 0) {
-      if constexpr (!SUM) ra.store(ta);
-      rb.store(tb);
-      rx.store(tx);
-    }
-    __syncthreads();
-    if (k + 1 < nch) load(k + 1);
+  auto load_bx = [&](int t0, int n, char* t) __attribute__((always_inline)) {
+    rb.load(pb + (int64_t)t0 * sb_b, sb_b, n, da, back, t, wave);
+    rxs.load(px + (int64_t)t0 * sx_b, sx_b, n, dx - x0, back, t + SA::BYTES, wave);
+  };
+  auto pair = [](int f, int& tt, int& sp) __attribute__((always_inline)) {
+    tt = KT == 4 ? (f < 2 ? f : 2 + ((f - 2) >> 1)) : f;
+    sp = KT == 4 && f >= 2 ? (f & 1) : 0;
+  };
+  int tab = -1;             // live tokens that rx and decay are for
+  float decay = 0.f;
+  bool slow = false;
 
-    caf4 y[KT];
-    if (!SUM && n > 0) {
-      // weights of pairs: tile (s, t) leaves a lane with s = 4g + r of its t = li
-#pragma unroll
-      for (int f0 = 0; f0 < NF; f0 += NW) {
-        const int f = f0 + wave;
-        if (f < NF) {
-          const int tt = KT == 4 ? (f < 2 ? f : 2 + ((f - 2) >> 1)) : f, sp = KT == 4 && f >= 2 ? (f & 1) : 0;
-          caf4 w[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int ss = 2 * sp + u;
-            w[u] = caf4{0.f, 0.f, 0.f, 0.f};
-            if (ss <= tt) {
-#pragma unroll
-              for (int c = 0; c < DA / 32; ++c) {
-                LaFrag fb[NP], fa[NP];
-#pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                  fb[p] = TA::frag(tb + p * SA::PLANE, 16 * ss, c, li, g);
-                  fa[p] = TA::frag(ta + p * SA::PLANE, 16 * tt, c, li, g);
-                }
-                w[u] = la_mma<NP, NP, MOST>(fb, fa, w[u]);
-              }
-              const int gap = 16 * (tt - ss) + li - 4 * g;
-#pragma unroll
-              for (int r = 0; r < 4; ++r) w[u][r] = gap >= r ? w[u][r] * (j.cp * pw[gap - r]) : 0.f;
-            }
-          }
-          LaFrag fp[NC];
-          la_split<NC>(w, fp);
-#pragma unroll
-          for (int p = 0; p < NC; ++p) tp[(f * NC + p) * 64 + lane] = __builtin_bit_cast(uint4, fp[p]);
-        }
+  if (nch > 0) {
+    int t0, n;
+    tokens(0, t0, n);
+    if (n > 0) {
+      load_bx(t0, n, buf0);
+      load_a(t0, n);
+    }
+  }
+  auto work = [&](int k, char* tb, char* next) __attribute__((always_inline)) {
+    int t0, n, t1 = 0, n1 = 0;
+    tokens(k, t0, n);
+    if (k + 1 < nch) tokens(k + 1, t1, n1);
+    char* tx = tb + SA::BYTES;
+    if constexpr (DMA) {
+      ca_wait_vmem();
+      __syncthreads();      // the chunk is in LDS, and every wave is done with the one before
+      if (n1 > 0) load_bx(t1, n1, next);
+    } else {
+      __syncthreads();
+      if (n > 0) {
+        if constexpr (!SUM) ra.store(ta);
+        rb.store(tb);
+        rxs.store(tx);
+      }
+      if (n1 > 0) {
+        load_bx(t1, n1, next);
+        load_a(t1, n1);
       }
     }
-    if constexpr (!SUM) __syncthreads();
-    if (n > 0) {
-      if constexpr (!SUM) {
-        // what the state gives: y^T = S^T A^T
+    if (n != tab) {
+      tab = n;
+      if ((int)threadIdx.x < C)
+        rx[threadIdx.x] = (int)threadIdx.x < n ? cu * expf(gd * (float)(n - 1 - (int)threadIdx.x + shift)) : 0.f;
+      const float an = expf(gd * (float)n);      // (la_decayed, one of its two forms for all)
+      slow = __builtin_amdgcn_readfirstlane(an >= 0.5f ? 1 : 0) != 0;
+      decay = slow ? expm1f(gd * (float)n) : an;
+      if constexpr (SUM && DMA) __syncthreads();
+    }
+    if constexpr (!DMA) __syncthreads();
+
+    caf4 y[SUM ? 1 : KT];
+    if constexpr (!SUM) {
 #pragma unroll
-        for (int t = 0; t < KT; ++t) y[t] = caf4{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < KT; ++u) y[u] = caf4{0.f, 0.f, 0.f, 0.f};
+      if (n > 0) {
+        // weights of pairs: tile (s, t) leaves a lane with s = 4g + r of its t = li.  Waves 0 and 1 have two pairs of tiles of
+        // the six; the operands of CG products of all a wave's pairs are read before the first.
+        {
+          constexpr int CG = DA == 64 ? 2 : NP == 1 ? 4 : 1;
+          caf4 w[NFW][2];
+          int tt[NFW], sp[NFW];
+          bool mine[NFW];
 #pragma unroll
-        for (int c = 0; c < DA / 32; ++c) {
-          LaFrag fs[NC];
-          la_split<NC>(&s[2 * c], fs);
+          for (int o = 0; o < NFW; ++o) {
+            const int f = NF == 6 ? (wave < 2 ? 2 * wave + o : wave + 2) : wave;
+            mine[o] = f < NF && (o == 0 || wave < 2);
+            pair(f, tt[o], sp[o]);
 #pragma unroll
-          for (int t = 0; t < KT; ++t) {
-            LaFrag fa[NP];
+            for (int u = 0; u < 2; ++u) w[o][u] = caf4{0.f, 0.f, 0.f, 0.f};
+          }
 #pragma unroll
-            for (int p = 0; p < NP; ++p) fa[p] = TA::frag(ta + p * SA::PLANE, 16 * t, c, li, g);
-            y[t] = la_mma<NC, NP, MOST>(fs, fa, y[t]);
+          for (int c0 = 0; c0 < DA / 32; c0 += CG) {
+            LaFrag fa[NFW][CG][NP], fb[NFW][CG][2][NP];
+#pragma unroll
+            for (int o = 0; o < NFW; ++o)
+              if (mine[o])
+#pragma unroll
+                for (int c = 0; c < CG; ++c)
+#pragma unroll
+                  for (int p = 0; p < NP; ++p) {
+                    fa[o][c][p] = TA::frag(ta + p * SA::PLANE, 16 * tt[o], c0 + c, li, g);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) fb[o][c][u][p] = TA::frag(tb + p * SA::PLANE, 32 * sp[o] + 16 * u, c0 + c, li, g);
+                  }
+            ca_fence();
+#pragma unroll
+            for (int o = 0; o < NFW; ++o)
+              if (mine[o])
+#pragma unroll
+                for (int c = 0; c < CG; ++c)
+#pragma unroll
+                  for (int i = 0; i < NP; ++i)
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+                      if (i + p <= MOST)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) w[o][u] = LaB::mma(fb[o][c][u][i], fa[o][c][p], w[o][u]);
+          }
+#pragma unroll
+          for (int o = 0; o < NFW; ++o)
+            if (mine[o]) {
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const int apart = tt[o] - 2 * sp[o] - u;      // tiles between the two
+                const float more = apart > 2 ? w16 * w16 : apart > 1 ? w16 : 1.f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)      // (what lies above the diagonal may be infinite)
+                  w[o][u][r] = 16 * apart + li >= 4 * g + r ? w[o][u][r] * (apart > 0 ? w1[r] * more : wd[r]) : 0.f;
+              }
+              LaFrag fp[NC];
+              la_split<NC>(w[o], fp);
+              const int f = NF == 6 ? (wave < 2 ? 2 * wave + o : wave + 2) : wave;
+#pragma unroll
+              for (int p = 0; p < NC; ++p) tp[(f * NC + p) * 64 + lane] = __builtin_bit_cast(uint4, fp[p]);
+            }
+        }
+        // what the state gives: y^T = S^T A^T, the next operands on their way
+        {
+          LaFrag fa[2][KT][NP], fs[2][NC];
+          auto get = [&](int c, LaFrag (*f)[NP]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < KT; ++u)
+#pragma unroll
+              for (int p = 0; p < NP; ++p) f[u][p] = TA::frag(ta + p * SA::PLANE, 16 * u, c, li, g);
+          };
+          get(0, fa[0]);
+          la_split<NC>(&s[0], fs[0]);
+#pragma unroll
+          for (int c = 0; c < DA / 32; ++c) {
+            if (c + 1 < DA / 32) get(c + 1, fa[(c + 1) & 1]);
+            ca_fence();
+            la_mma_all<NC, NP, MOST, KT>(fs[c & 1], fa[c & 1], y);
+            if (c + 1 < DA / 32) la_split<NC>(&s[2 * c + 2], fs[(c + 1) & 1]);
+            ca_fence();
           }
         }
 #pragma unroll
-        for (int t = 0; t < KT; ++t) y[t] *= j.ci * pw[16 * t + li + 1 - j.shift];
+        for (int u = 0; u < KT; ++u) y[u] *= wy[u];
       }
-      LaFrag fx[KT / 2][NP];
+      la_barrier();         // the weights are in LDS, and every wave is done with A
+      if constexpr (DMA) {
+        if (n1 > 0) load_a(t1, n1);
+      }
+    }
+    LaFrag fx[KT / 2][NP];
+    if (n > 0) {
 #pragma unroll
       for (int sp = 0; sp < KT / 2; ++sp)
 #pragma unroll
         for (int p = 0; p < NP; ++p) fx[sp][p] = TX::frag_t(tx + p * SX::PLANE, 32 * sp, wave, li, g);
       if constexpr (!SUM) {
+        constexpr int ORDER[6] = {0, 1, 2, 4, 3, 5};      // products in a row have results of their own
+        LaFrag fp[NF][NC];
 #pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          const int tt = KT == 4 ? (f < 2 ? f : 2 + ((f - 2) >> 1)) : f, sp = KT == 4 && f >= 2 ? (f & 1) : 0;
-          LaFrag fp[NC];
+        for (int f = 0; f < NF; ++f)
 #pragma unroll
-          for (int p = 0; p < NC; ++p) fp[p] = ca_frag<HCLSM_BF16>(tp[(f * NC + p) * 64 + lane]);
-          y[tt] = la_mma<NP, NC, MOST>(fx[sp], fp, y[tt]);
-        }
+          for (int p = 0; p < NC; ++p) fp[f][p] = ca_frag<HCLSM_BF16>(tp[(f * NC + p) * 64 + lane]);
+        ca_fence();
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int p = 0; p < NC; ++p)
+            if (i + p <= MOST)
+#pragma unroll
+              for (int o = 0; o < NF; ++o) {
+                const int f = NF == 6 ? ORDER[o] : o;
+                int tt, sp;
+                pair(f, tt, sp);
+                y[tt] = LaB::mma(fx[sp][i], fp[f][p], y[tt]);
+              }
       }
-      // the state behind the chunk
-      const float an = pw[n], less = em[n];
-#pragma unroll
-      for (int m = 0; m < NS; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[m][r] = la_decayed(s[m][r], an, less);
-#pragma unroll
-      for (int sp = 0; sp < KT / 2; ++sp) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int q = 32 * sp + 16 * (e >> 2) + 4 * g + (e & 3);
-          float x = 0.f;
-#pragma unroll
-          for (int p = NP - 1; p >= 0; --p) x += (float)fx[sp][p][e];
-          v[e] = q < n ? x * (j.cu * pw[n - 1 - q + j.shift]) : 0.f;
-        }
-        uint4 w[3];
-        la_split<3>(v, w);
-        LaFrag fw[3];
-#pragma unroll
-        for (int p = 0; p < 3; ++p) fw[p] = ca_frag<HCLSM_BF16>(w[p]);
-#pragma unroll
-        for (int m = 0; m < NS; ++m) {
-          LaFrag fb[NP];
-#pragma unroll
-          for (int p = 0; p < NP; ++p) fb[p] = la_frag_cols<DA>(tb + p * SA::PLANE, 32 * sp, m >> 1, m & 1, li, g);
-          s[m] = la_mma<NP, 3, 2>(fb, fw, s[m]);
-        }
-      }
-    } else if constexpr (!SUM) {
-#pragma unroll
-      for (int t = 0; t < KT; ++t) y[t] = caf4{0.f, 0.f, 0.f, 0.f};
     }
-    if constexpr (!SUM) {
-      const int col = xc + 4 * g;
-      if (j.y != nullptr && col < j.dx) {
+    if constexpr (!SUM) {      // (here, not at the end: the state's sum hides the stores)
+      if (wanted) {
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(py + (int64_t)t0 * yrow, 0, 0x7fffffff, kRawBufferWord3);
+        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        const int cb = (xc + 4 * g) * ysz;
+        auto put = [&](caf4 v, int off, int so) __attribute__((always_inline)) {
+          off = xc + 4 * g < dx ? off : (int)SA::NONE;
+          if (wide) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), rs, off, so, 0);
+          else if constexpr (DT != HCLSM_F32)
+            __builtin_amdgcn_raw_buffer_store_b64(u2{CaT<DT>::pack2(v[0], v[1]), CaT<DT>::pack2(v[2], v[3])}, rs, off, so, 0);
+        };
+        if (n == C) {
+          const int off = (back ? 15 - li : li) * yrow + cb;
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          const int r = 16 * t + li;
-          const int64_t tok = t0 + (r < n && back ? n - 1 - r : r);      // tokens that are not live get zeros
-          if (tok < t_end) {
-            const int64_t o = ((b * (int64_t)args.L + tok) * args.H + h) * j.dx + col;
-            const caf4 v = r < n ? y[t] : caf4{0.f, 0.f, 0.f, 0.f};
-            if (j.y32) *reinterpret_cast<caf4*>(j.y + o * 4) = v;
-            else ca_store4<DT>(j.y, o, v);
+          for (int u = 0; u < KT; ++u) put(y[u], off, (back ? KT - 1 - u : u) * 16 * yrow);
+        } else {      // tokens that are not live get zeros
+#pragma unroll
+          for (int u = 0; u < KT; ++u) {
+            const int r = 16 * u + li, tok = r < n && back ? n - 1 - r : r;
+            put(r < n ? y[u] : caf4{0.f, 0.f, 0.f, 0.f}, t0 + tok < t_end ? tok * yrow + cb : (int)SA::NONE, 0);
           }
         }
       }
     }
+    if (n > 0) {
+      // the state behind the chunk
+      if (slow) {
+#pragma unroll
+        for (int m = 0; m < NS; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[m][r] = fmaf(s[m][r], decay, s[m][r]);
+      } else {
+#pragma unroll
+        for (int m = 0; m < NS; ++m) s[m] *= decay;
+      }
+#pragma unroll
+      for (int sp = 0; sp < KT / 2; ++sp) {
+        float v[8];
+        const caf4 w0 = *reinterpret_cast<const caf4*>(rx + 32 * sp + 4 * g), w1 = *reinterpret_cast<const caf4*>(rx + 32 * sp + 16 + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float x = 0.f;
+#pragma unroll
+          for (int p = NP - 1; p >= 0; --p) x += (float)fx[sp][p][e];
+          v[e] = x * (e < 4 ? w0[e & 3] : w1[e & 3]);      // (rows that are not live are zeros)
+        }
+        if (fine) la_update<DA, NP, 3, SA::PLANE>(tb, 32 * sp, v, s, li, g);
+        else la_update<DA, NP, 2, SA::PLANE>(tb, 32 * sp, v, s, li, g);
+      }
+    }
+  };
+  if constexpr (DMA) {
+    for (int k = 0; k < nch; k += 2) {
+      work(k, buf0, buf1);
+      if (k + 1 < nch) work(k + 1, buf1, buf0);
+    }
+  } else {
+    for (int k = 0; k < nch; ++k) work(k, buf0, buf0);
   }
 
   float* out = SUM ? j.seg + ((int64_t)unit * args.nseg + seg) * state : args.nseg == 1 && j.s1 ? j.s1 + unit * state : nullptr;
   if (out != nullptr && xc + li < j.dx) {
-    const int64_t sr = SUM ? j.dx : j.s_r, sc = SUM ? 1 : j.s_c;
+    const int sr = SUM ? j.dx : j.s_r, sc = SUM ? 1 : j.s_c;
 #pragma unroll
     for (int m = 0; m < NS; ++m)
 #pragma unroll
@@ -353,24 +543,18 @@ __global__ void __launch_bounds__(64 * NW) la_kernel(const LaArgs args) {
   }
 }
 
-template <int DT, int DA, int NW>
-int la_launch_one(const LaArgs& a, bool sum, hipStream_t st) {
-  const dim3 grid(a.first[a.njobs]), block(64 * NW);
-  if (sum) hipLaunchKernelGGL((la_kernel<DT, DA, NW, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((la_kernel<DT, DA, NW, false>), grid, block, 0, st, a);
+template <int DT, int DA> int la_launch_one(const LaArgs& a, bool sum, hipStream_t st) {
+  const dim3 grid((a.by_xcd ? (a.items + 7) / 8 * 8 : a.items) * a.per), block(LA_THREADS);
+  if (sum) hipLaunchKernelGGL((la_kernel<DT, DA, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((la_kernel<DT, DA, false>), grid, block, 0, st, a);
   HCLSM_LAUNCH_CHECK();
   return 0;
 }
 
-template <int DT> int la_launch(const LaArgs& a, int da, int xt, bool sum, hipStream_t st) {
-  if (xt == 64) {
-    if (da == 64) return la_launch_one<DT, 64, 4>(a, sum, st);
-    if (da == 128) return la_launch_one<DT, 128, 4>(a, sum, st);
-    return la_launch_one<DT, 256, 4>(a, sum, st);
-  }
-  if (da == 64) return la_launch_one<DT, 64, 8>(a, sum, st);
-  if (da == 128) return la_launch_one<DT, 128, 8>(a, sum, st);
-  return la_launch_one<DT, 256, 8>(a, sum, st);
+template <int DT> int la_launch(const LaArgs& a, int da, bool sum, hipStream_t st) {
+  if (da == 64) return la_launch_one<DT, 64>(a, sum, st);
+  if (da == 128) return la_launch_one<DT, 128>(a, sum, st);
+  return la_launch_one<DT, 256>(a, sum, st);
 }
 
 }  // namespace hclsm

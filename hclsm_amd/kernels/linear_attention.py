@@ -20,6 +20,8 @@ _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 MAX_HEAD_DIM = 256
 _MAX_HEADS = 1 << 20        # heads of a call, B H
+_MAX_ROW = 1 << 23          # elements of a token, H max(dk, dv)
+_FAR = 1 << 22              # elements between tokens
 
 
 def _check(fn, q, k, v, log_decay, scale, token):
@@ -41,6 +43,8 @@ def _check(fn, q, k, v, log_decay, scale, token):
             raise ValueError(f"{fn}: heads of 8, 16, .. {MAX_HEAD_DIM} elements, got {name} = {d}")
     if q.shape[0] * H > _MAX_HEADS:
         raise ValueError(f"{fn}: at most {_MAX_HEADS} heads in a call, got {q.shape[0]} x {H}")
+    if H * max(dk, dv) >= _MAX_ROW:
+        raise ValueError(f"{fn}: fewer than {_MAX_ROW} elements in a token, got {H} x {max(dk, dv)}")
     if tuple(log_decay.shape) != (H,) or log_decay.dtype != torch.float32:
         raise ValueError(f"{fn}: log_decay must be ({H},) float32, got {tuple(log_decay.shape)} {log_decay.dtype}")
     if log_decay.requires_grad and torch.is_grad_enabled():
@@ -67,11 +71,13 @@ def _index_code(t):
 
 
 def _rows(t):
-    """t with rows on 16-byte boundaries (t itself where they are)."""
+    """t with rows on 16-byte boundaries and near enough to each other (t itself where they are): the kernels' offsets from
+    a chunk's first row are 31 bits."""
     n = 16 // t.element_size()
     sb, sl, sh, s = t.stride()
     B, L, H, _ = t.shape
-    if s == 1 and t.data_ptr() % 16 == 0 and (sb % n == 0 or B == 1) and (sl % n == 0 or L == 1) and (sh % n == 0 or H == 1):
+    if (s == 1 and t.data_ptr() % 16 == 0 and (sb % n == 0 or B == 1) and (L == 1 or (sl % n == 0 and sl < _FAR))
+            and (sh % n == 0 or H == 1)):
         return t
     if not t.is_contiguous():
         return t.contiguous()
@@ -175,7 +181,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
 
     q (B, L, H, dk); k (B, L, Hk, dk) and v (B, L, Hk, dv): head h reads key head h // (H // Hk).  One dtype among bfloat16,
         float16, float32; dk and dv multiples of 8 up to 256; any strides (rows that are not contiguous or not on 16-byte
-        boundaries are copied).  B H is at most 2^20.
+        boundaries, or very far apart, are copied).  B H is at most 2^20, H max(dk, dv) below 2^23.
     log_decay (H,) float32, at most 0 (0 sums without decay, -inf keeps the token itself alone); a constant: it has no
         gradient here, and one that requires grad is refused.
     initial_state (B, H, dk, dv) float32: the state in front of the first token; None: zeros.

@@ -743,7 +743,8 @@ int64_t hclsm_linear_attention_workspace(int64_t B, int64_t L, int64_t H, int64_
 /*
  * S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T (S_{-1} = state_in),  out_t = scale * q_t^T S_t,  state_out = S behind the last
  * live token.  Tokens from seq_lens[b] on are not read, get out = 0 and leave the state as it is.
- * dk and dv are multiples of 8 up to 256, H a multiple of Hk, B H at most 2^20 (HCLSM_ERR_UNSUPPORTED otherwise).
+ * dk and dv are multiples of 8 up to 256, H a multiple of Hk, B H at most 2^20, H max(dk, dv) below 2^23, tokens of q, k, v and
+ * g less than 16 MB apart (HCLSM_ERR_UNSUPPORTED otherwise).
  * Operands of the matrix products are float32 values in two bf16 parts (three for float32 inputs and for the state's own
  * update), sums and states float32.  No counterpart in the reference, whose time mixing is the selective scan
  * (kernels/ssm_scan_kernel.py).
