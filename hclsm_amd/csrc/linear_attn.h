@@ -23,7 +23,7 @@
 namespace hclsm {
 
 constexpr int LA_MAX_DIM = 256;
-constexpr int LA_MAX_SEGMENTS = 256;
+constexpr int LA_MAX_SEGMENTS = 256, LA_FEW_SEGMENTS = 8;
 
 struct LaTensor {
   const char* p;

@@ -67,8 +67,8 @@ bool la_aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int esz) {
   return (uintptr_t)p % 16 == 0 && s0 % n == 0 && s1 % n == 0 && s2 % n == 0;
 }
 
-// States in front of a call's segments, from the segments' sums, in place; the state behind the last one.  One thread per
-// element: the segments one after another, the next sums on their way.
+// States in front of a call's segments, from the sums of the segments before them, in place.  One thread per element: the segments
+// one after another, the next sums on their way.
 __global__ void __launch_bounds__(256) la_prefix_kernel(const LaArgs a) {
   const LaJob& j = a.job[blockIdx.y];
   const int n = j.da * j.dx, blocks = (n + 255) / 256, unit = (int)blockIdx.x / blocks, b = unit / a.H, h = unit - b * a.H;
@@ -79,21 +79,27 @@ __global__ void __launch_bounds__(256) la_prefix_kernel(const LaArgs a) {
   const int d = e / j.dx, c = e - d * j.dx;
   float* p = j.seg + (int64_t)unit * a.nseg * n + e;
   float s = j.s0 ? j.s0[(int64_t)unit * n + d * j.s_r + c * j.s_c] : 0.f;
-  constexpr int NB = 16;
+  int64_t of = a.seg_tokens;      // tokens that `an` and `less` are for
+  float an = expf(g * (float)of), less = expm1f(g * (float)of);
+  constexpr int NB = 32;
   for (int k0 = 0; k0 < a.nseg; k0 += NB) {
     float u[NB];
 #pragma unroll
-    for (int k = 0; k < NB; ++k) u[k] = k0 + k < a.nseg ? p[(int64_t)(k0 + k) * n] : 0.f;
+    for (int k = 0; k < NB; ++k) u[k] = k0 + k + 1 < a.nseg ? p[(int64_t)(k0 + k) * n] : 0.f;
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
       if (k0 + k >= a.nseg) break;
       const int64_t t0 = (int64_t)(j.back ? a.nseg - 1 - k0 - k : k0 + k) * a.seg_tokens;
       const int64_t m = live - t0 < 0 ? 0 : live - t0 > a.seg_tokens ? a.seg_tokens : live - t0;
       p[(int64_t)(k0 + k) * n] = s;
-      s = la_decayed(s, expf(g * (float)m), expm1f(g * (float)m)) + u[k];
+      if (m != of) {
+        of = m;
+        an = expf(g * (float)m);
+        less = expm1f(g * (float)m);
+      }
+      s = la_decayed(s, an, less) + u[k];
     }
   }
-  if (j.s1) j.s1[(int64_t)unit * n + d * j.s_r + c * j.s_c] = s;
 }
 
 // Gradients of shared heads: the sums of the heads of a group, rounded once.
@@ -125,8 +131,18 @@ int la_launch_any(const LaArgs& a, int dtype, int da, bool sum, hipStream_t st) 
 
 // All jobs of a call: sums of segments, states in front of them, outputs.  Jobs of the same padded sizes share a launch.
 int la_run(LaArgs a, int dtype, hipStream_t st) {
+  // Jobs of different padded sizes share a launch of the larger one where together they are on the chip at once: they then run
+  // side by side, and one after the other elsewhere.
+  int64_t all = 0;
+  int most = 0;
+  for (int i = 0; i < a.njobs; ++i) {
+    all += (int64_t)a.B * a.H * a.nseg * a.job[i].xtiles;
+    most = la_padded(a.job[i].da) > most ? la_padded(a.job[i].da) : most;
+  }
+  auto padded = [&](int i) { return all <= 512 ? most : la_padded(a.job[i].da); };
   for (int pass = a.nseg > 1 ? 0 : 2; pass < 3; ++pass) {
     if (pass == 1) {
+      if (a.nseg <= LA_FEW_SEGMENTS) continue;      // the main kernel adds them up itself
       const int64_t n = ((int64_t)a.job[0].da * a.job[0].dx + 255) / 256 * a.B * a.H;
       hipLaunchKernelGGL(la_prefix_kernel, dim3((unsigned)n, (unsigned)a.njobs), dim3(256), 0, st, a);
       HCLSM_LAUNCH_CHECK();
@@ -138,9 +154,9 @@ int la_run(LaArgs a, int dtype, hipStream_t st) {
       LaArgs one = a;
       one.njobs = 0;
       one.per = 0;
-      const int da = la_padded(a.job[i].da);
+      const int da = padded(i);
       for (int k = i; k < a.njobs; ++k) {
-        if (done[k] || la_padded(a.job[k].da) != da) continue;
+        if (done[k] || padded(k) != da) continue;
         done[k] = true;
         one.per += (uint32_t)a.job[k].xtiles;
         one.job[one.njobs++] = a.job[k];

@@ -157,7 +157,7 @@ template <int NA, int NB, int MOST, int T> __device__ __forceinline__ void la_mm
         for (int t = 0; t < T; ++t) acc[t] = LaB::mma(a[t][i], b[j], acc[t]);
 }
 
-// A barrier for what went through LDS: transfers from global memory to LDS stay in flight (__syncthreads waits for them).
+// A barrier for what went through LDS: loads and transfers from global memory stay in flight (__syncthreads waits for them).
 __device__ __forceinline__ void la_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0xc07f);      // LDS counter zero (gfx9 encoding), the others as they are
@@ -226,6 +226,7 @@ __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const 
   while (rest >= (uint32_t)args.job[ji].xtiles) rest -= (uint32_t)args.job[ji++].xtiles;
   const LaJob& j = args.job[ji];
   const int xt = (int)rest, unit = (int)(item / (uint32_t)args.nseg), seg = (int)(item - (uint32_t)unit * (uint32_t)args.nseg);
+  if (SUM && seg == args.nseg - 1) return;      // no segment has its sum in front of it
   const int b = unit / args.H, h = unit - b * args.H;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
   const int live = ca_len(args.lens, args.lens64, b, args.L);
@@ -259,20 +260,37 @@ __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const 
   // the state: tile m of 16 rows holds da = 32 (m / 2) + 8g + 4 (m & 1) + r of column xc + li
   caf4 s[NS];
   const int64_t state = (int64_t)j.da * j.dx;
+  // byte offset of tile m's row r of the lane's column in a state, past its end where there is none
+  auto place = [&](int m, int r, int sr, int sc) __attribute__((always_inline)) {
+    const int d = 32 * (m >> 1) + 8 * g + 4 * (m & 1) + r;
+    return d < j.da && xc + li < j.dx ? (d * sr + (xc + li) * sc) * 4 : (int)SA::NONE;
+  };
 #pragma unroll
   for (int m = 0; m < NS; ++m) s[m] = caf4{0.f, 0.f, 0.f, 0.f};
   if constexpr (!SUM) {
-    const float* p = args.nseg > 1 ? j.seg + ((int64_t)unit * args.nseg + seg) * state : j.s0 ? j.s0 + unit * state : nullptr;
-    const int sr = args.nseg > 1 ? j.dx : j.s_r, sc = args.nseg > 1 ? 1 : j.s_c;
-    if (p != nullptr && xc + li < j.dx) {
+    // few segments: the state in front of this one from the sums of those before it; many: as la_prefix_kernel left it
+    auto add = [&](const float* p, int sr, int sc, float an, float less) __attribute__((always_inline)) {
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)state * 4, kRawBufferWord3);
+      float v[NS][4];
 #pragma unroll
       for (int m = 0; m < NS; ++m)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int d = 32 * (m >> 1) + 8 * g + 4 * (m & 1) + r;
-          if (d < j.da) s[m][r] = p[d * sr + (xc + li) * sc];
-        }
-    }
+        for (int r = 0; r < 4; ++r) v[m][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, place(m, r, sr, sc), 0, 0));
+#pragma unroll
+      for (int m = 0; m < NS; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[m][r] = la_decayed(s[m][r], an, less) + v[m][r];
+    };
+    const float* sums = j.seg + (int64_t)unit * args.nseg * state;
+    const bool few = args.nseg <= LA_FEW_SEGMENTS;
+    if (few && j.s0) add(j.s0 + unit * state, j.s_r, j.s_c, 0.f, 0.f);
+    if (!few) add(sums + seg * state, j.dx, 1, 0.f, 0.f);
+    else
+      for (int k = 0; k < seg; ++k) {
+        const int64_t t0 = (int64_t)(back ? args.nseg - 1 - k : k) * args.seg_tokens, m = live - t0;
+        const float n = (float)(m < 0 ? 0 : m > args.seg_tokens ? args.seg_tokens : m);
+        add(sums + k * state, j.dx, 1, expf(gd * n), expm1f(gd * n));
+      }
   }
 
   const int64_t base_a = (b * j.a.sb + (h / j.a.group) * j.a.sh) * ESZ, base_b = (b * j.b.sb + (h / j.b.group) * j.b.sh) * ESZ,
@@ -325,7 +343,7 @@ __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const 
       __syncthreads();      // the chunk is in LDS, and every wave is done with the one before
       if (n1 > 0) load_bx(t1, n1, next);
     } else {
-      __syncthreads();
+      la_barrier();
       if (n > 0) {
         if constexpr (!SUM) ra.store(ta);
         rb.store(tb);
@@ -345,7 +363,7 @@ __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const 
       decay = slow ? expm1f(gd * (float)n) : an;
       if constexpr (SUM && DMA) __syncthreads();
     }
-    if constexpr (!DMA) __syncthreads();
+    if constexpr (!DMA) la_barrier();
 
     caf4 y[SUM ? 1 : KT];
     if constexpr (!SUM) {
@@ -530,16 +548,15 @@ __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const 
     for (int k = 0; k < nch; ++k) work(k, buf0, buf0);
   }
 
-  float* out = SUM ? j.seg + ((int64_t)unit * args.nseg + seg) * state : args.nseg == 1 && j.s1 ? j.s1 + unit * state : nullptr;
-  if (out != nullptr && xc + li < j.dx) {
+  float* out = SUM ? j.seg + ((int64_t)unit * args.nseg + seg) * state
+                   : seg == args.nseg - 1 && j.s1 ? j.s1 + unit * state : nullptr;
+  if (out != nullptr) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(out, 0, (int)state * 4, kRawBufferWord3);
     const int sr = SUM ? j.dx : j.s_r, sc = SUM ? 1 : j.s_c;
 #pragma unroll
     for (int m = 0; m < NS; ++m)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 32 * (m >> 1) + 8 * g + 4 * (m & 1) + r;
-        if (d < j.da) out[d * sr + (xc + li) * sc] = s[m][r];
-      }
+      for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s[m][r]), rs, place(m, r, sr, sc), 0, 0);
   }
 }
 
