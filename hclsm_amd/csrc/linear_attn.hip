@@ -5,15 +5,18 @@ namespace hclsm {
 
 namespace {
 
-// Segments of a call: where heads and columns alone do not fill the chip, the tokens are split, each segment's sum formed
-// first (from zero), the states in front of the segments from those, and then all segments at once.
+// Segments of a call: where heads and columns alone are fewer workgroups than the chip has CUs, the tokens are split, each segment's
+// sum formed first (from zero), the states in front of the segments from those, and then all segments at once, two workgroups to a
+// CU.  The sums read B and X once more.  Measured, 50176 tokens of 12 heads of 64: 21 segments 140 us, 32: 130, 42: 116, 53: 124, 64:
+// 119; training steps of 32 x 1024 tokens (384 workgroups forward): 173 unsplit, 183 with two segments; 8 x 4096, 16 heads of 128
+// (256): 605, with four 652.
 struct LaPlan {
   int nseg, seg_tokens;
 };
 
 LaPlan la_plan(int64_t workgroups, int64_t L, int chunk) {
   const int64_t chunks = (L + chunk - 1) / chunk;
-  int64_t n = workgroups > 0 ? (workgroups < 256 ? 768 / workgroups : 1) : 1;
+  int64_t n = workgroups > 0 ? (workgroups < 256 ? 512 / workgroups : 1) : 1;
   n = n > chunks / 4 ? chunks / 4 : n;
   n = n > LA_MAX_SEGMENTS ? LA_MAX_SEGMENTS : n;
   if (n <= 1) return {1, 0};
@@ -81,7 +84,7 @@ __global__ void __launch_bounds__(256) la_prefix_kernel(const LaArgs a) {
   float s = j.s0 ? j.s0[(int64_t)unit * n + d * j.s_r + c * j.s_c] : 0.f;
   int64_t of = a.seg_tokens;      // tokens that `an` and `less` are for
   float an = expf(g * (float)of), less = expm1f(g * (float)of);
-  constexpr int NB = 32;
+  constexpr int NB = 16;
   for (int k0 = 0; k0 < a.nseg; k0 += NB) {
     float u[NB];
 #pragma unroll

@@ -25,7 +25,20 @@ _FAR = 1 << 22              # elements between tokens
 
 
 def _check(fn, q, k, v, log_decay, scale, token):
-    """q (B, [L,] H, dk), k and v (B, [L,] Hk, dk / dv); token: no L."""
+    """q (B, [L,] H, dk), k and v (B, [L,] Hk, dk / dv); token: no L.  One test of everything, and what is wrong if it fails."""
+    qs, ks, vs, dt = q.shape, k.shape, v.shape, q.dtype
+    n = len(qs)
+    if not (n == (3 if token else 4) and len(ks) == n and len(vs) == n and dt in _CODE and k.dtype is dt and v.dtype is dt
+            and ks[:-2] == qs[:-2] and ks[-1] == qs[-1] and vs[:-1] == ks[:-1] and ks[-2] >= 1 and qs[-2] % ks[-2] == 0
+            and 8 <= qs[-1] <= MAX_HEAD_DIM and qs[-1] % 8 == 0 and 8 <= vs[-1] <= MAX_HEAD_DIM and vs[-1] % 8 == 0
+            and qs[0] * qs[-2] <= _MAX_HEADS and qs[-2] * max(qs[-1], vs[-1]) < _MAX_ROW
+            and log_decay.shape == qs[-2:-1] and log_decay.dtype is torch.float32 and 1e-38 <= scale <= 3e38):
+        _explain(fn, q, k, v, log_decay, scale, token)
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{fn}: log_decay has no gradient here; pass log_decay.detach()")
+
+
+def _explain(fn, q, k, v, log_decay, scale, token):
     dims, shape = (3, "(B, H, d)") if token else (4, "(B, L, H, d)")
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != dims:
@@ -47,10 +60,7 @@ def _check(fn, q, k, v, log_decay, scale, token):
         raise ValueError(f"{fn}: fewer than {_MAX_ROW} elements in a token, got {H} x {max(dk, dv)}")
     if tuple(log_decay.shape) != (H,) or log_decay.dtype != torch.float32:
         raise ValueError(f"{fn}: log_decay must be ({H},) float32, got {tuple(log_decay.shape)} {log_decay.dtype}")
-    if log_decay.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{fn}: log_decay has no gradient here; pass log_decay.detach()")
-    if not 1e-38 <= scale <= 3e38:
-        raise ValueError(f"{fn}: scale must be positive, as a float32 too, got {scale}")
+    raise ValueError(f"{fn}: scale must be positive, as a float32 too, got {scale}")
 
 
 def _check_index(fn, name, t, B):
@@ -233,32 +243,37 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
         raise RuntimeError(f"{fn}: the step has no gradient (it updates the state in place); use linear_attention, or "
                            "torch.no_grad()")
     B, H, dk = q.shape
-    Hk, dv = k.shape[1], v.shape[2]
-    _check_index(fn, "rows", rows, B)
-    _check_state(fn, state, B if rows is None else None, H, dk, dv)
+    if rows is not None:
+        _check_index(fn, "rows", rows, B)
+    _check_state(fn, state, B if rows is None else None, H, dk, v.shape[2])
     return _step(q, k, v, log_decay.contiguous(), state, _index(rows), scale)
 
 
 def _check_state(fn, state, N, H, dk, dv):
-    if (state.dim() != 4 or tuple(state.shape[1:]) != (H, dk, dv) or state.dtype != torch.float32
-            or (N is not None and state.shape[0] != N)):
+    shape = state.shape
+    if (len(shape) != 4 or shape[1] != H or shape[2] != dk or shape[3] != dv or state.dtype is not torch.float32
+            or (N is not None and shape[0] != N)):
         raise ValueError(f"{fn}: state must be ({'N' if N is None else N}, {H}, {dk}, {dv}) float32, got "
-                         f"{tuple(state.shape)} {state.dtype}")
+                         f"{tuple(shape)} {state.dtype}")
     sb, sh, sr, sc = state.stride()
-    if state.numel() and (sc != 1 or sr != dv or (sh != dk * dv and H > 1) or state.data_ptr() % 16
-                          or (state.shape[0] > 1 and (sb % 4 or sb < H * dk * dv))):
+    if (sc != 1 or sr != dv or (sh != dk * dv and H > 1) or state.data_ptr() % 16
+            or (shape[0] > 1 and (sb % 4 or sb < H * dk * dv))) and state.numel():
         raise ValueError(f"{fn}: the heads of a state must be contiguous, on 16-byte boundaries, and states apart (it is "
                          f"updated in place), got strides {state.stride()}")
 
 
 def _step(q, k, v, log_decay, state, rows, scale):
-    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+    qb, qh, qe = q.stride()
+    kb, kh, ke = k.stride()
+    vb, vh, ve = v.stride()
+    if qe != 1 or ke != 1 or ve != 1:
+        return _step(q.contiguous(), k.contiguous(), v.contiguous(), log_decay, state, rows, scale)
     B, H, dk = q.shape
-    dv = v.shape[2]
-    out = torch.empty((B, H, dv), dtype=q.dtype, device=q.device)
+    _, Hk, dv = v.shape
+    out = q.new_empty((B, H, dv))
     x = _lib.pack_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(), _ptr(rows),
-                       out.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                       state.stride(0), state.shape[0], B, H, k.shape[1], dk, dv, scale, _CODE[q.dtype], _index_code(rows))
+                       out.data_ptr(), qb, qh, kb, kh, vb, vh, state.stride(0), state.shape[0], B, H, Hk, dk, dv, scale,
+                       _CODE[q.dtype], _index_code(rows))
     with on_device(q.device):
         rc = _lib.lib().hclsm_linear_attention_step(x, _lib.stream_of(q))
     if rc:

@@ -20,9 +20,19 @@ _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 MAX_COLUMNS = 16384
 GROUPS = (32, 64, 128)
+_INF = float("inf")
 
 
 def _check(fn, x, residual, weight, eps):
+    """One test of everything, and what is wrong if it fails."""
+    shape, dt = x.shape, x.dtype
+    if not (shape and dt in _CODE and 1 <= shape[-1] <= MAX_COLUMNS
+            and (residual is None or (residual.shape == shape and residual.dtype in (dt, torch.float32)))
+            and (weight is None or (weight.shape == shape[-1:] and weight.dtype in _CODE)) and 0 <= eps < _INF):
+        _explain(fn, x, residual, weight, eps)
+
+
+def _explain(fn, x, residual, weight, eps):
     if x.dim() < 1:
         raise ValueError(f"{fn}: x must be (..., D), got a scalar")
     if x.dtype not in _FLOATS:
@@ -37,8 +47,7 @@ def _check(fn, x, residual, weight, eps):
             raise TypeError(f"{fn}: residual must be {x.dtype} or float32, got {residual.dtype}")
     if weight is not None and (tuple(weight.shape) != (D,) or weight.dtype not in _FLOATS):
         raise ValueError(f"{fn}: weight must be a float tensor of {D} elements, got {weight.dtype} {tuple(weight.shape)}")
-    if not 0 <= eps < float("inf"):
-        raise ValueError(f"{fn}: eps must be >= 0 and finite, got {eps}")
+    raise ValueError(f"{fn}: eps must be >= 0 and finite, got {eps}")
 
 
 def _rows2d(t):
@@ -56,7 +65,8 @@ def _ptr(t):
 
 
 def _like(t, dtype=None):
-    return torch.empty(t.shape, dtype=dtype or t.dtype, device=t.device)
+    """A new contiguous tensor of t's shape."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def _count(x):
