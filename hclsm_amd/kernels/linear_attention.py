@@ -29,7 +29,7 @@ def _check(fn, q, k, v, log_decay, scale, token):
     qs, ks, vs, dt = q.shape, k.shape, v.shape, q.dtype
     n = len(qs)
     if not (n == (3 if token else 4) and len(ks) == n and len(vs) == n and dt in _CODE and k.dtype is dt and v.dtype is dt
-            and ks[:-2] == qs[:-2] and ks[-1] == qs[-1] and vs[:-1] == ks[:-1] and ks[-2] >= 1 and qs[-2] % ks[-2] == 0
+            and ks[:-2] == qs[:-2] and ks[-1] == qs[-1] and vs[:-1] == ks[:-1] and 1 <= ks[-2] <= qs[-2] and qs[-2] % ks[-2] == 0
             and 8 <= qs[-1] <= MAX_HEAD_DIM and qs[-1] % 8 == 0 and 8 <= vs[-1] <= MAX_HEAD_DIM and vs[-1] % 8 == 0
             and qs[0] * qs[-2] <= _MAX_HEADS and qs[-2] * max(qs[-1], vs[-1]) < _MAX_ROW
             and log_decay.shape == qs[-2:-1] and log_decay.dtype is torch.float32 and 1e-38 <= scale <= 3e38):
@@ -49,7 +49,7 @@ def _explain(fn, q, k, v, log_decay, scale, token):
     if k.shape[:-2] != q.shape[:-2] or k.shape[-1] != dk or v.shape[:-1] != k.shape[:-1]:
         raise ValueError(f"{fn}: k must be {(*q.shape[:-2], 'Hk', dk)} and v {(*q.shape[:-2], 'Hk', 'dv')}, got "
                          f"{tuple(k.shape)} and {tuple(v.shape)}")
-    if Hk < 1 or H % Hk:
+    if Hk < 1 or H < 1 or H % Hk:
         raise ValueError(f"{fn}: {H} heads cannot share {Hk} key heads")
     for name, d in (("dk", dk), ("dv", dv)):
         if not 8 <= d <= MAX_HEAD_DIM or d % 8:
@@ -70,6 +70,13 @@ def _check_index(fn, name, t, B):
         raise TypeError(f"{fn}: {name} must be int32 or int64, got {t.dtype}")
     if tuple(t.shape) != (B,):
         raise ValueError(f"{fn}: {name} must be ({B},), got {tuple(t.shape)}")
+
+
+def _check_first(fn, state, q, v):
+    """A state (or its gradient) in front of or behind a sequence."""
+    want = (q.shape[0], q.shape[2], q.shape[3], v.shape[3])
+    if state is not None and (state.shape != want or state.dtype is not torch.float32):
+        raise ValueError(f"{fn}: initial_state must be {want} float32, got {tuple(state.shape)} {state.dtype}")
 
 
 def _index(t):
@@ -209,11 +216,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
         scale = q.shape[-1] ** -0.5 if q.shape[-1] else 1.0
     scale = float(scale)
     _check(fn, q, k, v, log_decay, scale, False)
-    B, H, dk, dv = q.shape[0], q.shape[2], q.shape[3], v.shape[3]
-    _check_index(fn, "seq_lens", seq_lens, B)
-    if initial_state is not None and (tuple(initial_state.shape) != (B, H, dk, dv) or initial_state.dtype != torch.float32):
-        raise ValueError(f"{fn}: initial_state must be {(B, H, dk, dv)} float32, got {tuple(initial_state.shape)} "
-                         f"{initial_state.dtype}")
+    _check_index(fn, "seq_lens", seq_lens, q.shape[0])
+    _check_first(fn, initial_state, q, v)
     log_decay, lens = log_decay.contiguous(), _index(seq_lens)
     s0 = None if initial_state is None else initial_state.contiguous()
     if _no_node((q, k, v) if s0 is None else (q, k, v, s0)):

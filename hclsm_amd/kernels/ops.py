@@ -53,6 +53,18 @@ adds tens of microseconds of Python dispatch per call, which is the size of the 
         float64; layout 0 half, 1 interleaved) (perception/vision_encoder.py:171-259)
     hclsm_hip::norm_rotary_bwd(x, weight?, turns?, positions?, g, rot_dim, layout, amplitude, eps) -> (gx, gweight)
         of the normed form; gweight has shape (0,) without a weight
+    hclsm_hip::linear_attention_fwd(q, k, v, log_decay, initial_state?, seq_lens?, scale, want_state) -> (out, state)
+        S_t = exp(log_decay) S_{t-1} + k_t v_t^T, out_t = scale q_t^T S_t; state has shape (0,) without want_state
+    hclsm_hip::linear_attention_bwd(q, k, v, log_decay, initial_state?, seq_lens?, g, gstate?, scale)
+        -> (dq, dk, dv, dinitial_state); the last has shape (0,) without an initial state
+    hclsm_hip::linear_attention_step(q, k, v, log_decay, state, rows?, scale) -> out
+        one token, state updated in place
+    hclsm_hip::residual_rms_norm_fwd(x, residual?, weight?, eps) -> (y, h)
+        h = x + residual (shape (0,) without one), y = its root-mean-square norm times weight
+    hclsm_hip::residual_rms_norm_fp8(x, residual?, weight?, eps, group) -> (y8, scale, h)
+        y in float8_e4m3fn with scales by row (group 0) or by 32, 64 or 128 columns
+    hclsm_hip::residual_rms_norm_bwd(h, weight?, gy, gh?, eps) -> (dx, dr, dweight)
+        dx in gy's type; dr in h's (shape (0,) where that is the same); dweight has shape (0,) without a weight
 """
 
 from __future__ import annotations
@@ -66,8 +78,14 @@ from hclsm_amd.kernels._common import require_gpu
 from hclsm_amd.kernels.cross_attention import (_backward as _cross_backward, _check as _cross_check,
                                                _forward as _cross_forward, _masks as _cross_masks)
 from hclsm_amd.kernels.event_attention import event_attention as _event_attention
+from hclsm_amd.kernels.linear_attention import (_backward as _la_backward, _check as _la_check_qkv,
+                                                _check_first as _la_check_first, _check_index as _la_check_index,
+                                                _check_state as _la_check_state, _forward as _la_forward,
+                                                _index as _la_index, _step as _la_step)
 from hclsm_amd.kernels.norm_rotary import (_check_heads, _check_positions, _check_weight, _forward as _nr_forward,
                                            _norm_backward as _nr_backward, _RawPlan)
+from hclsm_amd.kernels.residual_norm import (_backward as _rn_backward, _check as _rn_check, _check_group as _rn_check_group,
+                                             _forward as _rn_forward, _forward_fp8 as _rn_forward_fp8)
 from hclsm_amd.kernels.slot_attention_kernel import _core_raw
 from hclsm_amd.kernels.slot_iteration import SlotMode, SlotWeights, slot_attention_forward as _slot_forward
 from hclsm_amd.kernels.level1_packed import Level1Weights, level1_forward_packed
@@ -431,3 +449,115 @@ def norm_rotary_bwd(x: Tensor, weight: Optional[Tensor], turns: Optional[Tensor]
 @norm_rotary_bwd.register_fake
 def _(x, weight, turns, positions, g, rot_dim, layout, amplitude, eps):
     return x.new_empty(x.shape), (weight.new_empty(weight.shape) if weight is not None else x.new_empty((0,)))
+
+
+# --------------------------------------------------------------------------- linear attention, norms with the residual
+
+def _la_check(fn, q, k, v, log_decay, s0, lens, scale):
+    require_gpu(fn, q, k, v, log_decay, s0, lens)
+    _la_check_qkv(fn, q, k, v, log_decay, scale, False)
+    _la_check_index(fn, "seq_lens", lens, q.shape[0])
+    _la_check_first(fn, s0, q, v)
+
+
+@torch.library.custom_op("hclsm_hip::linear_attention_fwd", mutates_args=())
+def linear_attention_fwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, initial_state: Optional[Tensor],
+                         seq_lens: Optional[Tensor], scale: float, want_state: bool) -> tuple[Tensor, Tensor]:
+    _la_check("linear_attention_fwd", q, k, v, log_decay, initial_state, seq_lens, scale)
+    s0 = None if initial_state is None else initial_state.contiguous()
+    out, s1 = _la_forward(q, k, v, log_decay.contiguous(), s0, _la_index(seq_lens), scale, bool(want_state))
+    return out, _opt(s1, q, torch.float32)
+
+
+@linear_attention_fwd.register_fake
+def _(q, k, v, log_decay, initial_state, seq_lens, scale, want_state):
+    B, L, H, dk = q.shape
+    return (q.new_empty((B, L, H, v.shape[3])),
+            q.new_empty((B, H, dk, v.shape[3]) if want_state else (0,), dtype=torch.float32))
+
+
+@torch.library.custom_op("hclsm_hip::linear_attention_bwd", mutates_args=())
+def linear_attention_bwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, initial_state: Optional[Tensor],
+                         seq_lens: Optional[Tensor], g: Tensor, gstate: Optional[Tensor],
+                         scale: float) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    fn = "linear_attention_bwd"
+    _la_check(fn, q, k, v, log_decay, initial_state, seq_lens, scale)
+    require_gpu(fn, q, g, gstate)
+    if tuple(g.shape) != (*q.shape[:3], v.shape[3]):
+        raise ValueError(f"{fn}: g must be {(*q.shape[:3], v.shape[3])}, got {tuple(g.shape)}")
+    _la_check_first(fn, gstate, q, v)
+    s0 = None if initial_state is None else initial_state.contiguous()
+    dq, dk, dv, ds = _la_backward(q, k, v, log_decay.contiguous(), s0, _la_index(seq_lens), scale, g, gstate,
+                                  (True, True, True, s0 is not None))
+    return dq, dk, dv, _opt(ds, q, torch.float32)
+
+
+@linear_attention_bwd.register_fake
+def _(q, k, v, log_decay, initial_state, seq_lens, g, gstate, scale):
+    return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape),
+            q.new_empty((0,) if initial_state is None else initial_state.shape, dtype=torch.float32))
+
+
+@torch.library.custom_op("hclsm_hip::linear_attention_step", mutates_args=("state",))
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, rows: Optional[Tensor],
+                          scale: float) -> Tensor:
+    fn = "linear_attention_step"
+    require_gpu(fn, q, k, v, log_decay, state, rows)
+    _la_check_qkv(fn, q, k, v, log_decay, scale, True)
+    _la_check_index(fn, "rows", rows, q.shape[0])
+    _la_check_state(fn, state, q.shape[0] if rows is None else None, q.shape[1], q.shape[2], v.shape[2])
+    return _la_step(q, k, v, log_decay.contiguous(), state, _la_index(rows), scale)
+
+
+@linear_attention_step.register_fake
+def _(q, k, v, log_decay, state, rows, scale):
+    return q.new_empty((q.shape[0], q.shape[1], v.shape[2]))
+
+
+@torch.library.custom_op("hclsm_hip::residual_rms_norm_fwd", mutates_args=())
+def residual_rms_norm_fwd(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], eps: float) -> tuple[Tensor, Tensor]:
+    require_gpu("residual_rms_norm_fwd", x, residual, weight)
+    _rn_check("residual_rms_norm_fwd", x, residual, weight, eps)
+    y, h = _rn_forward(x, residual, None if weight is None else weight.contiguous(), eps)
+    return y, _opt(h, x)
+
+
+@residual_rms_norm_fwd.register_fake
+def _(x, residual, weight, eps):
+    return x.new_empty(x.shape), x.new_empty((0,)) if residual is None else residual.new_empty(residual.shape)
+
+
+@torch.library.custom_op("hclsm_hip::residual_rms_norm_fp8", mutates_args=())
+def residual_rms_norm_fp8(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], eps: float,
+                          group: int) -> tuple[Tensor, Tensor, Tensor]:
+    require_gpu("residual_rms_norm_fp8", x, residual, weight)
+    _rn_check("residual_rms_norm_fp8", x, residual, weight, eps)
+    _rn_check_group("residual_rms_norm_fp8", x, group or None)
+    y, scale, h = _rn_forward_fp8(x, residual, None if weight is None else weight.contiguous(), eps, group)
+    return y, scale, _opt(h, x)
+
+
+@residual_rms_norm_fp8.register_fake
+def _(x, residual, weight, eps, group):
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
+            x.new_empty((*x.shape[:-1], x.shape[-1] // group if group else 1), dtype=torch.float32),
+            x.new_empty((0,)) if residual is None else residual.new_empty(residual.shape))
+
+
+@torch.library.custom_op("hclsm_hip::residual_rms_norm_bwd", mutates_args=())
+def residual_rms_norm_bwd(h: Tensor, weight: Optional[Tensor], gy: Tensor, gh: Optional[Tensor],
+                          eps: float) -> tuple[Tensor, Tensor, Tensor]:
+    fn = "residual_rms_norm_bwd"
+    require_gpu(fn, h, weight, gy, gh)
+    _rn_check(fn, gy, h, weight, eps)
+    if gh is not None and gh.shape != h.shape:
+        raise ValueError(f"{fn}: gh must be {tuple(h.shape)}, got {tuple(gh.shape)}")
+    w = None if weight is None else weight.contiguous()
+    dx, dr, dw = _rn_backward(h, w, gy, gh, eps, gy.dtype, True, h.dtype is not gy.dtype, w is not None)
+    return dx, _opt(dr, h), _opt(dw, h)
+
+
+@residual_rms_norm_bwd.register_fake
+def _(h, weight, gy, gh, eps):
+    return (gy.new_empty(h.shape), h.new_empty(h.shape if h.dtype is not gy.dtype else (0,)),
+            h.new_empty((0,)) if weight is None else weight.new_empty(weight.shape))

@@ -50,6 +50,11 @@ def _explain(fn, x, residual, weight, eps):
     raise ValueError(f"{fn}: eps must be >= 0 and finite, got {eps}")
 
 
+def _check_group(fn, x, group):
+    if group is not None and (group not in GROUPS or x.shape[-1] % group):
+        raise ValueError(f"{fn}: group must be None or one of {GROUPS} that divides {x.shape[-1]}, got {group}")
+
+
 def _rows2d(t):
     """(rows, D) of a tensor, and the rows' stride: a view where the columns are contiguous and the rows evenly apart."""
     D = t.shape[-1]
@@ -201,8 +206,7 @@ def residual_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None = None,
     require_gpu(fn, x, residual, weight)
     eps = float(eps)
     _check(fn, x, residual, weight, eps)
-    if group is not None and (group not in GROUPS or x.shape[-1] % group):
-        raise ValueError(f"{fn}: group must be None or one of {GROUPS} that divides {x.shape[-1]}, got {group}")
+    _check_group(fn, x, group)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
         raise RuntimeError(f"{fn}: 8-bit outputs have no gradient; use residual_rms_norm, or torch.no_grad()")
     y, scale, h = _forward_fp8(x, residual, None if weight is None else weight.contiguous(), eps, group or 0)
