@@ -21,6 +21,7 @@ _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib
 MAX_COLUMNS = 16384
 GROUPS = (32, 64, 128)
 _INF = float("inf")
+_BWD_BLOCKS = 1024          # most partial sums of the weight's gradient (hclsm_residual_norm_backward_workspace)
 
 
 def _check(fn, x, residual, weight, eps):
@@ -123,28 +124,28 @@ def _on_boundaries(t, stride):
 
 def _backward(h, weight, gy, gh, eps, x_dtype, want_x, want_r, want_w):
     """Gradients of x, of the residual (None where it is that of x) and of the weight."""
-    D = h.shape[-1]
+    h_dtype, D = h.dtype, h.shape[-1]
     if gy is not None and gy.dtype is not x_dtype:
         gy = gy.to(x_dtype)
-    if gh is not None and gh.dtype is not h.dtype:
-        gh = gh.to(h.dtype)
-    same = h.dtype is x_dtype
+    if gh is not None and gh.dtype is not h_dtype:
+        gh = gh.to(h_dtype)
+    same = h_dtype is x_dtype
+    n = h.numel() // D
     dx = _like(h, x_dtype) if want_x or (same and want_r) else None
     dr = _like(h) if want_r and not same else None
-    dw = torch.empty((D,), dtype=weight.dtype, device=h.device) if want_w else None
-    n = _count(h)
+    dw = ws = None
+    wsb = 0
+    if want_w:
+        dw = torch.empty_like(weight)
+        wsb = (n if n < _BWD_BLOCKS else _BWD_BLOCKS) * D * 4
+        ws = torch.empty(wsb + 16, dtype=torch.uint8, device=h.device)
     h, hs = _rows2d(h)
     gy, gys = (None, 0) if gy is None else _rows2d(gy)
     gh, ghs = (None, 0) if gh is None else _rows2d(gh)
-    L = _lib.lib()
-    ws, wsb = None, 0
-    if want_w:
-        wsb = int(L.hclsm_residual_norm_backward_workspace(n, D))
-        ws = torch.empty(max(wsb, 16), dtype=torch.uint8, device=h.device)
     a = _lib.pack_residual(0, 0, _ptr(weight), h.data_ptr(), _ptr(gy), _ptr(gh), 0, 0, 0, _ptr(dx), _ptr(dr), _ptr(dw), 0, 0, hs,
-                           gys, ghs, n, D, 0, eps, _CODE[x_dtype], _CODE[h.dtype], 0 if weight is None else _CODE[weight.dtype])
+                           gys, ghs, n, D, 0, eps, _CODE[x_dtype], _CODE[h_dtype], 0 if weight is None else _CODE[weight.dtype])
     with on_device(h.device):
-        rc = L.hclsm_residual_norm_backward(a, None if ws is None else ws.data_ptr(), wsb, _lib.stream_of(h))
+        rc = _lib.lib().hclsm_residual_norm_backward(a, None if ws is None else ws.data_ptr(), wsb, _lib.stream_of(h))
     if rc:
         _lib.check(rc, "hclsm_residual_norm_backward")
     return dx, (dx if same else dr) if want_r else None, dw
@@ -155,7 +156,9 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
         y, h = _forward(x, residual, weight, eps)
-        ctx.save_for_backward(x if h is None else h, weight)
+        if h is None:
+            h = x           # an output too (a view of x): its gradient is added in the backward's one rounding
+        ctx.save_for_backward(h, weight)
         ctx.eps, ctx.x_dtype = eps, x.dtype
         ctx.set_materialize_grads(False)
         return y, h
@@ -166,12 +169,12 @@ class _ResidualNorm(torch.autograd.Function):
 
     @staticmethod
     def _back(ctx, gy, gh):
-        h, weight = ctx.saved_tensors
         if gy is None and gh is None:
             return None, None, None, None
-        need = ctx.needs_input_grad
-        dx, dr, dw = _backward(h, weight, gy, gh, ctx.eps, ctx.x_dtype, need[0], need[1], need[2])
-        return dx if need[0] else None, dr, dw, None
+        h, weight = ctx.saved_tensors
+        x, r, w, _ = ctx.needs_input_grad
+        dx, dr, dw = _backward(h, weight, gy, gh, ctx.eps, ctx.x_dtype, x, r, w)
+        return dx if x else None, dr, dw, None
 
 
 def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, weight: torch.Tensor | None = None, *,
@@ -179,7 +182,7 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, wei
     """(y, h): h = x + residual and y = h / sqrt(mean(h^2) + eps) * weight over the last dimension.
 
     x (..., D), bfloat16, float16 or float32, 1 <= D <= 16384; residual: x's shape, x's type or float32, or None (then h is
-    x itself); weight (D,) of any of the float types, None: ones.  Rows of (rows, D) views may lie any distance apart; other
+    x, or a view of it where gradients are recorded); weight (D,) of any of the float types, None: ones.  Rows of (rows, D) views may lie any distance apart; other
     views are copied.  y has x's type, h the residual's.  Differentiable in all three, through both outputs; float32 between
     the loads and the one rounding of each output."""
     fn = "residual_rms_norm"
@@ -191,7 +194,7 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, wei
     if _no_node([t for t in (x, residual, weight) if t is not None]):
         y, h = _forward(x, residual, weight, eps)
     else:
-        y, h = _ResidualNorm.apply(x, residual, weight, eps)
+        return _ResidualNorm.apply(x, residual, weight, eps)
     return y, (x if h is None else h)
 
 

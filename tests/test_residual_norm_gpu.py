@@ -49,7 +49,7 @@ def _compare(x, r, w, gy, gh, eps):
     ins = [None if t is None else t.detach().requires_grad_() for t in (x, r, w)]
     y, h = residual_rms_norm(*ins, eps=eps)
     if r is None:
-        assert h is ins[0]
+        assert h.data_ptr() == ins[0].data_ptr() and h.shape == x.shape
     else:
         assert h.dtype == r.dtype and torch.equal(h, (x.float() + r.float()).to(r.dtype))
     hn, wn = _np(h), _np(w)
@@ -62,11 +62,8 @@ def _compare(x, r, w, gy, gh, eps):
     i = 1 / np.sqrt((hn * hn).mean(-1, keepdims=True) + eps)
     n, gw = np.abs(hn * i), np.abs(_np(gy) * (1 if wn is None else wn))
     M = i * (gw + n * (gw * n).mean(-1, keepdims=True)) + np.abs(_np(gh))
-    if r is None:       # the gradient of h comes back as x's own, added to the norm's in x's type: two roundings more
-        e = torch.finfo(x.dtype).eps
-        assert (np.abs(_np(got[0]) - dh) <= e * (np.abs(dh) + M) + 120 * U * M + 2 * TINY[x.dtype]).all()
-    else:
-        _within(got[0], dh, M, 120, "dx")
+    _within(got[0], dh, M, 120, "dx")
+    if r is not None:
         _within(got[1], dh, M, 120, "dr")
         assert got[1].dtype == r.dtype
     assert got[0].dtype == x.dtype
