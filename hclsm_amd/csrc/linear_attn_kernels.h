@@ -47,16 +47,6 @@ template <int N> __device__ __forceinline__ void la_split(const caf4* t, LaFrag*
   for (int p = 0; p < N; ++p) out[p] = ca_frag<HCLSM_BF16>(w[p]);
 }
 
-// acc += sum over the planes whose orders add up to at most MOST (what is left out lies below the last plane kept).
-template <int NA, int NB, int MOST> __device__ __forceinline__ caf4 la_mma(const LaFrag* a, const LaFrag* b, caf4 acc) {
-#pragma unroll
-  for (int i = 0; i < NA; ++i)
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
-      if (i + j <= MOST) acc = LaB::mma(a[i], b[j], acc);
-  return acc;
-}
-
 // Rows of one chunk on their way from global memory to LDS: row r of the tile is token r, or n - 1 - r backwards, of the chunk's n
 // live ones; other rows and columns past d are zeros (a load past the buffer resource's end gives zeros).  bf16 goes straight
 // to LDS, the other types through registers, in which they are split into their planes.  The offsets stand for a number of live
@@ -137,7 +127,8 @@ template <int D> __device__ __forceinline__ LaFrag la_frag_cols(char* t, int row
   return __builtin_bit_cast(LaFrag, r);
 }
 
-// acc[t] += a b[t] for every t, over the planes as la_mma: products in a row have results of their own.
+// acc[t] += a b[t] for every t, over the planes whose orders add up to at most MOST (what is left out lies below the last plane
+// kept): products in a row have results of their own.
 template <int NA, int NB, int MOST, int T> __device__ __forceinline__ void la_mma_all(const LaFrag* a, const LaFrag (*b)[NB], caf4* acc) {
 #pragma unroll
   for (int i = 0; i < NA; ++i)
@@ -185,7 +176,7 @@ __device__ __forceinline__ void la_update(char* tb, int row0, const float* v, ca
   for (int p = 0; p < N; ++p) fw[p] = ca_frag<HCLSM_BF16>(w[p]);
 #pragma unroll
   for (int m = 0; m < M; m += 4) {
-    if (m + 4 < M) get(m + 4, fb[(m >> 2) + 1 & 1]);
+    if (m + 4 < M) get(m + 4, fb[((m >> 2) + 1) & 1]);
     ca_fence();
     la_mma_all<NP, N, N - 1, 4>(fb[(m >> 2) & 1], fw, s + m);
     ca_fence();
@@ -196,6 +187,16 @@ __device__ __forceinline__ void la_update(char* tb, int row0, const float* v, ca
 // tokens, chunk after chunk.  Wave w owns 16 columns of the state, in registers for the whole segment; the weights of
 // pairs (A_r . B_s) a^(r-s) are shared out over the waves and passed through LDS in the order in which the matrix unit
 // reads them.  Several workgroups of a CU hide each other's waits.  SUM: the state alone, from zero (the sum of a segment).
+//
+// Why 64 columns: A and B are read once for each column tile (from L2: the tiles of a head run on one XCD), and 64 leaves the
+// registers and LDS for two or three workgroups to a CU; 128 columns by eight waves, one workgroup to a CU, took 996 us where
+// this takes 600 (below).  Why 64 tokens: the state's share, 4 dk dv flops a token, does not depend on it, the pairs' grows with it,
+// and the planes of the state are formed once for each chunk.  Why two buffers of B and X: one of each took 746 us.
+// What bounds it, bf16: heads of 64, HBM (32 x 1024 tokens, 12 heads, with gradients: 173 us, 704 MB, 4.1 TB/s; 50176 tokens of 12
+// heads, split over time, main launch 78 us, 3.9 TB/s).  Heads of 128 (8 x 4096 tokens, 16 heads, with gradients: 600 us,
+// 3.1 TB/s): vector unit 41%, matrix unit 28%, LDS 29% of the backward's cycles, in turn, since two waves per SIMD do not cover
+// each other's waits.  float16 takes 1.5 to 2.4 times and float32 2.5 to 3.4 times as long: two and three planes for each
+// input, formed on the way to LDS.
 template <int DT, int DA, bool SUM>
 __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const LaArgs args) {
   constexpr int NT = LA_THREADS, NW = NT / 64, XT = LA_XT, C = la_chunk(DT, DA), KT = C / 16, NS = DA / 16, NP = LaT<DT>::NP,

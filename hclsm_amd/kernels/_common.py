@@ -53,6 +53,14 @@ def on_device(dev: torch.device):
     return _SAME_DEVICE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+def call_on(index: int, fn, *args):
+    """fn(*args) with device ``index`` as the current one (``on_device`` without the cost of a context where it is)."""
+    if torch.cuda.current_device() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
 class HipFallbackWarning(UserWarning):
     """A call ran the reference's math as torch ops on the GPU instead of an hclsm_amd kernel (autograd through a
     forward-only kernel, or a module structure / shape the kernel does not take)."""

@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from hclsm_amd import _lib
-from hclsm_amd.kernels._common import on_device, once, require_gpu
+from hclsm_amd.kernels._common import call_on, once, require_gpu
 from hclsm_amd.kernels.ssm_scan_kernel import _no_node
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -91,6 +91,9 @@ def _rows(t):
     """t with rows on 16-byte boundaries and near enough to each other (t itself where they are): the kernels' offsets from
     a chunk's first row are 31 bits."""
     n = 16 // t.element_size()
+    if t.is_contiguous():       # heads are multiples of 8 elements, rows smaller than _FAR unless there is one alone
+        if t.data_ptr() % 16 == 0 and (t.shape[1] < 2 or t.stride(1) < _FAR):
+            return t
     sb, sl, sh, s = t.stride()
     B, L, H, _ = t.shape
     if (s == 1 and t.data_ptr() % 16 == 0 and (sb % n == 0 or B == 1) and (L == 1 or (sl % n == 0 and sl < _FAR))
@@ -109,6 +112,14 @@ def _strides(t):
 
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
+
+
+def _run(name, t, *args):
+    """The library's entry on t's device and stream (its last argument)."""
+    index = t.get_device()
+    rc = call_on(index, getattr(_lib.lib(), name), *args, _lib.stream_of_device(index))
+    if rc:
+        _lib.check(rc, name)
 
 
 _WORKSPACE: dict = {}       # sizes -> bytes (a function of the sizes alone)
@@ -138,10 +149,7 @@ def _forward(q, k, v, log_decay, s0, lens, scale, want_state):
     x = _lib.pack_linear(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, log_decay.data_ptr(), _ptr(s0), _ptr(s1), 0, 0,
                          out.data_ptr(), 0, 0, 0, _ptr(lens), *_strides(q), *_strides(k), *_strides(v), 0, 0, 0, B, L, H,
                          k.shape[2], dk, dv, scale, _CODE[q.dtype], _index_code(lens))
-    with on_device(q.device):
-        rc = _lib.lib().hclsm_linear_attention_forward(x, None if ws is None else ws.data_ptr(), n, _lib.stream_of(q))
-    if rc:
-        _lib.check(rc, "hclsm_linear_attention_forward")
+    _run("hclsm_linear_attention_forward", q, x, _ptr(ws), n)
     return out, s1
 
 
@@ -162,10 +170,7 @@ def _backward(q, k, v, log_decay, s0, lens, scale, g, gs, want):
     x = _lib.pack_linear(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), log_decay.data_ptr(), _ptr(s0), 0, _ptr(gs),
                          _ptr(ds), 0, _ptr(dq), _ptr(dk_), _ptr(dv_), _ptr(lens), *_strides(q), *_strides(k), *_strides(v),
                          *_strides(g), B, L, H, k.shape[2], dk, dv, scale, _CODE[q.dtype], _index_code(lens))
-    with on_device(q.device):
-        rc = _lib.lib().hclsm_linear_attention_backward(x, None if ws is None else ws.data_ptr(), n, _lib.stream_of(q))
-    if rc:
-        _lib.check(rc, "hclsm_linear_attention_backward")
+    _run("hclsm_linear_attention_backward", q, x, _ptr(ws), n)
     return dq, dk_, dv_, ds
 
 
@@ -203,7 +208,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
         gradient here, and one that requires grad is refused.
     initial_state (B, H, dk, dv) float32: the state in front of the first token; None: zeros.
     seq_lens (B,) int32 or int64: tokens from seq_lens[b] on are not read (they may hold anything), give zeros, take part
-        in no gradient and leave the state as it is.
+        in no gradient and leave the state as it is.  Live tokens are to be finite: outputs of up to 63 tokens before one
+        that is not may be NaN too (tokens are taken in chunks).
     scale: dk ** -0.5 if None; positive.
 
     Returns out (B, L, H, dv), and with return_state the state behind each row's last live token, (B, H, dk, dv) float32,
@@ -278,8 +284,5 @@ def _step(q, k, v, log_decay, state, rows, scale):
     x = _lib.pack_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(), _ptr(rows),
                        out.data_ptr(), qb, qh, kb, kh, vb, vh, state.stride(0), state.shape[0], B, H, Hk, dk, dv, scale,
                        _CODE[q.dtype], _index_code(rows))
-    with on_device(q.device):
-        rc = _lib.lib().hclsm_linear_attention_step(x, _lib.stream_of(q))
-    if rc:
-        _lib.check(rc, "hclsm_linear_attention_step")
+    _run("hclsm_linear_attention_step", q, x)
     return out

@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from hclsm_amd import _lib
-from hclsm_amd.kernels._common import on_device, once, require_gpu
+from hclsm_amd.kernels._common import call_on, once, require_gpu
 from hclsm_amd.kernels.ssm_scan_kernel import _no_node
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -56,14 +56,13 @@ def _check_group(fn, x, group):
         raise ValueError(f"{fn}: group must be None or one of {GROUPS} that divides {x.shape[-1]}, got {group}")
 
 
-def _rows2d(t):
+def _rows2d(t, D):
     """(rows, D) of a tensor, and the rows' stride: a view where the columns are contiguous and the rows evenly apart."""
-    D = t.shape[-1]
+    if t.is_contiguous():
+        return t, D
     if t.dim() == 2 and (t.stride(1) == 1 or D == 1):
         return t, t.stride(0)
-    if not t.is_contiguous():
-        t = t.contiguous()
-    return t, D
+    return t.contiguous(), D
 
 
 def _ptr(t):
@@ -75,44 +74,46 @@ def _like(t, dtype=None):
     return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
-def _count(x):
-    return x.numel() // x.shape[-1]
+def _run(name, t, *args):
+    """The library's entry on t's device and stream (its last argument)."""
+    index = t.get_device()
+    rc = call_on(index, getattr(_lib.lib(), name), *args, _lib.stream_of_device(index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _forward(x, residual, weight, eps):
-    D = x.shape[-1]
-    y = _like(x)
-    h = None if residual is None else _like(residual)
-    x, xs = _rows2d(x)
-    r, rs = (None, 0) if residual is None else _rows2d(residual)
+    D, code = x.shape[-1], _CODE[x.dtype]
+    y, n = _like(x), x.numel() // D
+    x, xs = _rows2d(x, D)
+    if residual is None:
+        h, r, rs, hc = None, None, 0, code
+    else:
+        h, hc = _like(residual), _CODE[residual.dtype]
+        r, rs = _rows2d(residual, D)
     a = _lib.pack_residual(x.data_ptr(), _ptr(r), _ptr(weight), 0, 0, 0, y.data_ptr(), _ptr(h), 0, 0, 0, 0, xs, rs, 0, 0, 0,
-                           _count(x), D, 0, eps, _CODE[x.dtype], _CODE[x.dtype if r is None else r.dtype],
-                           0 if weight is None else _CODE[weight.dtype])
-    with on_device(x.device):
-        rc = _lib.lib().hclsm_residual_norm_forward(a, _lib.stream_of(x))
-    if rc:
-        _lib.check(rc, "hclsm_residual_norm_forward")
+                           n, D, 0, eps, code, hc, 0 if weight is None else _CODE[weight.dtype])
+    _run("hclsm_residual_norm_forward", x, a)
     return y, h
 
 
 def _forward_fp8(x, residual, weight, eps, group):
-    D = x.shape[-1]
-    y = _like(x, torch.float8_e4m3fn)
+    D, code = x.shape[-1], _CODE[x.dtype]
+    y, n = _like(x, torch.float8_e4m3fn), x.numel() // D
     scale = torch.empty((*x.shape[:-1], D // group if group else 1), dtype=torch.float32, device=x.device)
-    h = None if residual is None else _like(residual)
-    x, xs = _rows2d(x)
-    r, rs = (None, 0) if residual is None else _rows2d(residual)
+    x, xs = _rows2d(x, D)
+    if residual is None:
+        h, r, rs, hc = None, None, 0, code
+    else:
+        h, hc = _like(residual), _CODE[residual.dtype]
+        r, rs = _rows2d(residual, D)
     if group:       # a group's lanes read whole vectors
         x, xs = _on_boundaries(x, xs)
         if r is not None:
             r, rs = _on_boundaries(r, rs)
     a = _lib.pack_residual(x.data_ptr(), _ptr(r), _ptr(weight), 0, 0, 0, y.data_ptr(), _ptr(h), scale.data_ptr(), 0, 0, 0, xs,
-                           rs, 0, 0, 0, _count(x), D, group, eps, _CODE[x.dtype],
-                           _CODE[x.dtype if r is None else r.dtype], 0 if weight is None else _CODE[weight.dtype])
-    with on_device(x.device):
-        rc = _lib.lib().hclsm_residual_norm_fp8(a, _lib.stream_of(x))
-    if rc:
-        _lib.check(rc, "hclsm_residual_norm_fp8")
+                           rs, 0, 0, 0, n, D, group, eps, code, hc, 0 if weight is None else _CODE[weight.dtype])
+    _run("hclsm_residual_norm_fp8", x, a)
     return y, scale, h
 
 
@@ -139,15 +140,12 @@ def _backward(h, weight, gy, gh, eps, x_dtype, want_x, want_r, want_w):
         dw = torch.empty_like(weight)
         wsb = (n if n < _BWD_BLOCKS else _BWD_BLOCKS) * D * 4
         ws = torch.empty(wsb + 16, dtype=torch.uint8, device=h.device)
-    h, hs = _rows2d(h)
-    gy, gys = (None, 0) if gy is None else _rows2d(gy)
-    gh, ghs = (None, 0) if gh is None else _rows2d(gh)
+    h, hs = _rows2d(h, D)
+    gy, gys = (None, 0) if gy is None else _rows2d(gy, D)
+    gh, ghs = (None, 0) if gh is None else _rows2d(gh, D)
     a = _lib.pack_residual(0, 0, _ptr(weight), h.data_ptr(), _ptr(gy), _ptr(gh), 0, 0, 0, _ptr(dx), _ptr(dr), _ptr(dw), 0, 0, hs,
                            gys, ghs, n, D, 0, eps, _CODE[x_dtype], _CODE[h_dtype], 0 if weight is None else _CODE[weight.dtype])
-    with on_device(h.device):
-        rc = _lib.lib().hclsm_residual_norm_backward(a, None if ws is None else ws.data_ptr(), wsb, _lib.stream_of(h))
-    if rc:
-        _lib.check(rc, "hclsm_residual_norm_backward")
+    _run("hclsm_residual_norm_backward", h, a, _ptr(ws), wsb)
     return dx, (dx if same else dr) if want_r else None, dw
 
 
