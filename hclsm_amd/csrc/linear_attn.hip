@@ -62,8 +62,8 @@ int la_sizes(const LaSizes& z) {
   return 0;
 }
 
-// and so do its inputs
-bool la_near(int64_t sl, int esz) { return sl >= 0 && sl * esz < (1 << 24); }
+// and so do its inputs (chunks of float32 have 32 tokens)
+bool la_near(int64_t sl) { return sl >= 0 && sl < 1 << 23; }
 
 bool la_aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int esz) {
   const int64_t n = 16 / esz;
@@ -187,8 +187,7 @@ int la_args(const HclsmLinearAttention* x, bool bwd, LaSizes& z) {
     if (!x->q || !x->k || !x->v || (bwd ? !x->g : !x->out)) return HCLSM_ERR_NULL;
     if (!la_aligned(x->q, x->q_sb, x->q_sl, x->q_sh, esz) || !la_aligned(x->k, x->k_sb, x->k_sl, x->k_sh, esz) ||
         !la_aligned(x->v, x->v_sb, x->v_sl, x->v_sh, esz)) return HCLSM_ERR_UNSUPPORTED;
-    if (!la_near(x->q_sl, esz) || !la_near(x->k_sl, esz) || !la_near(x->v_sl, esz) || (bwd && !la_near(x->g_sl, esz)))
-      return HCLSM_ERR_UNSUPPORTED;
+    if (!la_near(x->q_sl) || !la_near(x->k_sl) || !la_near(x->v_sl) || (bwd && !la_near(x->g_sl))) return HCLSM_ERR_UNSUPPORTED;
     if (bwd ? !la_aligned(x->g, x->g_sb, x->g_sl, x->g_sh, esz) : !la_aligned(x->out, 0, 0, 0, esz)) return HCLSM_ERR_UNSUPPORTED;
     if (bwd && (!la_aligned(x->dq, 0, 0, 0, esz) || !la_aligned(x->dk_out, 0, 0, 0, esz) || !la_aligned(x->dv_out, 0, 0, 0, esz)))
       return HCLSM_ERR_UNSUPPORTED;

@@ -21,7 +21,7 @@ _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib
 MAX_HEAD_DIM = 256
 _MAX_HEADS = 1 << 20        # heads of a call, B H
 _MAX_ROW = 1 << 23          # elements of a token, H max(dk, dv)
-_FAR = 1 << 22              # elements between tokens
+_FAR = 1 << 23              # elements between tokens
 
 
 def _check(fn, q, k, v, log_decay, scale, token):
@@ -91,9 +91,8 @@ def _rows(t):
     """t with rows on 16-byte boundaries and near enough to each other (t itself where they are): the kernels' offsets from
     a chunk's first row are 31 bits."""
     n = 16 // t.element_size()
-    if t.is_contiguous():       # heads are multiples of 8 elements, rows smaller than _FAR unless there is one alone
-        if t.data_ptr() % 16 == 0 and (t.shape[1] < 2 or t.stride(1) < _FAR):
-            return t
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:        # (heads are multiples of 8 elements, tokens smaller than _FAR)
+        return t
     sb, sl, sh, s = t.stride()
     B, L, H, _ = t.shape
     if (s == 1 and t.data_ptr() % 16 == 0 and (sb % n == 0 or B == 1) and (L == 1 or (sl % n == 0 and sl < _FAR))

@@ -427,3 +427,22 @@ def test_step_refuses_gradients():
         linear_attention_step(x, x, x, d, s)
     with torch.no_grad():
         linear_attention_step(x, x, x, d, s)
+
+
+@pytest.mark.parametrize("dtype,H", [(F32, 16384 + 4), (BF16, 32768 - 4)])
+def test_many_heads_of_one_token(dtype, H):
+    """Tokens of 2^22 to 2^23 elements, forward and backward: some heads are as if alone."""
+    from hclsm_amd.kernels import linear_attention
+    L, d, some = 40, 256, [0, 1, H // 2, H - 1]
+    gen = torch.Generator("cuda").manual_seed(24)
+    q, k, v, go = (torch.randn(1, L, H, d, generator=gen, device="cuda", dtype=dtype) for _ in range(4))
+    decay = -torch.rand(H, generator=gen, device="cuda")
+
+    def run(q, k, v, decay, go):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = linear_attention(*leaves, decay)
+        return [o.detach(), *torch.autograd.grad(o, leaves, go)]
+    got = [t[:, :, some] for t in run(q, k, v, decay, go)]
+    want = run(*(t[:, :, some].contiguous() for t in (q, k, v)), decay[some], go[:, :, some].contiguous())
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
