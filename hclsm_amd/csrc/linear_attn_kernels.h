@@ -19,25 +19,29 @@ template <> struct LaT<HCLSM_F32> { static constexpr int NP = 3, NC = 3, RAW = 2
 using LaB = CaT<HCLSM_BF16>;
 using LaFrag = cab8;
 
-// N planes of eight float32 values.
-template <int N> __device__ __forceinline__ void la_split(const float* v, uint4* out) {
-  float r[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = v[i];
+// N planes of four and of eight float32 values.
+template <int N> __device__ __forceinline__ void la_split(caf4 v, uint2* out) {
 #pragma unroll
   for (int p = 0; p < N; ++p) {
-    uint32_t w[4];
+    uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
+    for (int i = 0; i < 2; ++i) {
+      w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
       if (p + 1 < N) {
         asm("" : "+v"(w[i]));      // (the pair as it is: otherwise each element's conversion is repeated for its rest)
-        r[2 * i] -= LaB::lo(w[i]);
-        r[2 * i + 1] -= LaB::hi(w[i]);
+        v[2 * i] -= LaB::lo(w[i]);
+        v[2 * i + 1] -= LaB::hi(w[i]);
       }
     }
-    out[p] = uint4{w[0], w[1], w[2], w[3]};
+    out[p] = uint2{w[0], w[1]};
   }
+}
+template <int N> __device__ __forceinline__ void la_split(const float* v, uint4* out) {
+  uint2 a[N], b[N];
+  la_split<N>(caf4{v[0], v[1], v[2], v[3]}, a);
+  la_split<N>(caf4{v[4], v[5], v[6], v[7]}, b);
+#pragma unroll
+  for (int p = 0; p < N; ++p) out[p] = uint4{a[p].x, a[p].y, b[p].x, b[p].y};
 }
 template <int N> __device__ __forceinline__ void la_split(const caf4* t, LaFrag* out) {
   const float v[8] = {t[0][0], t[0][1], t[0][2], t[0][3], t[1][0], t[1][1], t[1][2], t[1][3]};
@@ -199,10 +203,10 @@ __device__ __forceinline__ void la_update(char* tb, int row0, const float* v, ca
 // input, formed on the way to LDS.
 template <int DT, int DA, bool SUM>
 __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const LaArgs args) {
-  constexpr int NT = LA_THREADS, NW = NT / 64, XT = LA_XT, C = la_chunk(DT, DA), KT = C / 16, NS = DA / 16, NP = LaT<DT>::NP,
+  constexpr int NT = LA_THREADS, XT = LA_XT, C = la_chunk(DT, DA), KT = C / 16, NS = DA / 16, NP = LaT<DT>::NP,
                 NC = LaT<DT>::NC;
   constexpr int ESZ = DT == HCLSM_F32 ? 4 : 2, MOST = NC - 1;
-  constexpr int NF = KT == 4 ? 6 : 2, NFW = (NF + NW - 1) / NW;     // pairs of 16-token tiles at or below the diagonal
+  constexpr int NF = KT == 4 ? 6 : 2;     // 16 tokens by 32 at or below the diagonal
   using SA = LaStage<DT, C, DA, NT>;
   using SX = LaStage<DT, C, XT, NT>;
   using TA = CaTile<HCLSM_BF16, DA>;
@@ -322,6 +326,11 @@ __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const 
     tt = KT == 4 ? (f < 2 ? f : 2 + ((f - 2) >> 1)) : f;
     sp = KT == 4 && f >= 2 ? (f & 1) : 0;
   };
+  if constexpr (!SUM) {     // the tiles above the diagonal, beside those on it: zeros throughout
+    if (wave < KT / 2)
+#pragma unroll
+      for (int p = 0; p < NC; ++p) reinterpret_cast<uint2*>(tp)[((3 * wave * NC + p) * 64 + lane) * 2 + 1] = uint2{0, 0};
+  }
   int tab = -1;             // live tokens that rx and decay are for
   float decay = 0.f;
   bool slow = false;
@@ -371,65 +380,74 @@ __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const 
 #pragma unroll
       for (int u = 0; u < KT; ++u) y[u] = caf4{0.f, 0.f, 0.f, 0.f};
       if (n > 0) {
-        // weights of pairs: tile (s, t) leaves a lane with s = 4g + r of its t = li.  Waves 0 and 1 have two pairs of tiles of
-        // the six; the operands of CG products of all a wave's pairs are read before the first.
+        // weights of pairs: tile (s, t) leaves a lane with s = 4g + r of its t = li.  The ten tiles at or below the diagonal (three
+        // of 32 tokens) are shared out as evenly as they go: two for every wave and a third for waves 0 and 1 (one for
+        // waves 0 to 2); the operands of CG products of all a wave's tiles are read before the first.
         {
-          constexpr int CG = DA == 64 ? 2 : NP == 1 ? 4 : 1;
-          caf4 w[NFW][2];
-          int tt[NFW], sp[NFW];
-          bool mine[NFW];
-#pragma unroll
-          for (int o = 0; o < NFW; ++o) {
-            const int f = NF == 6 ? (wave < 2 ? 2 * wave + o : wave + 2) : wave;
-            mine[o] = f < NF && (o == 0 || wave < 2);
-            pair(f, tt[o], sp[o]);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) w[o][u] = caf4{0.f, 0.f, 0.f, 0.f};
+          constexpr int CG = DA == 64 ? 2 : NP == 1 ? 4 : 1, SUBS = KT == 4 ? 3 : 1, AS = KT == 4 ? 2 : 1;
+          caf4 w[SUBS];
+          int tt[SUBS], st[SUBS];
+          bool mine[SUBS];
+          if constexpr (KT == 4) {
+            tt[0] = tt[1] = wave < 2 ? wave + 1 : 3;
+            st[0] = wave < 3 ? 0 : 2;
+            st[1] = st[0] + 1;
+            tt[2] = st[2] = 2 * wave;
+            mine[0] = mine[1] = true;
+            mine[2] = wave < 2;
+          } else {
+            tt[0] = wave > 0 ? 1 : 0;
+            st[0] = wave > 1 ? 1 : 0;
+            mine[0] = wave < 3;
           }
 #pragma unroll
-          for (int c0 = 0; c0 < DA / 32; c0 += CG) {
-            LaFrag fa[NFW][CG][NP], fb[NFW][CG][2][NP];
+          for (int o = 0; o < SUBS; ++o) w[o] = caf4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int o = 0; o < NFW; ++o)
+          for (int c0 = 0; c0 < DA / 32; c0 += CG) {
+            LaFrag fa[AS][CG][NP], fb[SUBS][CG][NP];
+#pragma unroll
+            for (int o = 0; o < SUBS; ++o)
               if (mine[o])
 #pragma unroll
                 for (int c = 0; c < CG; ++c)
 #pragma unroll
                   for (int p = 0; p < NP; ++p) {
-                    fa[o][c][p] = TA::frag(ta + p * SA::PLANE, 16 * tt[o], c0 + c, li, g);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) fb[o][c][u][p] = TA::frag(tb + p * SA::PLANE, 32 * sp[o] + 16 * u, c0 + c, li, g);
+                    if (o != 1) fa[o >> 1][c][p] = TA::frag(ta + p * SA::PLANE, 16 * tt[o], c0 + c, li, g);
+                    fb[o][c][p] = TA::frag(tb + p * SA::PLANE, 16 * st[o], c0 + c, li, g);
                   }
             ca_fence();
 #pragma unroll
-            for (int o = 0; o < NFW; ++o)
-              if (mine[o])
+            for (int c = 0; c < CG; ++c)
 #pragma unroll
-                for (int c = 0; c < CG; ++c)
+              for (int i = 0; i < NP; ++i)
 #pragma unroll
-                  for (int i = 0; i < NP; ++i)
+                for (int p = 0; p < NP; ++p)
+                  if (i + p <= MOST) {
 #pragma unroll
-                    for (int p = 0; p < NP; ++p)
-                      if (i + p <= MOST)
+                    for (int o = 0; o < (KT == 4 ? 2 : 0); ++o) w[o] = LaB::mma(fb[o][c][i], fa[0][c][p], w[o]);
+                  }
+            if (mine[SUBS - 1])
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) w[o][u] = LaB::mma(fb[o][c][u][i], fa[o][c][p], w[o][u]);
+              for (int c = 0; c < CG; ++c)
+#pragma unroll
+                for (int i = 0; i < NP; ++i)
+#pragma unroll
+                  for (int p = 0; p < NP; ++p)
+                    if (i + p <= MOST) w[SUBS - 1] = LaB::mma(fb[SUBS - 1][c][i], fa[AS - 1][c][p], w[SUBS - 1]);
           }
 #pragma unroll
-          for (int o = 0; o < NFW; ++o)
+          for (int o = 0; o < SUBS; ++o)
             if (mine[o]) {
+              const int apart = tt[o] - st[o];      // tiles between the two
+              const float more = apart > 2 ? w16 * w16 : apart > 1 ? w16 : 1.f;
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const int apart = tt[o] - 2 * sp[o] - u;      // tiles between the two
-                const float more = apart > 2 ? w16 * w16 : apart > 1 ? w16 : 1.f;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)      // (what lies above the diagonal may be infinite)
-                  w[o][u][r] = 16 * apart + li >= 4 * g + r ? w[o][u][r] * (apart > 0 ? w1[r] * more : wd[r]) : 0.f;
-              }
-              LaFrag fp[NC];
+              for (int r = 0; r < 4; ++r)      // (what lies above the diagonal may be infinite)
+                w[o][r] = 16 * apart + li >= 4 * g + r ? w[o][r] * (apart > 0 ? w1[r] * more : wd[r]) : 0.f;
+              uint2 fp[NC];
               la_split<NC>(w[o], fp);
-              const int f = NF == 6 ? (wave < 2 ? 2 * wave + o : wave + 2) : wave;
+              const int f = KT == 4 ? (tt[o] < 2 ? tt[o] : 2 * tt[o] - 2 + (st[o] >> 1)) : tt[o];
 #pragma unroll
-              for (int p = 0; p < NC; ++p) tp[(f * NC + p) * 64 + lane] = __builtin_bit_cast(uint4, fp[p]);
+              for (int p = 0; p < NC; ++p) reinterpret_cast<uint2*>(tp)[((f * NC + p) * 64 + lane) * 2 + (st[o] & 1)] = fp[p];
             }
         }
         // what the state gives: y^T = S^T A^T, the next operands on their way
