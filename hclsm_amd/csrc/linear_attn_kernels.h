@@ -86,7 +86,7 @@ template <int DT, int C, int D, int NT> struct LaStage {
       // row r0 + u STEP, backwards C - 1 - r0 - u STEP
       const int off = c0 < d ? (back ? C - 1 - (U - 1) * STEP - r0 : r0) * sb + c0 * ESZ : (int)NONE;
 #pragma unroll
-      for (int u = 0; u < U; ++u) one(u, off, (back ? U - 1 - u : u) * STEP * sb);
+      for (int u = 0; u < U; ++u) one(u, off, __builtin_amdgcn_readfirstlane((back ? U - 1 - u : u) * STEP * sb));
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -164,11 +164,11 @@ __device__ __forceinline__ void la_barrier() {
 // operands of the next four on their way.
 template <int DA, int NP, int N, int PLANE>
 __device__ __forceinline__ void la_update(char* tb, int row0, const float* v, caf4* s, int li, int g) {
-  constexpr int M = DA / 16;
-  LaFrag fb[2][4][NP];
+  constexpr int M = DA / 16, T = DA == 256 ? 2 : 4;
+  LaFrag fb[2][T][NP];
   auto get = [&](int m0, LaFrag (*f)[NP]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < T; ++m)
 #pragma unroll
       for (int p = 0; p < NP; ++p) f[m][p] = la_frag_cols<DA>(tb + p * PLANE, row0, (m0 + m) >> 1, (m0 + m) & 1, li, g);
   };
@@ -179,10 +179,10 @@ __device__ __forceinline__ void la_update(char* tb, int row0, const float* v, ca
 #pragma unroll
   for (int p = 0; p < N; ++p) fw[p] = ca_frag<HCLSM_BF16>(w[p]);
 #pragma unroll
-  for (int m = 0; m < M; m += 4) {
-    if (m + 4 < M) get(m + 4, fb[((m >> 2) + 1) & 1]);
+  for (int m = 0; m < M; m += T) {
+    if (m + T < M) get(m + T, fb[(m / T + 1) & 1]);
     ca_fence();
-    la_mma_all<NP, N, N - 1, 4>(fb[(m >> 2) & 1], fw, s + m);
+    la_mma_all<NP, N, N - 1, T>(fb[m / T & 1], fw, s + m);
     ca_fence();
   }
 }
@@ -264,11 +264,12 @@ __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const 
 
   // the state: tile m of 16 rows holds da = 32 (m / 2) + 8g + 4 (m & 1) + r of column xc + li
   caf4 s[NS];
-  const int64_t state = (int64_t)j.da * j.dx;
+  const int da = j.da, dx = j.dx;
+  const int64_t state = (int64_t)da * dx;
   // byte offset of tile m's row r of the lane's column in a state, past its end where there is none
   auto place = [&](int m, int r, int sr, int sc) __attribute__((always_inline)) {
-    const int d = 32 * (m >> 1) + 8 * g + 4 * (m & 1) + r;
-    return d < j.da && xc + li < j.dx ? (d * sr + (xc + li) * sc) * 4 : (int)SA::NONE;
+    const int d = 32 * (m >> 1) + 8 * g + 4 * (m & 1) + r, at = (d * sr + (xc + li) * sc) * 4;
+    return d < da && xc + li < dx ? at : (int)SA::NONE;
   };
 #pragma unroll
   for (int m = 0; m < NS; ++m) s[m] = caf4{0.f, 0.f, 0.f, 0.f};
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const 
                 base_x = (b * j.x.sb + (h / j.x.group) * j.x.sh + x0) * ESZ;
   const char *pa = j.a.p + base_a, *pb = j.b.p + base_b, *px = j.x.p + base_x;
   const int sa_b = (int)j.a.sl * ESZ, sb_b = (int)j.b.sl * ESZ, sx_b = (int)j.x.sl * ESZ;      // bytes between tokens
-  const int da = j.da, dx = j.dx, ysz = j.y32 ? 4 : ESZ, yrow = args.H * dx * ysz;
+  const int ysz = j.y32 ? 4 : ESZ, yrow = args.H * dx * ysz;
   const bool wanted = j.y != nullptr, wide = DT == HCLSM_F32 || j.y32 != 0, fine = NC == 3 || args.fine != 0;
   char* py = j.y + ((int64_t)b * args.L * args.H + h) * dx * ysz;
   const float cu = j.cu;
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const 
     char* tx = tb + SA::BYTES;
     if constexpr (DMA) {
       ca_wait_vmem();
-      __syncthreads();      // the chunk is in LDS, and every wave is done with the one before
+      la_barrier();         // the chunk is in LDS, and every wave is done with the one before
       if (n1 > 0) load_bx(t1, n1, next);
     } else {
       la_barrier();
@@ -435,20 +436,32 @@ __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const 
                   for (int p = 0; p < NP; ++p)
                     if (i + p <= MOST) w[SUBS - 1] = LaB::mma(fb[SUBS - 1][c][i], fa[AS - 1][c][p], w[SUBS - 1]);
           }
+          auto weigh = [&](int o) __attribute__((always_inline)) {
+            const int apart = tt[o] - st[o];      // tiles between the two
+            const float more = apart > 2 ? w16 * w16 : apart > 1 ? w16 : 1.f;
 #pragma unroll
-          for (int o = 0; o < SUBS; ++o)
-            if (mine[o]) {
-              const int apart = tt[o] - st[o];      // tiles between the two
-              const float more = apart > 2 ? w16 * w16 : apart > 1 ? w16 : 1.f;
+            for (int r = 0; r < 4; ++r)      // (what lies above the diagonal may be infinite)
+              w[o][r] = 16 * apart + li >= 4 * g + r ? w[o][r] * (apart > 0 ? w1[r] * more : wd[r]) : 0.f;
+            return KT == 4 ? (tt[o] < 2 ? tt[o] : 2 * tt[o] - 2 + (st[o] >> 1)) : tt[o];
+          };
+          if constexpr (KT == 4) {
+            const int f = weigh(0);
+            weigh(1);
+            LaFrag fp[NC];
+            la_split<NC>(w, fp);
 #pragma unroll
-              for (int r = 0; r < 4; ++r)      // (what lies above the diagonal may be infinite)
-                w[o][r] = 16 * apart + li >= 4 * g + r ? w[o][r] * (apart > 0 ? w1[r] * more : wd[r]) : 0.f;
-              uint2 fp[NC];
-              la_split<NC>(w[o], fp);
-              const int f = KT == 4 ? (tt[o] < 2 ? tt[o] : 2 * tt[o] - 2 + (st[o] >> 1)) : tt[o];
+            for (int p = 0; p < NC; ++p) tp[(f * NC + p) * 64 + lane] = __builtin_bit_cast(uint4, fp[p]);
+          }
+          if (mine[SUBS - 1]) {
+            const int f = weigh(SUBS - 1);
+            uint2 fp[NC];
+            la_split<NC>(w[SUBS - 1], fp);
 #pragma unroll
-              for (int p = 0; p < NC; ++p) reinterpret_cast<uint2*>(tp)[((f * NC + p) * 64 + lane) * 2 + (st[o] & 1)] = fp[p];
+            for (int p = 0; p < NC; ++p) {
+              reinterpret_cast<uint2*>(tp)[((f * NC + p) * 64 + lane) * 2 + (st[SUBS - 1] & 1)] = fp[p];
+              asm volatile("" ::: "memory");      // (two writes in one instruction would wait for the transfers in flight)
             }
+          }
         }
         // what the state gives: y^T = S^T A^T, the next operands on their way
         {
@@ -509,26 +522,30 @@ __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const 
     if constexpr (!SUM) {      // (here, not at the end: the state's sum hides the stores)
       if (wanted) {
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(py + (int64_t)t0 * yrow, 0, 0x7fffffff, kRawBufferWord3);
-        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-        const int cb = (xc + 4 * g) * ysz;
-        auto put = [&](caf4 v, int off, int so) __attribute__((always_inline)) {
-          off = xc + 4 * g < dx ? off : (int)SA::NONE;
-          if (wide) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), rs, off, so, 0);
-          else if constexpr (DT != HCLSM_F32)
-            __builtin_amdgcn_raw_buffer_store_b64(u2{CaT<DT>::pack2(v[0], v[1]), CaT<DT>::pack2(v[2], v[3])}, rs, off, so, 0);
-        };
-        if (n == C) {
-          const int off = (back ? 15 - li : li) * yrow + cb;
+        const int cb = xc + 4 * g < dx ? (xc + 4 * g) * ysz : (int)SA::NONE;
+        auto put_all = [&](auto put) __attribute__((always_inline)) {
+          if (n == C) {
+            const int off = cb < 0 ? cb : (back ? 15 - li : li) * yrow + cb;
 #pragma unroll
-          for (int u = 0; u < KT; ++u) put(y[u], off, (back ? KT - 1 - u : u) * 16 * yrow);
-        } else {      // tokens that are not live get zeros
+            for (int u = 0; u < KT; ++u) put(y[u], rs, off, (back ? KT - 1 - u : u) * 16 * yrow);
+          } else {      // tokens that are not live get zeros
 #pragma unroll
-          for (int u = 0; u < KT; ++u) {
-            const int r = 16 * u + li, tok = r < n && back ? n - 1 - r : r;
-            put(r < n ? y[u] : caf4{0.f, 0.f, 0.f, 0.f}, t0 + tok < t_end ? tok * yrow + cb : (int)SA::NONE, 0);
+            for (int u = 0; u < KT; ++u) {
+              const int r = 16 * u + li, tok = r < n && back ? n - 1 - r : r;
+              put(r < n ? y[u] : caf4{0.f, 0.f, 0.f, 0.f}, rs, cb >= 0 && t0 + tok < t_end ? tok * yrow + cb : (int)SA::NONE, 0);
+            }
           }
-        }
+        };
+        if (wide)
+          put_all([](caf4 v, __amdgpu_buffer_rsrc_t rs, int off, int so) __attribute__((always_inline)) {
+            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), rs, off, so, 0);
+          });
+        else if constexpr (DT != HCLSM_F32)
+          put_all([](caf4 v, __amdgpu_buffer_rsrc_t rs, int off, int so) __attribute__((always_inline)) {
+            typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+            __builtin_amdgcn_raw_buffer_store_b64(u2{CaT<DT>::pack2(v[0], v[1]), CaT<DT>::pack2(v[2], v[3])}, rs, off, so, 0);
+          });
       }
     }
     if (n > 0) {
