@@ -9,7 +9,7 @@ namespace {
 // sum formed first (from zero), the states in front of the segments from those, and then all segments at once, two workgroups to a
 // CU.  The sums read B and X once more.  Measured, 50176 tokens of 12 heads of 64: 21 segments 140 us, 32: 130, 42: 116, 53: 124, 64:
 // 119; training steps of 32 x 1024 tokens (384 workgroups forward): 173 unsplit, 183 with two segments; 8 x 4096, 16 heads of 128
-// (256): 605, with four 652.
+// (256): 605, with four 652; forward alone 181, with two 188, and of 8 x 512 tokens 27 and 35.
 struct LaPlan {
   int nseg, seg_tokens;
 };

@@ -194,13 +194,15 @@ __device__ __forceinline__ void la_update(char* tb, int row0, const float* v, ca
 //
 // Why 64 columns: A and B are read once for each column tile (from L2: the tiles of a head run on one XCD), and 64 leaves the
 // registers and LDS for two or three workgroups to a CU; 128 columns by eight waves, one workgroup to a CU, took 996 us where
-// this takes 600 (below).  Why 64 tokens: the state's share, 4 dk dv flops a token, does not depend on it, the pairs' grows with it,
-// and the planes of the state are formed once for each chunk.  Why two buffers of B and X: one of each took 746 us.
-// What bounds it, bf16: heads of 64, HBM (32 x 1024 tokens, 12 heads, with gradients: 173 us, 704 MB, 4.1 TB/s; 50176 tokens of 12
-// heads, split over time, main launch 78 us, 3.9 TB/s).  Heads of 128 (8 x 4096 tokens, 16 heads, with gradients: 600 us,
-// 3.1 TB/s): vector unit 41%, matrix unit 28%, LDS 29% of the backward's cycles, in turn, since two waves per SIMD do not cover
-// each other's waits.  float16 takes 1.5 to 2.4 times and float32 2.5 to 3.4 times as long: two and three planes for each
-// input, formed on the way to LDS.
+// 64 took 746 (8 x 4096 tokens, below).  Why 64 tokens: the state's share, 4 dk dv flops a token, does not depend on it, the pairs' grows with it,
+// and the planes of the state are formed once for each chunk.  Why two buffers of B and X: with one of each the same call took
+// 746 us, before they were 653; two chunks ahead in three buffers, where the LDS has the room (sums alone), gained nothing.
+// What bounds it, bf16: heads of 64, HBM (32 x 1024 tokens, 12 heads, with gradients: 165 us, 704 MB, 4.3 TB/s; 50176 tokens of 12
+// heads, split over time, main launch 73 us, 4.2 TB/s).  Heads of 128 (8 x 4096 tokens, 16 heads, with gradients: 560 us,
+// 3.3 TB/s): vector unit 40%, matrix unit 30%, LDS 31% of the backward's cycles, in turn, since two waves per SIMD do not cover
+// each other's waits.  float16 takes 1.4 to 2.5 times and float32 2.1 to 3.8 times as long: two and three planes for each
+// input, formed on the way to LDS.  (Each wait on the transfers in flight that the compiler adds shows: for writes to LDS that
+// it joins, spills, stores that only some paths make.)
 template <int DT, int DA, bool SUM>
 __global__ void __launch_bounds__(LA_THREADS, la_waves(DT, DA)) la_kernel(const LaArgs args) {
   constexpr int NT = LA_THREADS, XT = LA_XT, C = la_chunk(DT, DA), KT = C / 16, NS = DA / 16, NP = LaT<DT>::NP,
