@@ -160,11 +160,11 @@ __device__ __forceinline__ void la_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// S += B^T X for 32 tokens' weighted X (v, the lane's column and tokens) in N planes; four tiles of S at a time, the
-// operands of the next four on their way.
+// S += B^T X for 32 tokens' weighted X (v, the lane's column and tokens) in N planes; two tiles of S at a time, the
+// operands of the next two on their way (four: heads of 256 spill, 217 -> 245 us, float16 of 128 192 for 186).
 template <int DA, int NP, int N, int PLANE>
 __device__ __forceinline__ void la_update(char* tb, int row0, const float* v, caf4* s, int li, int g) {
-  constexpr int M = DA / 16, T = DA == 256 ? 2 : 4;
+  constexpr int M = DA / 16, T = 2;
   LaFrag fb[2][T][NP];
   auto get = [&](int m0, LaFrag (*f)[NP]) __attribute__((always_inline)) {
 #pragma unroll
@@ -198,8 +198,8 @@ __device__ __forceinline__ void la_update(char* tb, int row0, const float* v, ca
 // and the planes of the state are formed once for each chunk.  Why two buffers of B and X: with one of each the same call took
 // 746 us, before they were 653; two chunks ahead in three buffers, where the LDS has the room (sums alone), gained nothing.
 // What bounds it, bf16: heads of 64, HBM (32 x 1024 tokens, 12 heads, with gradients: 165 us, 704 MB, 4.3 TB/s; 50176 tokens of 12
-// heads, split over time, main launch 73 us, 4.2 TB/s).  Heads of 128 (8 x 4096 tokens, 16 heads, with gradients: 560 us,
-// 3.3 TB/s): vector unit 40%, matrix unit 30%, LDS 31% of the backward's cycles, in turn, since two waves per SIMD do not cover
+// heads, split over time, main launch 73 us, 4.2 TB/s).  Heads of 128 (8 x 4096 tokens, 16 heads, with gradients: 555 to 585
+// us, 3.3 TB/s): vector unit 40%, matrix unit 30%, LDS 31% of the backward's cycles, in turn, since two waves per SIMD do not cover
 // each other's waits.  float16 takes 1.4 to 2.5 times and float32 2.1 to 3.8 times as long: two and three planes for each
 // input, formed on the way to LDS.  (Each wait on the transfers in flight that the compiler adds shows: for writes to LDS that
 // it joins, spills, stores that only some paths make.)
