@@ -143,8 +143,8 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) rn_kernel(const RnArgs 
   constexpr int NT = TPR > 256 ? TPR : 256, RPB = NT / TPR, WPR = TPR / 64;
   using VX = RnVec<DX, V>;
   using VS = RnVec<DS, V>;
-  __shared__ float red[2][WPR > 1 ? WPR : 1][2];
-  __shared__ float top[2][WPR > 1 ? WPR : 1];
+  __shared__ float red[2][RPB][WPR][2];
+  __shared__ float top[2][RPB][WPR];
   const int tid = threadIdx.x % TPR, rg = threadIdx.x / TPR, wave = tid >> 6;
   int parity = 0;
   // both sums over a row's threads
@@ -153,15 +153,15 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) rn_kernel(const RnArgs 
     if (MODE == RN_BWD) q = rn_wave_sum(q);
     if constexpr (WPR > 1) {      // two sets in turn: a set is written again only behind the next barrier
       if ((tid & 63) == 0) {
-        red[parity][wave][0] = p;
-        if (MODE == RN_BWD) red[parity][wave][1] = q;
+        red[parity][rg][wave][0] = p;
+        if (MODE == RN_BWD) red[parity][rg][wave][1] = q;
       }
       __syncthreads();
       p = q = 0.f;
 #pragma unroll
       for (int i = 0; i < WPR; ++i) {
-        p += red[parity][i][0];
-        if (MODE == RN_BWD) q += red[parity][i][1];
+        p += red[parity][rg][i][0];
+        if (MODE == RN_BWD) q += red[parity][rg][i][1];
       }
     }
   };
@@ -294,11 +294,11 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) rn_kernel(const RnArgs 
           for (int k = 1; k < U; ++k) all = rn_max(all, m[k]);
           all = rn_lane_max(all, 64);
           if constexpr (WPR > 1) {
-            if ((tid & 63) == 0) top[parity][wave] = all;
+            if ((tid & 63) == 0) top[parity][rg][wave] = all;
             __syncthreads();
-            all = top[parity][0];
+            all = top[parity][rg][0];
 #pragma unroll
-            for (int i = 1; i < WPR; ++i) all = rn_max(all, top[parity][i]);
+            for (int i = 1; i < WPR; ++i) all = rn_max(all, top[parity][rg][i]);
           }
 #pragma unroll
           for (int k = 0; k < U; ++k) m[k] = all;
@@ -332,12 +332,12 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) rn_kernel(const RnArgs 
     // dw of this workgroup: its rows' sums added in order
     if (a.part == nullptr) return;
     if constexpr (RPB > 1) {
-      __shared__ float acc[RPB - 1][64 * U * V];
+      __shared__ float acc[RPB - 1][TPR * U * V];
       if (rg > 0) {
 #pragma unroll
         for (int k = 0; k < U; ++k)
 #pragma unroll
-          for (int e = 0; e < V; ++e) acc[rg - 1][(k * V + e) * 64 + tid] = gw[k][e];
+          for (int e = 0; e < V; ++e) acc[rg - 1][(k * V + e) * TPR + tid] = gw[k][e];
       }
       __syncthreads();
       if (rg == 0) {
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) rn_kernel(const RnArgs 
 #pragma unroll
           for (int k = 0; k < U; ++k)
 #pragma unroll
-            for (int e = 0; e < V; ++e) gw[k][e] += acc[i][(k * V + e) * 64 + tid];
+            for (int e = 0; e < V; ++e) gw[k][e] += acc[i][(k * V + e) * TPR + tid];
       }
     }
     if (rg == 0) {
@@ -386,15 +386,18 @@ __global__ void __launch_bounds__(1024) rn_dw_kernel(const float* part, int n, v
 
 namespace {
 
-// Threads of a row and vectors of a thread: the fewest threads that hold the row in the registers.
+// Threads of a row and vectors of a thread: one vector each, the fewest threads of 64, 128, 256, 512 and 1024.  More vectors to fewer
+// threads, bf16: 64 x 768 4.1 us by two to 64 threads, 3.2 by one to 256; 8192 x 4096 58.2 by two to 256, 54.5 by one to 512;
+// 8192 x 8192 106.5 by four to 256, 101 by one to 1024, backward 132 and 121, 8 bits 101 and 92.  More threads than it takes: 50176 x
+// 384 30.5 by one to 64, 37.7 to 256; 32768 x 768 backward 37 by one to 128, 45 to 256 (42 by two to 64).
 struct RnShape {
   int tpr, u;
 };
 RnShape rn_shape(int64_t D, int v) {
   if (v == 1) return D <= 256 ? RnShape{64, 4} : D <= 1024 ? RnShape{256, 4} : D <= 4096 ? RnShape{1024, 4} : RnShape{1024, 16};
   const int64_t n = (D + v - 1) / v;
-  return n <= 64 ? RnShape{64, 1} : n <= 128 ? RnShape{64, 2} : n <= 256 ? RnShape{256, 1} : n <= 512 ? RnShape{256, 2}
-         : n <= 1024 ? RnShape{256, 4} : n <= 2048 ? RnShape{1024, 2} : RnShape{1024, 4};
+  return n <= 64 ? RnShape{64, 1} : n <= 128 ? RnShape{128, 1} : n <= 256 ? RnShape{256, 1} : n <= 512 ? RnShape{512, 1} : n <= 1024 ? RnShape{1024, 1}
+         : n <= 2048 ? RnShape{1024, 2} : RnShape{1024, 4};
 }
 int64_t rn_blocks(int64_t rows, int tpr, int mode) {
   const int64_t rpb = tpr < 256 ? 256 / tpr : 1, n = (rows + rpb - 1) / rpb;
@@ -417,12 +420,15 @@ template <int DX, int DS> void rn_launch(const RnArgs& a, int v, RnShape s, int 
     else if (s.u == 4) rn_launch_m<DX, DS, 1, 4, 1024>(a, mode, grid, st);
     else rn_launch_m<DX, DS, 1, 16, 1024>(a, mode, grid, st);
   } else if (s.tpr == 64) {
-    if (s.u == 1) rn_launch_m<DX, DS, V, 1, 64>(a, mode, grid, st);
-    else rn_launch_m<DX, DS, V, 2, 64>(a, mode, grid, st);
+    rn_launch_m<DX, DS, V, 1, 64>(a, mode, grid, st);
+  } else if (s.tpr == 128) {
+    rn_launch_m<DX, DS, V, 1, 128>(a, mode, grid, st);
   } else if (s.tpr == 256) {
-    if (s.u == 1) rn_launch_m<DX, DS, V, 1, 256>(a, mode, grid, st);
-    else if (s.u == 2) rn_launch_m<DX, DS, V, 2, 256>(a, mode, grid, st);
-    else rn_launch_m<DX, DS, V, 4, 256>(a, mode, grid, st);
+    rn_launch_m<DX, DS, V, 1, 256>(a, mode, grid, st);
+  } else if (s.tpr == 512) {
+    rn_launch_m<DX, DS, V, 1, 512>(a, mode, grid, st);
+  } else if (s.u == 1) {
+    rn_launch_m<DX, DS, V, 1, 1024>(a, mode, grid, st);
   } else if (s.u == 2) {
     rn_launch_m<DX, DS, V, 2, 1024>(a, mode, grid, st);
   } else if constexpr (V == 4) {
