@@ -238,6 +238,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
 
     q (B, H, dk); k (B, Hk, dk) and v (B, Hk, dv), as ``linear_attention``'s without L, of any strides.
     state (N, H, dk, dv) float32, the heads of one state contiguous, on 16-byte boundaries: updated in place.
+        A graph that has saved it (linear_attention's initial_state) raises in its backward, as behind torch's own writes.
     rows (B,) int32 or int64: which state is each stream's; None: stream b has state b, and N is B.  A row that is negative or
         not below N pads the batch: it gives zeros and touches no state.  Rows must differ from each other (of a state
         that two streams name, neither's update is certain).
@@ -255,6 +256,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     if rows is not None:
         _check_index(fn, "rows", rows, B)
     _check_state(fn, state, B if rows is None else None, H, dk, v.shape[2])
+    torch.autograd.graph.increment_version(state)
     return _step(q, k, v, log_decay.contiguous(), state, _index(rows), scale)
 
 
