@@ -45,6 +45,23 @@ def once(back, ctx, *grads):
     return once_differentiable(back)(ctx, *grads)
 
 
+def refuse_transforms(fn_name: str, *tensors: "torch.Tensor | None") -> None:
+    """For a call without an autograd function: refuse what does not see what the library does and would lose it without a
+    word, tangents of forward-mode AD, function transforms and traces."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"hclsm_amd.{fn_name}: a trace does not record this call; use torch.ops.hclsm_hip.{fn_name} in it")
+    transforms, level = torch._C._are_functorch_transforms_active(), torch.autograd.forward_ad._current_level
+    if not transforms and level < 0:
+        return
+    for t in tensors:
+        if t is None:
+            continue
+        if transforms and torch._C._functorch.is_functorch_wrapped_tensor(t):
+            raise RuntimeError(f"hclsm_amd.{fn_name}: no function transform (torch.func) goes through this call")
+        if level >= 0 and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"hclsm_amd.{fn_name}: an input has a tangent, and there is no forward-mode gradient here")
+
+
 _SAME_DEVICE = contextlib.nullcontext()
 
 

@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from hclsm_amd import _lib
-from hclsm_amd.kernels._common import call_on, once, require_gpu
+from hclsm_amd.kernels._common import call_on, once, refuse_transforms, require_gpu
 from hclsm_amd.kernels.ssm_scan_kernel import _no_node
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -242,9 +242,11 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     rows (B,) int32 or int64: which state is each stream's; None: stream b has state b, and N is B.  A row that is negative or
         not below N pads the batch: it gives zeros and touches no state.  Rows must differ from each other (of a state
         that two streams name, neither's update is certain).
-    Returns out (B, H, dv).  For inference: tensors that require grad are refused while gradients are recorded."""
+    Returns out (B, H, dv).  For inference: tensors that require grad are refused while gradients are recorded, and so are
+    tangents, function transforms and traces (torch.ops.hclsm_hip.linear_attention_step can be traced)."""
     fn = "linear_attention_step"
     require_gpu(fn, q, k, v, log_decay, state, rows)
+    refuse_transforms(fn, q, k, v, log_decay, state)
     if scale is None:
         scale = q.shape[-1] ** -0.5 if q.shape[-1] else 1.0
     scale = float(scale)

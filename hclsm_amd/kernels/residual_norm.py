@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from hclsm_amd import _lib
-from hclsm_amd.kernels._common import call_on, once, require_gpu
+from hclsm_amd.kernels._common import call_on, once, refuse_transforms, require_gpu
 from hclsm_amd.kernels.ssm_scan_kernel import _no_node
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -202,9 +202,11 @@ def residual_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None = None,
 
     group None: one scale for a row, scale (..., 1); 32, 64 or 128: one for each so many columns, scale (..., D / group).
     scale = max(max |y|, 2^-100) / 448, y8 = y / scale rounded to the nearest value.  A row with a NaN or an infinity
-    gives NaN.  For inference: tensors that require grad are refused while gradients are recorded."""
+    gives NaN.  For inference: tensors that require grad are refused while gradients are recorded, and so are tangents,
+    function transforms and traces (torch.ops.hclsm_hip.residual_rms_norm_fp8 can be traced)."""
     fn = "residual_rms_norm_fp8"
     require_gpu(fn, x, residual, weight)
+    refuse_transforms(fn, x, residual, weight)
     eps = float(eps)
     _check(fn, x, residual, weight, eps)
     _check_group(fn, x, group)

@@ -1,5 +1,5 @@
-"""linear_attention_step as a call that writes into a tensor of the user's: what autograd sees of it, and its state after
-thousands of tokens."""
+"""linear_attention_step as a call that writes into a tensor of the user's: what autograd, transforms and traces see of it, and
+its state after thousands of tokens."""
 
 from __future__ import annotations
 
@@ -76,3 +76,36 @@ def test_thousands_of_tokens(log_decay):
             most = max(most, ref.square().mean().sqrt().item())
     err = (s.double() - ref).square().mean().sqrt().item()
     assert err <= 2 * n ** 0.5 * 2.0 ** -24 * most, (err / most * 2 ** 24)
+
+
+def _with_tangents(t):
+    return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+
+@pytest.mark.gpu
+def test_tangents_transforms_and_traces_are_refused():
+    """None of these would see what the library does: a call drops tangents, and a trace would hold an empty tensor."""
+    from hclsm_amd.kernels import linear_attention_step, residual_rms_norm_fp8
+    q, k, v, d, s = _token(device="cuda")
+    x, w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    before = s.clone()
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        for i in range(5):
+            args = [_with_tangents(t) if j == i else t for j, t in enumerate((q, k, v, d, s))]
+            with pytest.raises(RuntimeError, match="tangent"):
+                linear_attention_step(*args)
+        for args in ((_with_tangents(x), x, w), (x, _with_tangents(x), w), (x, x, _with_tangents(w))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                residual_rms_norm_fp8(*args)
+        residual_rms_norm_fp8(x, x, w)      # no input has one
+        with pytest.raises(RuntimeError, match="tangent"):
+            torch.func.vmap(lambda t: t + residual_rms_norm_fp8(_with_tangents(x))[1].sum())(x)
+    with pytest.raises(RuntimeError, match="transform"):
+        torch.func.vmap(lambda t: linear_attention_step(t, k, v, d, s))(q[None])
+    with pytest.raises(RuntimeError, match="transform"), torch.no_grad():
+        torch.func.jvp(lambda t: residual_rms_norm_fp8(t)[1], (x,), (x,))
+    with pytest.raises(RuntimeError, match="trace"):
+        torch.jit.trace(lambda t: linear_attention_step(t, k, v, d, s), (q,))
+    with pytest.raises(RuntimeError, match="trace"):
+        torch.jit.trace(lambda t: residual_rms_norm_fp8(t)[1], (x,))
+    assert torch.equal(s, before)
