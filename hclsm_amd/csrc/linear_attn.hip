@@ -36,9 +36,8 @@ struct LaSizes {
     const int c = la_chunk(dtype, la_padded(dk)), d = la_chunk(dtype, la_padded(dv));
     return bwd && d > c ? d : c;
   }
-  LaPlan plan(bool bwd) const {
-    return la_plan(bwd ? units() * (tiles(dv) + 2 * tiles(dk)) : units() * tiles(dv), L, chunk(bwd));
-  }
+  int64_t column_tiles(bool bwd) const { return bwd ? tiles(dv) + 2 * tiles(dk) : tiles(dv); }      // of all jobs
+  LaPlan plan(bool bwd) const { return la_plan(units() * column_tiles(bwd), L, chunk(bwd)); }
   int64_t seg_bytes(bool bwd) const {
     const LaPlan p = plan(bwd);
     return p.nseg > 1 ? la_up(units() * p.nseg * dk * dv * 4) : 0;
@@ -135,16 +134,13 @@ int la_launch_any(const LaArgs& a, int dtype, int da, bool sum, hipStream_t st) 
 }
 
 // All jobs of a call: sums of segments, states in front of them, outputs.  Jobs of the same padded sizes share a launch.
-int la_run(LaArgs a, int dtype, hipStream_t st) {
+int la_run(LaArgs a, const LaSizes& z, bool bwd, hipStream_t st) {
   // Jobs of different padded sizes share a launch of the larger one where together they are on the chip at once (two workgroups
-  // to each of 256 CUs): they then run side by side.  Elsewhere the padding would cost, and they run one after the other.
-  int64_t all = 0;
-  int most = 0;
-  for (int i = 0; i < a.njobs; ++i) {
-    all += (int64_t)a.B * a.H * a.nseg * a.job[i].xtiles;
-    most = la_padded(a.job[i].da) > most ? la_padded(a.job[i].da) : most;
-  }
-  auto padded = [&](int i) { return all <= 512 ? most : la_padded(a.job[i].da); };
+  // to each of 256 CUs): they then run side by side.  Elsewhere the padding would cost, and they run one after the other.  All
+  // jobs that the sizes have count, wanted or not: a job's chunks, and so its bits, follow from its padded size.
+  const int64_t all = z.units() * a.nseg * z.column_tiles(bwd);
+  const int64_t most = bwd && z.dv > z.dk ? z.dv : z.dk;
+  auto padded = [&](int i) { return la_padded(all <= 512 ? most : a.job[i].da); };
   for (int pass = a.nseg > 1 ? 0 : 2; pass < 3; ++pass) {
     if (pass == 1) {
       if (a.nseg <= LA_FEW_SEGMENTS) continue;      // the main kernel adds them up itself
@@ -168,7 +164,7 @@ int la_run(LaArgs a, int dtype, hipStream_t st) {
       }
       one.items = a.B * a.H * a.nseg;
       one.by_xcd = one.items >= 64;
-      if (int rc = la_launch_any(one, dtype, da, pass == 0, st)) return rc;
+      if (int rc = la_launch_any(one, z.dtype, da, pass == 0, st)) return rc;
     }
   }
   return 0;
@@ -334,7 +330,7 @@ extern "C" int hclsm_linear_attention_forward(const HclsmLinearAttention* x, voi
   o.xtiles = (int)z.tiles(z.dv);
   o.cp = o.ci = x->scale;
   o.cu = 1.f;
-  return la_run(a, z.dtype, (hipStream_t)stream);
+  return la_run(a, z, false, (hipStream_t)stream);
 }
 
 extern "C" int hclsm_linear_attention_backward(const HclsmLinearAttention* x, void* workspace, int64_t workspace_bytes,
@@ -397,7 +393,7 @@ extern "C" int hclsm_linear_attention_backward(const HclsmLinearAttention* x, vo
     j->back = 1;
   }
   if (a.njobs == 0) return 0;
-  if (int rc = la_run(a, z.dtype, st)) return rc;
+  if (int rc = la_run(a, z, true, st)) return rc;
   if (G > 1 && x->dk_out)
     if (int rc = la_group(wk, x->dk_out, z.B * z.L * z.Hk, (int)G, z.dk, z.dtype, st)) return rc;
   if (G > 1 && x->dv_out)
