@@ -285,7 +285,7 @@ def _step(q, k, v, log_decay, state, rows, scale):
     _, Hk, dv = v.shape
     out = q.new_empty((B, H, dv))
     x = _lib.pack_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(), _ptr(rows),
-                       out.data_ptr(), qb, qh, kb, kh, vb, vh, state.stride(0), state.shape[0], B, H, Hk, dk, dv, scale,
-                       _CODE[q.dtype], _index_code(rows))
+                       out.data_ptr(), qb, qh, kb, kh, vb, vh, state.stride(0) if state.shape[0] > 1 else 0, state.shape[0], B, H,
+                       Hk, dk, dv, scale, _CODE[q.dtype], _index_code(rows))
     _run("hclsm_linear_attention_step", q, x)
     return out

@@ -109,3 +109,21 @@ def test_tangents_transforms_and_traces_are_refused():
     with pytest.raises(RuntimeError, match="trace"):
         torch.jit.trace(lambda t: residual_rms_norm_fp8(t)[1], (x,))
     assert torch.equal(s, before)
+
+
+def test_a_state_alone_in_its_pool_may_have_any_stride(no_launch):
+    from hclsm_amd import _lib
+    q, k, v, d, _ = _token(B=1)
+    s = torch.zeros(4, 3 * 16 * 24 + 1)[:, :-1].unflatten(1, (3, 16, 24))[:1]
+    assert s.stride(0) % 4 == 1
+    F.linear_attention_step(q, k, v, d, s)
+    assert _lib.HclsmLinearAttentionStep.from_buffer_copy(no_launch[0]).state_sb == 0
+
+
+@pytest.mark.gpu
+def test_a_state_alone_in_its_pool():
+    q, k, v, d, s = _token(B=1, device="cuda")
+    odd = torch.zeros(4, 3 * 16 * 24 + 1, device="cuda")[:, :-1].unflatten(1, (3, 16, 24))[:1]
+    odd.copy_(s)
+    assert torch.equal(F.linear_attention_step(q, k, v, d, odd), F.linear_attention_step(q, k, v, d, s))
+    assert torch.equal(odd, s)
