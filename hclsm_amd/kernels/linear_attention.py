@@ -218,7 +218,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     fn = "linear_attention"
     require_gpu(fn, q, k, v, log_decay, initial_state, seq_lens)
     if scale is None:
-        scale = q.shape[-1] ** -0.5 if q.shape[-1] else 1.0
+        scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
     scale = float(scale)
     _check(fn, q, k, v, log_decay, scale, False)
     _check_index(fn, "seq_lens", seq_lens, q.shape[0])
@@ -248,7 +248,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     require_gpu(fn, q, k, v, log_decay, state, rows)
     refuse_transforms(fn, q, k, v, log_decay, state)
     if scale is None:
-        scale = q.shape[-1] ** -0.5 if q.shape[-1] else 1.0
+        scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
     scale = float(scale)
     _check(fn, q, k, v, log_decay, scale, True)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):

@@ -127,3 +127,11 @@ def test_a_state_alone_in_its_pool():
     odd.copy_(s)
     assert torch.equal(F.linear_attention_step(q, k, v, d, odd), F.linear_attention_step(q, k, v, d, s))
     assert torch.equal(odd, s)
+
+
+def test_a_scalar_is_refused_as_any_other_shape(no_launch):
+    q, k, v, d, s = _token()
+    with pytest.raises(ValueError, match="q must be"):
+        F.linear_attention_step(q[0, 0, 0], k, v, d, s)
+    with pytest.raises(ValueError, match="q must be"):
+        F.linear_attention(q[0, 0, 0], k, v, d)
