@@ -182,7 +182,8 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, wei
     x (..., D), bfloat16, float16 or float32, 1 <= D <= 16384; residual: x's shape, x's type or float32, or None (then h is
     x, or a view of it where gradients are recorded); weight (D,) of any of the float types, None: ones.  Rows of (rows, D) views may lie any distance apart; other
     views are copied.  y has x's type, h the residual's.  Differentiable in all three, through both outputs; float32 between
-    the loads and the one rounding of each output."""
+    the loads and the one rounding of each output (a row whose squares add up to more than float32 holds, 3.4e38, gives
+    zeros)."""
     fn = "residual_rms_norm"
     require_gpu(fn, x, residual, weight)
     eps = float(eps)
@@ -201,8 +202,9 @@ def residual_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None = None,
     """(y8, scale, h): ``residual_rms_norm`` with y as y8 * scale, y8 of torch.float8_e4m3fn.
 
     group None: one scale for a row, scale (..., 1); 32, 64 or 128: one for each so many columns, scale (..., D / group).
-    scale = max(max |y|, 2^-100) / 448, y8 = y / scale rounded to the nearest value.  A row with a NaN or an infinity
-    gives NaN.  For inference: tensors that require grad are refused while gradients are recorded, and so are tangents,
+    scale = max(max |y|, 2^-100) / 448, y8 = y / scale rounded to the nearest value.  A NaN makes its row NaN, and so does
+    an infinity with one scale for a row; with groups, it makes its own group NaN and the row's other groups zeros (as
+    ``residual_rms_norm`` has them: the root is infinite).  For inference: tensors that require grad are refused while gradients are recorded, and so are tangents,
     function transforms and traces (torch.ops.hclsm_hip.residual_rms_norm_fp8 can be traced)."""
     fn = "residual_rms_norm_fp8"
     require_gpu(fn, x, residual, weight)
