@@ -1,13 +1,50 @@
-"""Linear attention's ways through its launches: the same bits whichever gradients are asked for."""
+"""Linear attention's ways through its launches: many segments of a long stream, jobs of different padded sizes with and without
+a launch in common, and the same bits whichever gradients are asked for.  Tolerances: test_linear_attention_gpu.py."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
-from test_linear_attention_gpu import BF16, F16, F32, _inputs
+from test_linear_attention_gpu import BF16, F16, F32, _compare, _inputs
 
 pytestmark = pytest.mark.gpu
+
+CODE = {F32: 0, BF16: 1, F16: 2}
+
+
+def _segments(B, L, H, dk, dv, dtype, backward):
+    from hclsm_amd import _lib
+    n = _lib.lib().hclsm_linear_attention_workspace(B, L, H, H, dk, dv, CODE[dtype], backward)
+    return n // ((3 if backward else 1) * B * H * dk * dv * 4)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("state", [False, True])
+def test_more_than_32_segments(dtype, state):
+    """Segments' states by a launch of their own, more than two of its rounds of 16; lengths inside a segment, on its border, one
+    token either side of it, and none."""
+    B, L, H, dk, dv = 2, 8700, 2, 32, 24
+    chunks = -(-L // (32 if dtype == F32 else 64))
+    n = [_segments(B, L, H, dk, dv, dtype, bwd) for bwd in (0, 1)]
+    assert min(n) > 32, n
+    border = 20 * -(-chunks // n[0]) * (32 if dtype == F32 else 64)
+    ins = list(_inputs(B, L, H, H, dk, dv, dtype, 31, state))
+    ins[4] = torch.tensor([-1e-3, -0.05])
+    for lens in (None, [border, border + 1], [border - 1, 5000], [0, 8699]):
+        print(f"{n} segments, {dtype}, {lens}", flush=True)
+        _compare(*ins, lens=lens)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", [(130, 70, 1, 1, 64, 128), (45, 70, 2, 1, 48, 256), (66, 37, 2, 2, 136, 64)])
+def test_a_launch_for_each_padded_size(shape, dtype):
+    """More workgroups than are on the chip at once: jobs of dk and of dv padded differently run one after the other."""
+    B, L, H, Hk, dk, dv = shape
+    tiles = lambda d: -(-d // 64)
+    assert B * H * (tiles(dv) + 2 * tiles(dk)) > 512 and _segments(B, L, H, dk, dv, dtype, 1) == 0
+    print(f"launches {shape} {dtype}", flush=True)
+    _compare(*_inputs(*shape, dtype, 32))
 
 
 @pytest.mark.parametrize("dtype,dk,dv", [(F16, 64, 128), (BF16, 64, 256), (F32, 128, 48), (F16, 256, 64), (BF16, 128, 64)])
