@@ -6,10 +6,19 @@ namespace hclsm {
 namespace {
 
 // Segments of a call: where heads and columns alone are fewer workgroups than the chip has CUs, the tokens are split, each segment's
-// sum formed first (from zero), the states in front of the segments from those, and then all segments at once, two workgroups to a
-// CU.  The sums read B and X once more.  Measured, 50176 tokens of 12 heads of 64: 21 segments 140 us, 32: 130, 42: 116, 53: 124, 64:
-// 119; training steps of 32 x 1024 tokens (384 workgroups forward): 173 unsplit, 183 with two segments; 8 x 4096, 16 heads of 128
-// (256): 605, with four 652; forward alone 181, with two 188, and of 8 x 512 tokens 27 and 35.
+// sum formed first (from zero), the states in front of the segments from those, and then all segments at once: two workgroups to a
+// CU, and four chunks or more to a segment.  The sums read B and X once more.  Measured (us):
+//   50176 tokens, 12 heads of 64, bf16: 21 segments 140, 32: 130, 42 (the rule's): 116, 53: 124, 64: 119
+//   2048 tokens in 1, 2, 3 and 4 segments, the rule's in brackets, by workgroups (64: eight segments)
+//                      64                128              160               192               224               256
+//     bf16 of 64      64 54 40 35 (34)   63 56 50 44 (44)  64 64 52 53 (50)  65 65 60 57 (64)  65 66 62 70 (64)  66 69 70 85 (64)
+//     bf16 of 128     80 66 50 43 (47)   79 68 64 58 (56)  79 85 67 77 (65)  80 85 88 82 (85)  81 86 90 97 (85)  82 93 101 104 (82)
+//     float16 of 64   98 80 58 48 (43)   98 82 74 61 (61)  99 102 76 88 (74) 101 102 100 89 (100) 102 102 104 102 (101) 103 105 108 109 (103)
+//     float32 of 64   145 119 88 68 (56) 147 123 110 93 (89) 147 152 117 118 (113) 149 155 135 130 (159) 150 163 149 165 (162) 155 174 165 179 (159)
+//   one prompt, 12 heads of 64, unsplit, in segments of two chunks (the rule's): bf16 128 tokens 8.1 11.1 (8.1), 256: 11.6 13.6
+//     (11.6), 512: 19.0 14.8 (18.7), 1024: 33.2 18.1 (20.1); float32 128: 12.6 12.7 (12.7), 256: 21.5 15.9 (21.3), 512: 38.5 19.3 (22.8)
+// So two segments of 171 to 255 workgroups take 5% less to 8% more, where four would take up to 13% less below 200 for heads of 64, and
+// segments of two chunks would gain a fifth for short prompts of six chunks or more.
 struct LaPlan {
   int nseg, seg_tokens;
 };
@@ -210,7 +219,7 @@ LaArgs la_common(const HclsmLinearAttention* x, const LaPlan& p) {
 
 // One token: S = a S + k v^T in place, o = c q^T S.  A workgroup has 64 columns of one head's state: 16 lanes of four columns,
 // 16 groups of rows.  Each state is read and written once, which bounds it (HBM); the loads of eight rows are in flight: 111 us for
-// 256 states of 16 heads of 128 x 128 (537 MB, 4.9 TB/s, a copy's rate), 4.8 for 16 of 12 heads of 64 x 64 (latency).
+// 256 states of 16 heads of 128 x 128 (537 MB, 4.9 TB/s, a copy's rate), 5.0 for 16 of 12 heads of 64 x 64 (latency).
 constexpr int LS_COLS = 64, LS_GROUPS = 16, LS_BATCH = 8;
 
 struct LsArgs {

@@ -10,7 +10,7 @@
 // elements where the columns or the alignment do not allow it), so that it is read once; the weight stays in registers while a
 // workgroup goes from row to row, the next row's loads in flight.  The backward's two sums travel together.
 // Measured, bf16: 50176 x 384 forward 29 us, backward 28 and dw's sums 4 (5.0 TB/s together); 32768 x 4096 to 8 bits 185 us,
-// 5.1 TB/s; 64 x 768 4.3 us (latency).  8027 x 1001 in single elements, float16 with a float32 stream: forward 21 us, backward 26,
+// 5.1 TB/s; 64 x 768 3.5 us (latency).  8027 x 1001 in single elements, float16 with a float32 stream: forward 21 us, backward 26,
 // 4.4 TB/s.  A copy of 1 GiB reaches 5.04.
 #include "internal.h"
 
@@ -387,9 +387,13 @@ __global__ void __launch_bounds__(1024) rn_dw_kernel(const float* part, int n, v
 namespace {
 
 // Threads of a row and vectors of a thread: one vector each, the fewest threads of 64, 128, 256, 512 and 1024.  More vectors to fewer
-// threads, bf16: 64 x 768 4.1 us by two to 64 threads, 3.2 by one to 256; 8192 x 4096 58.2 by two to 256, 54.5 by one to 512;
+// threads, bf16: 64 x 768 4.1 us by two to 64 threads, 3.5 by one to 128; 8192 x 4096 58.2 by two to 256, 54.5 by one to 512;
 // 8192 x 8192 106.5 by four to 256, 101 by one to 1024, backward 132 and 121, 8 bits 101 and 92.  More threads than it takes: 50176 x
 // 384 30.5 by one to 64, 37.7 to 256; 32768 x 768 backward 37 by one to 128, 45 to 256 (42 by two to 64).
+// Longer rows do not fit the 128 registers of 1024 threads in the backward, and the compiler spills (bytes a lane): two vectors 48 (bf16), 36
+// (float16), 168 (float32 stream), four of float32 204, 16 single elements 228 to 240, and 36 to 44 in their 8-bit form.  67 million elements,
+// backward by rows of 8192 and 16384: bf16 124 and 180 us, float32 stream 225 and 444, float32 225 and 427; by rows of 5001, backward 770 to
+// 1040, 8 bits 290 to 360, forward (without spills) 157 to 214.  Forward and 8 bits of 16384 run as shorter rows do, 4.8 to 5.2 TB/s.
 struct RnShape {
   int tpr, u;
 };
