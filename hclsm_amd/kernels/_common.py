@@ -38,7 +38,11 @@ def common_float_dtype(*tensors: torch.Tensor) -> torch.dtype:
 
 def once(back, ctx, *grads):
     """back(ctx, *grads), which cannot be differentiated again: where a graph of the gradients is asked for (create_graph),
-    differentiating it raises.  Elsewhere without the wrapper, which costs several us."""
+    differentiating it raises, and a gradient with a tangent is refused.  Elsewhere without the wrapper, which costs several us."""
+    if torch.autograd.forward_ad._current_level >= 0:
+        for g in grads:
+            if g is not None and torch.autograd.forward_ad.unpack_dual(g).tangent is not None:
+                raise RuntimeError("hclsm_amd: a gradient has a tangent, and there is no forward-mode derivative of this backward")
     if not torch.is_grad_enabled():
         return back(ctx, *grads)
     from torch.autograd.function import once_differentiable
